@@ -8,7 +8,7 @@ CSRC_DIR = os.path.join(PKG_DIR, 'csrc')
 LIB_NAME = 'libdlblas_fp8_gemm.so'
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 HOST_PATH = os.path.join(PKG_DIR, '_host.so')
-SOURCES = ['dlblas_fp8_gemm.hip', 'dlblas_fp8_moe.hip']
+SOURCES = ['dlblas_fp8_gemm.hip', 'dlblas_fp8_moe.hip', 'dlblas_decoder.hip']
 
 # packed fp32 VALU forms are switched off for every device compile of this library
 HIPCC_FLAGS = [
@@ -38,8 +38,8 @@ def build_library(verbose: bool = False, defines=(), out_path: str = LIB_PATH) -
 
 
 def build_host_module() -> str:
-    """Compile csrc/host_calls.cpp (the entry points as native calls on torch tensors; host code only) into _host.so next to
-    this file; always recompiles.  Returns its path."""
+    """Compile csrc/host_calls.cpp and host_steps.cpp (the entry points as native calls on torch tensors; host code only) into
+    _host.so next to this file; always recompiles.  Returns its path."""
     import sysconfig
 
     import torch
@@ -47,7 +47,8 @@ def build_host_module() -> str:
     include = [os.path.join(torch_dir, 'include'), os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'), sysconfig.get_paths()['include']]
     rocm = os.path.dirname(os.path.dirname(os.path.realpath(find_hipcc())))
     include.append(os.path.join(rocm, 'include'))
-    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-shared', '-fPIC', os.path.join(CSRC_DIR, 'host_calls.cpp'), '-DUSE_ROCM',
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-shared', '-fPIC', os.path.join(CSRC_DIR, 'host_calls.cpp'),
+           os.path.join(CSRC_DIR, 'host_steps.cpp'), '-DUSE_ROCM',
            '-D__HIP_PLATFORM_AMD__=1', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}']
     cmd += [f'-I{d}' for d in include] + [f'-L{os.path.join(torch_dir, "lib")}'] + [f'-l{lib}' for lib in ('c10', 'c10_hip', 'torch_cpu', 'torch_hip', 'torch_python')]
     cmd += ['-o', HOST_PATH]

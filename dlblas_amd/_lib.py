@@ -1,4 +1,4 @@
-"""ctypes binding of libdlblas_fp8_gemm.so (the C ABI declared in include/dlblas_fp8_gemm.h and dlblas_fp8_moe.h).
+"""ctypes binding of libdlblas_fp8_gemm.so (the C ABI declared in include/dlblas_fp8_gemm.h, dlblas_fp8_moe.h and dlblas_decoder.h).
 
 The library is the only implementation: when it has not been built, every op raises ImportError.  There is no
 PyTorch or CPU fallback.  The calling convention (``c_void_p(tensor.data_ptr())`` operands, the stream handle as
@@ -12,7 +12,7 @@ import torch
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 OUT_BF16, OUT_F32 = 0, 1
 WS_COUNTER_BYTES = 65536
 WORKSPACE_BYTES = WS_COUNTER_BYTES + (32 << 20)
@@ -25,7 +25,7 @@ ERR_NULL_POINTER, ERR_BAD_SHAPE, ERR_BAD_STRIDE, ERR_BAD_DTYPE, ERR_WORKSPACE, E
 
 _c_i64, _c_i32, _c_vp, _c_sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t
 
-# name -> (restype, argtypes); must list every symbol the headers under include/ declare
+# name -> (restype, argtypes); must list every symbol that dlblas_fp8_gemm.h and dlblas_fp8_moe.h declare
 SYMBOLS = {
     'dlb_abi_version': (ctypes.c_int, []),
     'dlb_last_error': (ctypes.c_char_p, []),
@@ -88,6 +88,25 @@ SYMBOLS = {
     'dlb_scale_relayout': (ctypes.c_int, [_c_vp, _c_vp] + [_c_i64] * 5 + [_c_vp]),
 }
 
+# the same for dlblas_decoder.h; the calls are in _decoder.py
+DECODER_SYMBOLS = {
+    'dlb_rms_norm': (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, ctypes.c_int, _c_vp, ctypes.c_int] + [_c_vp, _c_i64] * 2 + [_c_i64] * 2 + [ctypes.c_float, _c_vp]),
+    'dlb_rms_norm_quant':
+    (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp] + [_c_i64] * 3 + [ctypes.c_float] * 2 + [_c_vp]),
+    'dlb_rms_norm_backward_workspace_bytes': (_c_sz, [_c_i64] * 2),
+    'dlb_rms_norm_backward':
+    (ctypes.c_int, [_c_vp, _c_i64] * 3 + [ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, ctypes.c_float, _c_vp, _c_sz, _c_vp]),
+    'dlb_moe_sort_workspace_bytes': (_c_sz, [_c_i64] * 3),
+    'dlb_moe_sort': (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64] + [_c_vp] * 5 + [_c_i64] * 5 + [_c_vp, _c_sz, _c_vp]),
+    'dlb_moe_permute': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_i64, _c_i64] + [_c_vp] * 4 + [_c_i64] * 4 + [_c_vp]),
+    'dlb_moe_unpermute': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 3 + [_c_i64] * 5 + [_c_vp]),
+    'dlb_moe_unpermute_backward':
+    (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 4 + [_c_i64, _c_vp] + [_c_i64] * 4 + [_c_vp]),
+    'dlb_w4_gemm':
+    (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 5 + [_c_vp]),
+    'dlb_w4_quant': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 3 + [_c_i64] * 3 + [_c_vp]),
+}
+
 _lock = threading.Lock()
 _lib = None
 _workspaces = {}
@@ -118,7 +137,7 @@ def load() -> ctypes.CDLL:
             lib = ctypes.CDLL(path)
         except OSError as exc:
             raise ImportError(f'cannot load {path}: {exc}') from exc
-        for name, (restype, argtypes) in SYMBOLS.items():
+        for name, (restype, argtypes) in (SYMBOLS | DECODER_SYMBOLS).items():
             try:
                 fn = getattr(lib, name)
             except AttributeError:

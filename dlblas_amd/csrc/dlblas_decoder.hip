@@ -1,0 +1,405 @@
+// C ABI of the steps around the products of a decoder block: argument validation and launches.
+// The declarations and the contract of every entry point are in include/dlblas_decoder.h.
+#include "../../include/dlblas_decoder.h"
+
+#include <type_traits>
+
+#include "host_common.h"
+#include "moe_sort.h"
+#include "rms_norm.h"
+#include "w4_gemm.h"
+
+namespace dlb {
+namespace {
+
+int finish(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(DLB_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return DLB_OK;
+}
+
+bool bad_dtype(int d) { return d < kInBf16 || d > kInF32; }
+int64_t size_of(int d) { return d == kInF32 ? 4 : 2; }
+bool off_elements(const void* p, int dtype) { return misaligned(p, size_of(dtype)); }
+
+// Calls f with the type as a constant.
+template <typename F>
+void with_type(int dtype, F f) {
+  if (dtype == kInBf16)
+    f(std::integral_constant<int, kInBf16>());
+  else if (dtype == kInF16)
+    f(std::integral_constant<int, kInF16>());
+  else
+    f(std::integral_constant<int, kInF32>());
+}
+template <int... C, typename F>
+void with_chunks(int chunks, F f) {
+  (void)((chunks == C && (f(std::integral_constant<int, C>()), true)) || ...);
+}
+
+// ---- norms ------------------------------------------------------------------------------------------------------------
+
+// Threads of a workgroup and chunks of eight columns per thread for rows of H.
+struct RowShape {
+  int threads, chunks;
+};
+RowShape row_shape(int64_t H, int want_chunks) {
+  const int64_t chunks = ceil_div(H, 8);
+  int c = want_chunks;
+  while (c < 4 && ceil_div(chunks, c) > kNormMaxThreads) c *= 2;
+  return {static_cast<int>(ceil_div(ceil_div(chunks, c), 64) * 64), c};
+}
+
+int check_norm(const void* x, const void* residual, int dtype, const void* weight, int weight_dtype, const void* sum, int64_t rows,
+               int64_t H) {
+  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (weight_dtype != dtype && weight_dtype != kInF32)
+    return fail(DLB_ERR_BAD_DTYPE, "weight_dtype %d is neither the rows' type nor DLB_IN_F32", weight_dtype);
+  if (rows < 0 || H < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld H=%lld)", (long long)rows, (long long)H);
+  if (rows > (1ll << 31) - 1 || H > DLB_NORM_MAX_COLUMNS)
+    return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / H=%lld beyond the supported range (H at most %d)", (long long)rows, (long long)H,
+                DLB_NORM_MAX_COLUMNS);
+  if (rows == 0 || H == 0) return DLB_OK;
+  if (!x || !weight || (residual && !sum)) return fail(DLB_ERR_NULL_POINTER, "x, weight, or sum of a call with a residual is NULL");
+  if (off_elements(x, dtype) || off_elements(residual, dtype) || off_elements(sum, dtype) || off_elements(weight, weight_dtype))
+    return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
+  return DLB_OK;
+}
+
+template <bool QUANT>
+int launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
+  const RowShape shape = row_shape(a.H, 2);
+  const dim3 grid(static_cast<unsigned>(a.rows)), block(shape.threads);
+  with_type(dtype, [&](auto t) {
+    with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_kernel<t(), QUANT, c()>), grid, block, 0, st, a); });
+  });
+  return finish("rms_norm");
+}
+
+// Workgroups of the backward pass, each of which leaves a share of dw.
+int norm_grad_blocks(int64_t rows) { return static_cast<int>(rows < 512 ? rows : 512); }
+
+// ---- tokens by expert -------------------------------------------------------------------------------------------------
+
+int check_rows(int64_t tokens, int64_t H, int64_t topk, int64_t num_rows) {
+  if (tokens < 0 || H < 0 || num_rows < 0)
+    return fail(DLB_ERR_BAD_SHAPE, "negative dimension (tokens=%lld H=%lld num_rows=%lld)", (long long)tokens, (long long)H, (long long)num_rows);
+  if (topk < 1 || topk > kSortMaxTopk) return fail(DLB_ERR_BAD_SHAPE, "topk=%lld is not 1 ... %d", (long long)topk, kSortMaxTopk);
+  if (tokens * topk > (1ll << 31) - 1 || num_rows > (1ll << 31) - 1 || tokens > (1ll << 31) - 1)
+    return fail(DLB_ERR_BAD_SHAPE, "tokens * topk=%lld or num_rows=%lld does not fit the int32 tables", (long long)(tokens * topk), (long long)num_rows);
+  if (H > (1ll << 28)) return fail(DLB_ERR_BAD_SHAPE, "H=%lld beyond the supported range", (long long)H);
+  return DLB_OK;
+}
+
+int64_t sort_blocks(int64_t slots) { return slots > 0 ? ceil_div(slots, kSortBlockSlots) : 1; }
+
+// ---- 4-bit weights ----------------------------------------------------------------------------------------------------
+
+struct W4Shape {
+  int mt, nt, waves;
+};
+W4Shape w4_shape(int64_t rows_each, int64_t N, int64_t K) {
+  const int mt = rows_each <= 16 ? 1 : rows_each <= 32 ? 2 : 4;
+  const int nt = mt == 1 ? 1 : 2;
+  int64_t waves = ceil_div(K, 128);
+  if (waves > 8) waves = 8;
+  return {mt, nt, static_cast<int>(waves)};
+}
+
+template <int T, int STEPS>
+void launch_w4(const W4Args& a, const W4Shape& s, int64_t y_blocks, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * s.nt)), static_cast<unsigned>(y_blocks)), block(64 * s.waves);
+  const size_t lds = static_cast<size_t>(s.waves) * s.mt * s.nt * 1024;
+  if (s.mt == 1)
+    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 1, 1>), grid, block, lds, st, a);
+  else if (s.mt == 2)
+    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 2, 2>), grid, block, lds, st, a);
+  else
+    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 4, 2>), grid, block, lds, st, a);
+}
+
+}  // namespace
+}  // namespace dlb
+
+extern "C" {
+
+int dlb_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, int dtype,
+                 const void* weight, int weight_dtype, void* y, int64_t y_row_stride, void* sum, int64_t sum_row_stride,
+                 int64_t rows, int64_t H, float eps, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (int rc = check_norm(x, residual, dtype, weight, weight_dtype, sum, rows, H)) return rc;
+  if (rows == 0 || H == 0) return DLB_OK;
+  if (!y) return fail(DLB_ERR_NULL_POINTER, "y is NULL");
+  if (off_elements(y, dtype)) return fail(DLB_ERR_ALIGNMENT, "y is not aligned to its elements");
+  if (y_row_stride < H || (residual && sum_row_stride < H)) return fail(DLB_ERR_BAD_STRIDE, "a row stride of the outputs is smaller than H=%lld", (long long)H);
+  if (x_row_stride < 0 || residual_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  NormArgs a{};
+  a.x = x, a.res = residual, a.w = weight, a.y = y, a.sum = sum;
+  a.rows = rows, a.x_rs = x_row_stride, a.res_rs = residual_row_stride, a.y_rs = y_row_stride, a.sum_rs = sum_row_stride;
+  a.H = static_cast<int>(H), a.w_f32 = weight_dtype == kInF32, a.eps = eps;
+  return launch_norm<false>(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+int dlb_rms_norm_quant(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, int dtype,
+                       const void* weight, int weight_dtype, void* q, float* s, int64_t s_stride_m, int64_t s_stride_k,
+                       void* sum, int64_t sum_row_stride, int64_t rows, int64_t H, float eps, float quant_eps, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (int rc = check_norm(x, residual, dtype, weight, weight_dtype, sum, rows, H)) return rc;
+  if (H % kScaleBlock != 0) return fail(DLB_ERR_BAD_SHAPE, "H=%lld is not a multiple of the group size 128", (long long)H);
+  if (!(quant_eps >= 1e-30f)) return fail(DLB_ERR_BAD_SHAPE, "quant_eps=%g is below 1e-30: a scale could not be divided by", quant_eps);
+  if (rows == 0 || H == 0) return DLB_OK;
+  if (!q || !s) return fail(DLB_ERR_NULL_POINTER, "q or s is NULL");
+  if (misaligned(q, 8) || misaligned(s, 4)) return fail(DLB_ERR_ALIGNMENT, "q must be 8-byte, s 4-byte aligned");
+  if (s_stride_m < 0 || s_stride_k < 0 || x_row_stride < 0 || residual_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride");
+  if (residual && sum_row_stride < H) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of sum is smaller than H=%lld", (long long)sum_row_stride, (long long)H);
+  NormArgs a{};
+  a.x = x, a.res = residual, a.w = weight, a.sum = sum, a.q = static_cast<uint8_t*>(q), a.s = s;
+  a.rows = rows, a.x_rs = x_row_stride, a.res_rs = residual_row_stride, a.sum_rs = sum_row_stride, a.s_sm = s_stride_m, a.s_sk = s_stride_k;
+  a.H = static_cast<int>(H), a.w_f32 = weight_dtype == kInF32, a.eps = eps, a.qeps = quant_eps;
+  return launch_norm<true>(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t dlb_rms_norm_backward_workspace_bytes(int64_t rows, int64_t H) {
+  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::norm_grad_blocks(rows)) * H * sizeof(float) : 0;
+}
+
+int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
+                          int64_t h_row_stride, int dtype, const void* weight, int weight_dtype, void* dx, int64_t dx_row_stride,
+                          void* dw, int64_t rows, int64_t H, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (int rc = check_norm(h, dsum, dtype, weight, weight_dtype, dsum, rows, H)) return rc;
+  if (H == 0 || (rows == 0 && !dw)) return DLB_OK;
+  if (dw && off_elements(dw, weight_dtype)) return fail(DLB_ERR_ALIGNMENT, "dw is not aligned to its elements");
+  if (rows > 0) {
+    if (!dy || !dx) return fail(DLB_ERR_NULL_POINTER, "dy or dx is NULL");
+    if (off_elements(dy, dtype) || off_elements(dx, dtype)) return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
+    if (dx_row_stride < H) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of dx is smaller than H=%lld", (long long)dx_row_stride, (long long)H);
+    if (dy_row_stride < 0 || dsum_row_stride < 0 || h_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+    const size_t need = dlb_rms_norm_backward_workspace_bytes(rows, H);
+    if (dw && (!workspace || workspace_bytes < need))
+      return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (dw && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int blocks = norm_grad_blocks(rows);
+  if (rows > 0) {
+    NormGradArgs a{};
+    a.dy = dy, a.dsum = dsum, a.h = h, a.w = weight, a.dx = dx, a.dw_part = dw ? static_cast<float*>(workspace) : nullptr;
+    a.rows = rows, a.dy_rs = dy_row_stride, a.dsum_rs = dsum_row_stride, a.h_rs = h_row_stride, a.dx_rs = dx_row_stride;
+    a.H = static_cast<int>(H), a.w_f32 = weight_dtype == kInF32, a.eps = eps;
+    const RowShape shape = row_shape(H, 1);
+    const dim3 grid(blocks), block(shape.threads);
+    with_type(dtype, [&](auto t) {
+      with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_backward_kernel<t(), c()>), grid, block, 0, st, a); });
+    });
+    if (int rc = finish("rms_norm_backward")) return rc;
+  }
+  if (!dw) return DLB_OK;
+  const NormDwArgs d{static_cast<const float*>(workspace), dw, blocks, static_cast<int>(H), weight_dtype};
+  hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(H, 64))), dim3(256), 0, st, d);
+  return finish("rms_norm_backward (dw)");
+}
+
+size_t dlb_moe_sort_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts) {
+  if (tokens <= 0 || topk <= 0 || experts <= 0) return 0;
+  const int64_t blocks = dlb::sort_blocks(tokens * topk);
+  return blocks > 1 ? static_cast<size_t>(blocks) * experts * sizeof(int32_t) : 0;
+}
+
+int dlb_moe_sort(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, int32_t* row_index, int32_t* source,
+                 int32_t* m_indices, int32_t* row_start, int32_t* row_end, int64_t tokens, int64_t topk, int64_t experts,
+                 int64_t alignment, int64_t num_rows, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (ids_dtype != DLB_IDX_I32 && ids_dtype != DLB_IDX_I64) return fail(DLB_ERR_BAD_DTYPE, "ids_dtype %d is not DLB_IDX_I32 / I64", ids_dtype);
+  if (int rc = check_rows(tokens, 0, topk, num_rows)) return rc;
+  if (experts < 1 || experts > kSortMaxExperts) return fail(DLB_ERR_BAD_SHAPE, "experts=%lld is not 1 ... %d", (long long)experts, kSortMaxExperts);
+  if (alignment < 1 || alignment > (1 << 20)) return fail(DLB_ERR_BAD_SHAPE, "alignment=%lld is not 1 ... 2^20", (long long)alignment);
+  if (ids_stride_m < 0 || ids_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride of ids");
+  if ((tokens > 0 && (!ids || !row_index)) || (num_rows > 0 && (!source || !m_indices)) || !row_start || !row_end)
+    return fail(DLB_ERR_NULL_POINTER, "ids or a table is NULL");
+  if (misaligned(ids, ids_dtype == DLB_IDX_I64 ? 8 : 4) || misaligned(row_index, 4) || misaligned(source, 4) || misaligned(m_indices, 4) ||
+      misaligned(row_start, 4) || misaligned(row_end, 4))
+    return fail(DLB_ERR_ALIGNMENT, "ids or a table is not aligned to its elements");
+  const size_t need = dlb_moe_sort_workspace_bytes(tokens, topk, experts);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+  if (need > 0 && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  SortArgs a{};
+  a.ids = ids, a.row_index = row_index, a.source = source, a.m_indices = m_indices, a.row_start = row_start, a.row_end = row_end;
+  a.hist = static_cast<int32_t*>(workspace);
+  a.ids_s0 = ids_stride_m, a.ids_s1 = ids_stride_k, a.n = tokens * topk, a.R = num_rows;
+  a.ids_is64 = ids_dtype == DLB_IDX_I64, a.E = static_cast<int>(experts), a.topk = static_cast<int>(topk), a.align = static_cast<int>(alignment);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t blocks = sort_blocks(a.n);
+  if (blocks > 1) {
+    hipLaunchKernelGGL(moe_sort_count_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), static_cast<size_t>(a.E) * sizeof(int), st, a);
+    if (int rc = finish("moe_sort (count)")) return rc;
+  }
+  // further workgroups where the tables by row are longer than those by slot
+  int64_t grid = ceil_div(num_rows, 4 * kSortThreads);
+  if (grid > 256) grid = 256;
+  if (grid < blocks) grid = blocks;
+  const size_t lds = (static_cast<size_t>(3) * a.E + 1) * sizeof(int) + static_cast<size_t>(16) * a.E * sizeof(uint16_t);
+  hipLaunchKernelGGL(moe_sort_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(kSortThreads), lds, st, a, static_cast<int>(blocks));
+  return finish("moe_sort");
+}
+
+int dlb_moe_permute(const void* x, int64_t x_row_stride, int dtype, const float* x_s, int64_t xs_stride_m, int64_t xs_stride_k,
+                    void* rows, float* rows_s, const int32_t* row_index, const int32_t* source, int64_t tokens, int64_t H,
+                    int64_t topk, int64_t num_rows, void* stream) {
+  using namespace dlb;
+  clear_error();
+  const bool f8 = dtype == DLB_ROWS_E4M3;
+  if (!f8 && bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32 / DLB_ROWS_E4M3", dtype);
+  if (int rc = check_rows(tokens, H, topk, num_rows)) return rc;
+  if (f8 && H % kScaleBlock != 0) return fail(DLB_ERR_BAD_SHAPE, "H=%lld is not a multiple of 128", (long long)H);
+  if (num_rows == 0 || H == 0) return DLB_OK;
+  if (!rows || !source || (tokens > 0 && (!x || !row_index))) return fail(DLB_ERR_NULL_POINTER, "x, rows or a table is NULL");
+  if (f8 && (!rows_s || (tokens > 0 && !x_s))) return fail(DLB_ERR_NULL_POINTER, "e4m3 rows without their scales");
+  if (x_row_stride < 0 || xs_stride_m < 0 || xs_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride");
+  const int esz = f8 ? 1 : static_cast<int>(size_of(dtype));
+  if (f8 ? misaligned(x, 16) || misaligned(rows, 16) || x_row_stride % 16 != 0 || misaligned(x_s, 4) || misaligned(rows_s, 4)
+         : off_elements(x, dtype) || off_elements(rows, dtype))
+    return fail(DLB_ERR_ALIGNMENT, "x or rows is not aligned to its elements, or e4m3 rows not to 16 bytes");
+  SortCopyArgs a{};
+  a.x = static_cast<const char*>(x), a.rows = static_cast<char*>(rows), a.row_index = row_index, a.source = source;
+  if (f8) a.xs = x_s, a.rows_s = rows_s, a.xs_s0 = xs_stride_m, a.xs_s1 = xs_stride_k, a.groups = static_cast<int>(H / kScaleBlock);
+  a.x_stride = x_row_stride * esz, a.rows_stride = H * esz, a.T = tokens, a.R = num_rows;
+  a.row_bytes = static_cast<int>(H * esz), a.esz = esz, a.topk = static_cast<int>(topk);
+  constexpr int kWaves = kSortCopyThreads / 64;
+  a.token_blocks = static_cast<int>(ceil_div(tokens, kWaves) < 4096 ? ceil_div(tokens, kWaves) : 4096);
+  a.zero_blocks = static_cast<int>(ceil_div(num_rows, kWaves) < 1024 ? ceil_div(num_rows, kWaves) : 1024);
+  hipLaunchKernelGGL(moe_sort_copy_kernel, dim3(a.token_blocks + a.zero_blocks), dim3(kSortCopyThreads), 0, static_cast<hipStream_t>(stream), a);
+  return finish("moe_permute");
+}
+
+int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, const int32_t* row_index, const float* weights, void* out,
+                      int64_t out_row_stride, int64_t tokens, int64_t H, int64_t topk, int64_t num_rows, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (int rc = check_rows(tokens, H, topk, num_rows)) return rc;
+  if (tokens == 0 || H == 0) return DLB_OK;
+  if (!out || !row_index || (num_rows > 0 && !rows)) return fail(DLB_ERR_NULL_POINTER, "rows, row_index or out is NULL");
+  if (out_row_stride < H) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of out is smaller than H=%lld", (long long)out_row_stride, (long long)H);
+  if (rows_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  if (off_elements(rows, dtype) || off_elements(out, dtype) || misaligned(row_index, 4) || misaligned(weights, 4))
+    return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
+  int dev = 0;
+  const int cus = device_cu_count(&dev);
+  if (cus < 0) return fail(DLB_ERR_LAUNCH, "hipGetDevice failed");
+  const UnpermuteArgs a{rows, row_index, weights, out, rows_row_stride, out_row_stride, tokens, num_rows, static_cast<int>(H), static_cast<int>(topk)};
+  int64_t parts = ceil_div(H, 512);
+  if (parts > 64) parts = 64;
+  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(parts));
+  with_type(dtype, [&](auto t) { hipLaunchKernelGGL(moe_unpermute_kernel<t()>, grid, dim3(64), 0, static_cast<hipStream_t>(stream), a); });
+  return finish("moe_unpermute");
+}
+
+int dlb_moe_unpermute_backward(const void* dout, int64_t dout_row_stride, const void* rows, int64_t rows_row_stride, int dtype,
+                               const int32_t* row_index, const int32_t* source, const float* weights, void* drows,
+                               int64_t drows_row_stride, float* dweights, int64_t tokens, int64_t H, int64_t topk, int64_t num_rows,
+                               void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (int rc = check_rows(tokens, H, topk, num_rows)) return rc;
+  if (H < 1 || H > DLB_NORM_MAX_COLUMNS) return fail(DLB_ERR_BAD_SHAPE, "H=%lld is not 1 ... %d", (long long)H, DLB_NORM_MAX_COLUMNS);
+  if (tokens == 0 && num_rows == 0) return DLB_OK;
+  if ((tokens > 0 && (!dout || !row_index)) || (num_rows > 0 && (!drows || !source || (dweights && !rows))))
+    return fail(DLB_ERR_NULL_POINTER, "a tensor pointer is NULL");
+  if (drows_row_stride < H) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of drows is smaller than H=%lld", (long long)drows_row_stride, (long long)H);
+  if (dout_row_stride < 0 || rows_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  if (off_elements(dout, dtype) || off_elements(rows, dtype) || off_elements(drows, dtype) || misaligned(row_index, 4) || misaligned(source, 4) ||
+      misaligned(weights, 4) || misaligned(dweights, 4))
+    return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
+  UnpermuteGradArgs a{};
+  a.dout = dout, a.rows = rows, a.row_index = row_index, a.source = source, a.w = weights, a.drows = drows, a.dw = dweights;
+  a.dout_rs = dout_row_stride, a.rows_rs = rows_row_stride, a.drows_rs = drows_row_stride;
+  a.T = tokens, a.R = num_rows, a.H = static_cast<int>(H), a.topk = static_cast<int>(topk);
+  a.zero_blocks = static_cast<int>(num_rows < 1024 ? num_rows : 1024);
+  const RowShape shape = row_shape(H, 1);
+  const int64_t grid = tokens + a.zero_blocks;
+  if (grid > (1ll << 31) - 1) return fail(DLB_ERR_BAD_SHAPE, "tokens=%lld beyond the supported range", (long long)tokens);
+  with_type(dtype, [&](auto t) {
+    with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
+      hipLaunchKernelGGL((moe_unpermute_backward_kernel<t(), c()>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads), 0,
+                         static_cast<hipStream_t>(stream), a);
+    });
+  });
+  return finish("moe_unpermute_backward");
+}
+
+int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, int s_dtype, const void* z, void* y,
+                int64_t y_row_stride, const int32_t* row_start, const int32_t* row_end, int64_t rows, int64_t N, int64_t K,
+                int64_t group, int64_t experts, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16", dtype);
+  if (bad_dtype(s_dtype)) return fail(DLB_ERR_BAD_DTYPE, "s_dtype %d is not DLB_IN_BF16 / F16 / F32", s_dtype);
+  if (rows < 0 || N < 0 || K < 0 || experts < 0)
+    return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld N=%lld K=%lld experts=%lld)", (long long)rows, (long long)N, (long long)K, (long long)experts);
+  if (group != 32 && group != 64 && group != 128) return fail(DLB_ERR_BAD_SHAPE, "group=%lld is not 32, 64 or 128", (long long)group);
+  if (K % group != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of the group size %lld", (long long)K, (long long)group);
+  if (!row_start != !row_end) return fail(DLB_ERR_NULL_POINTER, "row_start and row_end come together");
+  if (!row_start && experts != 1) return fail(DLB_ERR_BAD_SHAPE, "%lld experts without row ranges", (long long)experts);
+  if (rows > (1ll << 31) - 1 || N > (1ll << 30) || K > (1ll << 28) || experts > (1 << 20))
+    return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / N=%lld / K=%lld / experts=%lld beyond the supported range", (long long)rows, (long long)N, (long long)K,
+                (long long)experts);
+  if (rows == 0 || N == 0 || experts == 0) return DLB_OK;
+  if (K == 0) return fail(DLB_ERR_BAD_SHAPE, "K=0: there is no product");
+  if (!x || !q || !s || !y) return fail(DLB_ERR_NULL_POINTER, "x, q, s or y is NULL");
+  if (x_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  if (y_row_stride < N) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of y is smaller than N=%lld", (long long)y_row_stride, (long long)N);
+  if (misaligned(q, 16) || off_elements(x, dtype) || off_elements(y, dtype) || off_elements(s, s_dtype) || misaligned(row_start, 4) || misaligned(row_end, 4))
+    return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte aligned, the others to their elements");
+  W4Args a{};
+  a.x = x, a.q = static_cast<const uint8_t*>(q), a.s = s, a.z = static_cast<const uint8_t*>(z), a.y = y, a.row_start = row_start, a.row_end = row_end;
+  a.x_rs = x_row_stride, a.y_rs = y_row_stride, a.rows = rows;
+  a.N = static_cast<int>(N), a.K = static_cast<int>(K), a.G = static_cast<int>(K / group), a.E = static_cast<int>(experts), a.s_type = s_dtype;
+  a.q_es = N * (K / 2), a.s_es = N * a.G;
+  const int64_t busy = experts < rows ? experts : rows;  // experts that can have a row
+  const W4Shape shape = w4_shape(row_start ? ceil_div(rows, busy) : rows, N, K);
+  const int64_t y_blocks = row_start ? busy : ceil_div(rows, 16 * shape.mt);
+  if (y_blocks > 65535) return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / experts=%lld beyond the supported range", (long long)rows, (long long)experts);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const auto launch = [&](auto t) {
+    if (group == 128)
+      launch_w4<t(), 4>(a, shape, y_blocks, st);
+    else if (group == 64)
+      launch_w4<t(), 2>(a, shape, y_blocks, st);
+    else
+      launch_w4<t(), 1>(a, shape, y_blocks, st);
+  };
+  if (dtype == kInBf16)
+    launch(std::integral_constant<int, kInBf16>());
+  else
+    launch(std::integral_constant<int, kInF16>());
+  return finish("w4_gemm");
+}
+
+int dlb_w4_quant(const void* w, int64_t w_row_stride, int dtype, void* q, void* s, void* z, int64_t rows, int64_t K, int64_t group,
+                 void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (rows < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld K=%lld)", (long long)rows, (long long)K);
+  if (group != 32 && group != 64 && group != 128) return fail(DLB_ERR_BAD_SHAPE, "group=%lld is not 32, 64 or 128", (long long)group);
+  if (K % group != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of the group size %lld", (long long)K, (long long)group);
+  if (K > (1ll << 28)) return fail(DLB_ERR_BAD_SHAPE, "K=%lld beyond the supported range", (long long)K);
+  if (rows == 0 || K == 0) return DLB_OK;
+  if (!w || !q || !s) return fail(DLB_ERR_NULL_POINTER, "w, q or s is NULL");
+  if (w_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  if (off_elements(w, dtype) || off_elements(s, dtype) || misaligned(q, 4)) return fail(DLB_ERR_ALIGNMENT, "w and s must be aligned to their elements, q to 4 bytes");
+  const W4QuantArgs a{w, static_cast<uint8_t*>(q), s, static_cast<uint8_t*>(z), rows, w_row_stride, static_cast<int>(K / group), static_cast<int>(group)};
+  const int64_t blocks = ceil_div(rows * a.G * (group / 8), 256);
+  const dim3 grid(static_cast<unsigned>(blocks < 8192 ? blocks : 8192));
+  with_type(dtype, [&](auto t) { hipLaunchKernelGGL(w4_quant_kernel<t()>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a); });
+  return finish("w4_quant");
+}
+
+}  // extern "C"

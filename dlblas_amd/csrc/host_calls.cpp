@@ -7,34 +7,9 @@
 // having enqueued anything.  None means "not a plain call": tensor subclasses, dispatch and function modes, tracing, inputs
 // that require grad or carry a tangent, arguments the checks refuse, layouts only the Python path handles.  The Python function then goes on as
 // it would without this module, through its custom op and its own checks and messages.
-#include <Python.h>
-
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/core/Tensor.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/record_function.h>
-#include <c10/core/DefaultDtype.h>
-#include <c10/core/GradMode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <algorithm>
-#include <cstdint>
-#include <cstring>
-#include <string>
-#include <unordered_map>
-#include <utility>
-#include <vector>
-
-#include "../../include/dlblas_fp8_gemm.h"
-#include "../../include/dlblas_fp8_moe.h"
+#include "host_tensors.h"
 
 namespace {
-
-constexpr int64_t kBlock = 128;
 
 // The entry points of the library that ctypes has loaded, by address (init() below): one library, whichever was chosen.
 struct Abi {
@@ -57,46 +32,6 @@ struct Abi {
   decltype(&dlb_ep_gather) gather;
 } abi;
 PyObject* g_make_workspace = nullptr;  // _lib.workspace: creates and keeps the buffer of a (device, stream)
-
-// ---- what a plain call is ---------------------------------------------------------------------------------------------
-
-const c10::DispatchKeySet kPlainKeys({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
-const c10::DispatchKeySet kPlainIncluded({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
-
-// (raw bits: set difference on DispatchKeySet leaves the backend bits alone)
-bool within(c10::DispatchKeySet keys, c10::DispatchKeySet allowed) { return (keys.raw_repr() & ~allowed.raw_repr()) == 0; }
-
-bool no_modes() { return within(c10::impl::tls_local_dispatch_key_set().included_, kPlainIncluded) && !at::impl::torch_function_mode_enabled(); }
-
-// A dense GPU tensor that nothing but its own storage stands behind; nullptr otherwise.
-const at::Tensor* plain(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || !t.is_cuda() || !within(t.key_set(), kPlainKeys)) return nullptr;
-  if (t.is_conj() || t.is_neg() || (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()) return nullptr;
-  return &t;
-}
-
-template <size_t N>
-bool all_plain(PyObject* const* args, const at::Tensor* (&out)[N]) {
-  if (!no_modes()) return false;
-  for (size_t i = 0; i < N; ++i) {
-    out[i] = plain(args[i]);
-    if (!out[i] || out[i]->get_device() != out[0]->get_device()) return false;
-  }
-  return true;
-}
-
-// Makes the tensors' device current for the scope (a no-op in the usual case).
-struct DeviceScope {
-  c10::DeviceIndex before, dev;
-  explicit DeviceScope(const at::Tensor& t) : before(c10::hip::current_device()), dev(t.get_device()) {
-    if (dev != before) c10::hip::set_device(dev);
-  }
-  ~DeviceScope() {
-    if (dev != before) c10::hip::set_device(before);
-  }
-};
 
 struct Workspace {
   void* ptr;
@@ -128,57 +63,6 @@ bool workspace_of(c10::DeviceIndex dev, hipStream_t stream, const at::Tensor& li
   return true;
 }
 
-hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-
-at::Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
-  return at::Tensor(at::detail::empty_cuda(size, dtype, like.device(), std::nullopt));
-}
-at::Tensor empty_strided(at::IntArrayRef size, at::IntArrayRef stride, at::ScalarType dtype, const at::Tensor& like) {
-  return at::Tensor(at::detail::empty_strided_cuda(size, stride, dtype, like.device()));
-}
-
-// A custom op that mutates an argument moves its version counter on.
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-void* ptr(const at::Tensor& t) { return t.numel() > 0 ? t.data_ptr() : nullptr; }
-float* fptr(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
-int32_t* iptr(const at::Tensor& t) { return static_cast<int32_t*>(ptr(t)); }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-bool is_f8(const at::Tensor& t) { return t.scalar_type() == at::kFloat8_e4m3fn; }
-bool is_f32(const at::Tensor& t) { return t.scalar_type() == at::kFloat; }
-int out_code(at::ScalarType t) { return t == at::kBFloat16 ? DLB_OUT_BF16 : t == at::kFloat ? DLB_OUT_F32 : -1; }
-int in_code(at::ScalarType t) { return t == at::kBFloat16 ? DLB_IN_BF16 : t == at::kHalf ? DLB_IN_F16 : t == at::kFloat ? DLB_IN_F32 : -1; }
-int idx_code(at::ScalarType t) { return t == at::kInt ? DLB_IDX_I32 : t == at::kLong ? DLB_IDX_I64 : -1; }
-
-// An op event of torch's profiler, as the custom ops of the Python path leave one; nothing when nobody records.
-struct OpRecord {
-  at::RecordFunction guard{at::RecordScope::FUNCTION};
-  std::vector<c10::IValue> inputs;
-  template <size_t N>
-  OpRecord(const char* name, const at::Tensor* const (&t)[N]) {
-    if (!guard.isActive()) return;
-    if (guard.needsInputs())
-      for (const at::Tensor* x : t) inputs.emplace_back(*x);
-    guard.before(name, c10::ArrayRef<const c10::IValue>(inputs.data(), inputs.size()));
-  }
-};
-
-// Allocations and launches run without the GIL: a launch waits while the hardware queue is full.  No Python object is touched
-// in such a scope.
-class NoGil {
- public:
-  NoGil() : state_(PyEval_SaveThread()) {}
-  ~NoGil() { PyEval_RestoreThread(state_); }
-  NoGil(const NoGil&) = delete;
-  NoGil& operator=(const NoGil&) = delete;
-
- private:
-  PyThreadState* state_;
-};
-
 // Keeps the launches of several library calls on one workspace together.  Inside a NoGil scope only: a thread that waits for
 // the lock must not keep its holder from finishing.
 class Together {
@@ -196,18 +80,6 @@ class Together {
 PyObject* launch_failed(int rc) {
   return PyErr_Format(PyExc_RuntimeError, "dlblas fp8_gemm error %d: %s", rc, abi.last_error());
 }
-
-#define NOT_PLAIN Py_RETURN_NONE
-#define HANDLE_EXCEPTIONS_BEGIN try {
-#define HANDLE_EXCEPTIONS_END                          \
-  }                                                    \
-  catch (const c10::OutOfMemoryError& e) {             \
-    NOT_PLAIN; /* the Python path raises torch's own */ \
-  }                                                    \
-  catch (const std::exception& e) {                    \
-    PyErr_SetString(PyExc_RuntimeError, e.what());     \
-    return nullptr;                                    \
-  }
 
 // ---- dense ------------------------------------------------------------------------------------------------------------
 
@@ -596,4 +468,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddFunctions(m, host_step_methods) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -1,0 +1,368 @@
+// Tokens sorted by expert and back, with their gradients, for gfx950.
+//
+//   slots      (t, j) with 0 <= ids[t, j] < E, ordered by (expert, t, j): a stable counting sort, the same in every run
+//   spans      expert e owns rows [start_e, end_e), start_e = sum over the experts before of their counts rounded up to `align`;
+//              what would lie at or past the last reserved row is dropped
+//   permute    rows[row_index[t, j]] = x[t], all other rows zero
+//   unpermute  out[t] = sum_j w[t, j] rows[row_index[t, j]] over the slots with a row, an fp32 FMA chain in slot order
+//   gradients  of permute: unpermute without weights.  Of unpermute: drows[row] = w dout[t] (zero in rows without a slot),
+//              dw[t, j] = sum over the columns of rows[row] dout[t]
+//
+// ep_scatter and ep_gather (moe_permute.h) are the forms for spans that a dispatcher has already sized on the host; here the
+// counts are found on the device and the rows carry gradients.  Copies and sums are bound by memory: a token's chunk is held in
+// registers while all of its rows are written or read, so either side is touched once.
+#pragma once
+
+#include "fp8_gemm_common.h"
+#include "rms_norm.h"
+
+namespace dlb {
+
+constexpr int kSortMaxTopk = 64;
+constexpr int kSortThreads = 1024;
+constexpr int kSortBlockSlots = 1024;     // slots whose rows one workgroup of the table kernel finds
+constexpr int kSortMaxExperts = 1024;  // tables of the workgroups in 64 KB of LDS
+
+struct SortArgs {
+  const void* ids;      // [T][topk], < 0 or >= E: no expert
+  int32_t* row_index;   // [T * topk]: row of every slot, -1: none
+  int32_t* source;      // [R]: slot of every row, -1: none
+  int32_t* m_indices;   // [R]: expert of every row of a span, -1 past the last span
+  int32_t* row_start;   // [E]
+  int32_t* row_end;     // [E]: one past the last row with a slot
+  int32_t* hist;        // [blocks][E], used by launches of more than one workgroup of slots
+  int64_t ids_s0, ids_s1;
+  int64_t n;            // T * topk
+  int64_t R;
+  int ids_is64, E, topk, align;
+};
+
+__device__ __forceinline__ int sort_id(const SortArgs& p, int64_t i) {
+  if (i >= p.n) return -1;
+  const int64_t t = p.n < (1ll << 31) ? static_cast<uint32_t>(i) / static_cast<uint32_t>(p.topk) : i / p.topk;
+  const int64_t at = t * p.ids_s0 + (i - t * p.topk) * p.ids_s1;
+  const int64_t id = p.ids_is64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p.ids)[at]);
+  return (id < 0 || id >= p.E) ? -1 : static_cast<int>(id);
+}
+
+__global__ void __launch_bounds__(kSortThreads) moe_sort_count_kernel(const SortArgs p) {
+  extern __shared__ int hist[];
+  for (int e = threadIdx.x; e < p.E; e += kSortThreads) hist[e] = 0;
+  __syncthreads();
+  const int id = sort_id(p, static_cast<int64_t>(blockIdx.x) * kSortBlockSlots + threadIdx.x);
+  if (id >= 0) atomicAdd(&hist[id], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += kSortThreads) p.hist[static_cast<int64_t>(blockIdx.x) * p.E + e] = hist[e];
+}
+
+// Rows of the slots of workgroup blockIdx, and its share of the tables by row.  Workgroups past the slots' share only the latter.
+// LDS: before [E], total [E], start [E + 1], wave_cnt [16][E] of 16-bit counts.
+__global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortArgs p, int slot_blocks) {
+  extern __shared__ int lds[];
+  const int E = p.E;
+  int* before = lds;           // slots of the expert in the workgroups before, then the expert's next row in this one
+  int* total = before + E;     // slots of the expert
+  int* start = total + E;      // [E + 1] first row of every span
+  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(start + E + 1);  // [16][E]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x;
+  for (int i = tid; i < 2 * E; i += kSortThreads) lds[i] = 0;
+  for (int i = tid; i < 16 * E; i += kSortThreads) wave_cnt[i] = 0;
+  __syncthreads();
+  const int64_t slot = static_cast<int64_t>(b) * kSortBlockSlots + tid;
+  const int id = b < slot_blocks ? sort_id(p, slot) : -1;
+  if (slot_blocks == 1) {
+    // one workgroup of slots: every workgroup counts them itself
+    const int mine = b == 0 ? id : sort_id(p, tid);
+    if (mine >= 0) atomicAdd(&total[mine], 1);
+  } else {
+    const int cols = min(E, kSortThreads), P = kSortThreads / cols;
+    const int my_part = tid / cols, my_col = tid % cols;
+    for (int e = my_col; e < E && my_part < P; e += cols) {
+      int all = 0, early = 0;
+      for (int r = my_part; r < slot_blocks; r += P) {
+        const int c = p.hist[static_cast<int64_t>(r) * E + e];
+        all += c;
+        if (r < b) early += c;
+      }
+      if (all) atomicAdd(&total[e], all);
+      if (early) atomicAdd(&before[e], early);
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int64_t carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      const int e = e0 + lane;
+      const int64_t c = e < E ? (static_cast<int64_t>(total[e]) + p.align - 1) / p.align * p.align : 0;
+      int64_t incl = c;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int64_t up = __shfl_up(incl, off);
+        if (lane >= off) incl += up;
+      }
+      if (e < E) start[e] = static_cast<int>(min(carry + incl - c, p.R));
+      carry += __shfl(incl, 63);
+    }
+    if (lane == 0) start[E] = static_cast<int>(min(carry, p.R));
+  }
+  // slots with the same expert: in the waves before (wave_cnt) and in the lanes before (one ballot per bit of the id)
+  uint64_t same = ~0ull;
+  if (b < slot_blocks) {
+    const uint64_t live = __ballot(id >= 0);
+    same = live;
+    for (int bit = 0; (E - 1) >> bit; ++bit) {
+      const uint64_t ones = __ballot((id >> bit) & 1);
+      same &= ((id >> bit) & 1) ? ones : ~ones;
+    }
+    if (id >= 0 && (same >> lane) == 1) wave_cnt[wave * E + id] = static_cast<uint16_t>(__popcll(same));
+  }
+  __syncthreads();
+  if (b < slot_blocks && slot < p.n) {
+    int64_t row = -1;
+    if (id >= 0) {
+      row = static_cast<int64_t>(start[id]) + before[id] + __popcll(same & ((1ull << lane) - 1));
+      for (int w = 0; w < wave; ++w) row += wave_cnt[w * E + id];
+      if (row >= p.R) row = -1;
+    }
+    p.row_index[slot] = static_cast<int32_t>(row);
+    if (row >= 0) p.source[row] = static_cast<int32_t>(slot);
+  }
+  if (b == 0)
+    for (int e = tid; e < E; e += kSortThreads) {
+      p.row_start[e] = start[e];
+      p.row_end[e] = static_cast<int>(min(static_cast<int64_t>(start[e]) + total[e], p.R));
+    }
+  for (int64_t r = static_cast<int64_t>(b) * kSortThreads + tid; r < p.R; r += static_cast<int64_t>(gridDim.x) * kSortThreads) {
+    int e = -1;
+    if (r < start[E]) {
+      int lo = 0, hi = E;  // the last e with start[e] <= r: an empty span before it starts at the same row
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= r)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      e = lo;
+    }
+    p.m_indices[r] = e;
+    if (e < 0 || r >= static_cast<int64_t>(start[e]) + total[e]) p.source[r] = -1;
+  }
+}
+
+// Rows moved as bytes in chunks of 16; the last chunk of a row may be short.
+__device__ __forceinline__ v4i load_bytes16(const char* p, int left, int esz) {
+  if (left >= 16) return *reinterpret_cast<const v4i_el*>(p);
+  v4i v{0, 0, 0, 0};
+  if (esz == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (2 * i < left) v[i / 2] |= static_cast<int>(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * i < left) v[i] = reinterpret_cast<const int*>(p)[i];
+  }
+  return v;
+}
+__device__ __forceinline__ void store_bytes16(char* p, const v4i& v, int left, int esz) {
+  if (left >= 16) {
+    *reinterpret_cast<v4i_el*>(p) = v;
+  } else if (esz == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (2 * i < left) reinterpret_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(static_cast<uint32_t>(v[i / 2]) >> (16 * (i & 1)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * i < left) reinterpret_cast<int*>(p)[i] = v[i];
+  }
+}
+
+struct SortCopyArgs {
+  const char* x;        // [T] rows of row_bytes
+  char* rows;           // [R]
+  const float* xs;      // scales of quantised tokens [T][groups] or NULL
+  float* rows_s;        // [R][groups]
+  const int32_t* row_index;
+  const int32_t* source;
+  int64_t x_stride, rows_stride;  // bytes
+  int64_t xs_s0, xs_s1;
+  int64_t T, R;
+  int row_bytes, esz, topk, groups;
+  int token_blocks, zero_blocks;
+};
+
+constexpr int kSortCopyThreads = 256;
+constexpr int kSortCopyChunks = 4;  // chunks of a row in flight per lane
+
+// One wave per token and stretch of its row: blocks [0, token_blocks) take the tokens, the others look for rows without a slot.
+__global__ void __launch_bounds__(kSortCopyThreads) moe_sort_copy_kernel(const SortCopyArgs p) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6, waves = kSortCopyThreads / 64;
+  constexpr int kSpan = kSortCopyChunks * 64 * 16;
+  if (static_cast<int>(blockIdx.x) < p.token_blocks) {
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * waves + wave; t < p.T; t += static_cast<int64_t>(p.token_blocks) * waves) {
+      const int32_t* index = p.row_index + t * p.topk;
+      const char* src = p.x + t * p.x_stride;
+      for (int c0 = 0; c0 < p.row_bytes; c0 += kSpan) {
+        v4i v[kSortCopyChunks];
+#pragma unroll
+        for (int u = 0; u < kSortCopyChunks; ++u) {
+          const int c = c0 + (u * 64 + lane) * 16;
+          if (c < p.row_bytes) v[u] = load_bytes16(src + c, p.row_bytes - c, p.esz);
+        }
+        for (int j = 0; j < p.topk; ++j) {
+          const int64_t row = index[j];
+          if (row < 0) continue;
+          char* dst = p.rows + row * p.rows_stride;
+#pragma unroll
+          for (int u = 0; u < kSortCopyChunks; ++u) {
+            const int c = c0 + (u * 64 + lane) * 16;
+            if (c < p.row_bytes) store_bytes16(dst + c, v[u], p.row_bytes - c, p.esz);
+          }
+        }
+      }
+      for (int g = lane; g < p.groups; g += 64) {
+        const float s = p.xs[t * p.xs_s0 + g * p.xs_s1];
+        for (int j = 0; j < p.topk; ++j) {
+          const int64_t row = index[j];
+          if (row >= 0) p.rows_s[row * p.groups + g] = s;
+        }
+      }
+    }
+    return;
+  }
+  const int64_t zb = static_cast<int64_t>(blockIdx.x) - p.token_blocks;
+  for (int64_t r = zb * waves + wave; r < p.R; r += static_cast<int64_t>(p.zero_blocks) * waves) {
+    if (p.source[r] >= 0) continue;
+    char* dst = p.rows + r * p.rows_stride;
+    for (int c = lane * 16; c < p.row_bytes; c += 64 * 16) store_bytes16(dst + c, v4i{0, 0, 0, 0}, p.row_bytes - c, p.esz);
+    for (int g = lane; g < p.groups; g += 64) p.rows_s[r * p.groups + g] = 0.f;
+  }
+}
+
+struct UnpermuteArgs {
+  const void* rows;         // [R][H]
+  const int32_t* row_index; // [T][topk]
+  const float* w;           // [T][topk] or NULL: all one
+  void* out;                // [T][H]
+  int64_t rows_rs, out_rs;  // elements
+  int64_t T, R;
+  int H, topk;
+};
+
+// One wave per token and stretch of 512 columns (one chunk a lane); the rows of two slots are on their way at a time.
+template <int T>
+__global__ void __launch_bounds__(64) moe_unpermute_kernel(const UnpermuteArgs p) {
+  const int lane = threadIdx.x;
+  const int64_t t = blockIdx.x;
+  const int32_t* index = p.row_index + t * p.topk;
+  const float* w = p.w ? p.w + t * p.topk : nullptr;
+  for (int64_t col = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * 8; col < p.H; col += static_cast<int64_t>(gridDim.y) * 512) {
+    const int left = static_cast<int>(p.H - col);
+    float acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+    for (int j0 = 0; j0 < p.topk; j0 += 4) {
+      Raw8 raw[4];
+      float wj[4];
+      bool on[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t row = j0 + u < p.topk ? index[j0 + u] : -1;
+        on[u] = row >= 0 && row < p.R;
+        if (!on[u]) continue;
+        raw[u] = load_raw8<T>(p.rows, row * p.rows_rs + col, left);
+        wj[u] = w ? w[j0 + u] : 1.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (!on[u]) continue;
+        float v[8];
+        quant_unpack8<T>(raw[u], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = fmaf(v[k], wj[u], acc[k]);
+      }
+    }
+    store_raw8<T>(p.out, t * p.out_rs + col, pack_raw8<T>(acc), left);
+  }
+}
+
+struct UnpermuteGradArgs {
+  const void* dout;         // [T][H]
+  const void* rows;         // [R][H], read for dw only
+  const int32_t* row_index;
+  const int32_t* source;    // [R]
+  const float* w;           // [T][topk] or NULL: all one
+  void* drows;              // [R][H]
+  float* dw;                // [T][topk] or NULL
+  int64_t dout_rs, rows_rs, drows_rs;
+  int64_t T, R;
+  int H, topk;
+  int zero_blocks;
+};
+
+// One workgroup per token, the chunks of its gradient in registers (CH a thread) while its rows pass; the workgroups behind the
+// tokens write the rows without a slot.  The waves' shares of a slot's product meet in LDS.
+template <int T, int CH>
+__global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel(const UnpermuteGradArgs p) {
+  __shared__ float part[kSortMaxTopk][kNormMaxWaves];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int chunks = (p.H + 7) / 8;
+  if (static_cast<int64_t>(blockIdx.x) >= p.T) {
+    Raw8 zero;
+    zero.a = v4i{0, 0, 0, 0}, zero.b = v4i{0, 0, 0, 0};
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) - p.T; r < p.R; r += p.zero_blocks) {
+      if (p.source[r] >= 0) continue;
+      for (int i = tid; i < chunks; i += threads) store_raw8<T>(p.drows, r * p.drows_rs + 8 * i, zero, p.H - 8 * i);
+    }
+    return;
+  }
+  const int64_t t = blockIdx.x;
+  const int32_t* index = p.row_index + t * p.topk;
+  const float* w = p.w ? p.w + t * p.topk : nullptr;
+  Raw8 g[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * threads + tid;
+    if (i < chunks) g[c] = load_raw8<T>(p.dout, t * p.dout_rs + 8 * i, p.H - 8 * i);
+  }
+  for (int j = 0; j < p.topk; ++j) {
+    const int64_t row = index[j];
+    float dot = 0.f;
+    if (row >= 0 && row < p.R) {
+      const float wj = w ? w[j] : 1.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int i = c * threads + tid;
+        if (i >= chunks) continue;
+        float d[8];
+        quant_unpack8<T>(g[c], d);
+        if (p.dw) {
+          float v[8];
+          quant_unpack8<T>(load_raw8<T>(p.rows, row * p.rows_rs + 8 * i, p.H - 8 * i), v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dot = fmaf(v[k], d[k], dot);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] *= wj;
+        store_raw8<T>(p.drows, row * p.drows_rs + 8 * i, pack_raw8<T>(d), p.H - 8 * i);
+      }
+    }
+    if (p.dw) {
+      dot = wave_sum(dot);
+      if ((tid & 63) == 0) part[j][tid >> 6] = dot;
+    }
+  }
+  if (!p.dw) return;
+  __syncthreads();
+  for (int j = tid; j < p.topk; j += threads) {
+    float s = 0.f;
+    for (int i = 0; i < threads / 64; ++i) s += part[j][i];
+    p.dw[t * p.topk + j] = s;
+  }
+}
+
+}  // namespace dlb

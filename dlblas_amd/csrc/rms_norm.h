@@ -1,0 +1,347 @@
+// Root-mean-square norm with the residual's addition, its gradient, and the form whose output is quantised 1 x 128, for gfx950.
+//
+//   h = x + res rounded to the rows' type (without a residual h = x),  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
+//   quantising:  s = max(max |y|, qeps) / 448 per 128 columns,  q = e4m3(clamp(y / s, +-448)); y itself is not rounded in between
+//   gradient:    dh = r (w dy) - h r^3 / H sum(w dy h) + dsum,   dw = sum over the rows of dy h r
+//
+// h is rounded before the norm reads it: it is what the next layer adds to and what the gradient starts from, so both see the same
+// rows.  Everything else is held in fp32 and rounded once at the store.
+//
+// All of it is bound by memory: a row is read once into registers (8 elements a chunk, CH chunks a thread), the sums cross the
+// workgroup once, and the results leave from the registers.  Chunks are consecutive over the lanes, so 16 lanes hold a group of
+// 128 columns and find its largest value among themselves.  Rows at any element boundary and widths that are no multiple of 8
+// take the same path: global memory serves a 16-byte access at its element's alignment, and the last chunk of a row may be short.
+#pragma once
+
+#include "fp8_gemm_common.h"
+#include "fp8_quant.h"
+
+namespace dlb {
+
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef v4h v4h_el __attribute__((aligned(2)));
+
+constexpr int kNormMaxThreads = 1024;
+constexpr int kNormMaxWaves = kNormMaxThreads / 64;
+
+// Eight consecutive elements as they lie in memory (16 bytes, 32 of fp32); `left` (at least 1) = elements left in the row, those
+// past it are zero.
+template <int T>
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t elem, int left) {
+  Raw8 r;
+  r.a = v4i{0, 0, 0, 0}, r.b = v4i{0, 0, 0, 0};
+  if (T == kInF32) {
+    typedef v4i v4i_f32 __attribute__((aligned(4)));
+    const float* q = static_cast<const float*>(p) + elem;
+    if (left >= 8) {
+      r.a = reinterpret_cast<const v4i_f32*>(q)[0], r.b = reinterpret_cast<const v4i_f32*>(q)[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < left) r.a[i] = __float_as_int(q[i]);
+        if (4 + i < left) r.b[i] = __float_as_int(q[4 + i]);
+      }
+    }
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(p) + elem;
+    if (left >= 8) {
+      r.a = *reinterpret_cast<const v4i_el*>(q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) r.a[i / 2] |= static_cast<int>(static_cast<uint32_t>(q[i]) << (16 * (i & 1)));
+    }
+  }
+  return r;
+}
+
+// Eight fp32 values rounded to nearest even into the type of the rows.
+template <int T>
+__device__ __forceinline__ Raw8 pack_raw8(const float (&v)[8]) {
+  Raw8 r;
+  if (T == kInF32) {
+    r.a = v4i{__float_as_int(v[0]), __float_as_int(v[1]), __float_as_int(v[2]), __float_as_int(v[3])};
+    r.b = v4i{__float_as_int(v[4]), __float_as_int(v[5]), __float_as_int(v[6]), __float_as_int(v[7])};
+  } else if (T == kInBf16) {
+    const v2i lo = __builtin_bit_cast(v2i, __builtin_convertvector(v4f{v[0], v[1], v[2], v[3]}, v4bf));
+    const v2i hi = __builtin_bit_cast(v2i, __builtin_convertvector(v4f{v[4], v[5], v[6], v[7]}, v4bf));
+    r.a = v4i{lo.x, lo.y, hi.x, hi.y};
+    r.b = r.a;
+  } else {
+    const v2i lo = __builtin_bit_cast(v2i, __builtin_convertvector(v4f{v[0], v[1], v[2], v[3]}, v4h));
+    const v2i hi = __builtin_bit_cast(v2i, __builtin_convertvector(v4f{v[4], v[5], v[6], v[7]}, v4h));
+    r.a = v4i{lo.x, lo.y, hi.x, hi.y};
+    r.b = r.a;
+  }
+  return r;
+}
+
+template <int T>
+__device__ __forceinline__ void store_raw8(void* p, int64_t elem, const Raw8& r, int left) {
+  if (T == kInF32) {
+    typedef v4i v4i_f32 __attribute__((aligned(4)));
+    float* q = static_cast<float*>(p) + elem;
+    if (left >= 8) {
+      reinterpret_cast<v4i_f32*>(q)[0] = r.a, reinterpret_cast<v4i_f32*>(q)[1] = r.b;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < left) q[i] = __int_as_float(r.a[i]);
+        if (4 + i < left) q[4 + i] = __int_as_float(r.b[i]);
+      }
+    }
+  } else {
+    uint16_t* q = static_cast<uint16_t*>(p) + elem;
+    if (left >= 8) {
+      *reinterpret_cast<v4i_el*>(q) = r.a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) q[i] = static_cast<uint16_t>(static_cast<uint32_t>(r.a[i / 2]) >> (16 * (i & 1)));
+    }
+  }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+struct NormArgs {
+  const void* x;
+  const void* res;  // or NULL
+  const void* w;    // [H], the rows' type or fp32
+  void* y;          // not written by the quantising form
+  void* sum;        // h, with a residual
+  uint8_t* q;       // quantising form: [rows][H]
+  float* s;
+  int64_t rows, x_rs, res_rs, y_rs, sum_rs, s_sm, s_sk;
+  int H;
+  int w_f32;
+  float eps, qeps;
+};
+
+template <int T>
+__device__ __forceinline__ void load_weight8(const void* w, int w_f32, int col, int left, float (&v)[8]) {
+  if (w_f32)
+    quant_unpack8<kInF32>(load_raw8<kInF32>(w, col, left), v);
+  else
+    quant_unpack8<T>(load_raw8<T>(w, col, left), v);
+}
+
+// One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each.
+template <int T, bool QUANT, int CH>
+__global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArgs p) {
+  __shared__ float part[kNormMaxWaves];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int64_t row = blockIdx.x;
+  const int chunks = (p.H + 7) / 8;
+  Raw8 h[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * threads + tid;
+    if (i < chunks) h[c] = load_raw8<T>(p.x, row * p.x_rs + 8 * i, p.H - 8 * i);
+  }
+  if (p.res) {
+    Raw8 res[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * threads + tid;
+      if (i < chunks) res[c] = load_raw8<T>(p.res, row * p.res_rs + 8 * i, p.H - 8 * i);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * threads + tid;
+      if (i >= chunks) continue;
+      float a[8], b[8];
+      quant_unpack8<T>(h[c], a);
+      quant_unpack8<T>(res[c], b);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] += b[k];
+      h[c] = pack_raw8<T>(a);
+      store_raw8<T>(p.sum, row * p.sum_rs + 8 * i, h[c], p.H - 8 * i);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    if (c * threads + tid >= chunks) continue;
+    float v[8];
+    quant_unpack8<T>(h[c], v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fmaf(v[k], v[k], ss);
+  }
+  ss = wave_sum(ss);
+  if (threads > 64) {
+    if ((tid & 63) == 0) part[tid >> 6] = ss;
+    __syncthreads();
+    ss = 0.f;
+    for (int i = 0; i < threads / 64; ++i) ss += part[i];
+  }
+  const float r = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * threads + tid;
+    if (i >= chunks) continue;  // whole groups of 16 lanes: a quantised row is a multiple of 128 wide
+    float v[8], w[8];
+    quant_unpack8<T>(h[c], v);
+    load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * r * w[k];
+    if (!QUANT) {
+      store_raw8<T>(p.y, row * p.y_rs + 8 * i, pack_raw8<T>(v), p.H - 8 * i);
+      continue;
+    }
+    // the largest value by the bits of |y|, which puts NaN above infinity: a group that holds one gets a scale that shows it
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
+    const float amax = __uint_as_float(top);
+    const float scale = (amax < p.qeps ? p.qeps : amax) / 448.0f;
+    const float inv_scale = 1.0f / scale;
+    int packed[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = div_by_scale(v[4 * k + j], scale, inv_scale);  // at most 448 and a rounding: no clamp
+      int word = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
+      packed[k] = __builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], word, true);
+    }
+    *reinterpret_cast<v2i*>(p.q + row * p.H + 8 * i) = v2i{packed[0], packed[1]};
+    if ((tid & 15) == 0) p.s[row * p.s_sm + (i >> 4) * p.s_sk] = scale;
+  }
+}
+
+struct NormGradArgs {
+  const void* dy;
+  const void* dsum;  // or NULL: gradient of h by its other use
+  const void* h;
+  const void* w;
+  void* dx;
+  float* dw_part;    // [gridDim.x][H] or NULL: sums over a workgroup's rows
+  int64_t rows, dy_rs, dsum_rs, h_rs, dx_rs;
+  int H;
+  int w_f32;
+  float eps;
+};
+
+// A workgroup takes rows blockIdx, blockIdx + gridDim, ... and keeps its share of dw in registers; the shares of all workgroups are
+// added by rms_norm_dw_kernel in workgroup order, so the gradient is the same in every run.
+template <int T, int CH>
+__global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(const NormGradArgs p) {
+  __shared__ float part[2][2][kNormMaxWaves];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int chunks = (p.H + 7) / 8;
+  float dw[CH][8];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dw[c][k] = 0.f;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    Raw8 dy[CH], h[CH], ds[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * threads + tid;
+      if (i >= chunks) continue;
+      h[c] = load_raw8<T>(p.h, row * p.h_rs + 8 * i, p.H - 8 * i);
+      dy[c] = load_raw8<T>(p.dy, row * p.dy_rs + 8 * i, p.H - 8 * i);
+      if (p.dsum) ds[c] = load_raw8<T>(p.dsum, row * p.dsum_rs + 8 * i, p.H - 8 * i);
+    }
+    float ss = 0.f, dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * threads + tid;
+      if (i >= chunks) continue;
+      float hv[8], g[8], w[8];
+      quant_unpack8<T>(h[c], hv);
+      quant_unpack8<T>(dy[c], g);
+      load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        ss = fmaf(hv[k], hv[k], ss);
+        dot = fmaf(g[k] * w[k], hv[k], dot);
+      }
+    }
+    ss = wave_sum(ss), dot = wave_sum(dot);
+    if (threads > 64) {
+      // two sets of sums in turn: a wave may be one row ahead of the others, never two
+      if ((tid & 63) == 0) part[turn][0][tid >> 6] = ss, part[turn][1][tid >> 6] = dot;
+      __syncthreads();
+      ss = dot = 0.f;
+      for (int i = 0; i < threads / 64; ++i) ss += part[turn][0][i], dot += part[turn][1][i];
+    }
+    const float r = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+    const float along = r * r * dot / static_cast<float>(p.H);  // dh = r (w dy - h along)
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * threads + tid;
+      if (i >= chunks) continue;
+      float hv[8], g[8], w[8];
+      quant_unpack8<T>(h[c], hv);
+      quant_unpack8<T>(dy[c], g);
+      load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        dw[c][k] = fmaf(g[k], hv[k] * r, dw[c][k]);
+        g[k] = r * (g[k] * w[k] - hv[k] * along);
+      }
+      if (p.dsum) {
+        float d[8];
+        quant_unpack8<T>(ds[c], d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[k] += d[k];
+      }
+      store_raw8<T>(p.dx, row * p.dx_rs + 8 * i, pack_raw8<T>(g), p.H - 8 * i);
+    }
+  }
+  if (!p.dw_part) return;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * threads + tid;
+    if (i < chunks) store_raw8<kInF32>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H + 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
+  }
+}
+
+// dw[col] = sum over the parts, in order within each of the four waves and then over the waves.
+struct NormDwArgs {
+  const float* part;
+  void* dw;
+  int parts, H, dw_type;
+};
+
+__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const NormDwArgs p) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (col < p.H) {
+    const int per = (p.parts + 3) / 4;
+    const int b1 = min(p.parts, (wave + 1) * per);
+    int b = wave * per;
+    for (; b + 8 <= b1; b += 8) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = p.part[static_cast<int64_t>(b + u) * p.H + col];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+    for (; b < b1; ++b) s += p.part[static_cast<int64_t>(b) * p.H + col];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || col >= p.H) return;
+  s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  if (p.dw_type == kInF32)
+    static_cast<float*>(p.dw)[col] = s;
+  else if (p.dw_type == kInBf16)
+    static_cast<__bf16*>(p.dw)[col] = static_cast<__bf16>(s);
+  else
+    static_cast<_Float16*>(p.dw)[col] = static_cast<_Float16>(s);
+}
+
+}  // namespace dlb

@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define DLB_ABI_VERSION 11
+#define DLB_ABI_VERSION 12
 
 /* output element type of C */
 #define DLB_OUT_BF16 0
