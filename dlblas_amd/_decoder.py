@@ -83,10 +83,13 @@ def moe_unpermute_backward(dout, rows, row_index, source, weights, drows, dweigh
 
 def w4_gemm(x, w_q, w_s, w_z, y, row_start, row_end, group):
     _require_gpu(*_present(x, w_q, w_s, w_z, y, row_start, row_end))
+    lib = load()
     E = w_q.size(0) if w_q.dim() == 3 else 1
     with torch.cuda.device(x.device):
-        check(load().dlb_w4_gemm(_ptr(x), _rs(x), IN_CODES[x.dtype], _ptr(w_q), _ptr(w_s), IN_CODES[w_s.dtype], _ptr(w_z), _ptr(y), _rs(y),
-                                 _ptr(row_start), _ptr(row_end), x.size(0), w_q.size(-2), x.size(1), group, E, _stream(x)))
+        need = lib.dlb_w4_gemm_workspace_bytes(x.size(0), w_q.size(-2), x.size(1), 0 if row_start is None else E)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        check(lib.dlb_w4_gemm(_ptr(x), _rs(x), IN_CODES[x.dtype], _ptr(w_q), _ptr(w_s), IN_CODES[w_s.dtype], _ptr(w_z), _ptr(y), _rs(y),
+                              _ptr(row_start), _ptr(row_end), x.size(0), w_q.size(-2), x.size(1), group, E, _ptr(ws), need, _stream(x)))
 
 
 def w4_quant(w, q, s, z, group):

@@ -103,7 +103,8 @@ DECODER_SYMBOLS = {
     'dlb_moe_unpermute_backward':
     (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 4 + [_c_i64, _c_vp] + [_c_i64] * 4 + [_c_vp]),
     'dlb_w4_gemm':
-    (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 5 + [_c_vp]),
+    (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 5 + [_c_vp, _c_sz, _c_vp]),
+    'dlb_w4_gemm_workspace_bytes': (_c_sz, [_c_i64] * 4),
     'dlb_w4_quant': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 3 + [_c_i64] * 3 + [_c_vp]),
 }
 

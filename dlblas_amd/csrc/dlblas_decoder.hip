@@ -95,27 +95,57 @@ int64_t sort_blocks(int64_t slots) { return slots > 0 ? ceil_div(slots, kSortBlo
 
 // ---- 4-bit weights ----------------------------------------------------------------------------------------------------
 
-struct W4Shape {
-  int mt, nt, waves;
+// What a product runs as: K split over the waves of a workgroup, or neighbouring tiles sharing x, in K slices of `chunks` chunks.
+struct W4Plan {
+  bool shared;
+  int mt, slices, chunks;
 };
-W4Shape w4_shape(int64_t rows_each, int64_t N, int64_t K) {
-  const int mt = rows_each <= 16 ? 1 : rows_each <= 32 ? 2 : 4;
-  const int nt = mt == 1 ? 1 : 2;
-  int64_t waves = ceil_div(K, 128);
-  if (waves > 8) waves = 8;
-  return {mt, nt, static_cast<int>(waves)};
+constexpr int kW4Cus = 256;
+
+int w4_columns(int mt) { return mt == 1 ? 64 : 128; }                       // of a workgroup that shares x
+int w4_chunk(int mt) { return mt == 1 ? 2 * kW4Unit : kW4Unit; }           // columns of x
+
+// rows_each: of one matrix.  Up to 8 MB of weights the workgroups that share x are too few to fill the chip, or pay a second launch
+// for their slices (1 x 2112 x 7168 7.6 against 8.1 us, 1 x 512 x 2048 4.3 / 5.6; 16 x 4096 x 7168, 15 MB, 12.0 / 10.6, 1 x 7168 x 18432
+// 28 / 21, 16 x 7168 x 18432 51 / 26.5, 32 experts x 4 rows x 4096 x 7168 197 / 102).  Above 16 rows tiles of 32 x 32 (32 x 7168 x 7168
+// 20.3 -> 17.9 us, 32 experts x 16 rows x 7168 x 2048 87 -> 66); above 8 rows per expert too, because experts have more than the mean.
+W4Plan w4_plan(int64_t rows_each, bool by_expert, int64_t matrices, int64_t N, int64_t K) {
+  const int mt = rows_each <= (by_expert ? 8 : 16) ? 1 : 2;
+  if (mt == 1 && matrices * N * (K / 2) <= (8 << 20)) return {false, 1, 1, 0};
+  const int chunks = static_cast<int>(ceil_div(K, w4_chunk(mt)));
+  W4Plan best{true, mt, 1, chunks};
+  if (by_expert) return best;
+  // time in chunks of one workgroup: rounds over the chip x chunks, which go in pairs, the second launch and the sums' way through memory
+  const int64_t base = ceil_div(N, w4_columns(mt)) * ceil_div(rows_each, 16 * mt);
+  double best_cost = 1e30;
+  for (int slices = 1; slices <= 16 && slices <= chunks; ++slices) {
+    const int each = static_cast<int>(ceil_div(chunks, slices));
+    if (ceil_div(chunks, each) != slices) continue;
+    const double cost = static_cast<double>(ceil_div(base * slices, kW4Cus)) * ((each + 1) / 2 * 2) + (slices > 1 ? 3 + 0.5 * slices : 0);
+    if (cost < best_cost) best_cost = cost, best.slices = slices, best.chunks = each;
+  }
+  return best;
 }
 
-template <int T, int STEPS>
-void launch_w4(const W4Args& a, const W4Shape& s, int64_t y_blocks, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * s.nt)), static_cast<unsigned>(y_blocks)), block(64 * s.waves);
-  const size_t lds = static_cast<size_t>(s.waves) * s.mt * s.nt * 1024;
-  if (s.mt == 1)
-    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 1, 1>), grid, block, lds, st, a);
-  else if (s.mt == 2)
-    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 2, 2>), grid, block, lds, st, a);
+template <int T, int GROUPS, bool ZEROS>
+void launch_w4(const W4Args& a, const W4Plan& plan, int64_t y_blocks, float* sums, hipStream_t st) {
+  if (!plan.shared) {
+    const int waves = 4;
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16)), static_cast<unsigned>(y_blocks));
+    hipLaunchKernelGGL((w4_gemm_kernel<T, GROUPS, ZEROS, 1, 1, 4>), grid, dim3(64 * waves), waves * 1024, st, a);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, w4_columns(plan.mt))), static_cast<unsigned>(y_blocks), static_cast<unsigned>(plan.slices));
+  const dim3 block(64 * kW4Waves);
+  float* const to = plan.slices > 1 ? sums : nullptr;
+  if (plan.mt == 2)
+    hipLaunchKernelGGL((w4_gemm_shared_kernel<T, GROUPS, ZEROS, 2, 2, 1, 4>), grid, block, 0, st, a, to, plan.chunks);
+  else if (!a.row_start && a.rows <= 4)
+    hipLaunchKernelGGL((w4_gemm_shared_kernel<T, GROUPS, ZEROS, 1, 1, 2, 1>), grid, block, 0, st, a, to, plan.chunks);
   else
-    hipLaunchKernelGGL((w4_gemm_kernel<T, STEPS, 4, 2>), grid, block, lds, st, a);
+    hipLaunchKernelGGL((w4_gemm_shared_kernel<T, GROUPS, ZEROS, 1, 1, 2, 4>), grid, block, 0, st, a, to, plan.chunks);
+  if (plan.slices > 1)
+    hipLaunchKernelGGL(w4_sum_kernel<T>, dim3(static_cast<unsigned>(ceil_div(a.rows * a.N, 256))), dim3(256), 0, st, sums, a.y, a.y_rs, a.rows, a.N, plan.slices);
 }
 
 }  // namespace
@@ -334,20 +364,26 @@ int dlb_moe_unpermute_backward(const void* dout, int64_t dout_row_stride, const 
   return finish("moe_unpermute_backward");
 }
 
+size_t dlb_w4_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t experts) {
+  if (experts != 0 || rows <= 0 || N <= 0 || K <= 0) return 0;
+  const dlb::W4Plan plan = dlb::w4_plan(rows, false, 1, N, K);
+  return plan.slices > 1 ? static_cast<size_t>(plan.slices) * rows * N * sizeof(float) : 0;
+}
+
 int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, int s_dtype, const void* z, void* y,
                 int64_t y_row_stride, const int32_t* row_start, const int32_t* row_end, int64_t rows, int64_t N, int64_t K,
-                int64_t group, int64_t experts, void* stream) {
+                int64_t group, int64_t experts, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace dlb;
   clear_error();
   if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16", dtype);
-  if (bad_dtype(s_dtype)) return fail(DLB_ERR_BAD_DTYPE, "s_dtype %d is not DLB_IN_BF16 / F16 / F32", s_dtype);
+  if (s_dtype != kInBf16 && s_dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "s_dtype %d is not DLB_IN_BF16 / F16", s_dtype);
   if (rows < 0 || N < 0 || K < 0 || experts < 0)
     return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld N=%lld K=%lld experts=%lld)", (long long)rows, (long long)N, (long long)K, (long long)experts);
   if (group != 32 && group != 64 && group != 128) return fail(DLB_ERR_BAD_SHAPE, "group=%lld is not 32, 64 or 128", (long long)group);
   if (K % group != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of the group size %lld", (long long)K, (long long)group);
   if (!row_start != !row_end) return fail(DLB_ERR_NULL_POINTER, "row_start and row_end come together");
   if (!row_start && experts != 1) return fail(DLB_ERR_BAD_SHAPE, "%lld experts without row ranges", (long long)experts);
-  if (rows > (1ll << 31) - 1 || N > (1ll << 30) || K > (1ll << 28) || experts > (1 << 20))
+  if (rows > (1ll << 31) - 1 || N > (1ll << 30) || K > (1ll << 30) || experts > (1 << 20))
     return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / N=%lld / K=%lld / experts=%lld beyond the supported range", (long long)rows, (long long)N, (long long)K,
                 (long long)experts);
   if (rows == 0 || N == 0 || experts == 0) return DLB_OK;
@@ -355,30 +391,40 @@ int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, c
   if (!x || !q || !s || !y) return fail(DLB_ERR_NULL_POINTER, "x, q, s or y is NULL");
   if (x_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
   if (y_row_stride < N) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of y is smaller than N=%lld", (long long)y_row_stride, (long long)N);
-  if (misaligned(q, 16) || off_elements(x, dtype) || off_elements(y, dtype) || off_elements(s, s_dtype) || misaligned(row_start, 4) || misaligned(row_end, 4))
-    return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte aligned, the others to their elements");
+  // a tile is one buffer of 32-bit offsets
+  if (x_row_stride > (1 << 24) || K > (1 << 24)) return fail(DLB_ERR_BAD_STRIDE, "x row stride %lld / K=%lld beyond 2^24", (long long)x_row_stride, (long long)K);
+  if (misaligned(q, 16) || misaligned(x, 4) || x_row_stride % 2 != 0 || off_elements(y, dtype) || off_elements(s, s_dtype) || misaligned(row_start, 4) ||
+      misaligned(row_end, 4))
+    return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte, rows of x 4-byte aligned, the others to their elements");
   W4Args a{};
   a.x = x, a.q = static_cast<const uint8_t*>(q), a.s = s, a.z = static_cast<const uint8_t*>(z), a.y = y, a.row_start = row_start, a.row_end = row_end;
   a.x_rs = x_row_stride, a.y_rs = y_row_stride, a.rows = rows;
   a.N = static_cast<int>(N), a.K = static_cast<int>(K), a.G = static_cast<int>(K / group), a.E = static_cast<int>(experts), a.s_type = s_dtype;
   a.q_es = N * (K / 2), a.s_es = N * a.G;
   const int64_t busy = experts < rows ? experts : rows;  // experts that can have a row
-  const W4Shape shape = w4_shape(row_start ? ceil_div(rows, busy) : rows, N, K);
-  const int64_t y_blocks = row_start ? busy : ceil_div(rows, 16 * shape.mt);
+  const W4Plan plan = row_start ? w4_plan(ceil_div(rows, busy), true, busy, N, K) : w4_plan(rows, false, 1, N, K);
+  const int64_t y_blocks = row_start ? busy : ceil_div(rows, 16 * plan.mt);
   if (y_blocks > 65535) return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / experts=%lld beyond the supported range", (long long)rows, (long long)experts);
+  const size_t need = plan.slices > 1 ? static_cast<size_t>(plan.slices) * rows * N * sizeof(float) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+  if (need > 0 && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  if (ceil_div(rows * N, 256) > (1ll << 31) - 1) return fail(DLB_ERR_BAD_SHAPE, "rows=%lld x N=%lld beyond the supported range", (long long)rows, (long long)N);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const auto launch = [&](auto t) {
+  float* const sums = static_cast<float*>(workspace);
+  const auto launch = [&](auto t, auto zeros) {
     if (group == 128)
-      launch_w4<t(), 4>(a, shape, y_blocks, st);
+      launch_w4<t(), 1, zeros()>(a, plan, y_blocks, sums, st);
     else if (group == 64)
-      launch_w4<t(), 2>(a, shape, y_blocks, st);
+      launch_w4<t(), 2, zeros()>(a, plan, y_blocks, sums, st);
     else
-      launch_w4<t(), 1>(a, shape, y_blocks, st);
+      launch_w4<t(), 4, zeros()>(a, plan, y_blocks, sums, st);
   };
+  const auto with_zeros = [&](auto t) { z ? launch(t, std::true_type()) : launch(t, std::false_type()); };
   if (dtype == kInBf16)
-    launch(std::integral_constant<int, kInBf16>());
+    with_zeros(std::integral_constant<int, kInBf16>());
   else
-    launch(std::integral_constant<int, kInF16>());
+    with_zeros(std::integral_constant<int, kInF16>());
   return finish("w4_gemm");
 }
 

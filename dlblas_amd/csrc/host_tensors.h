@@ -42,12 +42,15 @@ bool within(c10::DispatchKeySet keys, c10::DispatchKeySet allowed) { return (key
 
 bool no_modes() { return within(c10::impl::tls_local_dispatch_key_set().included_, kPlainIncluded) && !at::impl::torch_function_mode_enabled(); }
 
-// A dense GPU tensor that nothing but its own storage stands behind; nullptr otherwise.
-const at::Tensor* plain(PyObject* o) {
+// A dense GPU tensor that nothing but its own storage stands behind; nullptr otherwise.  *grad, where asked for: whether a gradient is
+// wanted for it; otherwise such a tensor is not plain.
+const at::Tensor* plain(PyObject* o, bool* grad = nullptr) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || !within(t.key_set(), kPlainKeys)) return nullptr;
-  if (t.is_conj() || t.is_neg() || (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()) return nullptr;
+  const bool wanted = c10::GradMode::is_enabled() && t.requires_grad();
+  if (t.is_conj() || t.is_neg() || (wanted && !grad) || t._fw_grad(0).defined()) return nullptr;
+  if (wanted) *grad = true;
   return &t;
 }
 

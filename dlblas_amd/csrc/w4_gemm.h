@@ -28,7 +28,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 struct W4Args {
   const void* x;
   const uint8_t* q;          // [E][N][K / 2], low nibble = even column
-  const void* s;             // [E][N][G] of s_type
+  const void* s;             // [E][N][G], bf16 or fp16 (s_type)
   const uint8_t* z;          // [E][N][G] or NULL
   void* y;                   // [rows][N]
   const int32_t* row_start;  // [E] or NULL: one matrix, all rows
@@ -46,11 +46,8 @@ __device__ __forceinline__ v4f mfma_16x16x32(const v4i& a, const v4i& b, const v
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float load_scale(const void* s, int type, int64_t i) {
-  if (type == kInF32) return static_cast<const float*>(s)[i];
-  const uint32_t w = static_cast<const uint16_t*>(s)[i];
-  if (type == kInBf16) return __uint_as_float(w << 16);
-  return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const uint8_t* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, bytes, 0x00020000);
 }
 
 // Words i of the four quarters of the wave change places with quarters i of the words: quarter q of word i then holds what
@@ -64,90 +61,170 @@ __device__ __forceinline__ void transpose_quarters(v4i& v) {
   v = v4i{static_cast<int>(c[0]), static_cast<int>(c[1]), static_cast<int>(d[0]), static_cast<int>(d[1])};
 }
 
-// STEPS = MFMA steps (32 columns) per group: 4, 2, 1 for groups of 128, 64, 32.  A tile is 16 MT rows of x by 16 NT rows of the
-// matrix.  Groups below a block of 128 need the 32 columns of a step to be neighbours, so the quarters of the wave exchange words;
-// otherwise a quarter keeps its 32 columns and x is read to match.
-template <int T, int STEPS, int MT, int NT>
+// The values of a lane's quarter in all quarters: v[i] of the result is what quarter i held.
+template <int N>
+__device__ __forceinline__ void spread_quarters(float v, float (&out)[N]) {
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  const unsigned u = __float_as_uint(v);
+  if (N == 1) {
+    out[0] = v;
+    return;
+  }
+  const v2u h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  if (N == 2) {
+    out[0] = __uint_as_float(h[0]), out[N - 1] = __uint_as_float(h[1]);
+    return;
+  }
+  const v2u lo = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+  const v2u hi = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+  out[0] = __uint_as_float(lo[0]), out[1 % N] = __uint_as_float(lo[1]), out[2 % N] = __uint_as_float(hi[0]), out[3 % N] = __uint_as_float(hi[1]);
+}
+
+// The which-th expert that has rows, -1: there are not so many.
+__device__ __forceinline__ int nth_expert(const W4Args& p, int which, int lane) {
+  for (int e0 = 0; e0 < p.E; e0 += 64) {
+    const int i = min(e0 + lane, p.E - 1);
+    uint64_t some = __ballot(e0 + lane < p.E && p.row_end[i] > p.row_start[i]);
+    const int n = __popcll(some);
+    if (which >= n) {
+      which -= n;
+      continue;
+    }
+    for (; which > 0; --which) some &= some - 1;
+    return __builtin_amdgcn_readfirstlane(e0 + __builtin_ctzll(some));
+  }
+  return -1;
+}
+
+// A barrier for what went through LDS; loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int N>
+__device__ __forceinline__ void spread_quarters(int v, int (&out)[N]) {
+  float f[N];
+  spread_quarters(__int_as_float(v), f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = __float_as_int(f[i]);
+}
+
+// Chunks of 256 columns with groups of 128: a quarter holds 64 columns, words of a and then of b.  Afterwards a holds the columns of the
+// first group and b those of the second: quarters 0 and 1 keep their place in a, 2 and 3 in b.
+__device__ __forceinline__ void exchange_halves(v4i& a, v4i& b) {
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const v2u h = __builtin_amdgcn_permlane32_swap(a[i], b[i], false, false);
+    a[i] = static_cast<int>(h[0]), b[i] = static_cast<int>(h[1]);
+  }
+}
+// The values of the halves of the wave in both.
+__device__ __forceinline__ void spread_halves(int s, int mz, bool zeros, float* s_out, int* m_out) {
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  const v2u h = __builtin_amdgcn_permlane32_swap(s, s, false, false);
+  s_out[0] = __uint_as_float(h[0]), s_out[1] = __uint_as_float(h[1]);
+  const v2u z = __builtin_amdgcn_permlane32_swap(mz, mz, false, false);
+  if (zeros) m_out[0] = static_cast<int>(z[0]), m_out[1] = static_cast<int>(z[1]);
+}
+
+// What a wave reads for one block of 128 columns: its weights, the scale (and zero point) of the quarter's group, its rows of x.
+template <int MT, int NT>
+struct W4Block {
+  v4i w[NT];
+  uint32_t s[NT], z[NT];
+  v4i x[MT][4];
+};
+
+// GROUPS = groups in a block of 128 columns: 1, 2, 4 for groups of 128, 64, 32.  A tile is 16 MT rows of x by 16 NT rows of the
+// matrix.  After the exchange of words between the quarters, step i of a block is columns 32 i to 32 i + 31, 8 a quarter.
+// DEPTH blocks are on their way to a wave at a time.  Loads return in the order they were issued in, so all that a block needs is
+// asked for together, and none of them stands behind a branch, because a wait counts the loads issued since: what lies outside
+// (rows past the tile, columns past the end, blocks past the last one) has an offset past the end of the buffer, which costs no
+// traffic and gives zero.
+template <int T, int GROUPS, bool ZEROS, int MT, int NT, int DEPTH>
 __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
   extern __shared__ float part[];  // [waves][MT][NT][256]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int quarter = lane >> 4, l16 = lane & 15;
-  constexpr bool kTranspose = STEPS < 4;
-  constexpr int kGroups = 4 / STEPS;  // of a block
-  const uint8_t* wq = p.q;
-  int64_t s_base = 0;
+  constexpr uint32_t kNowhere = 0x80000000u;  // every buffer is shorter
+  int64_t expert = 0;
   int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT, row_end = min(p.rows, row0 + 16 * MT);
   if (p.row_start) {
-    // the blockIdx.y-th expert that has rows
-    int left = blockIdx.y;
-    int e = -1;
-    for (int e0 = 0; e0 < p.E && e < 0; e0 += 64) {
-      const int i = e0 + lane;
-      uint64_t some = __ballot(i < p.E && p.row_end[i < p.E ? i : 0] > p.row_start[i < p.E ? i : 0]);
-      const int n = __popcll(some);
-      if (left >= n) {
-        left -= n;
-        continue;
-      }
-      for (; left > 0; --left) some &= some - 1;
-      e = e0 + __builtin_ctzll(some);
-    }
+    const int e = nth_expert(p, blockIdx.y, lane);
     if (e < 0) return;
-    e = __builtin_amdgcn_readfirstlane(e);
     row0 = max(p.row_start[e], 0), row_end = min(static_cast<int64_t>(p.row_end[e]), p.rows);
-    wq += e * p.q_es;
-    s_base = e * p.s_es;
+    expert = e;
   }
   const int blocks = (p.K + 127) / 128;
-  const int half = p.K / 2;  // bytes of a row
-  int n_row[NT];             // rows past the matrix read its last one and are not stored
+  const uint32_t half = p.K / 2;  // bytes of a row
+  const int n0 = static_cast<int>(blockIdx.x) * 16 * NT;
+  const int cols = min(16 * NT, p.N - n0);
+  const uint8_t* w_ptr = p.q + expert * p.q_es + static_cast<int64_t>(n0) * half;
+  const int64_t s0 = expert * p.s_es + static_cast<int64_t>(n0) * p.G;
+  const uint8_t *s_ptr = static_cast<const uint8_t*>(p.s) + 2 * s0, *z_ptr = ZEROS ? p.z + s0 : p.q;
+  const uint32_t w_bytes = cols * half, s_count = cols * p.G;
+  uint32_t w_off[NT], s_off[NT];  // of rows past the matrix: past the end
 #pragma unroll
-  for (int n = 0; n < NT; ++n) n_row[n] = min(static_cast<int>(blockIdx.x) * 16 * NT + 16 * n + l16, p.N - 1);
+  for (int n = 0; n < NT; ++n) w_off[n] = (16 * n + l16) * half + 16 * quarter, s_off[n] = (16 * n + l16) * p.G + quarter * GROUPS / 4;
+  // in registers, where one v_and_or_b32 takes both
+  int mask = T == kInBf16 ? 0x00780078 : 0x03c003c0, bits = T == kInBf16 ? 0x41804180 : 0x4c004c00;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bits));
   v4i ones;
 #pragma unroll
   for (int i = 0; i < 4; ++i) ones[i] = T == kInBf16 ? 0x3f803f80 : 0x3c003c00;
 
   for (; row0 < row_end; row0 += 16 * MT) {
+    const int rows = static_cast<int>(min(row_end - row0, static_cast<int64_t>(16 * MT)));
+    const uint32_t x_row = static_cast<uint32_t>(p.x_rs) * 2;
+    const uint8_t* x_ptr = static_cast<const uint8_t*>(p.x) + row0 * p.x_rs * 2;
+    const uint32_t x_bytes = (rows - 1) * x_row + 2u * p.K;
+    uint32_t x_off[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x_off[m] = 16 * m + l16 < rows ? (16 * m + l16) * x_row + 16 * quarter : kNowhere;
     v4f acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
-    const char* x_row[MT];
-    bool x_on[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t r = row0 + 16 * m + l16;
-      x_on[m] = r < row_end;
-      x_row[m] = static_cast<const char*>(p.x) + (x_on[m] ? r : row0) * p.x_rs * 2;
-    }
-    auto load_w = [&](int kb, v4i (&w)[NT]) {
-      const int off = kb * 64 + 16 * quarter;
+    // The place of a block travels in the scalar offset, so a load costs no vector instruction; past the last block the buffers are
+    // empty.  A lane past the last column of a row
+    // reads the next row's codes, which then meet zeros of x; the scale of such a group is replaced in multiply().
+    auto load = [&](int kb, W4Block<MT, NT>& b) {
+      const bool in = kb < blocks;
+      const uint32_t at = in ? kb : 0;
+      const auto w_src = make_rsrc(w_ptr, in ? w_bytes : 0), s_src = make_rsrc(s_ptr, in ? 2 * s_count : 0), z_src = make_rsrc(z_ptr, ZEROS && in ? s_count : 0);
+      const auto x_src = make_rsrc(x_ptr, in ? x_bytes : 0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        w[n] = v4i{0, 0, 0, 0};
-        if (off < half) w[n] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(wq + static_cast<int64_t>(n_row[n]) * half + off));
+        b.w[n] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(w_src, w_off[n], 64 * at, 2));
+        b.s[n] = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * s_off[n], 2 * GROUPS * at, 0);
+        if (ZEROS) b.z[n] = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off[n], GROUPS * at, 0);
       }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b.x[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, x_off[m] + 64 * i, 256 * at, 0));
     };
-    v4i w_now[NT];
-    if (wave < blocks) load_w(wave, w_now);
-    for (int kb = wave; kb < blocks; kb += waves) {
-      v4i w_next[NT];
-      if (kb + waves < blocks) load_w(kb + waves, w_next);
-      float sc[NT][kGroups], coef[NT][kGroups];
+    auto multiply = [&](int kb, W4Block<MT, NT>& b) {
+      float sc[NT][GROUPS], coef[NT][GROUPS];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        transpose_quarters(b.w[n]);
+        float s = p.s_type == kInBf16 ? __uint_as_float(b.s[n] << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s[n])));
+        if (GROUPS > 1 && kb * GROUPS + quarter * GROUPS / 4 >= p.G) s = 0.f;
+        spread_quarters(s, sc[n]);
+        if (ZEROS)
+          spread_quarters(-16.f - static_cast<float>(b.z[n]), coef[n]);
+        else
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const int64_t i = s_base + static_cast<int64_t>(n_row[n]) * p.G + min(kb * kGroups + g, p.G - 1);
-          sc[n][g] = load_scale(p.s, p.s_type, i);
-          coef[n][g] = -16.f - (p.z ? static_cast<float>(p.z[i]) : 8.f);
-        }
+          for (int g = 0; g < GROUPS; ++g) coef[n][g] = -24.f;
+      }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (kTranspose) transpose_quarters(w_now[n]);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
+      for (int g = 0; g < GROUPS; ++g) {
         v4f sum[MT][NT], xs[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -156,30 +233,30 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
           for (int n = 0; n < NT; ++n) sum[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
-        for (int i = g * STEPS; i < (g + 1) * STEPS; ++i) {
-          const int k = kb * 128 + (kTranspose ? 32 * i + 8 * quarter : 32 * quarter + 8 * i);
+        for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
+          // columns past the end: what was read there is the next row, and selecting byte 12 gives zero
+          const bool in = kb * 128 + 32 * i < p.K;
+          const uint32_t low = in ? 0x05040100u : 0x0c0c0c0cu, high = in ? 0x07060302u : 0x0c0c0c0cu;
           v4i xf[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            v4i v{0, 0, 0, 0};
-            if (x_on[m] && k < p.K) v = *reinterpret_cast<const v4i_el*>(x_row[m] + 2 * k);
-            xf[m][0] = __builtin_amdgcn_perm(v[2], v[0], 0x05040100);
-            xf[m][1] = __builtin_amdgcn_perm(v[2], v[0], 0x07060302);
-            xf[m][2] = __builtin_amdgcn_perm(v[3], v[1], 0x05040100);
-            xf[m][3] = __builtin_amdgcn_perm(v[3], v[1], 0x07060302);
+            const v4i v = b.x[m][i];
+            xf[m][0] = __builtin_amdgcn_perm(v[2], v[0], low);
+            xf[m][1] = __builtin_amdgcn_perm(v[2], v[0], high);
+            xf[m][2] = __builtin_amdgcn_perm(v[3], v[1], low);
+            xf[m][3] = __builtin_amdgcn_perm(v[3], v[1], high);
           }
 #pragma unroll
           for (int m = 0; m < MT; ++m) xs[m] = mfma_16x16x32<T>(xf[m], ones, xs[m]);
-          constexpr int kBits = T == kInBf16 ? 0x41804180 : 0x4c004c00;
-          constexpr int kMask = T == kInBf16 ? 0x00780078 : 0x03c003c0, kUp = T == kInBf16 ? 3 : 6;
+          constexpr int kUp = T == kInBf16 ? 3 : 6;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int word = w_now[n][i];
-            v4i b;
+            const int word = b.w[n][i];
+            v4i v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & kMask) | kBits;
+            for (int j = 0; j < 4; ++j) v[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & mask) | bits;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) sum[m][n] = mfma_16x16x32<T>(xf[m], b, sum[m][n]);
+            for (int m = 0; m < MT; ++m) sum[m][n] = mfma_16x16x32<T>(xf[m], v, sum[m][n]);
           }
         }
 #pragma unroll
@@ -189,8 +266,22 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(sc[n][g], fmaf(coef[n][g], xs[m][r], sum[m][n][r]), acc[m][n][r]);
       }
+    };
+    W4Block<MT, NT> on_way[DEPTH];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) w_now[n] = w_next[n];
+    for (int d = 0; d < DEPTH; ++d) {
+      load(wave + d * waves, on_way[d]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int kb = wave; kb < blocks; kb += DEPTH * waves) {
+      // whole turns: blocks past the last one multiply zeros; the order of loads and products stays as it is written
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        multiply(kb + d * waves, on_way[d]);
+        __builtin_amdgcn_sched_barrier(0);
+        load(kb + (DEPTH + d) * waves, on_way[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     // lane l holds rows 4 (l / 16) + r, column l % 16 of a tile
 #pragma unroll
@@ -202,18 +293,261 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
     __syncthreads();
     for (int i = tid; i < MT * NT * 256; i += blockDim.x) {
       const int m = i / (NT * 256), n = i / 256 % NT, e = i % 256;
-      const int64_t row = row0 + 16 * m + e / 16;
-      const int col = static_cast<int>(blockIdx.x) * 16 * NT + 16 * n + e % 16;
+      const int row = 16 * m + e / 16, col = 16 * n + e % 16;
       float sum = 0.f;
       for (int w = 0; w < waves; ++w) sum += part[w * MT * NT * 256 + i];
-      if (row >= row_end || col >= p.N) continue;
+      if (row >= rows || col >= cols) continue;
+      const int64_t at = (row0 + row) * p.y_rs + n0 + col;
       if (T == kInBf16)
-        static_cast<__bf16*>(p.y)[row * p.y_rs + col] = static_cast<__bf16>(sum);
+        static_cast<__bf16*>(p.y)[at] = static_cast<__bf16>(sum);
       else
-        static_cast<_Float16*>(p.y)[row * p.y_rs + col] = static_cast<_Float16>(sum);
+        static_cast<_Float16*>(p.y)[at] = static_cast<_Float16>(sum);
     }
     __syncthreads();
   }
+}
+
+// The same product for more than a little work.  Four waves take neighbouring tiles and ask memory for nothing but weights and scales, a
+// chunk of UNITS x 256 columns ahead; x goes through LDS once for all of them, in the order in which they read it.
+// A lane reads 32 bytes of a unit's 128 bytes of a row in two loads, so a load touches whole cache lines: 64 columns a quarter.
+// Eight steps of 32 columns follow, of one group each: for groups of 128 the halves of the wave exchange words, for smaller ones the
+// quarters.  Slices of K (gridDim.z) go to workgroups of their own, whose fp32 sums w4_sum_kernel adds in slice order.
+constexpr int kW4Waves = 4;
+constexpr int kW4Unit = 256;  // columns
+
+// PIECES = 16-byte pieces of x a thread moves per chunk: all rows of a tile take 2 MT UNITS, one is enough for 8 / UNITS rows (1 x 7168 x
+// 18432 22.9 -> 21.1 us).
+template <int T, int GROUPS, bool ZEROS, int MT, int NT, int UNITS, int PIECES>
+__global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4Args p, float* sums, int chunks_each) {
+  constexpr int kThreads = 64 * kW4Waves;
+  constexpr int kUnitGroups = 2 * GROUPS;
+  constexpr int kLoads = GROUPS == 4 ? 2 : 1;  // of scales per unit and tile
+  constexpr int kPitch = 128 * UNITS + 16;     // bytes of a row's steps in LDS, neighbouring rows on other banks
+  constexpr int kPlane = 16 * MT * kPitch;     // x of a quarter
+  __shared__ __attribute__((aligned(16))) char x_lds[2][4 * kPlane];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int quarter = lane >> 4, l16 = lane & 15;
+  constexpr uint32_t kNowhere = 0x80000000u;  // past the end of every buffer
+  int64_t expert = 0;
+  int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT, row_end = min(p.rows, row0 + 16 * MT);
+  if (p.row_start) {
+    const int e = nth_expert(p, blockIdx.y, lane);
+    if (e < 0) return;
+    row0 = max(p.row_start[e], 0), row_end = min(static_cast<int64_t>(p.row_end[e]), p.rows);
+    expert = e;
+  }
+  constexpr int kColumns = kW4Unit * UNITS;
+  const int first = blockIdx.z * chunks_each, last = min((p.K + kColumns - 1) / kColumns, first + chunks_each);
+  const uint32_t half = p.K / 2;
+  const int n0 = (static_cast<int>(blockIdx.x) * kW4Waves + wave) * 16 * NT;
+  const int cols = max(0, min(16 * NT, p.N - n0));
+  const int64_t n_base = min(n0, p.N - 1);
+  const uint8_t* w_ptr = p.q + expert * p.q_es + n_base * half;
+  const int64_t s0 = expert * p.s_es + n_base * p.G;
+  const uint8_t *s_ptr = static_cast<const uint8_t*>(p.s) + 2 * s0, *z_ptr = ZEROS ? p.z + s0 : p.q;
+  const uint32_t w_bytes = cols * half, s_count = cols * p.G;
+  // group of a unit whose scale this quarter reads (with groups of 32 also the next one)
+  const int my_group = GROUPS == 1 ? quarter >> 1 : GROUPS == 2 ? quarter : 2 * quarter;
+  uint32_t w_off[NT], s_off[NT];  // of rows past the matrix: past the end
+#pragma unroll
+  for (int n = 0; n < NT; ++n) w_off[n] = (16 * n + l16) * half + 32 * quarter, s_off[n] = (16 * n + l16) * p.G + my_group;
+  // in registers, where one v_and_or_b32 takes both
+  int mask = T == kInBf16 ? 0x00780078 : 0x03c003c0, bits = T == kInBf16 ? 0x41804180 : 0x4c004c00;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bits));
+  const char* const x_mine = &x_lds[0][quarter * kPlane + l16 * kPitch];
+
+  struct Chunk {
+    v4i w[NT][UNITS][2];
+    uint32_t s[NT][UNITS][kLoads], z[NT][UNITS][kLoads];
+  };
+  auto load = [&](int c, Chunk& b) {
+    const bool in = c < last && w_bytes > 0;  // a scalar offset stays below the length of its buffer
+    const uint32_t at = in ? c * UNITS : 0;
+    const auto w_src = make_rsrc(w_ptr, in ? w_bytes : 0), s_src = make_rsrc(s_ptr, in ? 2 * s_count : 0), z_src = make_rsrc(z_ptr, ZEROS && in ? s_count : 0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) b.w[n][u][k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(w_src, w_off[n] + 128 * u + 16 * k, 128 * at, 0));
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          b.s[n][u][j] = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * (s_off[n] + kUnitGroups * u + j), 2 * kUnitGroups * at, 0);
+          if (ZEROS) b.z[n][u][j] = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off[n] + kUnitGroups * u + j, kUnitGroups * at, 0);
+        }
+      }
+  };
+  for (; row0 < row_end; row0 += 16 * MT) {
+    const int rows = static_cast<int>(min(row_end - row0, static_cast<int64_t>(16 * MT)));
+    const uint32_t x_pitch = static_cast<uint32_t>(p.x_rs) * 2;
+    const uint8_t* x_ptr = static_cast<const uint8_t*>(p.x) + row0 * p.x_rs * 2;
+    const uint32_t x_bytes = (rows - 1) * x_pitch + 2u * p.K;
+    // piece j of a thread: 8 columns of row x_r + j rows_apart, for the step and quarter that read them
+    constexpr int kRowPieces = 32 * UNITS, kRowsApart = kThreads / kRowPieces;
+    const int x_r = tid / kRowPieces, x_col8 = tid % kRowPieces, in_unit = x_col8 & 31;
+    const int x_step = GROUPS > 1 ? in_unit >> 2 : 4 * (in_unit >> 4) + (in_unit & 3);
+    const int x_quarter = GROUPS > 1 ? in_unit & 3 : ((in_unit >> 3) & 1) + ((in_unit >> 2) & 1) * 2;
+    const int x_to = x_quarter * kPlane + x_r * kPitch + (x_col8 >> 5) * 128 + x_step * 16;
+    v4i piece[PIECES];
+    auto load_x = [&](int c) {
+      const auto x_src = make_rsrc(x_ptr, c < last ? x_bytes : 0);
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        const int r = x_r + j * kRowsApart;
+        piece[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, r < rows ? r * x_pitch + 16 * x_col8 : kNowhere, c < last ? c * (2u * kColumns) : 0, 0));
+      }
+    };
+    auto keep_x = [&](int c, int buf) {
+      // columns past the end: what was read there is the next row, and selecting byte 12 gives zero
+      const bool in = c * kColumns + 8 * x_col8 < p.K;
+      const uint32_t low = in ? 0x05040100u : 0x0c0c0c0cu, high = in ? 0x07060302u : 0x0c0c0c0cu;
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        const v4i v = piece[j];
+        const v4i o{static_cast<int>(__builtin_amdgcn_perm(v[2], v[0], low)), static_cast<int>(__builtin_amdgcn_perm(v[2], v[0], high)),
+                    static_cast<int>(__builtin_amdgcn_perm(v[3], v[1], low)), static_cast<int>(__builtin_amdgcn_perm(v[3], v[1], high))};
+        *reinterpret_cast<v4i*>(&x_lds[buf][x_to + j * kRowsApart * kPitch]) = o;
+      }
+    };
+    v4f acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int c, Chunk& b, int buf) {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        float sc[NT][kUnitGroups];
+        int minus[NT][kUnitGroups];  // -(16 + z) twice: the matrix through which the constant leaves
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j) {
+            float s = p.s_type == kInBf16 ? __uint_as_float(b.s[n][u][j] << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s[n][u][j])));
+            if ((c * UNITS + u) * kUnitGroups + my_group + j >= p.G) s = 0.f;  // past the row's last group: the next row's
+            const int mz = ZEROS ? static_cast<int>((b.z[n][u][j] << (T == kInBf16 ? 3 : 6)) * 0x10001u + (static_cast<uint32_t>(bits) | 0x80008000u)) : 0;
+            if (GROUPS == 1) {
+              spread_halves(__float_as_int(s), mz, ZEROS, sc[n], minus[n]);
+            } else {
+              float s4[4];
+              int m4[4] = {};
+              spread_quarters(s, s4);
+              if (ZEROS) spread_quarters(mz, m4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[n][(kLoads * i + j) % kUnitGroups] = s4[i], minus[n][(kLoads * i + j) % kUnitGroups] = m4[i];
+            }
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (GROUPS == 1)
+            exchange_halves(b.w[n][u][0], b.w[n][u][1]);
+          else
+            transpose_quarters(b.w[n][u][0]), transpose_quarters(b.w[n][u][1]);
+        }
+#pragma unroll
+        for (int g = 0; g < kUnitGroups; ++g) {
+          v4f sum[MT][NT];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sum[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = g * 4 / GROUPS; st < (g + 1) * 4 / GROUPS; ++st) {
+            v4i xf[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xf[m] = *reinterpret_cast<const v4i*>(x_mine + buf * 4 * kPlane + m * 16 * kPitch + u * 128 + st * 16);
+            constexpr int kUp = T == kInBf16 ? 3 : 6;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const int word = GROUPS == 1 ? b.w[n][u][st >> 2][st & 3] : b.w[n][u][st & 1][st >> 1];
+              v4i v, c16;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & mask) | bits;
+                c16[j] = ZEROS ? minus[n][g] : static_cast<int>(T == kInBf16 ? 0xc1c0c1c0 : 0xce00ce00);
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                sum[m][n] = mfma_16x16x32<T>(xf[m], c16, sum[m][n]);
+                sum[m][n] = mfma_16x16x32<T>(xf[m], v, sum[m][n]);
+              }
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(sc[n][g], sum[m][n][r], acc[m][n][r]);
+        }
+      }
+    };
+    Chunk even, odd;
+    load_x(first);
+    load(first, even);
+    __builtin_amdgcn_sched_barrier(0);
+    keep_x(first, 0);
+    lds_barrier();
+    for (int c = first; c < last; c += 2) {
+      // x before the weights: loads return in order.  Past the last chunk: zeros
+      load_x(c + 1);
+      load(c + 1, odd);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(c, even, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      keep_x(c + 1, 1);
+      lds_barrier();
+      load_x(c + 2);
+      load(c + 2, even);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(c + 1, odd, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      keep_x(c + 2, 0);
+      lds_barrier();
+    }
+    // lane l holds rows 4 (l / 16) + r, column l % 16 of a tile
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * m + 4 * quarter + r, col = 16 * n + l16;
+          if (row >= rows || col >= cols) continue;
+          if (sums) {
+            sums[(blockIdx.z * p.rows + row0 + row) * p.N + n0 + col] = acc[m][n][r];
+            continue;
+          }
+          const int64_t at = (row0 + row) * p.y_rs + n0 + col;
+          if (T == kInBf16)
+            static_cast<__bf16*>(p.y)[at] = static_cast<__bf16>(acc[m][n][r]);
+          else
+            static_cast<_Float16*>(p.y)[at] = static_cast<_Float16>(acc[m][n][r]);
+        }
+  }
+}
+
+// y = the sums of the slices of K, added in their order.
+template <int T>
+__global__ void __launch_bounds__(256) w4_sum_kernel(const float* sums, void* y, int64_t y_rs, int64_t rows, int N, int slices) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows * N) return;
+  float s = 0.f;
+  int z = 0;
+  for (; z + 4 <= slices; z += 4) {
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = sums[(z + u) * rows * N + i];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s += v[u];
+  }
+  for (; z < slices; ++z) s += sums[z * rows * N + i];
+  const int64_t row = i / N, at = row * y_rs + (i - row * N);
+  if (T == kInBf16)
+    static_cast<__bf16*>(y)[at] = static_cast<__bf16>(s);
+  else
+    static_cast<_Float16*>(y)[at] = static_cast<_Float16>(s);
 }
 
 // 4-bit quantiser: per group of 32, 64 or 128 columns of a row

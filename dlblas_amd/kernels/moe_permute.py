@@ -173,7 +173,7 @@ def moe_unpermute(rows: torch.Tensor, permutation: Union[MoePermutation, torch.T
     whole = isinstance(permutation, MoePermutation)
     row_index = permutation.row_index if whole else permutation
     if not torch.compiler.is_compiling():
-        out = _fast.moe_unpermute(rows, row_index, topk_weights)
+        out = _fast.moe_unpermute(rows, row_index, topk_weights, permutation.source if whole else None)
         if out is not None:
             return out
     if rows.dtype not in _lib.IN_CODES:

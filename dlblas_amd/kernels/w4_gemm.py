@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from .. import _decoder, _fast, _lib
+from .. import _decoder, _fast
 from ..utils import SymVar, Tensor, register_dlblas_op
 from .rms_norm import _bench
 
@@ -33,8 +33,8 @@ def _check(x, w_q, w_s, w_z, dims):
         raise TypeError(f'x must be bfloat16 or float16, got {x.dtype}')
     if w_q.dtype != torch.uint8:
         raise TypeError(f'w_q must be uint8 (two codes a byte), got {w_q.dtype}')
-    if w_s.dtype not in _lib.IN_CODES:
-        raise TypeError(f'w_s must be bfloat16, float16 or float32, got {w_s.dtype}')
+    if w_s.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f'w_s must be bfloat16 or float16, got {w_s.dtype}')
     if w_z is not None and w_z.dtype != torch.uint8:
         raise TypeError(f'w_z must be uint8, got {w_z.dtype}')
     if w_q.dim() != dims or w_s.dim() != dims or tuple(w_s.shape[:-1]) != tuple(w_q.shape[:-1]):
@@ -42,6 +42,8 @@ def _check(x, w_q, w_s, w_z, dims):
     if w_z is not None and w_z.shape != w_s.shape:
         raise ValueError(f'w_z must be like w_s {list(w_s.shape)}, got {list(w_z.shape)}')
     K = 2 * w_q.size(-1)
+    if K > 1 << 24:
+        raise ValueError(f'at most 2^24 columns are implemented, got {K}')
     if x.size(-1) != K:
         raise ValueError(f'x has {x.size(-1)} columns and w_q {K}')
     groups = w_s.size(-1)
@@ -57,11 +59,19 @@ def _columns_whole(t):
     return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
 
 
-def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x`` [..., K] (bf16 / fp16) times the 4-bit weights ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / group] (bf16, fp16 or
-    fp32) and zero points ``w_z`` (uint8 like w_s, 0 ... 15, or None: 8): [..., N] in the type of x; fp32 sums, one rounding.
+def _on_dwords(t):
+    """Rows as the kernel reads them: on 4 bytes and less than 2^25 bytes apart."""
+    t = _columns_whole(t)
+    if t.data_ptr() % 4 != 0 or t.stride(0) % 2 != 0 or t.stride(0) > 1 << 24:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
 
-    For up to a few dozen rows: the weights are read once per 64 of them.  A product of N(0, 1)-like rows is as exact as its rounding;
+
+def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` [..., K] (bf16 / fp16) times the 4-bit weights ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / group] (bf16 or fp16)
+    and zero points ``w_z`` (uint8 like w_s, 0 ... 15, or None: 8): [..., N] in the type of x; fp32 sums, one rounding.
+
+    For up to a few dozen rows: the weights are read once per 32 of them.  A product of N(0, 1)-like rows is as exact as its rounding;
     see include/dlblas_decoder.h for rows that are nearly constant.
     """
     if not torch.compiler.is_compiling():
@@ -73,15 +83,15 @@ def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional
     group = _check(x, w_q, w_s, w_z, 2)
     x2d = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
     y = torch.empty(x.shape[:-1] + (w_q.size(0), ), dtype=x.dtype, device=x.device)
-    _w4_op(_columns_whole(x2d), w_q, w_s, w_z, y.view(-1, w_q.size(0)), None, None, group)
+    _w4_op(_on_dwords(x2d), w_q, w_s, w_z, y.view(-1, w_q.size(0)), None, None, group)
     return y
 
 
 def w4_gemm_grouped(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, row_start: torch.Tensor, row_end: torch.Tensor,
                     w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``w_gemm`` by expert: the rows [row_start[e], row_end[e]) of ``x`` [R, K] times the weights of expert e, w_q [E, N, K / 2] and so on.
+    """``w4_gemm`` by expert: the rows [row_start[e], row_end[e]) of ``x`` [R, K] times the weights of expert e, w_q [E, N, K / 2] and so on.
     The ranges (int32 [E] on the device, clamped to 0 ... R) are those of ``moe_permute``; rows of no expert are not written.  For a decode
-    step: an expert's weights are read once per 64 of its rows, and those of experts without a row not at all."""
+    step: an expert's weights are read once per 16 or 32 of its rows, and those of experts without a row not at all."""
     if not torch.compiler.is_compiling():
         y = _fast.w4_gemm_grouped(x, w_q, w_s, row_start, row_end, w_z)
         if y is not None:
@@ -95,19 +105,19 @@ def w4_gemm_grouped(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, row_s
         if tuple(t.shape) != (w_q.size(0), ):
             raise ValueError(f'{name} must be [{w_q.size(0)}], got {list(t.shape)}')
     y = torch.empty((x.size(0), w_q.size(1)), dtype=x.dtype, device=x.device)
-    _w4_op(_columns_whole(x), w_q, w_s, w_z, y, row_start.contiguous(), row_end.contiguous(), group)
+    _w4_op(_on_dwords(x), w_q, w_s, w_z, y, row_start.contiguous(), row_end.contiguous(), group)
     return y
 
 
 def per_group_quant_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool = False):
-    """4-bit codes of a weight ``w`` [N, K] or [E, N, K] (bf16 / fp16 / fp32) for ``w4_gemm`` / ``w4_gemm_grouped``: returns
+    """4-bit codes of a weight ``w`` [N, K] or [E, N, K] (bf16 / fp16) for ``w4_gemm`` / ``w4_gemm_grouped``: returns
     ``(w_q, w_s, w_z)`` with w_q [..., K / 2] uint8, w_s [..., K / group_size] in the type of w and w_z uint8 like it, or None.
 
     Without zero points ``w_s = amax / 7`` and codes around 8; with them the range of a group from its lowest (at most 0) to its highest value
     (at least 0) is cut into 15 steps.
     """
-    if w.dtype not in _lib.IN_CODES:
-        raise TypeError(f'w must be bfloat16, float16 or float32, got {w.dtype}')
+    if w.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f'w must be bfloat16 or float16 (the type of its scales), got {w.dtype}')
     if w.dim() not in (2, 3):
         raise ValueError('w must be [N, K] or [E, N, K]')
     if group_size not in GROUP_SIZES:

@@ -113,22 +113,28 @@ int dlb_moe_unpermute_backward(const void* dout, int64_t dout_row_stride, const 
                                int64_t drows_row_stride, float* dweights, int64_t tokens, int64_t H, int64_t topk, int64_t num_rows,
                                void* stream);
 
+/* Bytes of scratch dlb_w4_gemm needs; experts = 0 for one matrix without row ranges (with them none is needed). */
+size_t dlb_w4_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t experts);
+
 /*
  * y[m, n] = sum over the groups g of K of s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]); fp32 sums, one rounding at the end.
+ * The sums of a group are those of x (16 + q) and x (16 + z): they are off by up to 24 * 2^-24 of 62 sum |x|.
  *
- *   x    [rows, K]         bf16 / fp16 (dtype), row stride x_row_stride
+ *   x    [rows, K]         bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^24), 4-byte aligned
  *   q    [experts, N, K/2] 4-bit codes, the even column in the low half of a byte; contiguous, 16-byte aligned
- *   s    [experts, N, K/group] scales, s_dtype DLB_IN_*, contiguous
- *   z    the same shape, one byte each (0 ... 15), or NULL: 8 everywhere
+ *   s    [experts, N, K/group] scales, bf16 / fp16 (s_dtype), contiguous
+ *   z    the same shape, one byte each (0 ... 15; other bits give other products), or NULL: 8 everywhere
  *   y    [rows, N]         dtype, row stride y_row_stride
  *   row_start, row_end [experts] int32 on the device: expert e multiplies the rows [row_start[e], row_end[e]), clamped to
  *        [0, rows]; rows of no expert are not written.  NULL with experts = 1: every row
+ *   workspace              4-byte aligned, dlb_w4_gemm_workspace_bytes(rows, N, K, row_start ? experts : 0), no initialisation
  *
- * group 32, 64 or 128; K % group == 0.  Meant for up to a few dozen rows (per expert): the weights are read once per 64 of them.
+ * group 32, 64 or 128; K % group == 0; K at most 2^24.  Meant for up to a few dozen rows (per expert): the weights are read once per
+ * 32 of them.
  */
 int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, int s_dtype, const void* z, void* y,
                 int64_t y_row_stride, const int32_t* row_start, const int32_t* row_end, int64_t rows, int64_t N, int64_t K,
-                int64_t group, int64_t experts, void* stream);
+                int64_t group, int64_t experts, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * 4-bit codes of a weight, per group of columns: without z  s = max |w| / 7, q = clamp(round(w / s) + 8, 0, 15);  with z

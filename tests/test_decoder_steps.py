@@ -96,12 +96,17 @@ def test_sort_entry_points_refuse():
 
 
 def test_w4_entry_points_refuse():
-    good = dict(x=fake, x_rs=256, dt=0, q=fake, s=fake, s_dt=0, z=null, y=fake, y_rs=64, rs=fake, re=fake, rows=4, N=64, K=256, g=128, E=2, st=null)
+    good = dict(x=fake, x_rs=256, dt=0, q=fake, s=fake, s_dt=0, z=null, y=fake, y_rs=64, rs=fake, re=fake, rows=4, N=64, K=256, g=128, E=2, ws=null, wsb=0, st=null)
     refused('dlb_w4_gemm', good, [
-        (dict(dt=2), DTYPE), (dict(s_dt=3), DTYPE), (dict(rows=-1), SHAPE), (dict(g=16), SHAPE), (dict(g=256), SHAPE), (dict(K=192), SHAPE), (dict(K=0), SHAPE),
+        (dict(dt=2), DTYPE), (dict(s_dt=2), DTYPE), (dict(rows=-1), SHAPE), (dict(g=16), SHAPE), (dict(g=256), SHAPE), (dict(K=192), SHAPE), (dict(K=0), SHAPE),
         (dict(rs=null), NULL), (dict(re=null), NULL), (dict(rs=null, re=null), SHAPE), (dict(x=null), NULL), (dict(q=null), NULL), (dict(s=null), NULL), (dict(y=null), NULL),
-        (dict(y_rs=63), STRIDE), (dict(x_rs=-1), STRIDE), (dict(q=at(4104)), ALIGN), (dict(x=at(4097)), ALIGN), (dict(s=at(4098), s_dt=2), ALIGN), (dict(rs=at(4098)), ALIGN),
-        (dict(rows=1 << 31), SHAPE), (dict(K=1 << 29), SHAPE), (dict(rows=0, x=null), OK), (dict(N=0, y=null), OK)])
+        (dict(y_rs=63), STRIDE), (dict(x_rs=-1), STRIDE), (dict(q=at(4104)), ALIGN), (dict(x=at(4098)), ALIGN), (dict(x_rs=257), ALIGN), (dict(x_rs=(1 << 24) + 2), STRIDE), (dict(s=at(4097)), ALIGN),
+        (dict(rs=at(4098)), ALIGN), (dict(rows=1 << 31), SHAPE), (dict(K=1 << 31), SHAPE), (dict(K=1 << 25), STRIDE), (dict(rows=0, x=null), OK), (dict(N=0, y=null), OK)])
+    lib = _lib.load()
+    need = lib.dlb_w4_gemm_workspace_bytes(16, 7168, 18432, 0)
+    assert need > 0 and lib.dlb_w4_gemm_workspace_bytes(16, 7168, 18432, 32) == 0 and lib.dlb_w4_gemm_workspace_bytes(1, 16, 128, 0) == 0
+    good.update(x_rs=18432, y_rs=7168, rs=null, re=null, rows=16, N=7168, K=18432, E=1, ws=fake, wsb=need)
+    refused('dlb_w4_gemm', good, [(dict(ws=null), WORKSPACE), (dict(wsb=need - 1), WORKSPACE), (dict(ws=at(4098)), ALIGN)])
     good = dict(w=fake, w_rs=256, dt=0, q=fake, s=fake, z=null, rows=4, K=256, g=128, st=null)
     refused('dlb_w4_quant', good, [
         (dict(dt=3), DTYPE), (dict(rows=-1), SHAPE), (dict(g=48), SHAPE), (dict(K=300), SHAPE), (dict(w=null), NULL), (dict(q=null), NULL), (dict(s=null), NULL),
@@ -151,7 +156,7 @@ def zeros(*size, dtype=bf16):
     (lambda: moe_unpermute(zeros(2, 8).requires_grad_(), MoePermutation(*(zeros(3, 1, dtype=i32), zeros(3, dtype=i32)) + (None, ) * 3)), ValueError),
     (lambda: w4_gemm(zeros(2, 256, dtype=f32), zeros(8, 128, dtype=u8), zeros(8, 2)), TypeError),
     (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=torch.int8), zeros(8, 2)), TypeError),
-    (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=u8), zeros(8, 2, dtype=i32)), TypeError),
+    (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=u8), zeros(8, 2, dtype=f32)), TypeError),
     (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=u8), zeros(7, 2)), ValueError),
     (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=u8), zeros(8, 1)), ValueError),
     (lambda: w4_gemm(zeros(2, 256), zeros(8, 128, dtype=u8), zeros(8, 0)), ValueError),
@@ -165,6 +170,7 @@ def zeros(*size, dtype=bf16):
     (lambda: w4_gemm_grouped(zeros(2, 256), zeros(3, 8, 128, dtype=u8), zeros(3, 8, 2), zeros(3, dtype=torch.int64), zeros(3, dtype=i32)), TypeError),
     (lambda: w4_gemm_grouped(zeros(2, 256), zeros(3, 8, 128, dtype=u8), zeros(3, 8, 2), zeros(3, dtype=i32), zeros(2, dtype=i32)), ValueError),
     (lambda: per_group_quant_w4(zeros(8, 256, dtype=u8)), TypeError),
+    (lambda: per_group_quant_w4(zeros(8, 256, dtype=f32)), TypeError),
     (lambda: per_group_quant_w4(zeros(256)), ValueError),
     (lambda: per_group_quant_w4(zeros(8, 256), 48), NotImplementedError),
     (lambda: per_group_quant_w4(zeros(8, 200), 128), AssertionError),

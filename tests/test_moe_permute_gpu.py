@@ -270,5 +270,38 @@ def test_native_path_takes_plain_calls(dev):
     ids = torch.zeros(5, 2, dtype=torch.int64, device=dev)
     assert mod._fast.moe_permute(x, None, ids, 4, 1, None) is not None
     assert mod._fast.moe_permute(*per_token_group_quant_fp8(x, 128), ids, 4, 128, 256) is not None
-    assert mod._fast.moe_unpermute(x, ids.int(), None) is not None
-    assert mod._fast.moe_unpermute(x, ids.int(), torch.ones(5, 2, device=dev, requires_grad=True)) is None
+    assert mod._fast.moe_unpermute(x, ids.int(), None, None) is not None
+    w = torch.ones(5, 2, device=dev, requires_grad=True)
+    assert mod._fast.moe_unpermute(x, ids.int(), w, None) is None  # no gradient from a table alone
+    rows, p = moe_permute(x, ids, 4)
+    assert mod._fast.moe_unpermute(rows, p.row_index, w, p.source).grad_fn is not None
+    assert mod._fast.moe_permute(x.requires_grad_(), None, ids, 4, 1, None)[0].grad_fn is not None
+
+
+def test_gradients_are_those_of_the_python_path(dev, monkeypatch):
+    T, topk, E, H = 30, 3, 4, 72
+    ids = routing(T, topk, E, seed=5).to(dev)
+    x, dout = (torch.randn(T, H, device=dev, dtype=bf16) for _ in range(2))
+    w = torch.randn(T, topk, device=dev)
+
+    def passes():
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        rows, p = moe_permute(xl, ids, E, 8)
+        out = moe_unpermute(rows, p, wl)
+        return (out, ) + torch.autograd.grad([out], [xl, wl], [dout])
+
+    fast = passes()
+    monkeypatch.setattr(mod._fast, 'moe_permute', lambda *a: None)
+    monkeypatch.setattr(mod._fast, 'moe_unpermute', lambda *a: None)
+    for a, b in zip(fast, passes()):
+        assert torch.equal(a, b)
+
+
+def test_a_second_derivative_raises(dev):
+    ids = routing(6, 2, 3).to(dev)
+    x = torch.randn(6, 16, device=dev).requires_grad_()
+    w = torch.randn(6, 2, device=dev).requires_grad_()
+    rows, p = moe_permute(x, ids, 3)
+    dx, dw = torch.autograd.grad([moe_unpermute(rows, p, w).sum()], [x, w], create_graph=True)
+    with pytest.raises(RuntimeError):
+        (dx.sum() + dw.sum()).backward()

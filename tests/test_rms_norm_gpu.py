@@ -225,8 +225,8 @@ def test_gradients_that_are_not_asked_for_and_shared_ones(dev):
     rms_norm(xl2, w).sum().backward()  # a gradient with stride 0
     ref = torch.autograd.grad(rms_norm(xl, w), [xl], [torch.ones_like(x)])[0]
     assert torch.equal(xl2.grad, ref)
+    d, = torch.autograd.grad(rms_norm(xl, w), [xl], [dy.requires_grad_()], create_graph=True)
     with pytest.raises(RuntimeError):
-        d, = torch.autograd.grad(rms_norm(xl, w), [xl], [dy.requires_grad_()], create_graph=True)
         d.sum().backward()
 
 
@@ -245,7 +245,25 @@ def test_native_path_takes_plain_calls(dev):
     x, w, res = (t.to(dev) for t in inputs(4, 256, bf16, True))
     assert mod._fast.rms_norm(x, w, 1e-6, res) is not None and mod._fast.rms_norm(x, w, 1e-6, None) is not None
     assert mod._fast.rms_norm_quant(x, w, 1e-6, res, 128, 1e-10, False) is not None
-    assert mod._fast.rms_norm(x.requires_grad_(), w, 1e-6, res) is None
+    assert mod._fast.rms_norm(x.requires_grad_(), w, 1e-6, res)[0].grad_fn is not None
+    assert mod._fast.rms_norm_quant(x, w, 1e-6, res, 128, 1e-10, False) is None
+
+
+@pytest.mark.parametrize('residual', [False, True])
+def test_gradients_are_those_of_the_python_path(dev, monkeypatch, residual):
+    x, w, res = (None if t is None else t.to(dev) for t in inputs(40, 520, bf16, residual))
+    dy, dsum = (torch.randn(40, 520, device=dev, dtype=bf16) for _ in range(2))
+
+    def passes():
+        leaves = [t.clone().requires_grad_() for t in (x, w, res) if t is not None]
+        out = rms_norm(leaves[0], leaves[1], 1e-6, leaves[2] if residual else None)
+        out = out if residual else (out, )
+        return tuple(out) + torch.autograd.grad(out, leaves, [dy, dsum][:len(out)])
+
+    fast = passes()
+    monkeypatch.setattr(mod._fast, 'rms_norm', lambda *a: None)
+    for a, b in zip(fast, passes()):
+        assert torch.equal(a, b)
 
 
 def test_registry(dev):

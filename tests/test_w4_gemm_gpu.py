@@ -43,6 +43,8 @@ def check(y, x, q, s, z, what):
 SHAPES = [  # M, N, K, group
     (1, 1, 32, 32), (1, 16, 128, 128), (1, 2112, 7168, 128), (2, 17, 64, 64), (3, 33, 96, 32), (5, 100, 160, 32), (7, 48, 1088, 64), (15, 31, 2944, 128), (16, 64, 4096, 64),
     (17, 65, 256, 128), (31, 20, 1056, 32), (32, 96, 512, 128), (33, 40, 704, 64), (64, 130, 1152, 128), (65, 18, 416, 32), (200, 24, 384, 128), (1, 5, 18432, 128),
+    # more than 8 MB of weights: tiles that share x, whole and in slices of K, a last chunk that is short
+    (3, 4096, 4224, 128), (4, 2049, 8224, 32), (5, 2100, 8320, 64), (16, 1100, 16512, 128), (20, 2048, 9280, 64), (33, 1030, 17152, 128), (64, 9000, 2208, 32),
 ]
 
 
@@ -58,7 +60,7 @@ def test_product(dev, M, N, K, group, zeros, dtype):
     check(y, x, q, s, z, f'{M}x{N}x{K}/{group}')
 
 
-@pytest.mark.parametrize('s_dtype', [bf16, f16, f32])
+@pytest.mark.parametrize('s_dtype', [bf16, f16])
 @pytest.mark.parametrize('dtype', [bf16, f16])
 def test_types_of_scales(dev, dtype, s_dtype):
     q, s, z = (t[0] for t in weights(1, 70, 320, 64, True, s_dtype))
@@ -70,7 +72,7 @@ def test_types_of_scales(dev, dtype, s_dtype):
 def test_every_code_of_every_place(dev, dtype):
     """One column of x at a time picks one code: the results are the weights themselves, exactly."""
     K = 160
-    q, s, z = (t[0] for t in weights(1, 48, K, 32, True, f32, seed=9))
+    q, s, z = (t[0] for t in weights(1, 48, K, 32, True, f16, seed=9))
     s = torch.full_like(s, 0.5)
     x = torch.eye(K).to(dtype)
     y = w4_gemm(*on(dev, x, q, s, z)).cpu().double()
@@ -126,6 +128,7 @@ def ranges(counts, gaps=0):
 @pytest.mark.parametrize('counts,gaps,N,K,group,zeros', [
     ([1], 0, 16, 128, 128, False), ([0, 3, 0, 1], 0, 40, 256, 64, True), ([5, 0, 0, 16, 17, 2, 0], 3, 33, 160, 32, True), ([40, 1, 70, 0], 0, 64, 384, 128, False),
     ([1] * 70 + [0] * 70 + [2] * 3, 0, 17, 128, 64, False), ([0, 0, 0], 2, 16, 128, 128, False), ([2] * 8, 1, 96, 2048, 128, True),
+    ([3, 0, 20, 1], 1, 1056, 8288, 32, True), ([40, 0, 9, 33, 12], 0, 1000, 4224, 64, False), ([1, 2, 1, 0, 0, 5, 1, 1], 2, 1025, 4480, 128, True),
 ])
 def test_product_by_expert(dev, counts, gaps, N, K, group, zeros, dtype):
     start, end, rows = ranges(counts, gaps)
@@ -154,7 +157,7 @@ def test_rows_of_no_expert_are_not_written_and_ranges_are_clamped(dev):
     check(y[11:], x[11:], q[2], s[2], None, 'last')
 
 
-@pytest.mark.parametrize('dtype', [bf16, f16, f32])
+@pytest.mark.parametrize('dtype', [bf16, f16])
 @pytest.mark.parametrize('group', [32, 64, 128])
 @pytest.mark.parametrize('zero_points', [False, True])
 @pytest.mark.parametrize('shape', [(1, 128), (7, 384), (3, 5, 256)])
