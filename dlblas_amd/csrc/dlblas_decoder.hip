@@ -32,6 +32,10 @@ void with_type(int dtype, F f) {
   else
     f(std::integral_constant<int, kInF32>());
 }
+template <typename F>
+void with_flag(bool flag, F f) {
+  flag ? f(std::true_type()) : f(std::false_type());
+}
 template <int... C, typename F>
 void with_chunks(int chunks, F f) {
   (void)((chunks == C && (f(std::integral_constant<int, C>()), true)) || ...);
@@ -71,7 +75,14 @@ int launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
   const RowShape shape = row_shape(a.H, 2);
   const dim3 grid(static_cast<unsigned>(a.rows)), block(shape.threads);
   with_type(dtype, [&](auto t) {
-    with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_kernel<t(), QUANT, c()>), grid, block, 0, st, a); });
+    with_flag(a.res != nullptr, [&](auto res) {
+      with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
+        if (QUANT || a.H % 8 == 0)
+          hipLaunchKernelGGL((rms_norm_kernel<t(), QUANT, res(), true, c()>), grid, block, 0, st, a);
+        else
+          hipLaunchKernelGGL((rms_norm_kernel<t(), false, res(), false, c()>), grid, block, 0, st, a);
+      });
+    });
   });
   return finish("rms_norm");
 }
@@ -223,13 +234,17 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
     const RowShape shape = row_shape(H, 1);
     const dim3 grid(blocks), block(shape.threads);
     with_type(dtype, [&](auto t) {
-      with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_backward_kernel<t(), c()>), grid, block, 0, st, a); });
+      with_flag(dsum != nullptr, [&](auto ds) {
+        with_flag(H % 8 == 0, [&](auto whole) {
+          with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_backward_kernel<t(), ds(), whole(), c()>), grid, block, 0, st, a); });
+        });
+      });
     });
     if (int rc = finish("rms_norm_backward")) return rc;
   }
   if (!dw) return DLB_OK;
   const NormDwArgs d{static_cast<const float*>(workspace), dw, blocks, static_cast<int>(H), weight_dtype};
-  hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(H, 64))), dim3(256), 0, st, d);
+  hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(H, 64))), dim3(64 * kDwWaves), 0, st, d);
   return finish("rms_norm_backward (dw)");
 }
 
@@ -300,10 +315,18 @@ int dlb_moe_permute(const void* x, int64_t x_row_stride, int dtype, const float*
   if (f8) a.xs = x_s, a.rows_s = rows_s, a.xs_s0 = xs_stride_m, a.xs_s1 = xs_stride_k, a.groups = static_cast<int>(H / kScaleBlock);
   a.x_stride = x_row_stride * esz, a.rows_stride = H * esz, a.T = tokens, a.R = num_rows;
   a.row_bytes = static_cast<int>(H * esz), a.esz = esz, a.topk = static_cast<int>(topk);
+  // a wave holds kSortCopyChunks KB of a row; parts down to one KB while there are fewer waves than the chip takes at once
   constexpr int kWaves = kSortCopyThreads / 64;
-  a.token_blocks = static_cast<int>(ceil_div(tokens, kWaves) < 4096 ? ceil_div(tokens, kWaves) : 4096);
+  const int64_t kbytes = ceil_div(a.row_bytes, 1024);
+  int64_t part = kSortCopyChunks;
+  while (part > 1 && tokens * ceil_div(kbytes, part) < 8192) part /= 2;
+  a.parts = static_cast<int>(ceil_div(kbytes, part)), a.part_bytes = static_cast<int>(part * 1024);
+  const int64_t units = ceil_div(tokens * a.parts, kWaves);
+  a.token_blocks = static_cast<int>(units < 16384 ? units : 16384);
   a.zero_blocks = static_cast<int>(ceil_div(num_rows, kWaves) < 1024 ? ceil_div(num_rows, kWaves) : 1024);
-  hipLaunchKernelGGL(moe_sort_copy_kernel, dim3(a.token_blocks + a.zero_blocks), dim3(kSortCopyThreads), 0, static_cast<hipStream_t>(stream), a);
+  with_flag(a.row_bytes % 16 == 0, [&](auto whole) {
+    hipLaunchKernelGGL(moe_sort_copy_kernel<whole()>, dim3(a.token_blocks + a.zero_blocks), dim3(kSortCopyThreads), 0, static_cast<hipStream_t>(stream), a);
+  });
   return finish("moe_permute");
 }
 
@@ -326,7 +349,9 @@ int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, cons
   int64_t parts = ceil_div(H, 512);
   if (parts > 64) parts = 64;
   const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(parts));
-  with_type(dtype, [&](auto t) { hipLaunchKernelGGL(moe_unpermute_kernel<t()>, grid, dim3(64), 0, static_cast<hipStream_t>(stream), a); });
+  with_type(dtype, [&](auto t) {
+    with_flag(H % 8 == 0, [&](auto whole) { hipLaunchKernelGGL((moe_unpermute_kernel<t(), whole()>), grid, dim3(64), 0, static_cast<hipStream_t>(stream), a); });
+  });
   return finish("moe_unpermute");
 }
 
@@ -356,9 +381,13 @@ int dlb_moe_unpermute_backward(const void* dout, int64_t dout_row_stride, const 
   const int64_t grid = tokens + a.zero_blocks;
   if (grid > (1ll << 31) - 1) return fail(DLB_ERR_BAD_SHAPE, "tokens=%lld beyond the supported range", (long long)tokens);
   with_type(dtype, [&](auto t) {
-    with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
-      hipLaunchKernelGGL((moe_unpermute_backward_kernel<t(), c()>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads), 0,
-                         static_cast<hipStream_t>(stream), a);
+    with_flag(dweights != nullptr, [&](auto dw) {
+      with_flag(H % 8 == 0, [&](auto whole) {
+        with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
+          hipLaunchKernelGGL((moe_unpermute_backward_kernel<t(), dw(), whole(), c()>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads), 0,
+                             static_cast<hipStream_t>(stream), a);
+        });
+      });
     });
   });
   return finish("moe_unpermute_backward");

@@ -25,15 +25,16 @@ constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWaves = kNormMaxThreads / 64;
 
 // Eight consecutive elements as they lie in memory (16 bytes, 32 of fp32); `left` (at least 1) = elements left in the row, those
-// past it are zero.
-template <int T>
+// past it are zero.  WHOLE: rows are a multiple of eight wide and there is no such case, nor the branch for it: waits for loads count
+// those issued since, and behind a branch the compiler takes the lower count, so that a row asked for ahead would be waited for at once.
+template <int T, bool WHOLE = false>
 __device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t elem, int left) {
   Raw8 r;
   r.a = v4i{0, 0, 0, 0}, r.b = v4i{0, 0, 0, 0};
   if (T == kInF32) {
     typedef v4i v4i_f32 __attribute__((aligned(4)));
     const float* q = static_cast<const float*>(p) + elem;
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
       r.a = reinterpret_cast<const v4i_f32*>(q)[0], r.b = reinterpret_cast<const v4i_f32*>(q)[1];
     } else {
 #pragma unroll
@@ -44,7 +45,7 @@ __device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t elem, int left)
     }
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(p) + elem;
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
       r.a = *reinterpret_cast<const v4i_el*>(q);
     } else {
 #pragma unroll
@@ -76,12 +77,12 @@ __device__ __forceinline__ Raw8 pack_raw8(const float (&v)[8]) {
   return r;
 }
 
-template <int T>
+template <int T, bool WHOLE = false>
 __device__ __forceinline__ void store_raw8(void* p, int64_t elem, const Raw8& r, int left) {
   if (T == kInF32) {
     typedef v4i v4i_f32 __attribute__((aligned(4)));
     float* q = static_cast<float*>(p) + elem;
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
       reinterpret_cast<v4i_f32*>(q)[0] = r.a, reinterpret_cast<v4i_f32*>(q)[1] = r.b;
     } else {
 #pragma unroll
@@ -92,7 +93,7 @@ __device__ __forceinline__ void store_raw8(void* p, int64_t elem, const Raw8& r,
     }
   } else {
     uint16_t* q = static_cast<uint16_t*>(p) + elem;
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
       *reinterpret_cast<v4i_el*>(q) = r.a;
     } else {
 #pragma unroll
@@ -106,6 +107,13 @@ __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
   return v;
+}
+
+// A barrier for what went through LDS; loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 struct NormArgs {
@@ -122,55 +130,50 @@ struct NormArgs {
   float eps, qeps;
 };
 
-template <int T>
+template <int T, bool WHOLE>
 __device__ __forceinline__ void load_weight8(const void* w, int w_f32, int col, int left, float (&v)[8]) {
   if (w_f32)
-    quant_unpack8<kInF32>(load_raw8<kInF32>(w, col, left), v);
+    quant_unpack8<kInF32>(load_raw8<kInF32, WHOLE>(w, col, left), v);
   else
-    quant_unpack8<T>(load_raw8<T>(w, col, left), v);
+    quant_unpack8<T>(load_raw8<T, WHOLE>(w, col, left), v);
 }
 
-// One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each.
-template <int T, bool QUANT, int CH>
+// One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each; a thread past the last chunk reads that one
+// again and leaves no trace.
+template <int T, bool QUANT, bool RES, bool WHOLE, int CH>
 __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArgs p) {
   __shared__ float part[kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int64_t row = blockIdx.x;
   const int chunks = (p.H + 7) / 8;
-  Raw8 h[CH];
+  int at[CH];
+  Raw8 h[CH], res[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int i = c * threads + tid;
-    if (i < chunks) h[c] = load_raw8<T>(p.x, row * p.x_rs + 8 * i, p.H - 8 * i);
+    at[c] = min(c * threads + tid, chunks - 1);
+    h[c] = load_raw8<T, WHOLE>(p.x, row * p.x_rs + 8 * at[c], p.H - 8 * at[c]);
+    if (RES) res[c] = load_raw8<T, WHOLE>(p.res, row * p.res_rs + 8 * at[c], p.H - 8 * at[c]);
   }
-  if (p.res) {
-    Raw8 res[CH];
+  if (RES) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = c * threads + tid;
-      if (i < chunks) res[c] = load_raw8<T>(p.res, row * p.res_rs + 8 * i, p.H - 8 * i);
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int i = c * threads + tid;
-      if (i >= chunks) continue;
       float a[8], b[8];
       quant_unpack8<T>(h[c], a);
       quant_unpack8<T>(res[c], b);
 #pragma unroll
       for (int k = 0; k < 8; ++k) a[k] += b[k];
       h[c] = pack_raw8<T>(a);
-      store_raw8<T>(p.sum, row * p.sum_rs + 8 * i, h[c], p.H - 8 * i);
+      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.sum, row * p.sum_rs + 8 * at[c], h[c], p.H - 8 * at[c]);
     }
   }
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    if (c * threads + tid >= chunks) continue;
-    float v[8];
+    float v[8], s = 0.f;
     quant_unpack8<T>(h[c], v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fmaf(v[k], v[k], ss);
+    for (int k = 0; k < 8; ++k) s = fmaf(v[k], v[k], s);
+    ss += c * threads + tid < chunks ? s : 0.f;
   }
   ss = wave_sum(ss);
   if (threads > 64) {
@@ -186,11 +189,11 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
     if (i >= chunks) continue;  // whole groups of 16 lanes: a quantised row is a multiple of 128 wide
     float v[8], w[8];
     quant_unpack8<T>(h[c], v);
-    load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+    load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = v[k] * r * w[k];
     if (!QUANT) {
-      store_raw8<T>(p.y, row * p.y_rs + 8 * i, pack_raw8<T>(v), p.H - 8 * i);
+      store_raw8<T, WHOLE>(p.y, row * p.y_rs + 8 * i, pack_raw8<T>(v), p.H - 8 * i);
       continue;
     }
     // the largest value by the bits of |y|, which puts NaN above infinity: a group that holds one gets a scale that shows it
@@ -230,48 +233,62 @@ struct NormGradArgs {
 };
 
 // A workgroup takes rows blockIdx, blockIdx + gridDim, ... and keeps its share of dw in registers; the shares of all workgroups are
-// added by rms_norm_dw_kernel in workgroup order, so the gradient is the same in every run.
-template <int T, int CH>
+// added by rms_norm_dw_kernel in a fixed order, so the gradient is the same in every run.  The next row is on its way while the sums of
+// this one cross the workgroup, where a row of two chunks a thread leaves the registers for it.  Threads past the last chunk as above.
+template <int T, bool DSUM, bool WHOLE, int CH>
 __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(const NormGradArgs p) {
+  constexpr bool kAhead = CH == 1 || (CH == 2 && T != kInF32);
   __shared__ float part[2][2][kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int chunks = (p.H + 7) / 8;
   float dw[CH][8];
+  int at[CH];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    at[c] = min(c * threads + tid, chunks - 1);
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[c][k] = 0.f;
-  int turn = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+  }
+  struct Row {
     Raw8 dy[CH], h[CH], ds[CH];
+  };
+  auto load = [&](int64_t row, Row& r) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = c * threads + tid;
-      if (i >= chunks) continue;
-      h[c] = load_raw8<T>(p.h, row * p.h_rs + 8 * i, p.H - 8 * i);
-      dy[c] = load_raw8<T>(p.dy, row * p.dy_rs + 8 * i, p.H - 8 * i);
-      if (p.dsum) ds[c] = load_raw8<T>(p.dsum, row * p.dsum_rs + 8 * i, p.H - 8 * i);
+      const int col = 8 * at[c];
+      r.h[c] = load_raw8<T, WHOLE>(p.h, row * p.h_rs + col, p.H - col);
+      r.dy[c] = load_raw8<T, WHOLE>(p.dy, row * p.dy_rs + col, p.H - col);
+      if (DSUM) r.ds[c] = load_raw8<T, WHOLE>(p.dsum, row * p.dsum_rs + col, p.H - col);
     }
+  };
+  Row now, next;
+  if (kAhead) load(blockIdx.x, now);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    if (kAhead)
+      load(min(row + gridDim.x, p.rows - 1), next);  // behind the last row that one again
+    else
+      load(row, now);
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = c * threads + tid;
-      if (i >= chunks) continue;
-      float hv[8], g[8], w[8];
-      quant_unpack8<T>(h[c], hv);
-      quant_unpack8<T>(dy[c], g);
-      load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+      float hv[8], g[8], w[8], s = 0.f, d = 0.f;
+      quant_unpack8<T>(now.h[c], hv);
+      quant_unpack8<T>(now.dy[c], g);
+      load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        ss = fmaf(hv[k], hv[k], ss);
-        dot = fmaf(g[k] * w[k], hv[k], dot);
+        s = fmaf(hv[k], hv[k], s);
+        d = fmaf(g[k] * w[k], hv[k], d);
       }
+      const bool live = c * threads + tid < chunks;
+      ss += live ? s : 0.f, dot += live ? d : 0.f;
     }
     ss = wave_sum(ss), dot = wave_sum(dot);
     if (threads > 64) {
       // two sets of sums in turn: a wave may be one row ahead of the others, never two
       if ((tid & 63) == 0) part[turn][0][tid >> 6] = ss, part[turn][1][tid >> 6] = dot;
-      __syncthreads();
+      lds_barrier();
       ss = dot = 0.f;
       for (int i = 0; i < threads / 64; ++i) ss += part[turn][0][i], dot += part[turn][1][i];
     }
@@ -279,63 +296,64 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
     const float along = r * r * dot / static_cast<float>(p.H);  // dh = r (w dy - h along)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = c * threads + tid;
-      if (i >= chunks) continue;
       float hv[8], g[8], w[8];
-      quant_unpack8<T>(h[c], hv);
-      quant_unpack8<T>(dy[c], g);
-      load_weight8<T>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+      quant_unpack8<T>(now.h[c], hv);
+      quant_unpack8<T>(now.dy[c], g);
+      load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         dw[c][k] = fmaf(g[k], hv[k] * r, dw[c][k]);
         g[k] = r * (g[k] * w[k] - hv[k] * along);
       }
-      if (p.dsum) {
+      if (DSUM) {
         float d[8];
-        quant_unpack8<T>(ds[c], d);
+        quant_unpack8<T>(now.ds[c], d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[k] += d[k];
       }
-      store_raw8<T>(p.dx, row * p.dx_rs + 8 * i, pack_raw8<T>(g), p.H - 8 * i);
+      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.dx, row * p.dx_rs + 8 * at[c], pack_raw8<T>(g), p.H - 8 * at[c]);
     }
+    if (kAhead) now = next;
   }
   if (!p.dw_part) return;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = c * threads + tid;
-    if (i < chunks) store_raw8<kInF32>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H + 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
+    if (i < chunks) store_raw8<kInF32, WHOLE>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H + 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
   }
 }
 
-// dw[col] = sum over the parts, in order within each of the four waves and then over the waves.
+// dw[col] = sum over the parts: a wave adds every kDwWaves-th, eight sums at a time, and the waves' sums are added in pairs.
 struct NormDwArgs {
   const float* part;
   void* dw;
   int parts, H, dw_type;
 };
+constexpr int kDwWaves = 16;
 
-__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const NormDwArgs p) {
-  __shared__ float sums[4][64];
+__global__ void __launch_bounds__(64 * kDwWaves) rms_norm_dw_kernel(const NormDwArgs p) {
+  __shared__ float sums[kDwWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (col < p.H) {
-    const int per = (p.parts + 3) / 4;
-    const int b1 = min(p.parts, (wave + 1) * per);
-    int b = wave * per;
-    for (; b + 8 <= b1; b += 8) {
-      float v[8];
+  float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = p.part[static_cast<int64_t>(b + u) * p.H + col];
+  for (int u = 0; u < 8; ++u) v[u] = 0.f;
+  const float* const mine = p.part + min(col, p.H - 1);
+  for (int b = wave; b < p.parts; b += 8 * kDwWaves) {
+    float e[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
-    }
-    for (; b < b1; ++b) s += p.part[static_cast<int64_t>(b) * p.H + col];
+    for (int u = 0; u < 8; ++u) e[u] = mine[static_cast<int64_t>(min(b + u * kDwWaves, p.parts - 1)) * p.H];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] += b + u * kDwWaves < p.parts ? e[u] : 0.f;
   }
-  sums[wave][lane] = s;
+  sums[wave][lane] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
   __syncthreads();
   if (wave != 0 || col >= p.H) return;
-  s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+#pragma unroll
+  for (int n = kDwWaves / 2; n >= 1; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) sums[i][lane] += sums[i + n][lane];
+  const float s = sums[0][lane];
   if (p.dw_type == kInF32)
     static_cast<float*>(p.dw)[col] = s;
   else if (p.dw_type == kInBf16)

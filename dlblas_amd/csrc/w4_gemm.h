@@ -96,13 +96,6 @@ __device__ __forceinline__ int nth_expert(const W4Args& p, int which, int lane) 
   return -1;
 }
 
-// A barrier for what went through LDS; loads from memory stay on their way.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <int N>
 __device__ __forceinline__ void spread_quarters(int v, int (&out)[N]) {
   float f[N];
