@@ -276,9 +276,8 @@ __global__ void __launch_bounds__(64) moe_unpermute_kernel(const UnpermuteArgs p
   const float my_w = lane < p.topk && p.w ? p.w[t * p.topk + lane] : 1.f;
   const uint64_t there = __ballot(mine >= 0);
   const int chunks = (p.H + 7) / 8;
-  for (int64_t c0 = static_cast<int64_t>(blockIdx.y) * 64; c0 < chunks; c0 += static_cast<int64_t>(gridDim.y) * 64) {
-    const int64_t col = min(c0 + lane, static_cast<int64_t>(chunks - 1)) * 8;
-    const int left = static_cast<int>(p.H - col);
+  for (int c0 = blockIdx.y * 64; c0 < chunks; c0 += gridDim.y * 64) {
+    const int col = min(c0 + lane, chunks - 1) * 8, left = p.H - col;
     float acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
@@ -293,7 +292,7 @@ __global__ void __launch_bounds__(64) moe_unpermute_kernel(const UnpermuteArgs p
         todo &= todo - 1;
         const int64_t row = __builtin_amdgcn_readlane(mine, j);
         wj[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_w), j));
-        raw[u] = load_raw8<T, WHOLE>(p.rows, row * p.rows_rs + col, left);
+        raw[u] = load_raw8<T, WHOLE>(p.rows, row * p.rows_rs, col, left);
       }
 #pragma unroll
       for (int u = 0; u < kUnpermuteRows; ++u) {
@@ -304,7 +303,7 @@ __global__ void __launch_bounds__(64) moe_unpermute_kernel(const UnpermuteArgs p
         for (int k = 0; k < 8; ++k) acc[k] = fmaf(v[k], wj[u], acc[k]);
       }
     }
-    if (c0 + lane < chunks) store_raw8<T, WHOLE>(p.out, t * p.out_rs + col, pack_raw8<T>(acc), left);
+    if (c0 + lane < chunks) store_raw8<T, WHOLE>(p.out, t * p.out_rs, col, pack_raw8<T>(acc), left);
   }
 }
 
@@ -335,7 +334,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel
     zero.a = v4i{0, 0, 0, 0}, zero.b = v4i{0, 0, 0, 0};
     for (int64_t r = static_cast<int64_t>(blockIdx.x) - p.T; r < p.R; r += p.zero_blocks) {
       if (p.source[r] >= 0) continue;
-      for (int i = tid; i < chunks; i += threads) store_raw8<T, WHOLE>(p.drows, r * p.drows_rs + 8 * i, zero, p.H - 8 * i);
+      for (int i = tid; i < chunks; i += threads) store_raw8<T, WHOLE>(p.drows, r * p.drows_rs, 8 * i, zero, p.H - 8 * i);
     }
     return;
   }
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     at[c] = min(c * threads + tid, chunks - 1);
-    g[c] = load_raw8<T, WHOLE>(p.dout, t * p.dout_rs + 8 * at[c], p.H - 8 * at[c]);
+    g[c] = load_raw8<T, WHOLE>(p.dout, t * p.dout_rs, 8 * at[c], p.H - 8 * at[c]);
   }
   constexpr int kAhead = CH == 1 ? 4 : 2;
   for (int j0 = 0; j0 < p.topk; j0 += kAhead) {
@@ -363,7 +362,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel
       if (row[u] >= p.R) row[u] = -1;
       if (!DW) continue;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) raw[u][c] = load_raw8<T, WHOLE>(p.rows, max(row[u], int64_t{0}) * p.rows_rs + 8 * at[c], p.H - 8 * at[c]);
+      for (int c = 0; c < CH; ++c) raw[u][c] = load_raw8<T, WHOLE>(p.rows, max(row[u], int64_t{0}) * p.rows_rs, 8 * at[c], p.H - 8 * at[c]);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel
           }
 #pragma unroll
           for (int k = 0; k < 8; ++k) d[k] *= wj;
-          store_raw8<T, WHOLE>(p.drows, row[u] * p.drows_rs + 8 * at[c], pack_raw8<T>(d), p.H - 8 * at[c]);
+          store_raw8<T, WHOLE>(p.drows, row[u] * p.drows_rs, 8 * at[c], pack_raw8<T>(d), p.H - 8 * at[c]);
         }
       }
       if (DW) {

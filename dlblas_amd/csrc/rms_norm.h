@@ -24,16 +24,23 @@ typedef v4h v4h_el __attribute__((aligned(2)));
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWaves = kNormMaxThreads / 64;
 
-// Eight consecutive elements as they lie in memory (16 bytes, 32 of fp32); `left` (at least 1) = elements left in the row, those
+// Where column `col` of the row at element `row` lies: the row's start is the same in every lane, which leaves 32 bits a lane to keep.
+template <int T>
+__device__ __forceinline__ const char* raw8_at(const void* p, int64_t row, int col) {
+  constexpr int kBytes = T == kInF32 ? 4 : 2;
+  return static_cast<const char*>(p) + row * kBytes + static_cast<uint32_t>(col) * kBytes;
+}
+
+// Eight consecutive elements of a row as they lie in memory (16 bytes, 32 of fp32); `left` (at least 1) = elements left in the row, those
 // past it are zero.  WHOLE: rows are a multiple of eight wide and there is no such case, nor the branch for it: waits for loads count
 // those issued since, and behind a branch the compiler takes the lower count, so that a row asked for ahead would be waited for at once.
 template <int T, bool WHOLE = false>
-__device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t elem, int left) {
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t row, int col, int left) {
   Raw8 r;
   r.a = v4i{0, 0, 0, 0}, r.b = v4i{0, 0, 0, 0};
   if (T == kInF32) {
     typedef v4i v4i_f32 __attribute__((aligned(4)));
-    const float* q = static_cast<const float*>(p) + elem;
+    const float* q = reinterpret_cast<const float*>(raw8_at<T>(p, row, col));
     if (WHOLE || left >= 8) {
       r.a = reinterpret_cast<const v4i_f32*>(q)[0], r.b = reinterpret_cast<const v4i_f32*>(q)[1];
     } else {
@@ -44,7 +51,7 @@ __device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t elem, int left)
       }
     }
   } else {
-    const uint16_t* q = static_cast<const uint16_t*>(p) + elem;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(raw8_at<T>(p, row, col));
     if (WHOLE || left >= 8) {
       r.a = *reinterpret_cast<const v4i_el*>(q);
     } else {
@@ -78,10 +85,10 @@ __device__ __forceinline__ Raw8 pack_raw8(const float (&v)[8]) {
 }
 
 template <int T, bool WHOLE = false>
-__device__ __forceinline__ void store_raw8(void* p, int64_t elem, const Raw8& r, int left) {
+__device__ __forceinline__ void store_raw8(void* p, int64_t row, int col, const Raw8& r, int left) {
   if (T == kInF32) {
     typedef v4i v4i_f32 __attribute__((aligned(4)));
-    float* q = static_cast<float*>(p) + elem;
+    float* q = reinterpret_cast<float*>(const_cast<char*>(raw8_at<T>(p, row, col)));
     if (WHOLE || left >= 8) {
       reinterpret_cast<v4i_f32*>(q)[0] = r.a, reinterpret_cast<v4i_f32*>(q)[1] = r.b;
     } else {
@@ -92,7 +99,7 @@ __device__ __forceinline__ void store_raw8(void* p, int64_t elem, const Raw8& r,
       }
     }
   } else {
-    uint16_t* q = static_cast<uint16_t*>(p) + elem;
+    uint16_t* q = reinterpret_cast<uint16_t*>(const_cast<char*>(raw8_at<T>(p, row, col)));
     if (WHOLE || left >= 8) {
       *reinterpret_cast<v4i_el*>(q) = r.a;
     } else {
@@ -133,9 +140,9 @@ struct NormArgs {
 template <int T, bool WHOLE>
 __device__ __forceinline__ void load_weight8(const void* w, int w_f32, int col, int left, float (&v)[8]) {
   if (w_f32)
-    quant_unpack8<kInF32>(load_raw8<kInF32, WHOLE>(w, col, left), v);
+    quant_unpack8<kInF32>(load_raw8<kInF32, WHOLE>(w, 0, col, left), v);
   else
-    quant_unpack8<T>(load_raw8<T, WHOLE>(w, col, left), v);
+    quant_unpack8<T>(load_raw8<T, WHOLE>(w, 0, col, left), v);
 }
 
 // One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each; a thread past the last chunk reads that one
@@ -151,8 +158,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     at[c] = min(c * threads + tid, chunks - 1);
-    h[c] = load_raw8<T, WHOLE>(p.x, row * p.x_rs + 8 * at[c], p.H - 8 * at[c]);
-    if (RES) res[c] = load_raw8<T, WHOLE>(p.res, row * p.res_rs + 8 * at[c], p.H - 8 * at[c]);
+    h[c] = load_raw8<T, WHOLE>(p.x, row * p.x_rs, 8 * at[c], p.H - 8 * at[c]);
+    if (RES) res[c] = load_raw8<T, WHOLE>(p.res, row * p.res_rs, 8 * at[c], p.H - 8 * at[c]);
   }
   if (RES) {
 #pragma unroll
@@ -163,7 +170,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
 #pragma unroll
       for (int k = 0; k < 8; ++k) a[k] += b[k];
       h[c] = pack_raw8<T>(a);
-      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.sum, row * p.sum_rs + 8 * at[c], h[c], p.H - 8 * at[c]);
+      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.sum, row * p.sum_rs, 8 * at[c], h[c], p.H - 8 * at[c]);
     }
   }
   float ss = 0.f;
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = v[k] * r * w[k];
     if (!QUANT) {
-      store_raw8<T, WHOLE>(p.y, row * p.y_rs + 8 * i, pack_raw8<T>(v), p.H - 8 * i);
+      store_raw8<T, WHOLE>(p.y, row * p.y_rs, 8 * i, pack_raw8<T>(v), p.H - 8 * i);
       continue;
     }
     // the largest value by the bits of |y|, which puts NaN above infinity: a group that holds one gets a scale that shows it
@@ -256,9 +263,9 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = 8 * at[c];
-      r.h[c] = load_raw8<T, WHOLE>(p.h, row * p.h_rs + col, p.H - col);
-      r.dy[c] = load_raw8<T, WHOLE>(p.dy, row * p.dy_rs + col, p.H - col);
-      if (DSUM) r.ds[c] = load_raw8<T, WHOLE>(p.dsum, row * p.dsum_rs + col, p.H - col);
+      r.h[c] = load_raw8<T, WHOLE>(p.h, row * p.h_rs, col, p.H - col);
+      r.dy[c] = load_raw8<T, WHOLE>(p.dy, row * p.dy_rs, col, p.H - col);
+      if (DSUM && CH < 4) r.ds[c] = load_raw8<T, WHOLE>(p.dsum, row * p.dsum_rs, col, p.H - col);
     }
   };
   Row now, next;
@@ -283,6 +290,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
       }
       const bool live = c * threads + tid < chunks;
       ss += live ? s : 0.f, dot += live ? d : 0.f;
+      if (CH == 4) __builtin_amdgcn_sched_barrier(0);  // four chunks fill the registers: one chunk's weights at a time
     }
     ss = wave_sum(ss), dot = wave_sum(dot);
     if (threads > 64) {
@@ -307,11 +315,13 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
       }
       if (DSUM) {
         float d[8];
+        if (CH == 4) now.ds[c] = load_raw8<T, WHOLE>(p.dsum, row * p.dsum_rs, 8 * at[c], p.H - 8 * at[c]);
         quant_unpack8<T>(now.ds[c], d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[k] += d[k];
       }
-      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.dx, row * p.dx_rs + 8 * at[c], pack_raw8<T>(g), p.H - 8 * at[c]);
+      if (c * threads + tid < chunks) store_raw8<T, WHOLE>(p.dx, row * p.dx_rs, 8 * at[c], pack_raw8<T>(g), p.H - 8 * at[c]);
+      if (CH == 4) __builtin_amdgcn_sched_barrier(0);
     }
     if (kAhead) now = next;
   }
@@ -319,7 +329,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = c * threads + tid;
-    if (i < chunks) store_raw8<kInF32, WHOLE>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H + 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
+    if (i < chunks) store_raw8<kInF32, WHOLE>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H, 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
   }
 }
 

@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const W4QuantArgs p) {
   for (int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / lanes; g < total; g += step) {
     const int64_t row = g / p.G, kg = g - row * p.G;
     float v[8];
-    quant_unpack8<T>(load_raw8<T>(p.w, row * p.w_rs + kg * p.group + 8 * sub, 8), v);
+    quant_unpack8<T>(load_raw8<T, true>(p.w, row * p.w_rs, static_cast<int>(kg * p.group) + 8 * sub, 8), v);
     float hi = 0.f, lo = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) hi = fmaxf(hi, v[i]), lo = fminf(lo, v[i]);
