@@ -46,24 +46,17 @@ def rms_norm_backward(dy, dsum, h, weight, dx, dw, eps):
                                         IN_CODES[weight.dtype], _ptr(dx), _rs(dx), _ptr(dw), rows, H, float(eps), _ptr(ws), need, _stream(h)))
 
 
-def moe_sort(ids, row_index, source, m_indices, row_start, row_end, alignment):
-    _require_gpu(ids, row_index, source, m_indices, row_start, row_end)
-    lib = load()
-    with torch.cuda.device(ids.device):
-        T, topk = ids.shape
-        E = row_start.numel()
-        need = lib.dlb_moe_sort_workspace_bytes(T, topk, E)
-        ws = torch.empty(need, dtype=torch.uint8, device=ids.device)
-        check(lib.dlb_moe_sort(_ptr(ids), IDX_CODES[ids.dtype], ids.stride(0), ids.stride(1), _ptr(row_index), _ptr(source), _ptr(m_indices),
-                               _ptr(row_start), _ptr(row_end), T, topk, E, alignment, source.numel(), _ptr(ws), need, _stream(ids)))
-
-
-def moe_permute(x, x_s, rows, rows_s, row_index, source):
-    _require_gpu(*_present(x, x_s, rows, rows_s, row_index, source))
+def moe_permute(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s, alignment):
+    _require_gpu(*_present(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s))
     code = ROWS_E4M3 if x.dtype == torch.float8_e4m3fn else IN_CODES[x.dtype]
+    lib = load()
     with torch.cuda.device(x.device):
-        check(load().dlb_moe_permute(_ptr(x), _rs(x), code, _ptr(x_s), _rs(x_s), 0 if x_s is None else x_s.stride(1), _ptr(rows), _ptr(rows_s),
-                                     _ptr(row_index), _ptr(source), x.size(0), x.size(1), row_index.size(1), rows.size(0), _stream(x)))
+        (T, topk), E = ids.shape, row_start.numel()
+        need = lib.dlb_moe_permute_workspace_bytes(T, topk, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        check(lib.dlb_moe_permute(_ptr(ids), IDX_CODES[ids.dtype], ids.stride(0), ids.stride(1), _ptr(x), _rs(x), code, _ptr(x_s), _rs(x_s),
+                                  0 if x_s is None else x_s.stride(1), _ptr(row_index), _ptr(source), _ptr(m_indices), _ptr(row_start), _ptr(row_end),
+                                  _ptr(rows), _ptr(rows_s), T, x.size(1), topk, E, alignment, source.numel(), _ptr(ws), need, _stream(x)))
 
 
 def moe_unpermute(rows, row_index, weights, out):

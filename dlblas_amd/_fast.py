@@ -19,7 +19,7 @@ _ABI = ('dlb_last_error', 'dlb_workspace_lock', 'dlb_workspace_unlock', 'dlb_fp8
 _FUNCTIONS = ('fp8_gemm', 'quant', 'grouped_contiguous', 'grouped_masked', 'low_latency_experts', 'ep_gather', 'fused_moe_v3')
 
 # the same for the StepAbi struct and the functions of csrc/host_steps.cpp
-_STEP_ABI = ('dlb_last_error', 'dlb_rms_norm_backward_workspace_bytes', 'dlb_rms_norm_backward', 'dlb_moe_unpermute_backward', 'dlb_rms_norm', 'dlb_rms_norm_quant', 'dlb_moe_sort_workspace_bytes', 'dlb_moe_sort', 'dlb_moe_permute', 'dlb_moe_unpermute', 'dlb_w4_gemm_workspace_bytes',
+_STEP_ABI = ('dlb_last_error', 'dlb_rms_norm_backward_workspace_bytes', 'dlb_rms_norm_backward', 'dlb_moe_unpermute_backward', 'dlb_rms_norm', 'dlb_rms_norm_quant', 'dlb_moe_permute_workspace_bytes', 'dlb_moe_permute', 'dlb_moe_unpermute', 'dlb_w4_gemm_workspace_bytes',
              'dlb_w4_gemm')
 _STEP_FUNCTIONS = ('rms_norm', 'rms_norm_quant', 'moe_permute', 'moe_unpermute', 'w4_gemm', 'w4_gemm_grouped')
 

@@ -2,6 +2,7 @@
 // The declarations and the contract of every entry point are in include/dlblas_decoder.h.
 #include "../../include/dlblas_decoder.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #include "host_common.h"
@@ -250,86 +251,95 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
   return finish("rms_norm_backward (dw)");
 }
 
-size_t dlb_moe_sort_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts) {
+size_t dlb_moe_permute_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts) {
   if (tokens <= 0 || topk <= 0 || experts <= 0) return 0;
   const int64_t blocks = dlb::sort_blocks(tokens * topk);
   return blocks > 1 ? static_cast<size_t>(blocks) * experts * sizeof(int32_t) : 0;
 }
 
-int dlb_moe_sort(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, int32_t* row_index, int32_t* source,
-                 int32_t* m_indices, int32_t* row_start, int32_t* row_end, int64_t tokens, int64_t topk, int64_t experts,
-                 int64_t alignment, int64_t num_rows, void* workspace, size_t workspace_bytes, void* stream) {
+int dlb_moe_permute(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, const void* x, int64_t x_row_stride,
+                    int dtype, const float* x_s, int64_t xs_stride_m, int64_t xs_stride_k, int32_t* row_index, int32_t* source,
+                    int32_t* m_indices, int32_t* row_start, int32_t* row_end, void* rows, float* rows_s, int64_t tokens, int64_t H,
+                    int64_t topk, int64_t experts, int64_t alignment, int64_t num_rows, void* workspace, size_t workspace_bytes,
+                    void* stream) {
   using namespace dlb;
   clear_error();
+  const bool f8 = dtype == DLB_ROWS_E4M3;
   if (ids_dtype != DLB_IDX_I32 && ids_dtype != DLB_IDX_I64) return fail(DLB_ERR_BAD_DTYPE, "ids_dtype %d is not DLB_IDX_I32 / I64", ids_dtype);
-  if (int rc = check_rows(tokens, 0, topk, num_rows)) return rc;
+  if (!f8 && bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32 / DLB_ROWS_E4M3", dtype);
+  if (int rc = check_rows(tokens, H, topk, num_rows)) return rc;
+  if (f8 && H % kScaleBlock != 0) return fail(DLB_ERR_BAD_SHAPE, "H=%lld is not a multiple of 128", (long long)H);
   if (experts < 1 || experts > kSortMaxExperts) return fail(DLB_ERR_BAD_SHAPE, "experts=%lld is not 1 ... %d", (long long)experts, kSortMaxExperts);
   if (alignment < 1 || alignment > (1 << 20)) return fail(DLB_ERR_BAD_SHAPE, "alignment=%lld is not 1 ... 2^20", (long long)alignment);
-  if (ids_stride_m < 0 || ids_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride of ids");
+  if (ids_stride_m < 0 || ids_stride_k < 0 || x_row_stride < 0 || xs_stride_m < 0 || xs_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride");
   if ((tokens > 0 && (!ids || !row_index)) || (num_rows > 0 && (!source || !m_indices)) || !row_start || !row_end)
     return fail(DLB_ERR_NULL_POINTER, "ids or a table is NULL");
   if (misaligned(ids, ids_dtype == DLB_IDX_I64 ? 8 : 4) || misaligned(row_index, 4) || misaligned(source, 4) || misaligned(m_indices, 4) ||
       misaligned(row_start, 4) || misaligned(row_end, 4))
     return fail(DLB_ERR_ALIGNMENT, "ids or a table is not aligned to its elements");
-  const size_t need = dlb_moe_sort_workspace_bytes(tokens, topk, experts);
+  const bool copies = num_rows > 0 && H > 0;
+  if (copies && (!rows || (tokens > 0 && !x))) return fail(DLB_ERR_NULL_POINTER, "x or rows is NULL");
+  if (copies && f8 && (!rows_s || (tokens > 0 && !x_s))) return fail(DLB_ERR_NULL_POINTER, "e4m3 rows without their scales");
+  if (f8 ? misaligned(x, 16) || misaligned(rows, 16) || x_row_stride % 16 != 0 || misaligned(x_s, 4) || misaligned(rows_s, 4)
+         : off_elements(x, dtype) || off_elements(rows, dtype))
+    return fail(DLB_ERR_ALIGNMENT, "x or rows is not aligned to its elements, or e4m3 rows not to 16 bytes");
+  const size_t need = dlb_moe_permute_workspace_bytes(tokens, topk, experts);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
   if (need > 0 && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+
   SortArgs a{};
   a.ids = ids, a.row_index = row_index, a.source = source, a.m_indices = m_indices, a.row_start = row_start, a.row_end = row_end;
   a.hist = static_cast<int32_t*>(workspace);
   a.ids_s0 = ids_stride_m, a.ids_s1 = ids_stride_k, a.n = tokens * topk, a.R = num_rows;
   a.ids_is64 = ids_dtype == DLB_IDX_I64, a.E = static_cast<int>(experts), a.topk = static_cast<int>(topk), a.align = static_cast<int>(alignment);
+  SortCopyArgs c{};
+  if (copies) {
+    const int esz = f8 ? 1 : static_cast<int>(size_of(dtype));
+    c.x = static_cast<const char*>(x), c.rows = static_cast<char*>(rows), c.row_index = row_index, c.source = source;
+    if (f8) c.xs = x_s, c.rows_s = rows_s, c.xs_s0 = xs_stride_m, c.xs_s1 = xs_stride_k, c.groups = static_cast<int>(H / kScaleBlock);
+    c.x_stride = x_row_stride * esz, c.rows_stride = H * esz, c.T = tokens, c.R = num_rows;
+    c.row_bytes = static_cast<int>(H * esz), c.esz = esz, c.topk = static_cast<int>(topk);
+    // a wave holds kSortCopyChunks KB of a row; parts down to one KB while there are fewer waves than the chip takes at once
+    const int64_t kbytes = ceil_div(c.row_bytes, 1024);
+    int64_t part = kSortCopyChunks;
+    while (part > 1 && tokens * ceil_div(kbytes, part) < 8192) part /= 2;
+    c.parts = static_cast<int>(ceil_div(kbytes, part)), c.part_bytes = static_cast<int>(part * 1024);
+  }
+  const bool whole_rows = c.row_bytes % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const size_t lds = (static_cast<size_t>(3) * a.E + 1) * sizeof(int) + static_cast<size_t>(16) * a.E * sizeof(uint16_t);
+
+  if (copies && a.n <= kSortBlockSlots) {
+    // 1024 slots, as many as one workgroup finds the rows of: one launch, 512 x 2 slots x 4096 bf16 6.6 us, 128 x 8 x 7168 among 256 experts
+    // 10.7, 16 x 8 x 7168 among 32 5.2.  One token more, in three launches: 513 x 2 10.0 us, 129 x 8 13.6.
+    const int threads = a.n <= 256 ? 256 : kSortThreads;
+    const int64_t want = ceil_div(std::max(tokens * c.parts, num_rows), threads / 64), most = 512 * (kSortThreads / threads);
+    const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+    with_flag(whole_rows, [&](auto whole) {
+      hipLaunchKernelGGL((moe_sort_rows_kernel<true, whole()>), grid, dim3(threads), lds + threads * sizeof(int), st, a, 1, c);
+    });
+    return finish("moe_permute");
+  }
   const int64_t blocks = sort_blocks(a.n);
   if (blocks > 1) {
     hipLaunchKernelGGL(moe_sort_count_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), static_cast<size_t>(a.E) * sizeof(int), st, a);
-    if (int rc = finish("moe_sort (count)")) return rc;
+    if (int rc = finish("moe_permute (count)")) return rc;
   }
   // further workgroups where the tables by row are longer than those by slot
   int64_t grid = ceil_div(num_rows, 4 * kSortThreads);
   if (grid > 256) grid = 256;
   if (grid < blocks) grid = blocks;
-  const size_t lds = (static_cast<size_t>(3) * a.E + 1) * sizeof(int) + static_cast<size_t>(16) * a.E * sizeof(uint16_t);
-  hipLaunchKernelGGL(moe_sort_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(kSortThreads), lds, st, a, static_cast<int>(blocks));
-  return finish("moe_sort");
-}
-
-int dlb_moe_permute(const void* x, int64_t x_row_stride, int dtype, const float* x_s, int64_t xs_stride_m, int64_t xs_stride_k,
-                    void* rows, float* rows_s, const int32_t* row_index, const int32_t* source, int64_t tokens, int64_t H,
-                    int64_t topk, int64_t num_rows, void* stream) {
-  using namespace dlb;
-  clear_error();
-  const bool f8 = dtype == DLB_ROWS_E4M3;
-  if (!f8 && bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32 / DLB_ROWS_E4M3", dtype);
-  if (int rc = check_rows(tokens, H, topk, num_rows)) return rc;
-  if (f8 && H % kScaleBlock != 0) return fail(DLB_ERR_BAD_SHAPE, "H=%lld is not a multiple of 128", (long long)H);
-  if (num_rows == 0 || H == 0) return DLB_OK;
-  if (!rows || !source || (tokens > 0 && (!x || !row_index))) return fail(DLB_ERR_NULL_POINTER, "x, rows or a table is NULL");
-  if (f8 && (!rows_s || (tokens > 0 && !x_s))) return fail(DLB_ERR_NULL_POINTER, "e4m3 rows without their scales");
-  if (x_row_stride < 0 || xs_stride_m < 0 || xs_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride");
-  const int esz = f8 ? 1 : static_cast<int>(size_of(dtype));
-  if (f8 ? misaligned(x, 16) || misaligned(rows, 16) || x_row_stride % 16 != 0 || misaligned(x_s, 4) || misaligned(rows_s, 4)
-         : off_elements(x, dtype) || off_elements(rows, dtype))
-    return fail(DLB_ERR_ALIGNMENT, "x or rows is not aligned to its elements, or e4m3 rows not to 16 bytes");
-  SortCopyArgs a{};
-  a.x = static_cast<const char*>(x), a.rows = static_cast<char*>(rows), a.row_index = row_index, a.source = source;
-  if (f8) a.xs = x_s, a.rows_s = rows_s, a.xs_s0 = xs_stride_m, a.xs_s1 = xs_stride_k, a.groups = static_cast<int>(H / kScaleBlock);
-  a.x_stride = x_row_stride * esz, a.rows_stride = H * esz, a.T = tokens, a.R = num_rows;
-  a.row_bytes = static_cast<int>(H * esz), a.esz = esz, a.topk = static_cast<int>(topk);
-  // a wave holds kSortCopyChunks KB of a row; parts down to one KB while there are fewer waves than the chip takes at once
+  hipLaunchKernelGGL((moe_sort_rows_kernel<false, true>), dim3(static_cast<unsigned>(grid)), dim3(kSortThreads), lds, st, a, static_cast<int>(blocks), c);
+  if (int rc = finish("moe_permute (tables)")) return rc;
+  if (!copies) return DLB_OK;
   constexpr int kWaves = kSortCopyThreads / 64;
-  const int64_t kbytes = ceil_div(a.row_bytes, 1024);
-  int64_t part = kSortCopyChunks;
-  while (part > 1 && tokens * ceil_div(kbytes, part) < 8192) part /= 2;
-  a.parts = static_cast<int>(ceil_div(kbytes, part)), a.part_bytes = static_cast<int>(part * 1024);
-  const int64_t units = ceil_div(tokens * a.parts, kWaves);
-  a.token_blocks = static_cast<int>(units < 16384 ? units : 16384);
-  a.zero_blocks = static_cast<int>(ceil_div(num_rows, kWaves) < 1024 ? ceil_div(num_rows, kWaves) : 1024);
-  with_flag(a.row_bytes % 16 == 0, [&](auto whole) {
-    hipLaunchKernelGGL(moe_sort_copy_kernel<whole()>, dim3(a.token_blocks + a.zero_blocks), dim3(kSortCopyThreads), 0, static_cast<hipStream_t>(stream), a);
+  c.token_blocks = static_cast<int>(std::min<int64_t>(ceil_div(tokens * c.parts, kWaves), 16384));
+  c.zero_blocks = static_cast<int>(std::min<int64_t>(ceil_div(num_rows, kWaves), 1024));
+  with_flag(whole_rows, [&](auto whole) {
+    hipLaunchKernelGGL(moe_sort_copy_kernel<whole()>, dim3(c.token_blocks + c.zero_blocks), dim3(kSortCopyThreads), 0, st, c);
   });
-  return finish("moe_permute");
+  return finish("moe_permute (copy)");
 }
 
 int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, const int32_t* row_index, const float* weights, void* out,

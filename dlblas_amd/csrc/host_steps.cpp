@@ -21,8 +21,7 @@ struct StepAbi {
   decltype(&dlb_moe_unpermute_backward) unpermute_backward;
   decltype(&dlb_rms_norm) norm;
   decltype(&dlb_rms_norm_quant) norm_quant;
-  decltype(&dlb_moe_sort_workspace_bytes) sort_ws;
-  decltype(&dlb_moe_sort) sort;
+  decltype(&dlb_moe_permute_workspace_bytes) permute_ws;
   decltype(&dlb_moe_permute) permute;
   decltype(&dlb_moe_unpermute) unpermute;
   decltype(&dlb_w4_gemm_workspace_bytes) w4_ws;
@@ -178,12 +177,11 @@ variable_list permute_forward(const at::Tensor& x, const at::Tensor* x_s, const 
   const at::Tensor tables = empty({T * topk + 2 * R + 2 * E}, at::kInt, x);
   int64_t at = 0;
   variable_list out{rows, part_of(tables, &at, {T, topk}), part_of(tables, &at, {R}), part_of(tables, &at, {R}), part_of(tables, &at, {E}), part_of(tables, &at, {E})};
-  const size_t need = abi.sort_ws(T, topk, E);
+  const size_t need = abi.permute_ws(T, topk, E);
   if (need > 0) scratch = empty({static_cast<int64_t>(need)}, at::kByte, x);
-  must(abi.sort(ptr(ids), idx_code(ids.scalar_type()), ids.stride(0), ids.stride(1), iptr(out[1]), iptr(out[2]), iptr(out[3]), iptr(out[4]), iptr(out[5]), T,
-                topk, E, align, R, need > 0 ? ptr(scratch) : nullptr, need, stream));
-  must(abi.permute(ptr(x), x.stride(0), x_s ? DLB_ROWS_E4M3 : in_code(x.scalar_type()), x_s ? fptr(*x_s) : nullptr, x_s ? x_s->stride(0) : 0,
-                   x_s ? x_s->stride(1) : 0, ptr(rows), x_s ? fptr(rows_s) : nullptr, iptr(out[1]), iptr(out[2]), T, H, topk, R, stream));
+  must(abi.permute(ptr(ids), idx_code(ids.scalar_type()), ids.stride(0), ids.stride(1), ptr(x), x.stride(0), x_s ? DLB_ROWS_E4M3 : in_code(x.scalar_type()),
+                   x_s ? fptr(*x_s) : nullptr, x_s ? x_s->stride(0) : 0, x_s ? x_s->stride(1) : 0, iptr(out[1]), iptr(out[2]), iptr(out[3]), iptr(out[4]),
+                   iptr(out[5]), ptr(rows), x_s ? fptr(rows_s) : nullptr, T, H, topk, E, align, R, need > 0 ? ptr(scratch) : nullptr, need, stream));
   if (x_s) out.push_back(rows_s);
   return out;
 }

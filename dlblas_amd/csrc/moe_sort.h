@@ -55,102 +55,6 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_count_kernel(const Sort
   for (int e = threadIdx.x; e < p.E; e += kSortThreads) p.hist[static_cast<int64_t>(blockIdx.x) * p.E + e] = hist[e];
 }
 
-// Rows of the slots of workgroup blockIdx, and its share of the tables by row.  Workgroups past the slots' share only the latter.
-// LDS: before [E], total [E], start [E + 1], wave_cnt [16][E] of 16-bit counts.
-__global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortArgs p, int slot_blocks) {
-  extern __shared__ int lds[];
-  const int E = p.E;
-  int* before = lds;           // slots of the expert in the workgroups before, then the expert's next row in this one
-  int* total = before + E;     // slots of the expert
-  int* start = total + E;      // [E + 1] first row of every span
-  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(start + E + 1);  // [16][E]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x;
-  for (int i = tid; i < 2 * E; i += kSortThreads) lds[i] = 0;
-  for (int i = tid; i < 16 * E; i += kSortThreads) wave_cnt[i] = 0;
-  __syncthreads();
-  const int64_t slot = static_cast<int64_t>(b) * kSortBlockSlots + tid;
-  const int id = b < slot_blocks ? sort_id(p, slot) : -1;
-  if (slot_blocks == 1) {
-    // one workgroup of slots: every workgroup counts them itself
-    const int mine = b == 0 ? id : sort_id(p, tid);
-    if (mine >= 0) atomicAdd(&total[mine], 1);
-  } else {
-    const int cols = min(E, kSortThreads), P = kSortThreads / cols;
-    const int my_part = tid / cols, my_col = tid % cols;
-    for (int e = my_col; e < E && my_part < P; e += cols) {
-      int all = 0, early = 0;
-      for (int r = my_part; r < slot_blocks; r += P) {
-        const int c = p.hist[static_cast<int64_t>(r) * E + e];
-        all += c;
-        if (r < b) early += c;
-      }
-      if (all) atomicAdd(&total[e], all);
-      if (early) atomicAdd(&before[e], early);
-    }
-  }
-  __syncthreads();
-  if (wave == 0) {
-    int64_t carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-      const int e = e0 + lane;
-      const int64_t c = e < E ? (static_cast<int64_t>(total[e]) + p.align - 1) / p.align * p.align : 0;
-      int64_t incl = c;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int64_t up = __shfl_up(incl, off);
-        if (lane >= off) incl += up;
-      }
-      if (e < E) start[e] = static_cast<int>(min(carry + incl - c, p.R));
-      carry += __shfl(incl, 63);
-    }
-    if (lane == 0) start[E] = static_cast<int>(min(carry, p.R));
-  }
-  // slots with the same expert: in the waves before (wave_cnt) and in the lanes before (one ballot per bit of the id)
-  uint64_t same = ~0ull;
-  if (b < slot_blocks) {
-    const uint64_t live = __ballot(id >= 0);
-    same = live;
-    for (int bit = 0; (E - 1) >> bit; ++bit) {
-      const uint64_t ones = __ballot((id >> bit) & 1);
-      same &= ((id >> bit) & 1) ? ones : ~ones;
-    }
-    if (id >= 0 && (same >> lane) == 1) wave_cnt[wave * E + id] = static_cast<uint16_t>(__popcll(same));
-  }
-  __syncthreads();
-  if (b < slot_blocks && slot < p.n) {
-    int64_t row = -1;
-    if (id >= 0) {
-      row = static_cast<int64_t>(start[id]) + before[id] + __popcll(same & ((1ull << lane) - 1));
-      for (int w = 0; w < wave; ++w) row += wave_cnt[w * E + id];
-      if (row >= p.R) row = -1;
-    }
-    p.row_index[slot] = static_cast<int32_t>(row);
-    if (row >= 0) p.source[row] = static_cast<int32_t>(slot);
-  }
-  if (b == 0)
-    for (int e = tid; e < E; e += kSortThreads) {
-      p.row_start[e] = start[e];
-      p.row_end[e] = static_cast<int>(min(static_cast<int64_t>(start[e]) + total[e], p.R));
-    }
-  for (int64_t r = static_cast<int64_t>(b) * kSortThreads + tid; r < p.R; r += static_cast<int64_t>(gridDim.x) * kSortThreads) {
-    int e = -1;
-    if (r < start[E]) {
-      int lo = 0, hi = E;  // the last e with start[e] <= r: an empty span before it starts at the same row
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= r)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      e = lo;
-    }
-    p.m_indices[r] = e;
-    if (e < 0 || r >= static_cast<int64_t>(start[e]) + total[e]) p.source[r] = -1;
-  }
-}
-
 // Rows moved as bytes in chunks of 16; the last chunk of a row may be short (not where rows are WHOLE chunks).
 template <bool WHOLE>
 __device__ __forceinline__ v4i load_bytes16(const char* p, int left, int esz) {
@@ -200,9 +104,165 @@ struct SortCopyArgs {
 constexpr int kSortCopyThreads = 256;
 constexpr int kSortCopyChunks = 4;  // of 16 bytes a lane holds while a token's rows are written
 
+// Part `part` of token t to all of its rows by one wave, lane j holding the row of slot j (-1: none).  A token without a row is not read.
+template <bool WHOLE>
+__device__ __forceinline__ void copy_token(const SortCopyArgs& p, int64_t t, int part, int mine, int lane) {
+  const uint64_t there = __ballot(mine >= 0);
+  if (there == 0) return;
+  const char* src = p.x + t * p.x_stride;
+  const int end = min(p.row_bytes, (part + 1) * p.part_bytes);
+  for (int c0 = part * p.part_bytes; c0 < end; c0 += kSortCopyChunks * 1024) {
+    v4i v[kSortCopyChunks];
+#pragma unroll
+    for (int k = 0; k < kSortCopyChunks; ++k) {
+      const int c = c0 + (k * 64 + lane) * 16;
+      if (c < end) v[k] = load_bytes16<WHOLE>(src + c, p.row_bytes - c, p.esz);
+    }
+    for (uint64_t left = there; left; left &= left - 1) {
+      char* dst = p.rows + static_cast<int64_t>(__builtin_amdgcn_readlane(mine, __builtin_ctzll(left))) * p.rows_stride;
+#pragma unroll
+      for (int k = 0; k < kSortCopyChunks; ++k) {
+        const int c = c0 + (k * 64 + lane) * 16;
+        if (c < end) store_bytes16<WHOLE>(dst + c, v[k], p.row_bytes - c, p.esz);
+      }
+    }
+  }
+  if (part != 0) return;
+  for (int g0 = 0; g0 < p.groups; g0 += 64) {
+    const int g = g0 + lane;
+    const float s = g < p.groups ? p.xs[t * p.xs_s0 + g * p.xs_s1] : 0.f;
+    for (uint64_t left = there; left; left &= left - 1) {
+      const int64_t row = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+      if (g < p.groups) p.rows_s[row * p.groups + g] = s;
+    }
+  }
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void clear_row(const SortCopyArgs& p, int64_t r, int lane) {
+  char* dst = p.rows + r * p.rows_stride;
+  for (int c = lane * 16; c < p.row_bytes; c += 64 * 16) store_bytes16<WHOLE>(dst + c, v4i{0, 0, 0, 0}, p.row_bytes - c, p.esz);
+  for (int g = lane; g < p.groups; g += 64) p.rows_s[r * p.groups + g] = 0.f;
+}
+
+// Rows of the slots of workgroup blockIdx, and its share of the tables by row.  Workgroups past the slots' share only the latter.
+// COPY: there is one workgroup's worth of slots, and every workgroup finds the rows of all of them and copies its share of the tokens, so
+// that a few tokens take one launch.  Then only the first workgroup writes the tables by slot and expert.
+// LDS: before [E], total [E], start [E + 1], wave_cnt [16][E] of 16-bit counts; COPY: rows [threads].
+template <bool COPY, bool WHOLE>
+__global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortArgs p, int slot_blocks, const SortCopyArgs c) {
+  extern __shared__ int lds[];
+  const int E = p.E;
+  int* before = lds;           // slots of the expert in the workgroups before, then the expert's next row in this one
+  int* total = before + E;     // slots of the expert
+  int* start = total + E;      // [E + 1] first row of every span
+  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(start + E + 1);  // [16][E]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = blockDim.x;
+  const int b = blockIdx.x;
+  const bool slots_here = COPY || b < slot_blocks;
+  int* const rows = reinterpret_cast<int*>(wave_cnt + 16 * E);  // an even number of them before
+  for (int i = tid; i < 2 * E; i += threads) lds[i] = 0;
+  for (int i = tid; i < 16 * E; i += threads) wave_cnt[i] = 0;
+  __syncthreads();
+  const int64_t slot = COPY ? tid : static_cast<int64_t>(b) * kSortBlockSlots + tid;
+  const int id = slots_here ? sort_id(p, slot) : -1;
+  if (slot_blocks == 1) {
+    // one workgroup of slots: every workgroup counts them itself
+    const int mine = COPY || b == 0 ? id : sort_id(p, tid);
+    if (mine >= 0) atomicAdd(&total[mine], 1);
+  } else {
+    const int cols = min(E, kSortThreads), P = kSortThreads / cols;
+    const int my_part = tid / cols, my_col = tid % cols;
+    for (int e = my_col; e < E && my_part < P; e += cols) {
+      int all = 0, early = 0;
+      for (int r = my_part; r < slot_blocks; r += P) {
+        const int c = p.hist[static_cast<int64_t>(r) * E + e];
+        all += c;
+        if (r < b) early += c;
+      }
+      if (all) atomicAdd(&total[e], all);
+      if (early) atomicAdd(&before[e], early);
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int64_t carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      const int e = e0 + lane;
+      const int64_t c = e < E ? (static_cast<int64_t>(total[e]) + p.align - 1) / p.align * p.align : 0;
+      int64_t incl = c;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int64_t up = __shfl_up(incl, off);
+        if (lane >= off) incl += up;
+      }
+      if (e < E) start[e] = static_cast<int>(min(carry + incl - c, p.R));
+      carry += __shfl(incl, 63);
+    }
+    if (lane == 0) start[E] = static_cast<int>(min(carry, p.R));
+  }
+  // slots with the same expert: in the waves before (wave_cnt) and in the lanes before (one ballot per bit of the id)
+  uint64_t same = ~0ull;
+  if (slots_here) {
+    const uint64_t live = __ballot(id >= 0);
+    same = live;
+    for (int bit = 0; (E - 1) >> bit; ++bit) {
+      const uint64_t ones = __ballot((id >> bit) & 1);
+      same &= ((id >> bit) & 1) ? ones : ~ones;
+    }
+    if (id >= 0 && (same >> lane) == 1) wave_cnt[wave * E + id] = static_cast<uint16_t>(__popcll(same));
+  }
+  __syncthreads();
+  if (slots_here && slot < p.n) {
+    int64_t row = -1;
+    if (id >= 0) {
+      row = static_cast<int64_t>(start[id]) + before[id] + __popcll(same & ((1ull << lane) - 1));
+      for (int w = 0; w < wave; ++w) row += wave_cnt[w * E + id];
+      if (row >= p.R) row = -1;
+    }
+    if (COPY) rows[tid] = static_cast<int>(row);
+    if (!COPY || b == 0) {
+      p.row_index[slot] = static_cast<int32_t>(row);
+      if (row >= 0) p.source[row] = static_cast<int32_t>(slot);
+    }
+  }
+  if (b == 0)
+    for (int e = tid; e < E; e += threads) {
+      p.row_start[e] = start[e];
+      p.row_end[e] = static_cast<int>(min(static_cast<int64_t>(start[e]) + total[e], p.R));
+    }
+  const auto expert_of = [&](int64_t r) {  // of row r, -1: past the last span
+    if (r >= start[E]) return -1;
+    int lo = 0, hi = E;  // the last e with start[e] <= r: an empty span before it starts at the same row
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  const auto vacant = [&](int64_t r, int e) { return e < 0 || r >= static_cast<int64_t>(start[e]) + total[e]; };
+  for (int64_t r = static_cast<int64_t>(b) * threads + tid; r < p.R; r += static_cast<int64_t>(gridDim.x) * threads) {
+    const int e = expert_of(r);
+    p.m_indices[r] = e;
+    if (vacant(r, e)) p.source[r] = -1;
+  }
+  if (!COPY) return;
+  __syncthreads();
+  const int waves = threads / 64;
+  for (uint32_t u = b * waves + wave; u < static_cast<uint32_t>(c.T * c.parts); u += gridDim.x * waves) {  // at most 1024 parts of 2^20 KB
+    const int t = static_cast<int>(u / static_cast<uint32_t>(c.parts));
+    copy_token<WHOLE>(c, t, static_cast<int>(u) - t * c.parts, lane < p.topk ? rows[t * p.topk + lane] : -1, lane);
+  }
+  for (int64_t r = static_cast<int64_t>(b) * waves + wave; r < p.R; r += static_cast<int64_t>(gridDim.x) * waves)
+    if (vacant(r, expert_of(r))) clear_row<WHOLE>(c, r, lane);
+}
+
 // A wave per token and part: blocks [0, token_blocks) take the tokens, the others look for rows without a slot.  The slots' rows come
-// in one load, a lane each; a token that none of them is here for is not read.  Few tokens are cut finer, so that there are waves
-// for the whole chip (16 tokens x 8 slots x 7168 bf16: 15.5 -> 4.1 us).
+// in one load, a lane each.  Few tokens are cut finer, so that there are waves for the whole chip.  4096 x 7168 bf16 to 8 rows each, 528 MB:
+// 93 us (5.7 TB/s), 8192 x 7168 e4m3 to 4 (294 MB) 26.
 template <bool WHOLE>
 __global__ void __launch_bounds__(kSortCopyThreads) moe_sort_copy_kernel(const SortCopyArgs p) {
   const int lane = threadIdx.x & 63;
@@ -211,46 +271,13 @@ __global__ void __launch_bounds__(kSortCopyThreads) moe_sort_copy_kernel(const S
   if (static_cast<int>(blockIdx.x) < p.token_blocks) {
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWaves + wave; u < p.T * p.parts; u += static_cast<int64_t>(p.token_blocks) * kWaves) {
       const int64_t t = u / p.parts;
-      const int part = static_cast<int>(u - t * p.parts);
-      const int mine = lane < p.topk ? p.row_index[t * p.topk + lane] : -1;
-      const uint64_t there = __ballot(mine >= 0);
-      if (there == 0) continue;
-      const char* src = p.x + t * p.x_stride;
-      const int end = min(p.row_bytes, (part + 1) * p.part_bytes);
-      for (int c0 = part * p.part_bytes; c0 < end; c0 += kSortCopyChunks * 1024) {
-        v4i v[kSortCopyChunks];
-#pragma unroll
-        for (int k = 0; k < kSortCopyChunks; ++k) {
-          const int c = c0 + (k * 64 + lane) * 16;
-          if (c < end) v[k] = load_bytes16<WHOLE>(src + c, p.row_bytes - c, p.esz);
-        }
-        for (uint64_t left = there; left; left &= left - 1) {
-          char* dst = p.rows + static_cast<int64_t>(__builtin_amdgcn_readlane(mine, __builtin_ctzll(left))) * p.rows_stride;
-#pragma unroll
-          for (int k = 0; k < kSortCopyChunks; ++k) {
-            const int c = c0 + (k * 64 + lane) * 16;
-            if (c < end) store_bytes16<WHOLE>(dst + c, v[k], p.row_bytes - c, p.esz);
-          }
-        }
-      }
-      if (part != 0) continue;
-      for (int g = lane; g < p.groups; g += 64) {
-        const float s = p.xs[t * p.xs_s0 + g * p.xs_s1];
-        for (int j = 0; j < p.topk; ++j) {
-          const int64_t row = p.row_index[t * p.topk + j];
-          if (row >= 0) p.rows_s[row * p.groups + g] = s;
-        }
-      }
+      copy_token<WHOLE>(p, t, static_cast<int>(u - t * p.parts), lane < p.topk ? p.row_index[t * p.topk + lane] : -1, lane);
     }
     return;
   }
   const int64_t zb = static_cast<int64_t>(blockIdx.x) - p.token_blocks;
-  for (int64_t r = zb * kWaves + wave; r < p.R; r += static_cast<int64_t>(p.zero_blocks) * kWaves) {
-    if (p.source[r] >= 0) continue;
-    char* dst = p.rows + r * p.rows_stride;
-    for (int c = lane * 16; c < p.row_bytes; c += 64 * 16) store_bytes16<WHOLE>(dst + c, v4i{0, 0, 0, 0}, p.row_bytes - c, p.esz);
-    for (int g = lane; g < p.groups; g += 64) p.rows_s[r * p.groups + g] = 0.f;
-  }
+  for (int64_t r = zb * kWaves + wave; r < p.R; r += static_cast<int64_t>(p.zero_blocks) * kWaves)
+    if (p.source[r] < 0) clear_row<WHOLE>(p, r, lane);
 }
 
 struct UnpermuteArgs {

@@ -21,16 +21,12 @@ class MoePermutation(NamedTuple):
     row_end: torch.Tensor    # [experts] one past its last row that holds a slot
 
 
-@torch.library.custom_op('dlblas::moe_sort', mutates_args=('row_index', 'source', 'm_indices', 'row_start', 'row_end'), device_types='cuda')
-def _sort_op(topk_ids: torch.Tensor, row_index: torch.Tensor, source: torch.Tensor, m_indices: torch.Tensor, row_start: torch.Tensor,
-             row_end: torch.Tensor, alignment: int) -> None:
-    _decoder.moe_sort(topk_ids, row_index, source, m_indices, row_start, row_end, alignment)
-
-
-@torch.library.custom_op('dlblas::moe_permute', mutates_args=('rows', 'rows_s'), device_types='cuda')
-def _permute_op(x: torch.Tensor, x_s: Optional[torch.Tensor], rows: torch.Tensor, rows_s: Optional[torch.Tensor], row_index: torch.Tensor,
-                source: torch.Tensor) -> None:
-    _decoder.moe_permute(x, x_s, rows, rows_s, row_index, source)
+@torch.library.custom_op('dlblas::moe_permute', mutates_args=('row_index', 'source', 'm_indices', 'row_start', 'row_end', 'rows', 'rows_s'),
+                         device_types='cuda')
+def _permute_op(topk_ids: torch.Tensor, x: torch.Tensor, x_s: Optional[torch.Tensor], row_index: torch.Tensor, source: torch.Tensor,
+                m_indices: torch.Tensor, row_start: torch.Tensor, row_end: torch.Tensor, rows: torch.Tensor, rows_s: Optional[torch.Tensor],
+                alignment: int) -> None:
+    _decoder.moe_permute(topk_ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s, alignment)
 
 
 @torch.library.custom_op('dlblas::moe_unpermute', mutates_args=('out', ), device_types='cuda')
@@ -48,13 +44,16 @@ def _columns_whole(t):
     return t if t is None or t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
 
 
-def _sorted(topk_ids, num_experts, alignment, num_rows):
+def _permuted(x, x_s, topk_ids, num_experts, alignment, num_rows):
+
     def table(*size):
-        return torch.empty(size, dtype=torch.int32, device=topk_ids.device)
+        return torch.empty(size, dtype=torch.int32, device=x.device)
 
     p = MoePermutation(table(*topk_ids.shape), table(num_rows), table(num_rows), table(num_experts), table(num_experts))
-    _sort_op(topk_ids, *p, alignment)
-    return p
+    rows = torch.empty((num_rows, x.size(1)), dtype=x.dtype, device=x.device)
+    rows_s = None if x_s is None else torch.empty((num_rows, x_s.size(1)), dtype=torch.float32, device=x.device)
+    _permute_op(topk_ids, x, x_s, *p, rows, rows_s, alignment)
+    return rows, rows_s, p
 
 
 def _unpermuted(rows, row_index, weights):
@@ -67,9 +66,7 @@ class _Permute(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, topk_ids, num_experts, alignment, num_rows):
-        p = _sorted(topk_ids, num_experts, alignment, num_rows)
-        rows = torch.empty((num_rows, x.size(1)), dtype=x.dtype, device=x.device)
-        _permute_op(_columns_whole(x), None, rows, None, p.row_index, p.source)
+        rows, _, p = _permuted(_columns_whole(x), None, topk_ids, num_experts, alignment, num_rows)
         ctx.save_for_backward(p.row_index)
         ctx.mark_non_differentiable(*p)
         return (rows, ) + tuple(p)
@@ -145,21 +142,16 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
         assert x.size(1) % 128 == 0, f'the last dimension of x {x.size(1)} must be divisible by 128'
         if tuple(x_s.shape) != (x.size(0), x.size(1) // 128):
             raise ValueError(f'scales must be {[x.size(0), x.size(1) // 128]}, got {list(x_s.shape)}')
-        p = _sorted(topk_ids, num_experts, alignment, num_rows)
-        rows = torch.empty((num_rows, x.size(1)), dtype=x.dtype, device=x.device)
-        rows_s = torch.empty((num_rows, x.size(1) // 128), dtype=torch.float32, device=x.device)
         if x.stride(1) != 1 or x.stride(0) % 16 != 0 or x.data_ptr() % 16 != 0:
             x = x.clone(memory_format=torch.contiguous_format)
-        _permute_op(x, x_s, rows, rows_s, p.row_index, p.source)
+        rows, rows_s, p = _permuted(x, x_s, topk_ids, num_experts, alignment, num_rows)
         return (rows, rows_s), p
     if x.dtype not in _lib.IN_CODES:
         raise TypeError(f'x must be bfloat16, float16 or float32, or float8_e4m3fn with its scales, got {x.dtype}')
     if torch.is_grad_enabled() and x.requires_grad:
         out = _Permute.apply(x, topk_ids, num_experts, alignment, num_rows)
         return out[0], MoePermutation(*out[1:])
-    p = _sorted(topk_ids, num_experts, alignment, num_rows)
-    rows = torch.empty((num_rows, x.size(1)), dtype=x.dtype, device=x.device)
-    _permute_op(_columns_whole(x), None, rows, None, p.row_index, p.source)
+    rows, _, p = _permuted(_columns_whole(x), None, topk_ids, num_experts, alignment, num_rows)
     return rows, p
 
 

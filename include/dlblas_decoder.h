@@ -21,8 +21,10 @@ extern "C" {
 
 /* widest row of the norms and of dlb_moe_unpermute_backward */
 #define DLB_NORM_MAX_COLUMNS 32768
-/* experts of dlb_moe_sort */
+/* experts of dlb_moe_permute */
 #define DLB_SORT_MAX_EXPERTS 1024
+/* element type of dlb_moe_permute beside DLB_IN_*: e4m3fn with fp32 scales of 1 x 128 */
+#define DLB_ROWS_E4M3 3
 
 /*
  * h = x + residual rounded to the element type (h = x without a residual), y = h * w / sqrt(mean(h^2) + eps); fp32 inside, one
@@ -61,36 +63,33 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
                           int64_t h_row_stride, int dtype, const void* weight, int weight_dtype, void* dx, int64_t dx_row_stride,
                           void* dw, int64_t rows, int64_t H, float eps, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of scratch dlb_moe_sort needs. */
-size_t dlb_moe_sort_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts);
+/* Bytes of scratch dlb_moe_permute needs. */
+size_t dlb_moe_permute_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts);
 
 /*
- * The tables of the tokens sorted by expert.  Slots (t, j) with 0 <= ids[t, j] < experts are ordered by (expert, t, j); expert e
- * gets the rows from row_start[e] on, its count rounded up to `alignment`.  Slots whose row would be num_rows or more get none.
+ * Tokens copied next to the other tokens of each expert they are routed to, and the tables that say where.  Slots (t, j) with
+ * 0 <= ids[t, j] < experts are ordered by (expert, t, j); expert e gets the rows from row_start[e] on, its count rounded up to
+ * `alignment`.  Slots whose row would be num_rows or more get none.  rows[r] = x[source[r] / topk], zeros where source[r] < 0.
  *
  *   ids        [tokens, topk]  int32 / int64 (ids_dtype, DLB_IDX_*) through two strides; topk <= 64
+ *   x          [tokens, H]     bf16 / fp16 / fp32 (DLB_IN_*) or e4m3fn (DLB_ROWS_E4M3: H % 128 == 0, rows of x and `rows` 16-byte
+ *                              aligned)
+ *   x_s        [tokens, H/128] fp32 through two strides with e4m3fn rows, else NULL
  *   row_index  [tokens, topk]  int32, contiguous, OUT: row of every slot, -1 where it has none
  *   source     [num_rows]      int32, OUT: slot t * topk + j of every row, -1 where it holds none
  *   m_indices  [num_rows]      int32, OUT: expert of every row of a span, -1 past the last span (the form that
  *                              dlb_fp8_gemm_grouped_contiguous takes with alignment 128)
  *   row_start, row_end [experts] int32, OUT: rows of every expert that hold a slot (the form dlb_fp8_gemm_grouped_ragged and
  *                              dlb_w4_gemm take); at most num_rows
- */
-int dlb_moe_sort(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, int32_t* row_index, int32_t* source,
-                 int32_t* m_indices, int32_t* row_start, int32_t* row_end, int64_t tokens, int64_t topk, int64_t experts,
-                 int64_t alignment, int64_t num_rows, void* workspace, size_t workspace_bytes, void* stream);
-
-/*
- * rows[r] = x[source[r] / topk], zeros where source[r] < 0, with the tables of dlb_moe_sort.
+ *   rows       [num_rows, H]   contiguous, OUT;   rows_s [num_rows, H/128] fp32, contiguous, OUT with e4m3fn rows
  *
- *   x     [tokens, H]    bf16 / fp16 / fp32 (DLB_IN_*) or e4m3fn (DLB_ROWS_E4M3: H % 128 == 0, rows of x and `rows` 16-byte aligned)
- *   x_s   [tokens, H/128] fp32 through two strides with e4m3fn rows, else NULL
- *   rows  [num_rows, H]   contiguous, OUT;   rows_s [num_rows, H/128] fp32, contiguous, OUT
+ * With H = 0 the tables alone are written.
  */
-#define DLB_ROWS_E4M3 3
-int dlb_moe_permute(const void* x, int64_t x_row_stride, int dtype, const float* x_s, int64_t xs_stride_m, int64_t xs_stride_k,
-                    void* rows, float* rows_s, const int32_t* row_index, const int32_t* source, int64_t tokens, int64_t H,
-                    int64_t topk, int64_t num_rows, void* stream);
+int dlb_moe_permute(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, const void* x, int64_t x_row_stride,
+                    int dtype, const float* x_s, int64_t xs_stride_m, int64_t xs_stride_k, int32_t* row_index, int32_t* source,
+                    int32_t* m_indices, int32_t* row_start, int32_t* row_end, void* rows, float* rows_s, int64_t tokens, int64_t H,
+                    int64_t topk, int64_t experts, int64_t alignment, int64_t num_rows, void* workspace, size_t workspace_bytes,
+                    void* stream);
 
 /*
  * out[t] = sum over the slots j with 0 <= row_index[t, j] < num_rows, in slot order, of weights[t, j] * rows[row_index[t, j]]; an fp32
@@ -102,7 +101,7 @@ int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, cons
                       int64_t out_row_stride, int64_t tokens, int64_t H, int64_t topk, int64_t num_rows, void* stream);
 
 /*
- * The gradients of dlb_moe_unpermute with the tables of dlb_moe_sort (every row is named by one slot at most):
+ * The gradients of dlb_moe_unpermute with the tables of dlb_moe_permute (every row is named by one slot at most):
  * drows[row] = weights[t, j] * dout[t], zeros in rows without a slot; dweights[t, j] = sum over the columns of rows[row] * dout[t], 0 for
  * a slot without a row.
  *

@@ -71,20 +71,19 @@ def test_norm_entry_points_refuse():
 
 def test_sort_entry_points_refuse():
     lib = _lib.load()
-    need = lib.dlb_moe_sort_workspace_bytes(100000, 8, 64)
-    assert need > 0 and lib.dlb_moe_sort_workspace_bytes(0, 8, 64) == 0
-    good = dict(ids=fake, dt=0, s0=8, s1=1, ri=fake, src=fake, mi=fake, rs=fake, re=fake, T=100000, topk=8, E=64, al=1, R=100, ws=fake, wsb=need, st=null)
-    refused('dlb_moe_sort', good, [
-        (dict(dt=2), DTYPE), (dict(T=-1), SHAPE), (dict(topk=0), SHAPE), (dict(topk=65), SHAPE), (dict(E=0), SHAPE), (dict(E=1025), SHAPE), (dict(al=0), SHAPE),
-        (dict(al=(1 << 20) + 1), SHAPE), (dict(R=-1), SHAPE), (dict(R=1 << 31), SHAPE), (dict(T=1 << 29), SHAPE), (dict(s0=-8), STRIDE), (dict(ids=null), NULL),
-        (dict(ri=null), NULL), (dict(src=null), NULL), (dict(mi=null), NULL), (dict(rs=null), NULL), (dict(re=null), NULL), (dict(ws=null), WORKSPACE),
-        (dict(wsb=need - 1), WORKSPACE), (dict(ids=at(4100), dt=1), ALIGN), (dict(src=at(4098)), ALIGN), (dict(ws=at(4098)), ALIGN)])
-    good = dict(x=fake, x_rs=256, dt=0, xs=null, xs0=0, xs1=0, rows=fake, rs=null, ri=fake, src=fake, T=10, H=256, topk=2, R=20, st=null)
+    need = lib.dlb_moe_permute_workspace_bytes(100000, 8, 64)
+    assert need > 0 and lib.dlb_moe_permute_workspace_bytes(0, 8, 64) == 0 and lib.dlb_moe_permute_workspace_bytes(128, 8, 64) == 0
+    good = dict(ids=fake, i_dt=0, s0=8, s1=1, x=fake, x_rs=256, dt=0, xs=null, xs0=0, xs1=0, ri=fake, src=fake, mi=fake, st=fake, en=fake, rows=fake, rs=null,
+                T=100000, H=256, topk=8, E=64, al=1, R=100, ws=fake, wsb=need, stream=null)
     f8 = dict(dt=3, xs=fake, rs=fake, xs0=2, xs1=1)
     refused('dlb_moe_permute', good, [
-        (dict(dt=4), DTYPE), (dict(H=-1), SHAPE), (dict(topk=0), SHAPE), (dict(x=null), NULL), (dict(rows=null), NULL), (dict(ri=null), NULL), (dict(src=null), NULL),
+        (dict(i_dt=2), DTYPE), (dict(T=-1), SHAPE), (dict(topk=0), SHAPE), (dict(topk=65), SHAPE), (dict(E=0), SHAPE), (dict(E=1025), SHAPE), (dict(al=0), SHAPE),
+        (dict(al=(1 << 20) + 1), SHAPE), (dict(R=-1), SHAPE), (dict(R=1 << 31), SHAPE), (dict(T=1 << 29), SHAPE), (dict(s0=-8), STRIDE), (dict(ids=null), NULL),
+        (dict(ri=null), NULL), (dict(src=null), NULL), (dict(mi=null), NULL), (dict(st=null), NULL), (dict(en=null), NULL), (dict(ws=null), WORKSPACE),
+        (dict(wsb=need - 1), WORKSPACE), (dict(ids=at(4100), i_dt=1), ALIGN), (dict(src=at(4098)), ALIGN), (dict(ws=at(4098)), ALIGN),
+        (dict(dt=4), DTYPE), (dict(H=-1), SHAPE), (dict(x=null), NULL), (dict(rows=null), NULL),
         (dict(x_rs=-1), STRIDE), (dict(x=at(4097)), ALIGN), (dict(f8, H=200), SHAPE), (dict(f8, xs=null), NULL), (dict(f8, rs=null), NULL), (dict(f8, x=at(4104)), ALIGN),
-        (dict(f8, x_rs=264), ALIGN), (dict(f8, xs0=-1), STRIDE), (dict(R=0, rows=null), OK), (dict(H=0, x=null), OK)])
+        (dict(f8, x_rs=264), ALIGN), (dict(f8, xs0=-1), STRIDE)])
     good = dict(rows=fake, rs=256, dt=0, ri=fake, w=fake, out=fake, o_rs=256, T=10, H=256, topk=2, R=20, st=null)
     refused('dlb_moe_unpermute', good, [
         (dict(dt=3), DTYPE), (dict(T=-1), SHAPE), (dict(topk=65), SHAPE), (dict(rows=null), NULL), (dict(ri=null), NULL), (dict(out=null), NULL), (dict(o_rs=255), STRIDE),
