@@ -1,7 +1,7 @@
 // Root-mean-square norm with the residual's addition, its gradient, and the form whose output is quantised 1 x 128, for gfx950.
 //
 //   h = x + res rounded to the rows' type (without a residual h = x),  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
-//   quantising:  s = max(max |y|, qeps) / 448 per 128 columns,  q = e4m3(clamp(y / s, +-448)); y itself is not rounded in between
+//   quantising:  s = max(max |y|, qeps) / 448 per 128 columns,  q = e4m3(y / s); y itself is not rounded in between
 //   gradient:    dh = r (w dy) - h r^3 / H sum(w dy h) + dsum,   dw = sum over the rows of dy h r
 //
 // h is rounded before the norm reads it: it is what the next layer adds to and what the gradient starts from, so both see the same
@@ -145,6 +145,16 @@ __device__ __forceinline__ void load_weight8(const void* w, int w_f32, int col, 
     quant_unpack8<T>(load_raw8<T, WHOLE>(w, 0, col, left), v);
 }
 
+// The largest |y| of 16 lanes, or the largest |h w|, as bits, which put NaN above infinity: a group that holds one gets a scale that shows it.
+__device__ __forceinline__ uint32_t group_max(bool hw, const float (&h)[8], const float (&w)[8], const float (&y)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(hw ? h[k] * w[k] : y[k]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 8; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
+  return top;
+}
+
 // One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each; a thread past the last chunk reads that one
 // again and leaves no trace.
 template <int T, bool QUANT, bool RES, bool WHOLE, int CH>
@@ -197,27 +207,38 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
     float v[8], w[8];
     quant_unpack8<T>(h[c], v);
     load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * i, p.H - 8 * i, w);
+    float y[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] * r * w[k];
+    for (int k = 0; k < 8; ++k) y[k] = v[k] * r * w[k];
     if (!QUANT) {
-      store_raw8<T, WHOLE>(p.y, row * p.y_rs, 8 * i, pack_raw8<T>(v), p.H - 8 * i);
+      store_raw8<T, WHOLE>(p.y, row * p.y_rs, 8 * i, pack_raw8<T>(y), p.H - 8 * i);
       continue;
     }
-    // the largest value by the bits of |y|, which puts NaN above infinity: a group that holds one gets a scale that shows it
-    uint32_t top = 0;
+    // y / s = 448 h w / max |h w|: r cancels, and for 16-bit rows and weights the operands of that quotient are exact, so a value half way
+    // between two codes stays there (with y rounded first 1 of 10^4 codes of bf16 rows differed, with these operands none of 3 10^6).
+    // Rows of fp32 take y, as the quantiser does that reads it from memory, and so do groups whose h w is close to the ends of fp32.
+    constexpr bool kExact = T != kInF32;
+    float num[8], den;
+    uint32_t top = group_max(kExact, v, w, y);
+    float scale = __uint_as_float(top) * r / 448.0f;
+    if (kExact && top - (27u << 23) < (200u << 23) && scale * 448.0f >= p.qeps) {  // 2^-100 to 2^100
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+      for (int k = 0; k < 8; ++k) num[k] = v[k] * w[k] * 448.0f;
+      den = __uint_as_float(top);
+    } else {
+      if (kExact) top = group_max(false, v, w, y);
+      const float amax = __uint_as_float(top);
+      scale = den = (amax < p.qeps ? p.qeps : amax) / 448.0f;
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
-    const float amax = __uint_as_float(top);
-    const float scale = (amax < p.qeps ? p.qeps : amax) / 448.0f;
-    const float inv_scale = 1.0f / scale;
+      for (int k = 0; k < 8; ++k) num[k] = y[k];
+    }
+    const float inv_den = 1.0f / den;
     int packed[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = div_by_scale(v[4 * k + j], scale, inv_scale);  // at most 448 and a rounding: no clamp
+      for (int j = 0; j < 4; ++j) e[j] = div_by_scale(num[4 * k + j], den, inv_den);  // at most 448 and a rounding: no clamp
       int word = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
       packed[k] = __builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], word, true);
     }

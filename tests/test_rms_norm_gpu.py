@@ -92,6 +92,21 @@ def test_norm_quant(dev, rows, H, residual, dtype, column_major):
     assert float(off.max()) <= 0
 
 
+@pytest.mark.parametrize('dtype', [bf16, f16])
+@pytest.mark.parametrize('rows,H', [(64, 7168), (5, 384)])
+def test_codes_half_way_between_two_stay_there(dev, rows, H, dtype):
+    """y / s = 448 h w / max |h w| does not depend on r.  bf16: both operands are exact in fp32 (8 + 8 + 3 bits), so the codes are those of
+    the fp32 quotient, ties to even among them.  fp16: 448 h w takes up to 25 bits, a rounding of 2^-24, so beside a quotient that is
+    within 2^-22 of the middle of two codes nothing may differ."""
+    x, w, res = inputs(rows, H, dtype, True)
+    q = rms_norm_quant(*on(dev, x, w), 1e-5, res.to(dev))[0].cpu()
+    hw = (orc.norm_input(x, res).double() * w.double()).reshape(rows, -1, 128)
+    v = hw * 448.0 / hw.abs().amax(-1, keepdim=True)
+    low, high = ((v * (1 + k * 2.0**-22)).float().to(torch.float8_e4m3fn).reshape(rows, H).float() for k in (-1, 1))
+    exact = v.float().to(torch.float8_e4m3fn).reshape(rows, H).float()
+    assert torch.equal(q.float(), exact) if dtype == bf16 else bool(((q.float() == exact) | (low != high)).all())
+
+
 @pytest.mark.parametrize('rows,H', [(1, 128), (9, 2048), (3, 7168)])
 def test_fp32_rows_quantise_to_the_bits_of_the_two_steps(dev, rows, H):
     """y of fp32 rows is not rounded on its way to memory, so norm and quantiser apart are the same arithmetic."""
@@ -271,3 +286,18 @@ def test_registry(dev):
     assert torch.equal(dlblas_amd.get_op('rms_norm', (x, w))(x, w), rms_norm(x, w))
     q, s = dlblas_amd.get_op('rms_norm_quant', (x, w))(x, w)
     assert torch.equal(s, rms_norm_quant(x, w)[1])
+
+
+@pytest.mark.parametrize('up', [2.0**-60, 2.0**55, 2.0**110])
+def test_quantiser_near_the_ends_of_fp32(dev, up):
+    """Groups whose h w leaves the range in which r cancels: y itself is ordinary."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(3, 256, generator=g).to(bf16)
+    w = (torch.rand(256, generator=g) + 0.5).to(bf16)
+    h = (x.double() * 2.0**-55).to(bf16) if up != 2.0**-60 else x
+    wide = (w.double() * up).to(bf16)
+    q, s = rms_norm_quant(*on(dev, h, wide), 1e-38)
+    ref_s, v = orc.quant_1x128(orc.rms_norm(h, wide, 1e-38))
+    assert float(((s.cpu().double() - ref_s).abs() / ref_s).max()) <= 42 * FP32
+    half = (v.abs() * 2.0**-4).clamp_min(2.0**-10)
+    assert float(((q.cpu().double() - v).abs() - half - 90 * FP32 * v.abs()).max()) <= 0
