@@ -123,7 +123,7 @@ int w4_chunk(int mt) { return mt == 1 ? 2 * kW4Unit : kW4Unit; }           // co
 // 20.3 -> 17.9 us, 32 experts x 16 rows x 7168 x 2048 87 -> 66); above 8 rows per expert too, because experts have more than the mean.
 W4Plan w4_plan(int64_t rows_each, bool by_expert, int64_t matrices, int64_t N, int64_t K) {
   const int mt = rows_each <= (by_expert ? 8 : 16) ? 1 : 2;
-  if (mt == 1 && matrices * N * (K / 2) <= (8 << 20)) return {false, 1, 1, 0};
+  if ((mt == 1 && matrices * N * (K / 2) <= (8 << 20)) || N * (K / 128) < 4) return {false, 1, 1, 0};
   const int chunks = static_cast<int>(ceil_div(K, w4_chunk(mt)));
   W4Plan best{true, mt, 1, chunks};
   if (by_expert) return best;

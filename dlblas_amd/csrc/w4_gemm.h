@@ -16,6 +16,8 @@
 // The waves of a workgroup take blocks of 128 columns in turn and add their sums through LDS in wave order at the end.
 #pragma once
 
+#include <type_traits>
+
 #include "fp8_gemm_common.h"
 #include "fp8_quant.h"
 #include "rms_norm.h"
@@ -96,14 +98,6 @@ __device__ __forceinline__ int nth_expert(const W4Args& p, int which, int lane) 
   return -1;
 }
 
-template <int N>
-__device__ __forceinline__ void spread_quarters(int v, int (&out)[N]) {
-  float f[N];
-  spread_quarters(__int_as_float(v), f);
-#pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = __float_as_int(f[i]);
-}
-
 // Chunks of 256 columns with groups of 128: a quarter holds 64 columns, words of a and then of b.  Afterwards a holds the columns of the
 // first group and b those of the second: quarters 0 and 1 keep their place in a, 2 and 3 in b.
 __device__ __forceinline__ void exchange_halves(v4i& a, v4i& b) {
@@ -114,13 +108,38 @@ __device__ __forceinline__ void exchange_halves(v4i& a, v4i& b) {
     a[i] = static_cast<int>(h[0]), b[i] = static_cast<int>(h[1]);
   }
 }
-// The values of the halves of the wave in both.
-__device__ __forceinline__ void spread_halves(int s, int mz, bool zeros, float* s_out, int* m_out) {
+// N consecutive values of 1 or 2 bytes in one load at any alignment of theirs.
+template <typename E, int N>
+__device__ __forceinline__ uint64_t load_packed(const E* p) {
+  constexpr int kBytes = sizeof(E) * N;
+  typedef std::conditional_t<kBytes == 8, uint64_t, std::conditional_t<kBytes == 4, uint32_t, std::conditional_t<kBytes == 2, uint16_t, uint8_t>>> word;
+  typedef word word_el __attribute__((aligned(sizeof(E))));
+  return *reinterpret_cast<const word_el*>(p);
+}
+// A word of every lane as the lanes of each half have it, in all lanes of both.
+struct Halves {
+  uint32_t low, high;
+};
+__device__ __forceinline__ Halves halves(uint32_t v) {
   typedef unsigned v2u __attribute__((ext_vector_type(2)));
-  const v2u h = __builtin_amdgcn_permlane32_swap(s, s, false, false);
-  s_out[0] = __uint_as_float(h[0]), s_out[1] = __uint_as_float(h[1]);
-  const v2u z = __builtin_amdgcn_permlane32_swap(mz, mz, false, false);
-  if (zeros) m_out[0] = static_cast<int>(z[0]), m_out[1] = static_cast<int>(z[1]);
+  const v2u h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return {h[0], h[1]};
+}
+// And as the lanes of each quarter have it; `same`: both quarters of a half hold the same.
+__device__ __forceinline__ void quarters(const Halves& h, uint32_t (&out)[4], bool low, bool same, bool high) {
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  if (same) {
+    out[0] = out[1] = h.low, out[2] = out[3] = h.high;
+    return;
+  }
+  if (low) {
+    const v2u l = __builtin_amdgcn_permlane16_swap(h.low, h.low, false, false);
+    out[0] = l[0], out[1] = l[1];
+  }
+  if (high) {
+    const v2u g = __builtin_amdgcn_permlane16_swap(h.high, h.high, false, false);
+    out[2] = g[0], out[3] = g[1];
+  }
 }
 
 // What a wave reads for one block of 128 columns: its weights, the scale (and zero point) of the quarter's group, its rows of x.
@@ -314,7 +333,9 @@ template <int T, int GROUPS, bool ZEROS, int MT, int NT, int UNITS, int PIECES>
 __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4Args p, float* sums, int chunks_each) {
   constexpr int kThreads = 64 * kW4Waves;
   constexpr int kUnitGroups = 2 * GROUPS;
-  constexpr int kLoads = GROUPS == 4 ? 2 : 1;  // of scales per unit and tile
+  constexpr int kChunkGroups = kUnitGroups * UNITS;
+  constexpr int kMine = kChunkGroups / 4 > 0 ? kChunkGroups / 4 : 1;  // of them a quarter reads the scales of, in one load
+  constexpr int kWords = (kMine + 1) / 2;                             // of them
   constexpr int kPitch = 128 * UNITS + 16;     // bytes of a row's steps in LDS, neighbouring rows on other banks
   constexpr int kPlane = 16 * MT * kPitch;     // x of a quarter
   __shared__ __attribute__((aligned(16))) char x_lds[2][4 * kPlane];
@@ -337,39 +358,51 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
   const int64_t n_base = min(n0, p.N - 1);
   const uint8_t* w_ptr = p.q + expert * p.q_es + n_base * half;
   const int64_t s0 = expert * p.s_es + n_base * p.G;
-  const uint8_t *s_ptr = static_cast<const uint8_t*>(p.s) + 2 * s0, *z_ptr = ZEROS ? p.z + s0 : p.q;
-  const uint32_t w_bytes = cols * half, s_count = cols * p.G;
-  // group of a unit whose scale this quarter reads (with groups of 32 also the next one)
-  const int my_group = GROUPS == 1 ? quarter >> 1 : GROUPS == 2 ? quarter : 2 * quarter;
-  uint32_t w_off[NT], s_off[NT];  // of rows past the matrix: past the end
+  const uint16_t* s_ptr = static_cast<const uint16_t*>(p.s) + s0;
+  const uint8_t* z_ptr = ZEROS ? p.z + s0 : nullptr;
+  const int s_last = static_cast<int>(min(p.E * p.s_es - s0, int64_t{1} << 30)) - kMine;  // where the last load of them can start
+  const uint32_t w_bytes = cols * half;
+  const int my_group = kChunkGroups < 4 ? quarter >> 1 : quarter * kMine;
+  uint32_t w_off[NT];  // of rows past the matrix: past the end
+  int s_off[NT];       // of rows past the matrix: the last row's
 #pragma unroll
-  for (int n = 0; n < NT; ++n) w_off[n] = (16 * n + l16) * half + 32 * quarter, s_off[n] = (16 * n + l16) * p.G + my_group;
+  for (int n = 0; n < NT; ++n) w_off[n] = (16 * n + l16) * half + 32 * quarter, s_off[n] = max(0, min(16 * n + l16, cols - 1)) * p.G + my_group;
   // in registers, where one v_and_or_b32 takes both
   int mask = T == kInBf16 ? 0x00780078 : 0x03c003c0, bits = T == kInBf16 ? 0x41804180 : 0x4c004c00;
   asm("" : "+s"(mask));
   asm("" : "+v"(bits));
+  uint32_t s_bf16 = p.s_type == kInBf16 ? ~0u : 0u;
+  asm("" : "+v"(s_bf16));
   const char* const x_mine = &x_lds[0][quarter * kPlane + l16 * kPitch];
 
   struct Chunk {
     v4i w[NT][UNITS][2];
-    uint32_t s[NT][UNITS][kLoads], z[NT][UNITS][kLoads];
+    uint64_t s[NT];  // kMine scales
+    uint32_t z[NT];
   };
   auto load = [&](int c, Chunk& b) {
     const bool in = c < last && w_bytes > 0;  // a scalar offset stays below the length of its buffer
     const uint32_t at = in ? c * UNITS : 0;
-    const auto w_src = make_rsrc(w_ptr, in ? w_bytes : 0), s_src = make_rsrc(s_ptr, in ? 2 * s_count : 0), z_src = make_rsrc(z_ptr, ZEROS && in ? s_count : 0);
+    const auto w_src = make_rsrc(w_ptr, in ? w_bytes : 0);
+    const auto s_src = make_rsrc(reinterpret_cast<const uint8_t*>(s_ptr), in ? 2u * cols * p.G : 0), z_src = make_rsrc(ZEROS ? z_ptr : p.q, ZEROS && in ? cols * p.G : 0);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
+      for (int u = 0; u < UNITS; ++u)
 #pragma unroll
         for (int k = 0; k < 2; ++k) b.w[n][u][k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(w_src, w_off[n] + 128 * u + 16 * k, 128 * at, 0));
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          b.s[n][u][j] = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * (s_off[n] + kUnitGroups * u + j), 2 * kUnitGroups * at, 0);
-          if (ZEROS) b.z[n][u][j] = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off[n] + kUnitGroups * u + j, kUnitGroups * at, 0);
-        }
+      // A load touches 16 cache lines however little it takes of each, and beside the matrices' bytes that is what these kernels wait for:
+      // one load for all that the lane needs (32 experts x 4 rows x 4096 x 7168, groups of 32 with zero points, a load for each scale
+      // 175 us, so 137).  Near the end of the tensor it starts earlier and the rest moves down in multiply().
+      if (kMine == 1) {
+        b.s[n] = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * s_off[n], 2 * kUnitGroups * at, 0);
+        if (ZEROS) b.z[n] = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off[n], kUnitGroups * at, 0);
+      } else {
+        const int from = min(s_off[n] + c * kChunkGroups, s_last);
+        b.s[n] = load_packed<uint16_t, kMine>(s_ptr + from);
+        if (ZEROS) b.z[n] = static_cast<uint32_t>(load_packed<uint8_t, kMine>(z_ptr + from));
       }
+    }
   };
   for (; row0 < row_end; row0 += 16 * MT) {
     const int rows = static_cast<int>(min(row_end - row0, static_cast<int64_t>(16 * MT)));
@@ -409,28 +442,47 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](int c, Chunk& b, int buf) {
+      // a scale in the upper 16 bits; not by a branch, which would part the products
+      const auto widened = [&](uint32_t up) {
+        const uint32_t from_half = __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(up >> 16))));
+        return __uint_as_float((up & s_bf16) | (from_half & ~s_bf16));
+      };
+      // scales (widened where a lane read one) and zero points, of the quarters 0, 1 and 2, 3 in words of their own
+      Halves sh[NT][kWords], zh[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int mine = p.G - (c * kChunkGroups + my_group);  // groups left in the row
+        if (kMine == 1) {
+          sh[n][0] = halves(mine > 0 ? __float_as_uint(widened(static_cast<uint32_t>(b.s[n]) << 16)) : 0u);
+          if (ZEROS) zh[n] = halves(b.z[n]);
+          continue;
+        }
+        const int down = max(0, min(s_off[n] + c * kChunkGroups - s_last, kMine - 1));
+        const uint64_t s = mine >= kMine ? b.s[n] >> (16 * down) : b.s[n] >> (16 * down) & ((uint64_t{1} << (16 * max(0, mine))) - 1);
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) sh[n][j] = halves(static_cast<uint32_t>(s >> (32 * j)));
+        if (ZEROS) zh[n] = halves(b.z[n] >> (8 * down));
+      }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        float sc[NT][kUnitGroups];
-        int minus[NT][kUnitGroups];  // -(16 + z) twice: the matrix through which the constant leaves
+        uint32_t sw[NT][kWords][4], zw[NT][4];  // by quarter; of the unit's alone
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int j = 0; j < kLoads; ++j) {
-            float s = p.s_type == kInBf16 ? __uint_as_float(b.s[n][u][j] << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s[n][u][j])));
-            if ((c * UNITS + u) * kUnitGroups + my_group + j >= p.G) s = 0.f;  // past the row's last group: the next row's
-            const int mz = ZEROS ? static_cast<int>((b.z[n][u][j] << (T == kInBf16 ? 3 : 6)) * 0x10001u + (static_cast<uint32_t>(bits) | 0x80008000u)) : 0;
-            if (GROUPS == 1) {
-              spread_halves(__float_as_int(s), mz, ZEROS, sc[n], minus[n]);
-            } else {
-              float s4[4];
-              int m4[4] = {};
-              spread_quarters(s, s4);
-              if (ZEROS) spread_quarters(mz, m4);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sc[n][(kLoads * i + j) % kUnitGroups] = s4[i], minus[n][(kLoads * i + j) % kUnitGroups] = m4[i];
-            }
-          }
+          for (int j = 0; j < kWords; ++j) quarters(sh[n][j], sw[n][j], UNITS == 1 || u == 0, kChunkGroups < 4, UNITS == 1 || u == 1);
+          if (ZEROS) quarters(zh[n], zw[n], UNITS == 1 || u == 0, kChunkGroups < 4, UNITS == 1 || u == 1);
+        }
+        const auto scale = [&](int n, int g) {  // g of the chunk
+          const int q = kChunkGroups < 4 ? 2 * g : g / kMine, j = kChunkGroups < 4 ? 0 : g % kMine;
+          const uint32_t word = sw[n][j / 2][q];
+          return kMine == 1 ? __uint_as_float(word) : widened(j % 2 ? word & 0xffff0000u : word << 16);
+        };
+        // -(16 + z) of a group twice: the matrix through which the constant leaves
+        const auto minus = [&](int n, int g) {
+          const int q = kChunkGroups < 4 ? 2 * g : g / kMine, j = kChunkGroups < 4 ? 0 : g % kMine;
+          const uint32_t z = (zw[n][q] >> (8 * j)) & 0xffu;
+          return static_cast<int>(z * (T == kInBf16 ? 0x80008u : 0x400040u) + (static_cast<uint32_t>(bits) | 0x80008000u));
+        };
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (GROUPS == 1)
@@ -441,6 +493,10 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
 #pragma unroll
         for (int g = 0; g < kUnitGroups; ++g) {
           v4f sum[MT][NT];
+          float sc[NT];
+          int constant[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sc[n] = scale(n, u * kUnitGroups + g), constant[n] = ZEROS ? minus(n, u * kUnitGroups + g) : static_cast<int>(T == kInBf16 ? 0xc1c0c1c0 : 0xce00ce00);
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -458,7 +514,7 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 v[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & mask) | bits;
-                c16[j] = ZEROS ? minus[n][g] : static_cast<int>(T == kInBf16 ? 0xc1c0c1c0 : 0xce00ce00);
+                c16[j] = constant[n];
               }
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
@@ -472,7 +528,7 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(sc[n][g], sum[m][n][r], acc[m][n][r]);
+              for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(sc[n], sum[m][n][r], acc[m][n][r]);
         }
       }
     };

@@ -222,3 +222,19 @@ def test_native_path_takes_plain_calls_and_registry(dev):
     start, end = on(dev, *ranges([4, 0, 16])[:2])
     assert mod._fast.w4_gemm(x, q[0], s[0], None) is not None and mod._fast.w4_gemm_grouped(x, q, s, start, end, z) is not None
     assert torch.equal(dlblas_amd.get_op('w4_gemm', (x, q[0], s[0]))(x, q[0], s[0]), w4_gemm(x, q[0], s[0]))
+
+
+@pytest.mark.parametrize('zeros', [False, True])
+@pytest.mark.parametrize('M,N,K,group', [(20, 3, 288, 32), (33, 1, 544, 32), (17, 2, 320, 64), (40, 129, 96, 32), (3, 8203, 2080, 32), (16, 8195, 2112, 64),
+                                         (2, 8193, 2176, 128)])
+def test_scales_at_the_end_of_their_tensor(dev, M, N, K, group, zeros):
+    """A lane reads several scales at once: rows with an odd number of groups, and a last row whose scales are the last bytes there are
+    (a NaN behind them would show)."""
+    q, s, z = (None if t is None else t[0] for t in weights(1, N, K, group, zeros, bf16))
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(N)).to(bf16)
+    room = torch.full((s.numel() + 8, ), float('nan'), dtype=bf16, device=dev)
+    sd = room[:s.numel()].view(s.shape).copy_(s)
+    qd, zd, xd = on(dev, q, z, x)
+    check(w4_gemm(xd, qd, sd, zd), x, q, s, z, f'{M}x{N}x{K}/{group}')
+    room = torch.full((s.numel() + 8, ), float('nan'), dtype=bf16, device=dev)
+    check(w4_gemm(xd, qd, room[7:7 + s.numel()].view(s.shape).copy_(s), zd), x, q, s, z, f'{M}x{N}x{K}/{group}, other place')
