@@ -127,13 +127,20 @@ W4Plan w4_plan(int64_t rows_each, bool by_expert, int64_t matrices, int64_t N, i
   const int chunks = static_cast<int>(ceil_div(K, w4_chunk(mt)));
   W4Plan best{true, mt, 1, chunks};
   if (by_expert) return best;
-  // time in chunks of one workgroup: rounds over the chip x chunks, which go in pairs, the second launch and the sums' way through memory
+  // Time in chunks of one workgroup alone on its CU, about a microsecond each: rounds over the chip x chunks, which go in pairs, and with
+  // slices the second launch and the sums' way through memory at 5 TB/s.  Workgroups that share a CU overlap, the more the less they
+  // have to compute.  Slices that this picks, and others (us): 1 x 7168 x 18432 nine 20.6, two 24.0, four 21.2; 16 rows nine 24.7, two
+  // 25.0, four 26.0; 1 x 7168 x 7168 four 11.6, one 16.1, seven 12.5; 64 x 36864 x 7168 two 87, one 92, seven 99; over 18 shapes of 1 to 64 rows
+  // 1.3 % behind the best number for each.
   const int64_t base = ceil_div(N, w4_columns(mt)) * ceil_div(rows_each, 16 * mt);
+  const double beside = rows_each <= 4 ? 0.75 : 0.85;
   double best_cost = 1e30;
   for (int slices = 1; slices <= 16 && slices <= chunks; ++slices) {
     const int each = static_cast<int>(ceil_div(chunks, slices));
     if (ceil_div(chunks, each) != slices) continue;
-    const double cost = static_cast<double>(ceil_div(base * slices, kW4Cus)) * ((each + 1) / 2 * 2) + (slices > 1 ? 3 + 0.5 * slices : 0);
+    const int64_t rounds = ceil_div(base * slices, kW4Cus);
+    const double sums = slices > 1 ? 3 + 0.3 * slices + 8e-6 / 5 * slices * static_cast<double>(rows_each) * static_cast<double>(N) : 0;
+    const double cost = (rounds == 1 ? 1 : beside * static_cast<double>(rounds)) * ((each + 1) / 2 * 2) + sums;
     if (cost < best_cost) best_cost = cost, best.slices = slices, best.chunks = each;
   }
   return best;
