@@ -117,31 +117,37 @@ constexpr int kW4Cus = 256;
 int w4_columns(int mt) { return mt == 1 ? 64 : 128; }                       // of a workgroup that shares x
 int w4_chunk(int mt) { return mt == 1 ? 2 * kW4Unit : kW4Unit; }           // columns of x
 
-// rows_each: of one matrix.  Up to 8 MB of weights the workgroups that share x are too few to fill the chip, or pay a second launch
-// for their slices (1 x 2112 x 7168 7.6 against 8.1 us, 1 x 512 x 2048 4.3 / 5.6; 16 x 4096 x 7168, 15 MB, 12.0 / 10.6, 1 x 7168 x 18432
-// 28 / 21, 16 x 7168 x 18432 51 / 26.5, 32 experts x 4 rows x 4096 x 7168 197 / 102).  Above 16 rows tiles of 32 x 32 (32 x 7168 x 7168
-// 20.3 -> 17.9 us, 32 experts x 16 rows x 7168 x 2048 87 -> 66); above 8 rows per expert too, because experts have more than the mean.
+// rows_each: of one matrix.  Above 16 rows tiles of 32 x 32 (32 x 7168 x 7168 20.3 -> 17.9 us, 32 experts x 16 rows x 7168 x 2048 87 -> 66);
+// above 8 rows per expert too, because experts have more than the mean.  Below, whichever of the two kernels is estimated faster, in us:
+//   shared x   a chunk of a workgroup alone on its CU is about one; rounds over the chip x chunks, which go in pairs.  Workgroups beside
+//              each other on a CU overlap, the more the less they have to compute.  With slices a second launch and the sums' way through
+//              memory at 5 TB/s.  Slices that this picks, and others: 1 x 7168 x 18432 nine 20.6, two 24.0, four 21.2; 16 rows nine 24.7, two
+//              25.0, four 26.0; 1 x 7168 x 7168 four 11.6, one 16.1, seven 12.5; 64 x 36864 x 7168 two 87, one 92, seven 99.
+//   K over the waves   a launch, the columns of K, each the longer the more rows there are, further rounds, at most 2.4 TB/s.
+// Measured, K over the waves / shared: 1 x 512 x 2048 4.3 / 5.9, 16 x 512 x 2048 5.6 / 6.9, 1 x 2112 x 7168 7.6 / 7.6, 16 x 2112 x 7168 11.8 / 8.4,
+// 1 x 128 x 18432 14.5 / 8.4, 16 x 1024 x 14336 21.3 / 10.2, 1 x 16384 x 1024 9.2 / 4.8, 1 x 4096 x 4096 5.8 / 6.9, 8 experts x 1 row x 512 x 7168
+// 8.1 / 17.1, 32 experts x 4 rows x 4096 x 7168 197 / 102.
 W4Plan w4_plan(int64_t rows_each, bool by_expert, int64_t matrices, int64_t N, int64_t K) {
   const int mt = rows_each <= (by_expert ? 8 : 16) ? 1 : 2;
-  if ((mt == 1 && matrices * N * (K / 2) <= (8 << 20)) || N * (K / 128) < 4) return {false, 1, 1, 0};
+  const W4Plan waves{false, 1, 1, 0};
+  if (N * (K / 128) < 4) return waves;  // fewer scales than a lane of the other kernel reads at once
   const int chunks = static_cast<int>(ceil_div(K, w4_chunk(mt)));
   W4Plan best{true, mt, 1, chunks};
-  if (by_expert) return best;
-  // Time in chunks of one workgroup alone on its CU, about a microsecond each: rounds over the chip x chunks, which go in pairs, and with
-  // slices the second launch and the sums' way through memory at 5 TB/s.  Workgroups that share a CU overlap, the more the less they
-  // have to compute.  Slices that this picks, and others (us): 1 x 7168 x 18432 nine 20.6, two 24.0, four 21.2; 16 rows nine 24.7, two
-  // 25.0, four 26.0; 1 x 7168 x 7168 four 11.6, one 16.1, seven 12.5; 64 x 36864 x 7168 two 87, one 92, seven 99; over 18 shapes of 1 to 64 rows
-  // 1.3 % behind the best number for each.
-  const int64_t base = ceil_div(N, w4_columns(mt)) * ceil_div(rows_each, 16 * mt);
-  const double beside = rows_each <= 4 ? 0.75 : 0.85;
+  const int64_t base = matrices * ceil_div(N, w4_columns(mt)) * ceil_div(rows_each, 16 * mt);
+  const double beside = rows_each <= 4 ? 0.75 : 0.85, rows = static_cast<double>(rows_each), n = static_cast<double>(N), k = static_cast<double>(K);
   double best_cost = 1e30;
-  for (int slices = 1; slices <= 16 && slices <= chunks; ++slices) {
+  for (int slices = 1; slices <= (by_expert ? 1 : 16) && slices <= chunks; ++slices) {
     const int each = static_cast<int>(ceil_div(chunks, slices));
     if (ceil_div(chunks, each) != slices) continue;
     const int64_t rounds = ceil_div(base * slices, kW4Cus);
-    const double sums = slices > 1 ? 3 + 0.3 * slices + 8e-6 / 5 * slices * static_cast<double>(rows_each) * static_cast<double>(N) : 0;
+    const double sums = slices > 1 ? 3 + 0.3 * slices + 8e-6 / 5 * slices * rows * n : 0;
     const double cost = (rounds == 1 ? 1 : beside * static_cast<double>(rounds)) * ((each + 1) / 2 * 2) + sums;
     if (cost < best_cost) best_cost = cost, best.slices = slices, best.chunks = each;
+  }
+  if (mt == 1) {
+    const double rounds = static_cast<double>(ceil_div(matrices * ceil_div(N, 16), kW4Cus));
+    const double by_columns = 6.2e-4 * k * (1 + 0.055 * rows) + 1.5 * (rounds - 1), by_bytes = static_cast<double>(matrices) * n * k / 2 / 2.4e6;
+    if (2.9 + std::max(by_columns, by_bytes) < best_cost + (best.slices > 1 ? 0.5 : 2.6) + 0.05 * rows) return waves;
   }
   return best;
 }

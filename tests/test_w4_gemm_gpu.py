@@ -129,6 +129,7 @@ def ranges(counts, gaps=0):
     ([1], 0, 16, 128, 128, False), ([0, 3, 0, 1], 0, 40, 256, 64, True), ([5, 0, 0, 16, 17, 2, 0], 3, 33, 160, 32, True), ([40, 1, 70, 0], 0, 64, 384, 128, False),
     ([1] * 70 + [0] * 70 + [2] * 3, 0, 17, 128, 64, False), ([0, 0, 0], 2, 16, 128, 128, False), ([2] * 8, 1, 96, 2048, 128, True),
     ([3, 0, 20, 1], 1, 1056, 8288, 32, True), ([40, 0, 9, 33, 12], 0, 1000, 4224, 64, False), ([1, 2, 1, 0, 0, 5, 1, 1], 2, 1025, 4480, 128, True),
+    ([3, 0, 20, 1], 1, 4105, 544, 32, True), ([1, 2, 1, 0, 0, 5, 1, 1], 0, 5003, 1056, 32, False), ([1] * 12, 0, 2051, 1088, 64, True), ([2, 1, 4, 0] * 4, 2, 4100, 640, 128, False),
 ])
 def test_product_by_expert(dev, counts, gaps, N, K, group, zeros, dtype):
     start, end, rows = ranges(counts, gaps)
@@ -226,7 +227,7 @@ def test_native_path_takes_plain_calls_and_registry(dev):
 
 @pytest.mark.parametrize('zeros', [False, True])
 @pytest.mark.parametrize('M,N,K,group', [(20, 3, 288, 32), (33, 1, 544, 32), (17, 2, 320, 64), (40, 129, 96, 32), (3, 8203, 2080, 32), (16, 8195, 2112, 64),
-                                         (2, 8193, 2176, 128)])
+                                         (2, 8193, 2176, 128), (3, 203, 18464, 32), (16, 195, 12352, 64), (2, 193, 9344, 128), (3, 16401, 544, 32), (16, 9003, 608, 32)])
 def test_scales_at_the_end_of_their_tensor(dev, M, N, K, group, zeros):
     """A lane reads several scales at once: rows with an odd number of groups, and a last row whose scales are the last bytes there are
     (a NaN behind them would show)."""
