@@ -82,11 +82,11 @@ __device__ __forceinline__ void spread_quarters(float v, float (&out)[N]) {
   out[0] = __uint_as_float(lo[0]), out[1 % N] = __uint_as_float(lo[1]), out[2 % N] = __uint_as_float(hi[0]), out[3 % N] = __uint_as_float(hi[1]);
 }
 
-// The which-th expert that has rows, -1: there are not so many.
+// The which-th expert that has rows among those there are, -1: there are not so many.
 __device__ __forceinline__ int nth_expert(const W4Args& p, int which, int lane) {
   for (int e0 = 0; e0 < p.E; e0 += 64) {
     const int i = min(e0 + lane, p.E - 1);
-    uint64_t some = __ballot(e0 + lane < p.E && p.row_end[i] > p.row_start[i]);
+    uint64_t some = __ballot(e0 + lane < p.E && min(static_cast<int64_t>(p.row_end[i]), p.rows) > max(p.row_start[i], 0));
     const int n = __popcll(some);
     if (which >= n) {
       which -= n;

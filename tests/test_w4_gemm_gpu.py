@@ -239,3 +239,14 @@ def test_scales_at_the_end_of_their_tensor(dev, M, N, K, group, zeros):
     check(w4_gemm(xd, qd, sd, zd), x, q, s, z, f'{M}x{N}x{K}/{group}')
     room = torch.full((s.numel() + 8, ), float('nan'), dtype=bf16, device=dev)
     check(w4_gemm(xd, qd, room[7:7 + s.numel()].view(s.shape).copy_(s), zd), x, q, s, z, f'{M}x{N}x{K}/{group}, other place')
+
+
+@pytest.mark.parametrize('N,K', [(48, 256), (4105, 544)])
+def test_ranges_outside_the_rows_take_no_place(dev, N, K):
+    """One row and eight experts: seven ranges name rows that there are not, and only the last one's is there."""
+    q, s, _ = weights(8, N, K, 32, False, bf16)
+    x = torch.randn(1, K, generator=torch.Generator().manual_seed(8)).to(bf16)
+    start = torch.tensor([1, 5, -4, 1000, 2, 3, 1, 0], dtype=torch.int32)
+    end = torch.tensor([4, 9, 0, 2000, 3, 9, 2, 1], dtype=torch.int32)
+    y = w4_gemm_grouped(*on(dev, x, q, s, start, end))
+    check(y, x, q[7], s[7], None, f'{N}x{K}')
