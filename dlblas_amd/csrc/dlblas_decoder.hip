@@ -55,6 +55,24 @@ RowShape row_shape(int64_t H, int want_chunks) {
   return {static_cast<int>(ceil_div(ceil_div(chunks, c), 64) * 64), c};
 }
 
+// Rows of a multiple of eight up to 256 columns share waves: 2^20 x 128, the norm 266 -> 98 us (5.5 TB/s), with quantiser 324 -> 105, its gradient
+// 2807 -> 296; 64 x 128 3.9 -> 3.8.
+constexpr int kNarrowThreads = 256;  // of a workgroup
+constexpr std::integral_constant<int, 1> kOne;
+constexpr std::integral_constant<int, 64> kWave;
+template <typename F>
+bool with_lanes(int64_t H, F f) {
+  if (H > 256) return false;
+  H <= 128 ? f(std::integral_constant<int, 16>()) : f(std::integral_constant<int, 32>());
+  return true;
+}
+
+// A grid of `blocks` workgroups in two dimensions.
+dim3 row_grid(int64_t blocks) {
+  constexpr int64_t kMost = 1 << 21;  // of up to 1024 threads, of which one dimension holds fewer than 2^32
+  return dim3(static_cast<unsigned>(std::min(blocks, kMost)), static_cast<unsigned>(ceil_div(blocks, kMost)));
+}
+
 int check_norm(const void* x, const void* residual, int dtype, const void* weight, int weight_dtype, const void* sum, int64_t rows,
                int64_t H) {
   if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
@@ -73,23 +91,38 @@ int check_norm(const void* x, const void* residual, int dtype, const void* weigh
 
 template <bool QUANT>
 int launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
-  const RowShape shape = row_shape(a.H, 2);  // 8192 x 7168 quantised: one chunk a thread 95 us, two 78, four 78; a single row 3.5, 3.7, 4.9
-  const dim3 grid(static_cast<unsigned>(a.rows)), block(shape.threads);
+  const auto launch = [&](auto t, auto res, auto whole, auto c, auto lanes, int threads, int beside) {
+    hipLaunchKernelGGL((rms_norm_kernel<t(), QUANT, res(), whole(), c(), lanes()>), row_grid(ceil_div(a.rows, beside)), dim3(threads, beside), 0, st, a);
+  };
   with_type(dtype, [&](auto t) {
     with_flag(a.res != nullptr, [&](auto res) {
+      if (a.H % 8 == 0) {
+        constexpr std::true_type whole;
+        if (with_lanes(a.H, [&](auto lanes) { launch(t, res, whole, kOne, lanes, lanes(), kNarrowThreads / lanes()); })) return;
+      }
+      const RowShape shape = row_shape(a.H, 2);  // 8192 x 7168 quantised: one chunk a thread 95 us, two 78, four 78; a single row 3.5, 3.7, 4.9
       with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
         if (QUANT || a.H % 8 == 0)
-          hipLaunchKernelGGL((rms_norm_kernel<t(), QUANT, res(), true, c()>), grid, block, 0, st, a);
-        else
-          hipLaunchKernelGGL((rms_norm_kernel<t(), false, res(), false, c()>), grid, block, 0, st, a);
+          launch(t, res, std::true_type(), c, kWave, shape.threads, 1);
+        else if constexpr (!QUANT)
+          launch(t, res, std::false_type(), c, kWave, shape.threads, 1);
       });
     });
   });
   return finish("rms_norm");
 }
 
-// Workgroups of the backward pass, each of which leaves a share of dw (4096 x 7168: 256 of them 65 us, 384 61, 512 51, 768 64, 1024 58).
-int norm_grad_blocks(int64_t rows) { return static_cast<int>(rows < 512 ? rows : 512); }
+// Shares of dw that the backward pass leaves, one of a workgroup (4096 x 7168: 256 of them 65 us, 384 61, 512 51, 768 64, 1024 58).  Of fewer
+// than eight waves more where each has eight rows or more, for waves enough: 131072 x 512 390 -> 113 us, 65536 x 2048
+// 307 -> 197; of narrow rows one of a wave.
+int norm_grad_shares(int64_t rows, int64_t H) {
+  if (H % 8 != 0 || H > 256) {
+    const int64_t most = std::max<int64_t>(512, 4096 / ceil_div(H, 512));
+    return static_cast<int>(std::min(rows, std::max<int64_t>(512, std::min(most, rows / 8))));
+  }
+  const int64_t rows_each = kNarrowThreads / (H <= 128 ? 16 : 32);
+  return static_cast<int>(std::min<int64_t>(ceil_div(rows, rows_each), 512) * (kNarrowThreads / 64));
+}
 
 // ---- tokens by expert -------------------------------------------------------------------------------------------------
 
@@ -103,6 +136,9 @@ int check_rows(int64_t tokens, int64_t H, int64_t topk, int64_t num_rows) {
   return DLB_OK;
 }
 
+// Whether a launch of its own adds up the counts of the workgroups of slots before each, instead of each for itself, which goes with the
+// square of their number: 60000 tokens x 8 slots, 256 experts 43 and 43 us, 66000 44 and 63, 10^6 498 and 7727, 131072 x 8, 32 experts 62 and 28.
+bool sort_scans(int64_t blocks, int64_t experts) { return blocks * blocks * experts > 60000000; }
 int64_t sort_blocks(int64_t slots) { return slots > 0 ? ceil_div(slots, kSortBlockSlots) : 1; }
 
 // ---- 4-bit weights ----------------------------------------------------------------------------------------------------
@@ -217,7 +253,7 @@ int dlb_rms_norm_quant(const void* x, int64_t x_row_stride, const void* residual
 }
 
 size_t dlb_rms_norm_backward_workspace_bytes(int64_t rows, int64_t H) {
-  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::norm_grad_blocks(rows)) * H * sizeof(float) : 0;
+  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::norm_grad_shares(rows, H)) * H * sizeof(float) : 0;
 }
 
 int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
@@ -239,27 +275,33 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
     if (dw && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int blocks = norm_grad_blocks(rows);
+  const int shares = norm_grad_shares(rows, H);
   if (rows > 0) {
     NormGradArgs a{};
     a.dy = dy, a.dsum = dsum, a.h = h, a.w = weight, a.dx = dx, a.dw_part = dw ? static_cast<float*>(workspace) : nullptr;
     a.rows = rows, a.dy_rs = dy_row_stride, a.dsum_rs = dsum_row_stride, a.h_rs = h_row_stride, a.dx_rs = dx_row_stride;
     a.H = static_cast<int>(H), a.w_f32 = weight_dtype == kInF32, a.eps = eps;
-    // Two workgroups of up to 512 threads fit a CU beside each other at these registers.  One and two chunks a thread, 4096 rows: of 4096
-    // columns in 16 bits 24 and 29 us, of 5120 44 and 35, of 7168 64 and 51; of 4096 in fp32 40 and 47, of 8192 in fp32 90 and 97.
-    const RowShape shape = row_shape(H, dtype != kInF32 && H > 4096 ? 2 : 1);
-    const dim3 grid(blocks), block(shape.threads);
+    const auto launch = [&](auto t, auto ds, auto whole, auto c, auto lanes, int grid, int threads, int beside) {
+      hipLaunchKernelGGL((rms_norm_backward_kernel<t(), ds(), whole(), c(), lanes()>), dim3(grid), dim3(threads, beside), 0, st, a);
+    };
     with_type(dtype, [&](auto t) {
       with_flag(dsum != nullptr, [&](auto ds) {
+        if (H % 8 == 0) {
+          constexpr std::true_type whole;
+          if (with_lanes(H, [&](auto lanes) { launch(t, ds, whole, kOne, lanes, shares / (kNarrowThreads / 64), lanes(), kNarrowThreads / lanes()); })) return;
+        }
+        // Two workgroups of up to 512 threads fit a CU beside each other at these registers.  One and two chunks a thread, 4096 rows: of 4096
+        // columns in 16 bits 24 and 29 us, of 5120 44 and 35, of 7168 64 and 51; of 4096 in fp32 40 and 47, of 8192 in fp32 90 and 97.
+        const RowShape shape = row_shape(H, dtype != kInF32 && H > 4096 ? 2 : 1);
         with_flag(H % 8 == 0, [&](auto whole) {
-          with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { hipLaunchKernelGGL((rms_norm_backward_kernel<t(), ds(), whole(), c()>), grid, block, 0, st, a); });
+          with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, ds, whole, c, kWave, shares, shape.threads, 1); });
         });
       });
     });
     if (int rc = finish("rms_norm_backward")) return rc;
   }
   if (!dw) return DLB_OK;
-  const NormDwArgs d{static_cast<const float*>(workspace), dw, blocks, static_cast<int>(H), weight_dtype};
+  const NormDwArgs d{static_cast<const float*>(workspace), dw, shares, static_cast<int>(H), weight_dtype};
   hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(H, 64))), dim3(64 * kDwWaves), 0, st, d);
   return finish("rms_norm_backward (dw)");
 }
@@ -267,7 +309,7 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
 size_t dlb_moe_permute_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts) {
   if (tokens <= 0 || topk <= 0 || experts <= 0) return 0;
   const int64_t blocks = dlb::sort_blocks(tokens * topk);
-  return blocks > 1 ? static_cast<size_t>(blocks) * experts * sizeof(int32_t) : 0;
+  return blocks > 1 ? static_cast<size_t>(dlb::sort_scans(blocks, experts) ? blocks + 1 : blocks) * experts * sizeof(int32_t) : 0;
 }
 
 int dlb_moe_permute(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k, const void* x, int64_t x_row_stride,
@@ -330,20 +372,25 @@ int dlb_moe_permute(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_
     const int64_t want = ceil_div(std::max(tokens * c.parts, num_rows), threads / 64), most = 512 * (kSortThreads / threads);
     const dim3 grid(static_cast<unsigned>(want < most ? want : most));
     with_flag(whole_rows, [&](auto whole) {
-      hipLaunchKernelGGL((moe_sort_rows_kernel<true, whole()>), grid, dim3(threads), lds + threads * sizeof(int), st, a, 1, c);
+      hipLaunchKernelGGL((moe_sort_rows_kernel<true, whole()>), grid, dim3(threads), lds + threads * sizeof(int), st, a, 1, false, c);
     });
     return finish("moe_permute");
   }
   const int64_t blocks = sort_blocks(a.n);
+  const bool summed = sort_scans(blocks, a.E);
   if (blocks > 1) {
     hipLaunchKernelGGL(moe_sort_count_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), static_cast<size_t>(a.E) * sizeof(int), st, a);
     if (int rc = finish("moe_permute (count)")) return rc;
+    if (summed) {
+      hipLaunchKernelGGL(moe_sort_scan_kernel, dim3(static_cast<unsigned>(ceil_div(a.E, 64))), dim3(64), 0, st, a, static_cast<int>(blocks));
+      if (int rc = finish("moe_permute (scan)")) return rc;
+    }
   }
   // further workgroups where the tables by row are longer than those by slot
   int64_t grid = ceil_div(num_rows, 4 * kSortThreads);
   if (grid > 256) grid = 256;
   if (grid < blocks) grid = blocks;
-  hipLaunchKernelGGL((moe_sort_rows_kernel<false, true>), dim3(static_cast<unsigned>(grid)), dim3(kSortThreads), lds, st, a, static_cast<int>(blocks), c);
+  hipLaunchKernelGGL((moe_sort_rows_kernel<false, true>), dim3(static_cast<unsigned>(grid)), dim3(kSortThreads), lds, st, a, static_cast<int>(blocks), summed, c);
   if (int rc = finish("moe_permute (tables)")) return rc;
   if (!copies) return DLB_OK;
   constexpr int kWaves = kSortCopyThreads / 64;
@@ -373,7 +420,7 @@ int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, cons
   const UnpermuteArgs a{rows, row_index, weights, out, rows_row_stride, out_row_stride, tokens, num_rows, static_cast<int>(H), static_cast<int>(topk)};
   int64_t parts = ceil_div(H, 512);
   if (parts > 64) parts = 64;
-  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(parts));
+  const dim3 rows_grid = row_grid(tokens), grid(rows_grid.x, static_cast<unsigned>(parts), rows_grid.y);
   with_type(dtype, [&](auto t) {
     with_flag(H % 8 == 0, [&](auto whole) { hipLaunchKernelGGL((moe_unpermute_kernel<t(), whole()>), grid, dim3(64), 0, static_cast<hipStream_t>(stream), a); });
   });
@@ -404,12 +451,11 @@ int dlb_moe_unpermute_backward(const void* dout, int64_t dout_row_stride, const 
   a.zero_blocks = static_cast<int>(num_rows < 1024 ? num_rows : 1024);
   const RowShape shape = row_shape(H, 2);  // 4096 tokens of 7168 x 8 rows: one chunk a thread 219 us, two 195, four 197
   const int64_t grid = tokens + a.zero_blocks;
-  if (grid > (1ll << 31) - 1) return fail(DLB_ERR_BAD_SHAPE, "tokens=%lld beyond the supported range", (long long)tokens);
   with_type(dtype, [&](auto t) {
     with_flag(dweights != nullptr, [&](auto dw) {
       with_flag(H % 8 == 0, [&](auto whole) {
         with_chunks<1, 2, 4>(shape.chunks, [&](auto c) {
-          hipLaunchKernelGGL((moe_unpermute_backward_kernel<t(), dw(), whole(), c()>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads), 0,
+          hipLaunchKernelGGL((moe_unpermute_backward_kernel<t(), dw(), whole(), c()>), row_grid(grid), dim3(shape.threads), 0,
                              static_cast<hipStream_t>(stream), a);
         });
       });
@@ -437,7 +483,7 @@ int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, c
   if (K % group != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of the group size %lld", (long long)K, (long long)group);
   if (!row_start != !row_end) return fail(DLB_ERR_NULL_POINTER, "row_start and row_end come together");
   if (!row_start && experts != 1) return fail(DLB_ERR_BAD_SHAPE, "%lld experts without row ranges", (long long)experts);
-  if (rows > (1ll << 31) - 1 || N > (1ll << 30) || K > (1ll << 30) || experts > (1 << 20))
+  if (rows > (1ll << 31) - 1 || N > (1ll << 27) || K > (1ll << 30) || experts > (1 << 20))
     return fail(DLB_ERR_BAD_SHAPE, "rows=%lld / N=%lld / K=%lld / experts=%lld beyond the supported range", (long long)rows, (long long)N, (long long)K,
                 (long long)experts);
   if (rows == 0 || N == 0 || experts == 0) return DLB_OK;

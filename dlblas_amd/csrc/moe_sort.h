@@ -30,7 +30,7 @@ struct SortArgs {
   int32_t* m_indices;   // [R]: expert of every row of a span, -1 past the last span
   int32_t* row_start;   // [E]
   int32_t* row_end;     // [E]: one past the last row with a slot
-  int32_t* hist;        // [blocks][E], used by launches of more than one workgroup of slots
+  int32_t* hist;        // [blocks][E], used by launches of more than one workgroup of slots; summed: [blocks + 1][E], slots before
   int64_t ids_s0, ids_s1;
   int64_t n;            // T * topk
   int64_t R;
@@ -145,13 +145,32 @@ __device__ __forceinline__ void clear_row(const SortCopyArgs& p, int64_t r, int 
   for (int g = lane; g < p.groups; g += 64) p.rows_s[r * p.groups + g] = 0.f;
 }
 
+// Counts to slots in the workgroups before, an expert a thread, the totals in a row of their own.
+__global__ void __launch_bounds__(64) moe_sort_scan_kernel(const SortArgs p, int slot_blocks) {
+  const int e = blockIdx.x * 64 + threadIdx.x;
+  if (e >= p.E) return;
+  int sum = 0;
+  for (int b = 0; b < slot_blocks; b += 16) {
+    int c[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) c[u] = p.hist[static_cast<int64_t>(min(b + u, slot_blocks - 1)) * p.E + e];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      if (b + u >= slot_blocks) break;
+      p.hist[static_cast<int64_t>(b + u) * p.E + e] = sum;
+      sum += c[u];
+    }
+  }
+  p.hist[static_cast<int64_t>(slot_blocks) * p.E + e] = sum;
+}
+
 // Rows of the slots of workgroup blockIdx, and its share of the tables by row.  Workgroups past the slots' share only the latter.
 // COPY: there is one workgroup's worth of slots, and every workgroup finds the rows of all of them and copies its share of the tokens, so
 // that a few tokens take one launch.  Then only the first workgroup writes the tables by slot and expert.
 // 32768 slots 5.8 us and 4.7 for the counts before it, both latency: loads, LDS atomics, barriers.
 // LDS: before [E], total [E], start [E + 1], wave_cnt [16][E] of 16-bit counts; COPY: rows [threads].
 template <bool COPY, bool WHOLE>
-__global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortArgs p, int slot_blocks, const SortCopyArgs c) {
+__global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortArgs p, int slot_blocks, bool summed, const SortCopyArgs c) {
   extern __shared__ int lds[];
   const int E = p.E;
   int* before = lds;           // slots of the expert in the workgroups before, then the expert's next row in this one
@@ -171,6 +190,11 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_rows_kernel(const SortA
     // one workgroup of slots: every workgroup counts them itself
     const int mine = COPY || b == 0 ? id : sort_id(p, tid);
     if (mine >= 0) atomicAdd(&total[mine], 1);
+  } else if (summed) {
+    for (int e = tid; e < E; e += threads) {
+      total[e] = p.hist[static_cast<int64_t>(slot_blocks) * E + e];
+      before[e] = b < slot_blocks ? p.hist[static_cast<int64_t>(b) * E + e] : 0;
+    }
   } else {
     const int cols = min(E, kSortThreads), P = kSortThreads / cols;
     const int my_part = tid / cols, my_col = tid % cols;
@@ -301,7 +325,8 @@ constexpr int kUnpermuteRows = 4;
 template <int T, bool WHOLE>
 __global__ void __launch_bounds__(64) moe_unpermute_kernel(const UnpermuteArgs p) {
   const int lane = threadIdx.x;
-  const int64_t t = blockIdx.x;
+  const int64_t t = static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
+  if (t >= p.T) return;
   int mine = lane < p.topk ? p.row_index[t * p.topk + lane] : -1;
   if (mine >= p.R) mine = -1;
   const float my_w = lane < p.topk && p.w ? p.w[t * p.topk + lane] : 1.f;
@@ -361,16 +386,16 @@ __global__ void __launch_bounds__(kNormMaxThreads) moe_unpermute_backward_kernel
   __shared__ float part[kSortMaxTopk][kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int chunks = (p.H + 7) / 8;
-  if (static_cast<int64_t>(blockIdx.x) >= p.T) {
+  const int64_t t = grid_row();
+  if (t >= p.T) {
     Raw8 zero;
     zero.a = v4i{0, 0, 0, 0}, zero.b = v4i{0, 0, 0, 0};
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) - p.T; r < p.R; r += p.zero_blocks) {
+    for (int64_t r = t - p.T; r < p.R && t < p.T + p.zero_blocks; r += p.zero_blocks) {
       if (p.source[r] >= 0) continue;
       for (int i = tid; i < chunks; i += threads) store_raw8<T, WHOLE>(p.drows, r * p.drows_rs, 8 * i, zero, p.H - 8 * i);
     }
     return;
   }
-  const int64_t t = blockIdx.x;
   if (p.R == 0) {
     if (DW && tid < p.topk) p.dw[t * p.topk + tid] = 0.f;
     return;

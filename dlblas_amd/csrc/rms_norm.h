@@ -110,10 +110,18 @@ __device__ __forceinline__ void store_raw8(void* p, int64_t row, int col, const 
   }
 }
 
+// Over neighbouring LANES of a wave.
+template <int LANES = 64>
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
+  for (int off = LANES / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off);
   return v;
+}
+
+// The row, or the worker, of this thread among the blockDim.y beside each other in a workgroup: the same for a wave of one row.
+template <int LANES>
+__device__ __forceinline__ int beside() {
+  return LANES < 64 ? static_cast<int>(threadIdx.y) : __builtin_amdgcn_readfirstlane(threadIdx.y);
 }
 
 // A barrier for what went through LDS; loads from memory stay on their way.
@@ -155,14 +163,19 @@ __device__ __forceinline__ uint32_t group_max(bool hw, const float (&h)[8], cons
   return top;
 }
 
-// One workgroup per row, blockDim = the threads that the row's chunks need at CH chunks each; a thread past the last chunk reads that one
+// A workgroup's place in a grid of two dimensions: one of them holds fewer than 2^32 threads.
+__device__ __forceinline__ int64_t grid_row() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
+// One workgroup per row, blockDim.x = the threads that the row's chunks need at CH chunks each, or blockDim.y narrow rows
+// (up to 16 or 32 chunks: LANES of a wave a row); a thread past the last chunk reads that one
 // again and leaves no trace.  8192 x 7168 bf16 with residual, quantised, 413 MB: 77 us, 5.3 TB/s (a large copy reaches 5.0 here); 4096 x 7168
 // with residual, not quantised, 235 MB: 40 us, 5.8 TB/s, part of it from the cache; one row 3.7 us, launch and latency.
-template <int T, bool QUANT, bool RES, bool WHOLE, int CH>
+template <int T, bool QUANT, bool RES, bool WHOLE, int CH, int LANES>
 __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArgs p) {
   __shared__ float part[kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = grid_row() * blockDim.y + beside<LANES>();
+  if (row >= p.rows) return;  // with rows beside each other in a workgroup there is no barrier
   const int chunks = (p.H + 7) / 8;
   int at[CH];
   Raw8 h[CH], res[CH];
@@ -193,8 +206,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
     for (int k = 0; k < 8; ++k) s = fmaf(v[k], v[k], s);
     ss += c * threads + tid < chunks ? s : 0.f;
   }
-  ss = wave_sum(ss);
-  if (threads > 64) {
+  ss = wave_sum<LANES>(ss);
+  if (LANES == 64 && threads > 64) {
     if ((tid & 63) == 0) part[tid >> 6] = ss;
     __syncthreads();
     ss = 0.f;
@@ -254,22 +267,24 @@ struct NormGradArgs {
   const void* h;
   const void* w;
   void* dx;
-  float* dw_part;    // [gridDim.x][H] or NULL: sums over a workgroup's rows
+  float* dw_part;    // [shares][H] or NULL: sums over the rows of a workgroup, of narrow rows those of a wave
   int64_t rows, dy_rs, dsum_rs, h_rs, dx_rs;
   int H;
   int w_f32;
   float eps;
 };
 
-// A workgroup takes rows blockIdx, blockIdx + gridDim, ... and keeps its share of dw in registers; the shares of all workgroups are
+// A worker takes rows worker, worker + workers, ... and keeps its share of dw in registers; the shares of all workers are
 // added by rms_norm_dw_kernel in a fixed order, so the gradient is the same in every run.  The next row is on its way while the sums of
 // this one cross the workgroup, where a row of two chunks a thread leaves the registers for it.  Threads past the last chunk as above.
 // 4096 x 7168 bf16 with the sum's gradient, 235 MB and 15 of shares: 52 us, 4.8 TB/s; 1237 x 2050 fp32 13 us.
-template <int T, bool DSUM, bool WHOLE, int CH>
+template <int T, bool DSUM, bool WHOLE, int CH, int LANES>
 __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(const NormGradArgs p) {
   constexpr bool kAhead = CH == 1 || (CH == 2 && T != kInF32);
   __shared__ float part[2][2][kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
+  // workers: workgroups, or where a wave or part of one has room for a row these
+  const int worker = blockIdx.x * blockDim.y + beside<LANES>(), workers = gridDim.x * blockDim.y;
   const int chunks = (p.H + 7) / 8;
   float dw[CH][8];
   int at[CH];
@@ -292,11 +307,11 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
     }
   };
   Row now, next;
-  if (kAhead) load(blockIdx.x, now);
+  if (kAhead) load(min(static_cast<int64_t>(worker), p.rows - 1), now);
   int turn = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+  for (int64_t row = worker; row < p.rows; row += workers, turn ^= 1) {
     if (kAhead)
-      load(min(row + gridDim.x, p.rows - 1), next);  // behind the last row that one again
+      load(min(row + workers, p.rows - 1), next);  // behind the last row that one again
     else
       load(row, now);
     float ss = 0.f, dot = 0.f;
@@ -315,8 +330,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
       ss += live ? s : 0.f, dot += live ? d : 0.f;
       if (CH == 4) __builtin_amdgcn_sched_barrier(0);  // four chunks fill the registers: one chunk's weights at a time
     }
-    ss = wave_sum(ss), dot = wave_sum(dot);
-    if (threads > 64) {
+    ss = wave_sum<LANES>(ss), dot = wave_sum<LANES>(dot);
+    if (LANES == 64 && threads > 64) {
       // two sets of sums in turn: a wave may be one row ahead of the others, never two
       if ((tid & 63) == 0) part[turn][0][tid >> 6] = ss, part[turn][1][tid >> 6] = dot;
       lds_barrier();
@@ -350,9 +365,14 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
   }
   if (!p.dw_part) return;
 #pragma unroll
+  for (int off = LANES; off < 64; off <<= 1)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dw[0][k] += __shfl_xor(dw[0][k], off);
+  if (worker % (64 / LANES) != 0) return;
+#pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int i = c * threads + tid;
-    if (i < chunks) store_raw8<kInF32, WHOLE>(p.dw_part, static_cast<int64_t>(blockIdx.x) * p.H, 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
+    if (i < chunks) store_raw8<kInF32, WHOLE>(p.dw_part, static_cast<int64_t>(worker / (64 / LANES)) * p.H, 8 * i, pack_raw8<kInF32>(dw[c]), p.H - 8 * i);
   }
 }
 

@@ -368,3 +368,51 @@ def test_experts_whose_offsets_pass_32_bits(dev):
     for i, e in enumerate((0, 200, 318, 319)):
         ref, bound = orc.w4_gemm(x[i:i + 1].cpu(), q[e, -64:].cpu(), s[e, -64:].cpu(), None)
         within(y[i, -64:], ref[0], (BF16 * (ref.abs() + bound) + bound)[0])
+
+
+def test_more_rows_than_a_launch_has_threads_in_one_dimension(dev):
+    rows, H = 2**28 + 1003, 8  # 16 lanes a row
+    x = torch.ones(rows, H, device=dev, dtype=bf16)
+    tail = torch.randn(3000, H, device=dev, generator=torch.Generator(device=dev).manual_seed(4)).to(bf16)
+    x[-3000:] = tail
+    w = torch.full((H, ), 2.0, device=dev, dtype=bf16)
+    y = rms_norm(x, w)
+    assert torch.equal(y[-3000:], rms_norm(tail, w)) and bool((y[:-3000:100003] == 2).all())
+
+
+def test_more_tokens_than_a_launch_has_threads_in_one_dimension(dev):
+    """65537 workgroups of slots as well, whose counts are added up in a launch of their own."""
+    T, E, H = 2**26 + 77, 4, 8
+    g = torch.Generator(device=dev).manual_seed(5)
+    ids = torch.randint(0, E, (T, 1), device=dev, generator=g, dtype=torch.int32)
+    x = torch.randn(T, H, device=dev, generator=g).to(bf16).requires_grad_()
+    rows, p = moe_permute(x, ids, E)
+    order = torch.sort(ids.flatten(), stable=True).indices
+    assert torch.equal(p.source.long(), order)
+    del order
+    assert torch.equal(rows[-5000:], x[p.source[-5000:].long()])
+    weights = torch.rand(T, 1, device=dev, generator=g).requires_grad_()
+    out = moe_unpermute(rows, p, weights)
+    dx, dweights = torch.autograd.grad(out, (x, weights), x.detach())
+    for lo in (0, T - 5000):
+        part, factor = x.detach()[lo:lo + 5000].float(), weights.detach()[lo:lo + 5000]
+        assert torch.equal(out.detach()[lo:lo + 5000], (part * factor).to(bf16)) and torch.equal(dx[lo:lo + 5000], (part * factor).to(bf16))
+        ref = part.double().square().sum(1, keepdim=True)
+        assert float(((dweights[lo:lo + 5000].double() - ref).abs() - 60 * FP32 * ref).max()) <= 0
+
+
+@pytest.mark.parametrize('T,topk,E', [(50000, 8, 1024), (140000, 8, 33)])
+def test_many_slots(dev, T, topk, E):
+    ids = torch.randint(-1, E, (T, topk), device=dev, generator=torch.Generator(device=dev).manual_seed(6))
+    _, p = moe_permute(torch.zeros(T, 8, device=dev, dtype=bf16), ids, E, alignment=16)
+    flat = ids.flatten()
+    order = torch.sort(flat, stable=True).indices[int((flat < 0).sum()):]
+    row = p.row_index.flatten()[order].long()
+    counts = torch.bincount(flat[flat >= 0], minlength=E)
+    start = torch.cumsum((counts + 15) // 16 * 16, 0) - (counts + 15) // 16 * 16
+    first = torch.cumsum(counts, 0) - counts
+    expert = flat[order]
+    assert torch.equal(row, start[expert] + torch.arange(order.numel(), device=dev) - first[expert])
+    assert torch.equal(p.source[row].long(), order) and int((p.source >= 0).sum()) == order.numel()
+    assert torch.equal(p.row_start.long(), start) and torch.equal(p.row_end.long(), start + counts)
+    assert bool((p.row_index.flatten()[flat < 0] == -1).all())

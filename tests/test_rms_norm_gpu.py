@@ -179,7 +179,8 @@ def test_rows_of_zeros_and_values_that_are_no_numbers(dev):
 
 @pytest.mark.parametrize('dtype', [bf16, f16, f32])
 @pytest.mark.parametrize('residual', [False, True])
-@pytest.mark.parametrize('rows,H', [(1, 1), (2, 9), (5, 64), (4, 127), (1100, 136), (600, 513), (7, 2050), (33, 7168), (2, 9000), (3, 20001)])
+@pytest.mark.parametrize('rows,H', [(1, 1), (2, 9), (5, 64), (4, 127), (1100, 136), (600, 513), (7, 2050), (33, 7168), (2, 9000), (3, 20001),
+                                    (17, 128), (9001, 64), (5003, 256), (8301, 520), (2, 8), (33, 248)])
 def test_gradients(dev, rows, H, residual, dtype):
     x, w, res = inputs(rows, H, dtype, residual, seed=1)
     g = torch.Generator().manual_seed(rows + H)
