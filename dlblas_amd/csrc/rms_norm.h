@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_backward_kernel(cons
   }
 }
 
-// dw[col] = sum over the parts: a wave adds every kDwWaves-th, eight sums at a time, and the waves' sums are added in pairs.
+// dw[col] = sum over the parts: a wave adds every kDwWaves-th, eight sums at a time, and the waves' sums are added in pairs.  512 shares of
+// 7168: 4 to 5 us (15 MB); four waves instead of sixteen 8, loads behind a branch 12.
 struct NormDwArgs {
   const float* part;
   void* dw;

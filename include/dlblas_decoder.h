@@ -125,7 +125,7 @@ size_t dlb_w4_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t e
  *   z    the same shape, one byte each (0 ... 15; other bits give other products), or NULL: 8 everywhere
  *   y    [rows, N]         dtype, row stride y_row_stride
  *   row_start, row_end [experts] int32 on the device: expert e multiplies the rows [row_start[e], row_end[e]), clamped to
- *        [0, rows]; rows of no expert are not written.  NULL with experts = 1: every row
+ *        [0, rows]; ranges share no row, rows of no expert are not written.  NULL with experts = 1: every row
  *   workspace              4-byte aligned, dlb_w4_gemm_workspace_bytes(rows, N, K, row_start ? experts : 0), no initialisation
  *
  * group 32, 64 or 128; K % group == 0; K at most 2^24.  Meant for up to a few dozen rows (per expert): the weights are read once per
