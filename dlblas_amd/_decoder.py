@@ -14,20 +14,27 @@ def _present(*tensors):
     return [t for t in tensors if t is not None]
 
 
+def _require_one_gpu(*tensors):
+    _require_gpu(*tensors)
+    for t in tensors:
+        if t.device != tensors[0].device:
+            raise RuntimeError(f'all tensors of a call must be on one GPU, got {tensors[0].device} and {t.device}')
+
+
 def _rs(t):
     """Row stride of a [rows, columns] tensor; 0 for none."""
     return 0 if t is None else t.stride(0)
 
 
 def rms_norm(x, weight, residual, y, summed, eps):
-    _require_gpu(*_present(x, weight, residual, y, summed))
+    _require_one_gpu(*_present(x, weight, residual, y, summed))
     with torch.cuda.device(x.device):
         check(load().dlb_rms_norm(_ptr(x), _rs(x), _ptr(residual), _rs(residual), IN_CODES[x.dtype], _ptr(weight), IN_CODES[weight.dtype], _ptr(y),
                                   _rs(y), _ptr(summed), _rs(summed), x.size(0), x.size(1), float(eps), _stream(x)))
 
 
 def rms_norm_quant(x, weight, residual, q, s, summed, eps, quant_eps):
-    _require_gpu(*_present(x, weight, residual, q, s, summed))
+    _require_one_gpu(*_present(x, weight, residual, q, s, summed))
     with torch.cuda.device(x.device):
         check(load().dlb_rms_norm_quant(_ptr(x), _rs(x), _ptr(residual), _rs(residual), IN_CODES[x.dtype], _ptr(weight), IN_CODES[weight.dtype],
                                         _ptr(q), _ptr(s), s.stride(0), s.stride(1), _ptr(summed), _rs(summed), x.size(0), x.size(1), float(eps),
@@ -35,7 +42,7 @@ def rms_norm_quant(x, weight, residual, q, s, summed, eps, quant_eps):
 
 
 def rms_norm_backward(dy, dsum, h, weight, dx, dw, eps):
-    _require_gpu(*_present(dy, dsum, h, weight, dx, dw))
+    _require_one_gpu(*_present(dy, dsum, h, weight, dx, dw))
     lib = load()
     with torch.cuda.device(h.device):
         rows, H = h.shape
@@ -47,7 +54,7 @@ def rms_norm_backward(dy, dsum, h, weight, dx, dw, eps):
 
 
 def moe_permute(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s, alignment):
-    _require_gpu(*_present(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s))
+    _require_one_gpu(*_present(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s))
     code = ROWS_E4M3 if x.dtype == torch.float8_e4m3fn else IN_CODES[x.dtype]
     lib = load()
     with torch.cuda.device(x.device):
@@ -60,14 +67,14 @@ def moe_permute(ids, x, x_s, row_index, source, m_indices, row_start, row_end, r
 
 
 def moe_unpermute(rows, row_index, weights, out):
-    _require_gpu(*_present(rows, row_index, weights, out))
+    _require_one_gpu(*_present(rows, row_index, weights, out))
     with torch.cuda.device(rows.device):
         check(load().dlb_moe_unpermute(_ptr(rows), _rs(rows), IN_CODES[rows.dtype], _ptr(row_index), _ptr(weights), _ptr(out), _rs(out), out.size(0),
                                        out.size(1), row_index.size(1), rows.size(0), _stream(rows)))
 
 
 def moe_unpermute_backward(dout, rows, row_index, source, weights, drows, dweights):
-    _require_gpu(*_present(dout, rows, row_index, source, weights, drows, dweights))
+    _require_one_gpu(*_present(dout, rows, row_index, source, weights, drows, dweights))
     with torch.cuda.device(dout.device):
         check(load().dlb_moe_unpermute_backward(_ptr(dout), _rs(dout), _ptr(rows), _rs(rows), IN_CODES[dout.dtype], _ptr(row_index), _ptr(source),
                                                 _ptr(weights), _ptr(drows), _rs(drows), _ptr(dweights), dout.size(0), dout.size(1),
@@ -75,7 +82,7 @@ def moe_unpermute_backward(dout, rows, row_index, source, weights, drows, dweigh
 
 
 def w4_gemm(x, w_q, w_s, w_z, y, row_start, row_end, group):
-    _require_gpu(*_present(x, w_q, w_s, w_z, y, row_start, row_end))
+    _require_one_gpu(*_present(x, w_q, w_s, w_z, y, row_start, row_end))
     lib = load()
     E = w_q.size(0) if w_q.dim() == 3 else 1
     with torch.cuda.device(x.device):
@@ -86,6 +93,6 @@ def w4_gemm(x, w_q, w_s, w_z, y, row_start, row_end, group):
 
 
 def w4_quant(w, q, s, z, group):
-    _require_gpu(*_present(w, q, s, z))
+    _require_one_gpu(*_present(w, q, s, z))
     with torch.cuda.device(w.device):
         check(load().dlb_w4_quant(_ptr(w), _rs(w), IN_CODES[w.dtype], _ptr(q), _ptr(s), _ptr(z), w.size(0), w.size(1), group, _stream(w)))

@@ -326,8 +326,9 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
 // Eight steps of 32 columns follow, of one group each: for groups of 128 the halves of the wave exchange words, for smaller ones the
 // quarters.  Slices of K (gridDim.z) go to workgroups of their own, whose fp32 sums w4_sum_kernel adds in slice order.
 // 32 experts x 4 rows x 4096 x 7168, 482 MB: 102 us, 4.7 TB/s, the memory's; 16 x 7168 x 18432, 69 MB in nine slices: 20 us and 4 for the
-// sums, instructions of the few waves per SIMD and the start of the stream; 64 x 7168 x 18432 47 us, products.  Three chunks on their way
-// instead of one made the latter two slower (30 and 52): registers, waves, and no wait for memory that they shorten.
+// sums, instructions of the few waves per SIMD and the start of the stream; 64 x 7168 x 18432 47 us, where a SIMD has 13 us of products and 15
+// of other vector instructions to issue and its one or two waves overlap them badly (a third of their time each waiting for issue, waiting for
+// LDS and memory, issuing).  Two chunks on their way instead of one 28 and 49 us, three 30 and 52.
 constexpr int kW4Waves = 4;
 constexpr int kW4Unit = 256;  // columns
 

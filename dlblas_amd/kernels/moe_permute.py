@@ -26,6 +26,9 @@ class MoePermutation(NamedTuple):
 def _permute_op(topk_ids: torch.Tensor, x: torch.Tensor, x_s: Optional[torch.Tensor], row_index: torch.Tensor, source: torch.Tensor,
                 m_indices: torch.Tensor, row_start: torch.Tensor, row_end: torch.Tensor, rows: torch.Tensor, rows_s: Optional[torch.Tensor],
                 alignment: int) -> None:
+    # inside the op, because an address is none that a compiled caller has
+    if x_s is not None and (x.stride(1) != 1 or x.stride(0) % 16 != 0 or x.data_ptr() % 16 != 0):
+        x = x.clone(memory_format=torch.contiguous_format)
     _decoder.moe_permute(topk_ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s, alignment)
 
 
@@ -142,8 +145,6 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
         assert x.size(1) % 128 == 0, f'the last dimension of x {x.size(1)} must be divisible by 128'
         if tuple(x_s.shape) != (x.size(0), x.size(1) // 128):
             raise ValueError(f'scales must be {[x.size(0), x.size(1) // 128]}, got {list(x_s.shape)}')
-        if x.stride(1) != 1 or x.stride(0) % 16 != 0 or x.data_ptr() % 16 != 0:
-            x = x.clone(memory_format=torch.contiguous_format)
         rows, rows_s, p = _permuted(x, x_s, topk_ids, num_experts, alignment, num_rows)
         return (rows, rows_s), p
     if x.dtype not in _lib.IN_CODES:

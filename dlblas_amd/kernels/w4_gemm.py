@@ -16,10 +16,23 @@ from .rms_norm import _bench
 GROUP_SIZES = (32, 64, 128)
 
 
+def _columns_whole(t):
+    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def _on_dwords(t):
+    """Rows as the kernel reads them: on 4 bytes and less than 2^25 bytes apart.  Inside the op, because an address is none that a compiled
+    caller has."""
+    t = _columns_whole(t)
+    if t.data_ptr() % 4 != 0 or t.stride(0) % 2 != 0 or t.stride(0) > 1 << 24:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 @torch.library.custom_op('dlblas::w4_gemm', mutates_args=('y', ), device_types='cuda')
 def _w4_op(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional[torch.Tensor], y: torch.Tensor, row_start: Optional[torch.Tensor],
            row_end: Optional[torch.Tensor], group_size: int) -> None:
-    _decoder.w4_gemm(x, w_q, w_s, w_z, y, row_start, row_end, group_size)
+    _decoder.w4_gemm(_on_dwords(x), w_q, w_s, w_z, y, row_start, row_end, group_size)
 
 
 @torch.library.custom_op('dlblas::per_group_quant_w4', mutates_args=('w_q', 'w_s', 'w_z'), device_types='cuda')
@@ -55,18 +68,6 @@ def _check(x, w_q, w_s, w_z, dims):
     return K // groups
 
 
-def _columns_whole(t):
-    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
-
-
-def _on_dwords(t):
-    """Rows as the kernel reads them: on 4 bytes and less than 2^25 bytes apart."""
-    t = _columns_whole(t)
-    if t.data_ptr() % 4 != 0 or t.stride(0) % 2 != 0 or t.stride(0) > 1 << 24:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
 def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` [..., K] (bf16 / fp16) times the 4-bit weights ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / group] (bf16 or fp16)
     and zero points ``w_z`` (uint8 like w_s, 0 ... 15, or None: 8): [..., N] in the type of x; fp32 sums, one rounding.
@@ -83,7 +84,7 @@ def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional
     group = _check(x, w_q, w_s, w_z, 2)
     x2d = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
     y = torch.empty(x.shape[:-1] + (w_q.size(0), ), dtype=x.dtype, device=x.device)
-    _w4_op(_on_dwords(x2d), w_q, w_s, w_z, y.view(-1, w_q.size(0)), None, None, group)
+    _w4_op(x2d, w_q, w_s, w_z, y.view(-1, w_q.size(0)), None, None, group)
     return y
 
 
@@ -105,7 +106,7 @@ def w4_gemm_grouped(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, row_s
         if tuple(t.shape) != (w_q.size(0), ):
             raise ValueError(f'{name} must be [{w_q.size(0)}], got {list(t.shape)}')
     y = torch.empty((x.size(0), w_q.size(1)), dtype=x.dtype, device=x.device)
-    _w4_op(_on_dwords(x), w_q, w_s, w_z, y, row_start.contiguous(), row_end.contiguous(), group)
+    _w4_op(x, w_q, w_s, w_z, y, row_start.contiguous(), row_end.contiguous(), group)
     return y
 
 

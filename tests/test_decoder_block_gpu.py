@@ -303,6 +303,40 @@ def test_blocks_from_threads(dev):
     assert not wrong
 
 
+@pytest.mark.parametrize('kind', ['serve_fp8', 'serve_w4', 'train'])
+def test_steps_under_the_tracing_compiler(dev, kind):
+    """The Python functions trace into one graph of the registered ops; the numbers are those of the native calls."""
+    layer = Block(dev)
+    x, res, ids, weights = (t.to(dev) for t in batch(20, layer.H, layer.E, 2))
+    q, s, z = layer.w4['gate_up']
+
+    def serve_fp8(x):
+        q, s, h = rms_norm_quant(x, layer.norm_dev, EPS, res)
+        rows, p = moe_permute((q, s), ids, layer.E, alignment=128)
+        return rows[0], rows[1], h, p.row_index, p.m_indices
+
+    def serve_w4(x):
+        y, h = rms_norm(x, layer.norm_dev, EPS, res)
+        rows, p = moe_permute(y, ids, layer.E, num_rows=32)
+        return moe_unpermute(w4_gemm_grouped(rows, q, s, p.row_start, p.row_end, z), p, weights), w4_gemm(y, q[0], s[0], z[0]), h
+
+    def train(x):
+        y, h = rms_norm(x, layer.norm_dev, EPS, res)
+        rows, p = moe_permute(y, ids, layer.E)
+        return moe_unpermute(rows, p, weights) + h
+
+    fn = dict(serve_fp8=serve_fp8, serve_w4=serve_w4, train=train)[kind]
+    torch._dynamo.reset()
+    traced = torch.compile(fn, backend='aot_eager', fullgraph=True)
+    if kind == 'train':
+        leaf, other = x.clone().requires_grad_(), x.clone().requires_grad_()
+        assert torch.equal(*(torch.autograd.grad(f(t), t, res)[0] for f, t in ((traced, leaf), (fn, other))))
+    else:
+        for a, b in zip(traced(x), fn(x)):
+            assert torch.equal(a.view(torch.uint8) if a.dtype == e4m3 else a, b.view(torch.uint8) if b.dtype == e4m3 else b)
+    torch._dynamo.reset()
+
+
 # ---- offsets that pass 32 bits -----------------------------------------------------------------------------------------
 
 

@@ -222,3 +222,15 @@ def test_sorted_order_is_stable_and_spans_are_aligned():
 
 def test_4_bit_codes_in_a_byte():
     assert orc.w4_codes(torch.tensor([[0x21, 0xf8]], dtype=u8)).tolist() == [[1, 2, 8, 15]]
+
+
+def test_tensors_of_two_devices_are_refused():
+    class On:
+        is_cuda = True
+
+        def __init__(self, index):
+            self.device = torch.device('cuda', index)
+
+    _decoder._require_one_gpu(On(0), On(0))
+    with pytest.raises(RuntimeError, match='one GPU'):
+        _decoder._require_one_gpu(On(0), On(0), On(1))
