@@ -136,9 +136,10 @@ int check_rows(int64_t tokens, int64_t H, int64_t topk, int64_t num_rows) {
   return DLB_OK;
 }
 
-// Whether a launch of its own adds up the counts of the workgroups of slots before each, instead of each for itself, which goes with the
-// square of their number: 60000 tokens x 8 slots, 256 experts 43 and 43 us, 66000 44 and 63, 10^6 498 and 7727, 131072 x 8, 32 experts 62 and 28.
-bool sort_scans(int64_t blocks, int64_t experts) { return blocks * blocks * experts > 60000000; }
+// Whether a launch of its own adds up the counts of the workgroups of slots before each, instead of each reading all of them: tables of 8192
+// tokens x 8 slots, 256 experts 13.1 and 13.7 us, 16384 13.5 and 17.8, 60000 19.9 and 42.6, 10^6 190 and 7733; 32 experts 8192 11.2 and 8.9,
+// 60000 16.5 and 13.5, 131072 26.6 and 28.1.
+bool sort_scans(int64_t blocks, int64_t experts) { return blocks * experts > 16384; }
 int64_t sort_blocks(int64_t slots) { return slots > 0 ? ceil_div(slots, kSortBlockSlots) : 1; }
 
 // ---- 4-bit weights ----------------------------------------------------------------------------------------------------
@@ -382,7 +383,7 @@ int dlb_moe_permute(const void* ids, int ids_dtype, int64_t ids_stride_m, int64_
     hipLaunchKernelGGL(moe_sort_count_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), static_cast<size_t>(a.E) * sizeof(int), st, a);
     if (int rc = finish("moe_permute (count)")) return rc;
     if (summed) {
-      hipLaunchKernelGGL(moe_sort_scan_kernel, dim3(static_cast<unsigned>(ceil_div(a.E, 64))), dim3(64), 0, st, a, static_cast<int>(blocks));
+      hipLaunchKernelGGL(moe_sort_scan_kernel, dim3(static_cast<unsigned>(ceil_div(a.E, 64))), dim3(64 * kScanWaves), 0, st, a, static_cast<int>(blocks));
       if (int rc = finish("moe_permute (scan)")) return rc;
     }
   }

@@ -45,6 +45,7 @@ __device__ __forceinline__ int sort_id(const SortArgs& p, int64_t i) {
   return (id < 0 || id >= p.E) ? -1 : static_cast<int>(id);
 }
 
+// Slots of every expert among the workgroup's 1024: 32768 slots 4.7 us, launch and latency.
 __global__ void __launch_bounds__(kSortThreads) moe_sort_count_kernel(const SortArgs p) {
   extern __shared__ int hist[];
   for (int e = threadIdx.x; e < p.E; e += kSortThreads) hist[e] = 0;
@@ -145,23 +146,45 @@ __device__ __forceinline__ void clear_row(const SortCopyArgs& p, int64_t r, int 
   for (int g = lane; g < p.groups; g += 64) p.rows_s[r * p.groups + g] = 0.f;
 }
 
-// Counts to slots in the workgroups before, an expert a thread, the totals in a row of their own.
-__global__ void __launch_bounds__(64) moe_sort_scan_kernel(const SortArgs p, int slot_blocks) {
-  const int e = blockIdx.x * 64 + threadIdx.x;
-  if (e >= p.E) return;
+// Counts to slots in the workgroups before, the totals in a row of their own.  A lane an expert, the waves take stretches of the
+// workgroups of slots: their sums first, then again from the sums of the waves before.  516 workgroups, 256 experts 7.1 us, 7813 69 (one
+// wave for all of them 26 and 372).
+constexpr int kScanWaves = 16;
+
+__global__ void __launch_bounds__(64 * kScanWaves) moe_sort_scan_kernel(const SortArgs p, int slot_blocks) {
+  __shared__ int sums[kScanWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int e = blockIdx.x * 64 + lane;
+  int32_t* const hist = p.hist + min(e, p.E - 1);
+  const int each = (slot_blocks + kScanWaves - 1) / kScanWaves;
+  const int first = min(wave * each, slot_blocks), last = min(first + each, slot_blocks);
+  const auto counts = [&](int b, int (&c)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) c[u] = hist[static_cast<int64_t>(min(b + u, slot_blocks - 1)) * p.E];
+  };
   int sum = 0;
-  for (int b = 0; b < slot_blocks; b += 16) {
-    int c[16];
+  for (int b = first; b < last; b += 8) {
+    int c[8];
+    counts(b, c);
 #pragma unroll
-    for (int u = 0; u < 16; ++u) c[u] = p.hist[static_cast<int64_t>(min(b + u, slot_blocks - 1)) * p.E + e];
+    for (int u = 0; u < 8; ++u) sum += b + u < last ? c[u] : 0;
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int w = 0; w < wave; ++w) sum += sums[w][lane];
+  if (e >= p.E) return;
+  for (int b = first; b < last; b += 8) {
+    int c[8];
+    counts(b, c);
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      if (b + u >= slot_blocks) break;
-      p.hist[static_cast<int64_t>(b + u) * p.E + e] = sum;
+    for (int u = 0; u < 8; ++u) {
+      if (b + u >= last) break;
+      hist[static_cast<int64_t>(b + u) * p.E] = sum;
       sum += c[u];
     }
   }
-  p.hist[static_cast<int64_t>(slot_blocks) * p.E + e] = sum;
+  if (wave == kScanWaves - 1) hist[static_cast<int64_t>(slot_blocks) * p.E] = sum;
 }
 
 // Rows of the slots of workgroup blockIdx, and its share of the tables by row.  Workgroups past the slots' share only the latter.
