@@ -14,6 +14,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -128,11 +129,21 @@ class NoGil {
 };
 
 #define NOT_PLAIN Py_RETURN_NONE
+// An exception raised in Python, by a hook on saved tensors for one, goes on as what it is: checkpointing ends a recomputation with
+// one of its own.
 #define HANDLE_EXCEPTIONS_BEGIN try {
 #define HANDLE_EXCEPTIONS_END                          \
   }                                                    \
   catch (const c10::OutOfMemoryError& e) {             \
     NOT_PLAIN; /* the Python path raises torch's own */ \
+  }                                                    \
+  catch (py::error_already_set & e) {                  \
+    e.restore();                                       \
+    return nullptr;                                    \
+  }                                                    \
+  catch (python_error & e) {                           \
+    e.restore();                                       \
+    return nullptr;                                    \
   }                                                    \
   catch (const std::exception& e) {                    \
     PyErr_SetString(PyExc_RuntimeError, e.what());     \
