@@ -1,6 +1,7 @@
 """The calls of include/dlblas_decoder.h on torch tensors: pointers, strides, device and stream.  Shapes and types are the business of
 the functions in kernels/, which call these through their custom ops."""
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import IDX_CODES, IN_CODES, _ptr, _require_gpu, _stream, check, load
 
@@ -19,6 +20,14 @@ def _require_one_gpu(*tensors):
     for t in tensors:
         if t.device != tensors[0].device:
             raise RuntimeError(f'all tensors of a call must be on one GPU, got {tensors[0].device} and {t.device}')
+
+
+def no_tangents(*tensors):
+    """Forward-mode derivatives are not implemented, and the ops write into outputs that no tangent follows: without this a tensor with a
+    tangent would come back as one whose derivative is zero."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError('forward-mode derivatives of the steps around the products are not implemented')
 
 
 def _rs(t):

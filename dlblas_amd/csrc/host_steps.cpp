@@ -114,6 +114,12 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// Nor in forward mode: the kernels write into outputs that no tangent follows.
+void no_tangent(const at::Tensor& grad) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!grad.defined() || !grad._fw_grad(0).defined(),
+                              "forward-mode derivatives of the steps around the products are not implemented");
+}
+
 at::Tensor whole_columns(const at::Tensor& t) { return row_stride(t) < 0 ? t.contiguous() : t; }
 std::optional<at::Tensor> optional_of(const at::Tensor* t) { return t ? std::optional<at::Tensor>(*t) : std::nullopt; }
 
@@ -141,6 +147,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const at::Tensor &h = saved[0], &w = saved[1];
     const bool with_res = ctx->saved_data["res"].toBool();
     const at::Tensor dsum_given = with_res ? grads[1] : at::Tensor();
+    no_tangent(grads[0]), no_tangent(dsum_given);
     if (!grads[0].defined()) return once({dsum_given, {}, with_res ? dsum_given : at::Tensor(), {}});  // only the sum went on, or nothing
     DeviceScope scope(h);
     const at::Tensor dy = whole_columns(grads[0]), dsum = dsum_given.defined() ? whole_columns(dsum_given) : dsum_given;
@@ -204,6 +211,7 @@ struct Permute : torch::autograd::Function<Permute> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
+    no_tangent(grads[0]);
     DeviceScope scope(grads[0]);
     return once({unpermute_forward(whole_columns(grads[0]), ctx->get_saved_variables()[0], nullptr), {}, {}, {}, {}});
   }
@@ -220,6 +228,7 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}};
+    no_tangent(grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &rows = saved[0], &w = saved[1], &index = saved[2], &source = saved[3];
     DeviceScope scope(grads[0]);

@@ -77,6 +77,7 @@ class _Permute(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows, *_):
+        _decoder.no_tangents(drows)
         row_index, = ctx.saved_tensors
         return _unpermuted(_columns_whole(drows), row_index, None), None, None, None, None
 
@@ -92,6 +93,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _decoder.no_tangents(dout)
         rows, weights, row_index, source = ctx.saved_tensors
         drows = torch.empty((ctx.num_rows, dout.size(1)), dtype=dout.dtype, device=dout.device)
         dweights = torch.empty(weights.shape, dtype=torch.float32, device=dout.device) if ctx.needs_input_grad[1] else None
@@ -116,7 +118,8 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
     num_rows   rows to return; slots whose row would lie past them are dropped (row_index -1).  By default enough for any routing, which
                with many experts and a large alignment is far more than one routing fills
 
-    Rows are in the order of (expert, token, j); rows that hold no slot are zero.  Differentiable in x.
+    Rows are in the order of (expert, token, j); rows that hold no slot are zero.  Differentiable in x, once and
+    in reverse mode.
     """
     quantised = isinstance(x, (tuple, list))
     x, x_s = x if quantised else (x, None)
@@ -125,6 +128,7 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
         if out is not None:
             rows = (out[0], out[1]) if quantised else out[0]
             return rows, MoePermutation(*out[2:])
+    _decoder.no_tangents(x, x_s)
     if x.dim() != 2 or topk_ids.dim() != 2 or topk_ids.size(0) != x.size(0):
         raise ValueError(f'x must be [T, H] and topk_ids [T, topk], got {list(x.shape)} and {list(topk_ids.shape)}')
     if topk_ids.dtype not in _lib.IDX_CODES:
@@ -161,7 +165,7 @@ def moe_unpermute(rows: torch.Tensor, permutation: Union[MoePermutation, torch.T
 
     rows [R, H] bf16 / fp16 / fp32; permutation as ``moe_permute`` returned it, or any int32 [T, topk] table of rows (entries outside
     0 ... R - 1 name none); topk_weights [T, topk] float32, all one by default.  fp32 sums in slot order, one rounding; a token without a
-    row gets zeros.  Differentiable in rows and topk_weights, for which it needs the permutation, not a table alone.
+    row gets zeros.  Differentiable in rows and topk_weights, once and in reverse mode, for which it needs the permutation, not a table alone.
     """
     whole = isinstance(permutation, MoePermutation)
     row_index = permutation.row_index if whole else permutation
@@ -169,6 +173,7 @@ def moe_unpermute(rows: torch.Tensor, permutation: Union[MoePermutation, torch.T
         out = _fast.moe_unpermute(rows, row_index, topk_weights, permutation.source if whole else None)
         if out is not None:
             return out
+    _decoder.no_tangents(rows, topk_weights)
     if rows.dtype not in _lib.IN_CODES:
         raise TypeError(f'rows must be bfloat16, float16 or float32, got {rows.dtype}')
     if row_index.dtype != torch.int32:

@@ -33,6 +33,7 @@ def _norm_backward_op(dy: torch.Tensor, dsum: Optional[torch.Tensor], h: torch.T
 
 
 def _check(x, weight, residual, eps):
+    _decoder.no_tangents(x, weight, residual)
     if x.dtype not in _lib.IN_CODES:
         raise TypeError(f'x must be bfloat16, float16 or float32, got {x.dtype}')
     if x.dim() < 1 or x.size(-1) < 1:
@@ -79,6 +80,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
+        _decoder.no_tangents(dy, dsum)
         h, weight = ctx.saved_tensors
         if dy is None:  # only the sum went on
             return dsum, None, dsum if ctx.needs_input_grad[2] else None, None
@@ -93,7 +95,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """RMS norm of ``x`` [..., H] (bf16 / fp16 / fp32) with ``weight`` [H] of the same type or fp32, in the type of x.
 
     Returns ``y``; with a ``residual`` like x ``(y, h)``, where ``h = x + residual`` is what the next residual starts from.
-    Differentiable in x, weight and residual; sums over rows are added in a fixed order.
+    Differentiable in x, weight and residual, once and in reverse mode; sums over rows are added in a fixed order.
     """
     if not torch.compiler.is_compiling():
         out = _fast.rms_norm(x, weight, eps, residual)

@@ -42,6 +42,7 @@ def _quant_op(w: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Option
 
 def _check(x, w_q, w_s, w_z, dims):
     """Types, shapes and layouts of a product; returns the group size."""
+    _decoder.no_tangents(x, w_s)
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f'x must be bfloat16 or float16, got {x.dtype}')
     if w_q.dtype != torch.uint8:
@@ -117,6 +118,7 @@ def per_group_quant_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool
     Without zero points ``w_s = amax / 7`` and codes around 8; with them the range of a group from its lowest (at most 0) to its highest value
     (at least 0) is cut into 15 steps.
     """
+    _decoder.no_tangents(w)
     if w.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f'w must be bfloat16 or float16 (the type of its scales), got {w.dtype}')
     if w.dim() not in (2, 3):
