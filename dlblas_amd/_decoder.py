@@ -30,6 +30,14 @@ def no_tangents(*tensors):
             raise NotImplementedError('forward-mode derivatives of the steps around the products are not implemented')
 
 
+def given_back(t, grad, dtype, shape):
+    """A saved tensor as a hook on saved tensors gave it back: the kernels are told nothing but its address."""
+    if t.device != grad.device or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise RuntimeError('a tensor saved for a gradient of dlblas_amd came back from its hook on another device, of another type or with other '
+                           f'sizes: {t.device}, {t.dtype}, {list(t.shape)}')
+    return t
+
+
 def _rs(t):
     """Row stride of a [rows, columns] tensor; 0 for none."""
     return 0 if t is None else t.stride(0)

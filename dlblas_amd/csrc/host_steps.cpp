@@ -120,6 +120,14 @@ void no_tangent(const at::Tensor& grad) {
                               "forward-mode derivatives of the steps around the products are not implemented");
 }
 
+// A saved tensor as a hook on saved tensors gave it back.  Its layout may be another one; the kernels are told nothing but its address, so
+// its device, type and sizes may not.
+const at::Tensor& given_back(const at::Tensor& t, at::ScalarType type, at::IntArrayRef size, const at::Tensor& grad) {
+  TORCH_CHECK(t.defined() && t.device() == grad.device() && t.scalar_type() == type && t.sizes() == size,
+              "a tensor saved for a gradient of dlblas_amd came back from its hook on another device, of another type or with other sizes");
+  return t;
+}
+
 at::Tensor whole_columns(const at::Tensor& t) { return row_stride(t) < 0 ? t.contiguous() : t; }
 std::optional<at::Tensor> optional_of(const at::Tensor* t) { return t ? std::optional<at::Tensor>(*t) : std::nullopt; }
 
@@ -144,14 +152,16 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &h = saved[0], &w = saved[1];
     const bool with_res = ctx->saved_data["res"].toBool();
     const at::Tensor dsum_given = with_res ? grads[1] : at::Tensor();
     no_tangent(grads[0]), no_tangent(dsum_given);
     if (!grads[0].defined()) return once({dsum_given, {}, with_res ? dsum_given : at::Tensor(), {}});  // only the sum went on, or nothing
-    DeviceScope scope(h);
-    const at::Tensor dy = whole_columns(grads[0]), dsum = dsum_given.defined() ? whole_columns(dsum_given) : dsum_given;
-    const int64_t H = h.size(-1), rows = h.numel() / H;
+    const at::Tensor& g = grads[0];
+    DeviceScope scope(g);
+    const int64_t H = g.size(-1), rows = g.numel() / H;
+    const at::Tensor h = whole_columns(given_back(saved[0], g.scalar_type(), g.sizes(), g));
+    const at::Tensor w = given_back(saved[1], is_f32(saved[1]) ? at::kFloat : g.scalar_type(), {H}, g).contiguous();
+    const at::Tensor dy = whole_columns(g), dsum = dsum_given.defined() ? whole_columns(dsum_given) : dsum_given;
     at::Tensor dx = empty(h.sizes(), h.scalar_type(), h), dw, shares;
     size_t need = 0;
     if (ctx->needs_input_grad(1)) {
@@ -205,6 +215,8 @@ struct Permute : torch::autograd::Function<Permute> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids, int64_t E, int64_t align, int64_t R) {
     variable_list out = permute_forward(x, nullptr, ids, E, align, R);
     ctx->save_for_backward({out[1]});
+    ctx->saved_data["topk"] = ids.size(1);
+    ctx->saved_data["tokens"] = ids.size(0);
     ctx->mark_non_differentiable({out.begin() + 1, out.end()});
     ctx->set_materialize_grads(false);
     return out;
@@ -212,15 +224,17 @@ struct Permute : torch::autograd::Function<Permute> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
     no_tangent(grads[0]);
+    const variable_list saved = ctx->get_saved_variables();
     DeviceScope scope(grads[0]);
-    return once({unpermute_forward(whole_columns(grads[0]), ctx->get_saved_variables()[0], nullptr), {}, {}, {}, {}});
+    const at::Tensor index = given_back(saved[0], at::kInt, {ctx->saved_data["tokens"].toInt(), ctx->saved_data["topk"].toInt()}, grads[0]).contiguous();
+    return once({unpermute_forward(whole_columns(grads[0]), index, nullptr), {}, {}, {}, {}});
   }
 };
 
 struct Unpermute : torch::autograd::Function<Unpermute> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const std::optional<at::Tensor>& w, const at::Tensor& index, const at::Tensor& source) {
     ctx->saved_data["rows"] = rows.size(0);
-    ctx->saved_data["w"] = w.has_value();
+    ctx->saved_data["topk"] = index.size(1);
     // the rows themselves are needed for the gradient of the weights alone
     ctx->save_for_backward({w && w->requires_grad() ? rows : at::Tensor(), w ? *w : at::Tensor(), index, source});
     ctx->set_materialize_grads(false);
@@ -230,15 +244,17 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
     if (!grads[0].defined()) return {{}, {}, {}, {}};
     no_tangent(grads[0]);
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &rows = saved[0], &w = saved[1], &index = saved[2], &source = saved[3];
     DeviceScope scope(grads[0]);
     const at::Tensor dout = whole_columns(grads[0]);
-    const int64_t R = ctx->saved_data["rows"].toInt(), T = index.size(0), H = dout.size(1);
-    const bool want_w = w.defined() && rows.defined() && ctx->needs_input_grad(1);
+    const int64_t R = ctx->saved_data["rows"].toInt(), topk = ctx->saved_data["topk"].toInt(), T = dout.size(0), H = dout.size(1);
+    const bool want_w = saved[1].defined() && saved[0].defined() && ctx->needs_input_grad(1);
+    const at::Tensor rows = want_w ? whole_columns(given_back(saved[0], dout.scalar_type(), {R, H}, dout)) : at::Tensor();
+    const at::Tensor w = saved[1].defined() ? given_back(saved[1], at::kFloat, {T, topk}, dout).contiguous() : at::Tensor();
+    const at::Tensor index = given_back(saved[2], at::kInt, {T, topk}, dout).contiguous(), source = given_back(saved[3], at::kInt, {R}, dout).contiguous();
     at::Tensor drows = empty({R, H}, dout.scalar_type(), dout), dw;
     if (want_w) dw = empty(w.sizes(), at::kFloat, dout);
     must(abi.unpermute_backward(ptr(dout), row_stride(dout), want_w ? ptr(rows) : nullptr, want_w ? rows.stride(0) : 0, in_code(dout.scalar_type()), iptr(index),
-                                iptr(source), w.defined() ? fptr(w) : nullptr, ptr(drows), H, want_w ? fptr(dw) : nullptr, T, H, index.size(1), R, stream_of(dout)));
+                                iptr(source), w.defined() ? fptr(w) : nullptr, ptr(drows), H, want_w ? fptr(dw) : nullptr, T, H, topk, R, stream_of(dout)));
     return once({drows, dw, {}, {}});
   }
 };

@@ -71,6 +71,7 @@ class _Permute(torch.autograd.Function):
     def forward(ctx, x, topk_ids, num_experts, alignment, num_rows):
         rows, _, p = _permuted(_columns_whole(x), None, topk_ids, num_experts, alignment, num_rows)
         ctx.save_for_backward(p.row_index)
+        ctx.slots = topk_ids.shape
         ctx.mark_non_differentiable(*p)
         return (rows, ) + tuple(p)
 
@@ -78,7 +79,7 @@ class _Permute(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows, *_):
         _decoder.no_tangents(drows)
-        row_index, = ctx.saved_tensors
+        row_index = _decoder.given_back(ctx.saved_tensors[0], drows, torch.int32, ctx.slots).contiguous()
         return _unpermuted(_columns_whole(drows), row_index, None), None, None, None, None
 
 
@@ -87,7 +88,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, row_index, source):
         ctx.save_for_backward(rows if weights is not None and weights.requires_grad else None, weights, row_index, source)
-        ctx.num_rows = rows.size(0)
+        ctx.num_rows, ctx.slots = rows.size(0), row_index.shape
         return _unpermuted(_columns_whole(rows), row_index, None if weights is None else weights.contiguous())
 
     @staticmethod
@@ -95,10 +96,14 @@ class _Unpermute(torch.autograd.Function):
     def backward(ctx, dout):
         _decoder.no_tangents(dout)
         rows, weights, row_index, source = ctx.saved_tensors
+        row_index = _decoder.given_back(row_index, dout, torch.int32, ctx.slots).contiguous()
+        source = _decoder.given_back(source, dout, torch.int32, (ctx.num_rows, )).contiguous()
+        weights = None if weights is None else _decoder.given_back(weights, dout, torch.float32, ctx.slots).contiguous()
         drows = torch.empty((ctx.num_rows, dout.size(1)), dtype=dout.dtype, device=dout.device)
         dweights = torch.empty(weights.shape, dtype=torch.float32, device=dout.device) if ctx.needs_input_grad[1] else None
-        _unpermute_backward_op(_columns_whole(dout), _columns_whole(rows) if dweights is not None else None, row_index, source,
-                               None if weights is None else weights.contiguous(), drows, dweights)
+        if dweights is not None:
+            rows = _columns_whole(_decoder.given_back(rows, dout, dout.dtype, drows.shape))
+        _unpermute_backward_op(_columns_whole(dout), rows if dweights is not None else None, row_index, source, weights, drows, dweights)
         return drows if ctx.needs_input_grad[0] else None, dweights, None, None
 
 

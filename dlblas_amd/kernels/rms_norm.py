@@ -84,7 +84,9 @@ class _RmsNorm(torch.autograd.Function):
         h, weight = ctx.saved_tensors
         if dy is None:  # only the sum went on
             return dsum, None, dsum if ctx.needs_input_grad[2] else None, None
-        H = h.size(-1)
+        H = dy.size(-1)
+        h = _decoder.given_back(h, dy, dy.dtype, dy.shape)
+        weight = _decoder.given_back(weight, dy, torch.float32 if weight.dtype == torch.float32 else dy.dtype, (H, ))
         dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         _norm_backward_op(_rows(dy), _rows(dsum), _rows(h), weight.contiguous(), dx.view(-1, H), dw, float(ctx.eps))

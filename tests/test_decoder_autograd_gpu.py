@@ -128,3 +128,62 @@ def test_batched_gradients_are_refused(dev, fn):
     out = fn(*ins)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, ins, torch.ones((2, ) + out.shape, dtype=bf16, device=dev), is_grads_batched=True, allow_unused=True)
+
+
+def spread(t):
+    """The same values in another layout."""
+    wide = t.new_zeros(t.shape + (3, ))
+    wide[..., 1] = t
+    return wide[..., 1]
+
+
+CHANGES = {
+    'another device': lambda t: t.cpu(),
+    'another type': lambda t: t.double() if t.is_floating_point() else t.long(),
+    'a narrower type': lambda t: t.half() if t.is_floating_point() else t.short(),
+    'fewer elements': lambda t: t[:1],
+    'another shape': lambda t: t.reshape(-1, 1),
+}
+
+
+@pytest.mark.parametrize('native', [True, False])
+@pytest.mark.parametrize('change', list(CHANGES) + ['another layout'])
+@pytest.mark.parametrize('fn,saved,which', [(fn, n, i) for fn, n in ((norm, 2), (norm_with_residual, 2), (permute, 1), (back_alone, 4)) for i in range(n)])
+def test_what_a_hook_gives_back_is_looked_at(dev, fn, saved, which, change, native, monkeypatch):
+    """The kernels are told nothing but addresses: a saved tensor that is another one raises before anything is enqueued, one that lies
+    differently is the same."""
+    if not native:
+        from dlblas_amd import _fast
+        for name in ('rms_norm', 'moe_permute', 'moe_unpermute'):
+            monkeypatch.setattr(_fast, name, lambda *a: None)
+    want = gradients(fn, dev)
+    count = [0]
+
+    def around(fn, ins):
+        if fn is back_alone:  # repeat() saves nothing
+            rows = ins[0].repeat(TOPK, 1)
+            with torch.no_grad():
+                _, p = moe_permute(ins[0], routing(dev), E)
+            call = lambda: moe_unpermute(rows[:p.source.numel()], p, ins[3])
+        else:
+            call = lambda: fn(*ins)
+
+        def pack(t):
+            count[0] += 1
+            return count[0] - 1, t
+
+        def unpack(packed):
+            n, t = packed
+            if n != which:
+                return t
+            return spread(t) if change == 'another layout' else CHANGES[change](t)
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            return call()
+
+    if change == 'another layout':
+        same(gradients(fn, dev, around), want)
+        return
+    with pytest.raises(RuntimeError, match='came back from its hook'):
+        gradients(fn, dev, around)
+    assert count[0] == saved
