@@ -124,7 +124,7 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
                with many experts and a large alignment is far more than one routing fills
 
     Rows are in the order of (expert, token, j); rows that hold no slot are zero.  Differentiable in x, once and
-    in reverse mode.
+    in reverse mode; quantised tokens are not.
     """
     quantised = isinstance(x, (tuple, list))
     x, x_s = x if quantised else (x, None)
@@ -154,6 +154,8 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_
         assert x.size(1) % 128 == 0, f'the last dimension of x {x.size(1)} must be divisible by 128'
         if tuple(x_s.shape) != (x.size(0), x.size(1) // 128):
             raise ValueError(f'scales must be {[x.size(0), x.size(1) // 128]}, got {list(x_s.shape)}')
+        if torch.is_grad_enabled() and (x.requires_grad or x_s.requires_grad):
+            raise NotImplementedError('quantised tokens have no gradient: permute them under torch.no_grad()')
         rows, rows_s, p = _permuted(x, x_s, topk_ids, num_experts, alignment, num_rows)
         return (rows, rows_s), p
     if x.dtype not in _lib.IN_CODES:

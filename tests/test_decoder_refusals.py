@@ -1,0 +1,16 @@
+"""What the Python functions of the steps around the products refuse, beside tests/test_decoder_steps.py: without a GPU."""
+import pytest
+import torch
+
+from dlblas_amd.kernels.moe_permute import moe_permute
+
+
+@pytest.mark.parametrize('which', ['scales', 'codes', 'both'])
+def test_quantised_tokens_have_no_gradient(which):
+    """They came back without one where their scales were leaves of a graph."""
+    codes, scales = torch.zeros(2, 128, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.ones(2, 1)
+    for t, name in ((codes, 'codes'), (scales, 'scales')):
+        if which in (name, 'both'):
+            t.requires_grad_()
+    with pytest.raises(NotImplementedError, match='no gradient'):
+        moe_permute((codes, scales), torch.zeros(2, 1, dtype=torch.int32), 4)
