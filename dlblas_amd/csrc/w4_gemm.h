@@ -607,7 +607,9 @@ __global__ void __launch_bounds__(256) w4_sum_kernel(const float* sums, void* y,
 // 4-bit quantiser: per group of 32, 64 or 128 columns of a row
 //   without zero points  s = max |w| / 7 rounded to its type,             q = clamp(round(w / s) + 8, 0, 15)
 //   with them            s = (max(w, 0) - min(w, 0)) / 15 rounded,        z = round(-min(w, 0) / s),  q = clamp(round(w / s) + z, 0, 15)
-// A group of zeros has s = 0 and q = 8 (z = 0, q = 0 with zero points).  8 columns a lane, one store of 4 bytes.
+// A group of zeros has s = 0 and q = 8 (z = 0, q = 0 with zero points); so has one whose s rounds to 0.  A group that holds a NaN or an
+// infinity, or whose range fp32 does not hold, has s = NaN: minima and maxima pass NaN over, and its codes would be those of ordinary
+// weights.  8 columns a lane, one store of 4 bytes.
 struct W4QuantArgs {
   const void* w;
   uint8_t* q;   // [rows][K / 2]
@@ -636,10 +638,17 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const W4QuantArgs p) {
     float v[8];
     quant_unpack8<T>(load_raw8<T, true>(p.w, row * p.w_rs, static_cast<int>(kg * p.group) + 8 * sub, 8), v);
     float hi = 0.f, lo = 0.f;
+    uint32_t top = 0;  // the largest magnitude as bits, which put infinity above all numbers and NaN above infinity
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi = fmaxf(hi, v[i]), lo = fminf(lo, v[i]);
-    for (int off = lanes / 2; off >= 1; off >>= 1) hi = fmaxf(hi, __shfl_xor(hi, off, lanes)), lo = fminf(lo, __shfl_xor(lo, off, lanes));
-    const float s = round_to_type<T>(p.z ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
+    for (int i = 0; i < 8; ++i) hi = fmaxf(hi, v[i]), lo = fminf(lo, v[i]), top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int off = lanes / 2; off >= 1; off >>= 1) {
+      hi = fmaxf(hi, __shfl_xor(hi, off, lanes)), lo = fminf(lo, __shfl_xor(lo, off, lanes));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, lanes)));
+    }
+    const float range = p.z ? hi - lo : fmaxf(hi, -lo);
+    constexpr uint32_t kInf = 0x7f800000u;
+    const bool numbers = top < kInf && __float_as_uint(fabsf(range)) < kInf;
+    const float s = numbers ? round_to_type<T>(range / (p.z ? 15.0f : 7.0f)) : __uint_as_float(0x7fc00000u);
     const float zero = p.z ? (s > 0.f ? fminf(rintf(-lo / s), 15.f) : 0.f) : 8.f;
     uint32_t word = 0;
 #pragma unroll

@@ -116,7 +116,7 @@ def per_group_quant_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool
     ``(w_q, w_s, w_z)`` with w_q [..., K / 2] uint8, w_s [..., K / group_size] in the type of w and w_z uint8 like it, or None.
 
     Without zero points ``w_s = amax / 7`` and codes around 8; with them the range of a group from its lowest (at most 0) to its highest value
-    (at least 0) is cut into 15 steps.
+    (at least 0) is cut into 15 steps.  A group that holds an infinity or a NaN gets a scale of NaN, so its products show it.
     """
     _decoder.no_tangents(w)
     if w.dtype not in (torch.bfloat16, torch.float16):

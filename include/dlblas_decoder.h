@@ -138,7 +138,8 @@ int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, c
 /*
  * 4-bit codes of a weight, per group of columns: without z  s = max |w| / 7, q = clamp(round(w / s) + 8, 0, 15);  with z
  * s = (max(w, 0) - min(w, 0)) / 15, z = round(-min(w, 0) / s), q = clamp(round(w / s) + z, 0, 15); s rounded to the type of w before it
- * divides.  A group of zeros has s = 0.
+ * divides.  A group of zeros has s = 0, and so has one whose s rounds to 0.  A group that holds an infinity or a NaN, or whose max - min
+ * passes fp32, has s = NaN and dequantises to NaN.
  *
  *   w [rows, K] bf16 / fp16 / fp32, row stride w_row_stride;  q [rows, K/2], 4-byte aligned;  s [rows, K/group] of w's type;  z or NULL
  */
