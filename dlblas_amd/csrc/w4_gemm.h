@@ -42,6 +42,10 @@ struct W4Args {
   int s_type;
 };
 
+// Zero points are 0 to 15, and 16, which a checkpoint that keeps z - 1 comes to: 16 + z is 32 then, still exact in every form here.  A byte
+// above that is none, and its group's scale is taken as NaN, so that its column shows it whichever kernel runs.
+constexpr uint32_t kMaxZero = 16;
+
 template <int T>
 __device__ __forceinline__ v4f mfma_16x16x32(const v4i& a, const v4i& b, const v4f& c) {
   if (T == kInBf16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -115,6 +119,14 @@ __device__ __forceinline__ uint64_t load_packed(const E* p) {
   typedef std::conditional_t<kBytes == 8, uint64_t, std::conditional_t<kBytes == 4, uint32_t, std::conditional_t<kBytes == 2, uint16_t, uint8_t>>> word;
   typedef word word_el __attribute__((aligned(sizeof(E))));
   return *reinterpret_cast<const word_el*>(p);
+}
+// Two 16-bit scales of which those are NaN whose zero point, byte 2 J or 2 J + 1 of z, is none: bit 7 of a byte shows it, moved up to bit
+// 15 of a half, from where a borrow fills the bits below.
+template <int J>
+__device__ __forceinline__ uint32_t mark_bad_zeros(uint32_t scales, uint32_t z) {
+  const uint32_t over = ((z & 0x7f7f7f7fu) + 0x01010101u * (0x7fu - kMaxZero)) | z;
+  const uint32_t top = __builtin_amdgcn_perm(over & 0x80808080u, 0, J == 0 ? 0x050c040cu : 0x070c060cu);
+  return scales | (top - (top >> 15));
 }
 // A word of every lane as the lanes of each half have it, in all lanes of both.
 struct Halves {
@@ -228,6 +240,7 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
       for (int n = 0; n < NT; ++n) {
         transpose_quarters(b.w[n]);
         float s = p.s_type == kInBf16 ? __uint_as_float(b.s[n] << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s[n])));
+        if (ZEROS && b.z[n] > kMaxZero) s = __builtin_nanf("");
         if (GROUPS > 1 && kb * GROUPS + quarter * GROUPS / 4 >= p.G) s = 0.f;
         spread_quarters(s, sc[n]);
         if (ZEROS)
@@ -458,15 +471,22 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_shared_kernel(const W4A
       for (int n = 0; n < NT; ++n) {
         const int mine = p.G - (c * kChunkGroups + my_group);  // groups left in the row
         if (kMine == 1) {
-          sh[n][0] = halves(mine > 0 ? __float_as_uint(widened(static_cast<uint32_t>(b.s[n]) << 16)) : 0u);
+          const uint32_t s = ZEROS && b.z[n] > kMaxZero ? 0x7fc00000u : __float_as_uint(widened(static_cast<uint32_t>(b.s[n]) << 16));
+          sh[n][0] = halves(mine > 0 ? s : 0u);
           if (ZEROS) zh[n] = halves(b.z[n]);
           continue;
         }
         const int down = max(0, min(s_off[n] + c * kChunkGroups - s_last, kMine - 1));
-        const uint64_t s = mine >= kMine ? b.s[n] >> (16 * down) : b.s[n] >> (16 * down) & ((uint64_t{1} << (16 * max(0, mine))) - 1);
+        uint64_t s = b.s[n] >> (16 * down);
+        if (ZEROS) {
+          const uint32_t z = b.z[n] >> (8 * down);
+          zh[n] = halves(z);
+          const uint64_t high = kWords > 1 ? mark_bad_zeros<1>(static_cast<uint32_t>(s >> 32), z) : 0u;
+          s = high << 32 | mark_bad_zeros<0>(static_cast<uint32_t>(s), z);
+        }
+        if (mine < kMine) s &= (uint64_t{1} << (16 * max(0, mine))) - 1;
 #pragma unroll
         for (int j = 0; j < kWords; ++j) sh[n][j] = halves(static_cast<uint32_t>(s >> (32 * j)));
-        if (ZEROS) zh[n] = halves(b.z[n] >> (8 * down));
       }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {

@@ -71,7 +71,8 @@ def _check(x, w_q, w_s, w_z, dims):
 
 def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` [..., K] (bf16 / fp16) times the 4-bit weights ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / group] (bf16 or fp16)
-    and zero points ``w_z`` (uint8 like w_s, 0 ... 15, or None: 8): [..., N] in the type of x; fp32 sums, one rounding.
+    and zero points ``w_z`` (uint8 like w_s, 0 ... 16, or None: 8; a byte above 16 makes its column NaN): [..., N] in the type of x; fp32
+    sums, one rounding.
 
     For up to a few dozen rows: the weights are read once per 32 of them.  A product of N(0, 1)-like rows is as exact as its rounding;
     see include/dlblas_decoder.h for rows that are nearly constant.

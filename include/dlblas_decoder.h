@@ -122,7 +122,7 @@ size_t dlb_w4_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t e
  *   x    [rows, K]         bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^24), 4-byte aligned
  *   q    [experts, N, K/2] 4-bit codes, the even column in the low half of a byte; contiguous, 16-byte aligned
  *   s    [experts, N, K/group] scales, bf16 / fp16 (s_dtype), contiguous
- *   z    the same shape, one byte each (0 ... 15; other bits give other products), or NULL: 8 everywhere
+ *   z    the same shape, one byte each (0 ... 16; a byte above makes its column of y NaN), or NULL: 8 everywhere
  *   y    [rows, N]         dtype, row stride y_row_stride
  *   row_start, row_end [experts] int32 on the device: expert e multiplies the rows [row_start[e], row_end[e]), clamped to
  *        [0, rows]; ranges share no row, rows of no expert are not written.  NULL with experts = 1: every row
