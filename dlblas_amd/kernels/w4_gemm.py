@@ -75,7 +75,8 @@ def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional
     sums, one rounding.
 
     For up to a few dozen rows: the weights are read once per 32 of them.  A product of N(0, 1)-like rows is as exact as its rounding;
-    see include/dlblas_decoder.h for rows that are nearly constant.
+    see include/dlblas_decoder.h for rows that are nearly constant or close to the end of fp32.  An infinity in a row of x makes that
+    row of the product NaN.
     """
     if not torch.compiler.is_compiling():
         y = _fast.w4_gemm(x, w_q, w_s, w_z)

@@ -117,7 +117,9 @@ size_t dlb_w4_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t e
 
 /*
  * y[m, n] = sum over the groups g of K of s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]); fp32 sums, one rounding at the end.
- * The sums of a group are those of x (16 + q) and x (16 + z): they are off by up to 24 * 2^-24 of 62 sum |x|.
+ * The sums of a group are those of x (16 + q) and x (16 + z): they are off by up to 24 * 2^-24 of 62 sum |x|, as long as fp32 holds
+ * 32 sum |x| (fp16 rows: always; bf16 rows: |x| below 8 * 10^34 will do).  Past that, and for an infinity, whose sign and weight the
+ * definition would keep, the two sums leave NaN.
  *
  *   x    [rows, K]         bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^24), 4-byte aligned
  *   q    [experts, N, K/2] 4-bit codes, the even column in the low half of a byte; contiguous, 16-byte aligned

@@ -1,4 +1,5 @@
-"""Products with 4-bit weights at the values where they can go wrong: zero points at and past the end of their range.
+"""Products with 4-bit weights at the values where they can go wrong: zero points at and past the end of their range, rows that are nearly
+constant, rows close to the end of fp32.
 
 The sizes of MATRICES are served by both kernels: few weights by the one whose waves split K, many by the one whose tiles share x."""
 import pytest
@@ -87,3 +88,33 @@ def test_zero_points_by_expert(dev, N, K, group):
     end[2], start[3] = 6, 6
     y = w4_gemm_grouped(*on(dev, x, q, s, start, end, z)).cpu()
     assert bool(y[4:6, 7].isnan().all()) and int(y.isnan().sum()) == 2
+
+
+# ---- rows ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('dtype', [bf16, f16])
+@pytest.mark.parametrize('M,N,K,group', MATRICES)
+def test_rows_that_are_nearly_constant(dev, M, N, K, group, dtype):
+    """sum x (16 + q) and (16 + z) sum x are both large then and their difference is not: the case the bound is made for."""
+    q, s, z = weights(N, K, group, dtype)
+    g = torch.Generator().manual_seed(M)
+    x = (3 * (1 + 2.0**-6 * torch.randn(M, K, generator=g))).to(dtype)
+    codes = orc.w4_codes(q).reshape(N, -1, group)
+    z = codes.float().mean(-1).round().to(torch.uint8)
+    check(w4_gemm(*on(dev, x, q, s, z)), x, q, s, z, f'{M}x{N}x{K}/{group}')
+    check(w4_gemm(*on(dev, x, q, s)), x, q, s, None, f'{M}x{N}x{K}/{group}, no zero points')
+
+
+@pytest.mark.parametrize('M,N,K,group', MATRICES)
+def test_rows_close_to_the_end_of_fp32(dev, M, N, K, group):
+    """What the bound covers: 32 sum |x| of a group below 2^128.  Rows just inside are products like any other; an infinity gives NaN,
+    whatever its weight, since both sums hold it."""
+    q, s, z = weights(N, K, group, bf16)
+    s = (s.double() * 2.0**-20).to(bf16)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M))
+    x = (x * (2.0**122 / x.abs().reshape(M, -1, group).sum(-1).max())).to(bf16)  # 2^127 with the factor 32, and bf16's rounding
+    check(w4_gemm(*on(dev, x, q, s, z)), x, q, s, z, f'{M}x{N}x{K}/{group}')
+    x[0, K // 2] = float('inf')
+    y = w4_gemm(*on(dev, x, q, s, z)).cpu()
+    assert bool(y[0].isnan().all()) and bool(y[1:].isfinite().all())
