@@ -415,9 +415,6 @@ int dlb_moe_unpermute(const void* rows, int64_t rows_row_stride, int dtype, cons
   if (rows_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
   if (off_elements(rows, dtype) || off_elements(out, dtype) || misaligned(row_index, 4) || misaligned(weights, 4))
     return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
-  int dev = 0;
-  const int cus = device_cu_count(&dev);
-  if (cus < 0) return fail(DLB_ERR_LAUNCH, "hipGetDevice failed");
   const UnpermuteArgs a{rows, row_index, weights, out, rows_row_stride, out_row_stride, tokens, num_rows, static_cast<int>(H), static_cast<int>(topk)};
   int64_t parts = ceil_div(H, 512);
   if (parts > 64) parts = 64;
