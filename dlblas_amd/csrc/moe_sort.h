@@ -39,7 +39,7 @@ struct SortArgs {
 
 __device__ __forceinline__ int sort_id(const SortArgs& p, int64_t i) {
   if (i >= p.n) return -1;
-  const int64_t t = p.n < (1ll << 31) ? static_cast<uint32_t>(i) / static_cast<uint32_t>(p.topk) : i / p.topk;
+  const int64_t t = static_cast<uint32_t>(i) / static_cast<uint32_t>(p.topk);  // n fits the int32 tables
   const int64_t at = t * p.ids_s0 + (i - t * p.topk) * p.ids_s1;
   const int64_t id = p.ids_is64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p.ids)[at]);
   return (id < 0 || id >= p.E) ? -1 : static_cast<int>(id);
