@@ -530,7 +530,7 @@ int dlb_w4_quant(const void* w, int64_t w_row_stride, int dtype, void* q, void* 
                  void* stream) {
   using namespace dlb;
   clear_error();
-  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16, the types of scales", dtype);
   if (rows < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld K=%lld)", (long long)rows, (long long)K);
   if (group != 32 && group != 64 && group != 128) return fail(DLB_ERR_BAD_SHAPE, "group=%lld is not 32, 64 or 128", (long long)group);
   if (K % group != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of the group size %lld", (long long)K, (long long)group);
@@ -542,7 +542,8 @@ int dlb_w4_quant(const void* w, int64_t w_row_stride, int dtype, void* q, void* 
   const W4QuantArgs a{w, static_cast<uint8_t*>(q), s, static_cast<uint8_t*>(z), rows, w_row_stride, static_cast<int>(K / group), static_cast<int>(group)};
   const int64_t blocks = ceil_div(rows * a.G * (group / 8), 256);
   const dim3 grid(static_cast<unsigned>(blocks < 8192 ? blocks : 8192));
-  with_type(dtype, [&](auto t) { hipLaunchKernelGGL(w4_quant_kernel<t()>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a); });
+  const auto launch = [&](auto t) { hipLaunchKernelGGL(w4_quant_kernel<t()>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a); };
+  dtype == kInBf16 ? launch(std::integral_constant<int, kInBf16>()) : launch(std::integral_constant<int, kInF16>());
   return finish("w4_quant");
 }
 

@@ -642,8 +642,7 @@ struct W4QuantArgs {
 template <int T>
 __device__ __forceinline__ float round_to_type(float v) {
   if (T == kInBf16) return static_cast<float>(static_cast<__bf16>(v));
-  if (T == kInF16) return static_cast<float>(static_cast<_Float16>(v));
-  return v;
+  return static_cast<float>(static_cast<_Float16>(v));
 }
 
 // A group's lanes hold eight columns each.  Run once per weight: 4096 x 7168 28 us, 2.6 TB/s, its divisions.
@@ -678,9 +677,7 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const W4QuantArgs p) {
     }
     reinterpret_cast<uint32_t*>(p.q)[g * lanes + sub] = word;
     if (sub == 0) {
-      if (T == kInF32)
-        static_cast<float*>(p.s)[g] = s;
-      else if (T == kInBf16)
+      if (T == kInBf16)
         static_cast<__bf16*>(p.s)[g] = static_cast<__bf16>(s);
       else
         static_cast<_Float16*>(p.s)[g] = static_cast<_Float16>(s);

@@ -143,7 +143,7 @@ int dlb_w4_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, c
  * divides.  A group of zeros has s = 0, and so has one whose s rounds to 0.  A group that holds an infinity or a NaN, or whose max - min
  * passes fp32, has s = NaN and dequantises to NaN.
  *
- *   w [rows, K] bf16 / fp16 / fp32, row stride w_row_stride;  q [rows, K/2], 4-byte aligned;  s [rows, K/group] of w's type;  z or NULL
+ *   w [rows, K] bf16 / fp16, row stride w_row_stride;  q [rows, K/2], 4-byte aligned;  s [rows, K/group] of w's type;  z or NULL
  */
 int dlb_w4_quant(const void* w, int64_t w_row_stride, int dtype, void* q, void* s, void* z, int64_t rows, int64_t K, int64_t group,
                  void* stream);

@@ -1,7 +1,10 @@
-"""What the Python functions of the steps around the products refuse, beside tests/test_decoder_steps.py: without a GPU."""
+"""What the steps around the products refuse, beside tests/test_decoder_steps.py: without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
+from dlblas_amd import _lib
 from dlblas_amd.kernels.moe_permute import moe_permute
 
 
@@ -14,3 +17,9 @@ def test_quantised_tokens_have_no_gradient(which):
             t.requires_grad_()
     with pytest.raises(NotImplementedError, match='no gradient'):
         moe_permute((codes, scales), torch.zeros(2, 1, dtype=torch.int32), 4)
+
+
+def test_the_4_bit_quantiser_takes_the_types_that_scales_have():
+    """Its scales have the type of the weights, and no product takes scales in 32 bits."""
+    fake, null = ctypes.c_void_p(4096), ctypes.c_void_p(0)
+    assert _lib.load().dlb_w4_quant(fake, 256, _lib.IN_CODES[torch.float32], fake, fake, null, 4, 256, 128, null) == _lib.ERR_BAD_DTYPE
