@@ -192,9 +192,8 @@ W4Plan w4_plan(int64_t rows_each, bool by_expert, int64_t matrices, int64_t N, i
 template <int T, int GROUPS, bool ZEROS>
 void launch_w4(const W4Args& a, const W4Plan& plan, int64_t y_blocks, float* sums, hipStream_t st) {
   if (!plan.shared) {
-    const int waves = 4;
     const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16)), static_cast<unsigned>(y_blocks));
-    hipLaunchKernelGGL((w4_gemm_kernel<T, GROUPS, ZEROS, 1, 1, 4>), grid, dim3(64 * waves), waves * 1024, st, a);
+    hipLaunchKernelGGL((w4_gemm_kernel<T, GROUPS, ZEROS>), grid, dim3(64 * kW4Waves), 0, st, a);
     return;
   }
   const dim3 grid(static_cast<unsigned>(ceil_div(a.N, w4_columns(plan.mt))), static_cast<unsigned>(y_blocks), static_cast<unsigned>(plan.slices));

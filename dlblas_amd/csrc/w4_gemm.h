@@ -154,29 +154,32 @@ __device__ __forceinline__ void quarters(const Halves& h, uint32_t (&out)[4], bo
   }
 }
 
+constexpr int kW4Waves = 4;  // of a workgroup, in both kernels
+
 // What a wave reads for one block of 128 columns: its weights, the scale (and zero point) of the quarter's group, its rows of x.
-template <int MT, int NT>
 struct W4Block {
-  v4i w[NT];
-  uint32_t s[NT], z[NT];
-  v4i x[MT][4];
+  v4i w;
+  uint32_t s, z;
+  v4i x[4];
 };
 
-// GROUPS = groups in a block of 128 columns: 1, 2, 4 for groups of 128, 64, 32.  A tile is 16 MT rows of x by 16 NT rows of the
+// GROUPS = groups in a block of 128 columns: 1, 2, 4 for groups of 128, 64, 32.  A tile is 16 rows of x by 16 rows of the
 // matrix.  After the exchange of words between the quarters, step i of a block is columns 32 i to 32 i + 31, 8 a quarter.
-// DEPTH blocks are on their way to a wave at a time.  Loads return in the order they were issued in, so all that a block needs is
+// kW4Depth blocks are on their way to a wave at a time.  Loads return in the order they were issued in, so all that a block needs is
 // asked for together, and none of them stands behind a branch, because a wait counts the loads issued since: what lies outside
 // (rows past the tile, columns past the end, blocks past the last one) has an offset past the end of the buffer, which costs no
 // traffic and gives zero.  For products whose launch and latency count: 1 x 2112 x 7168 7.0 us (7.8 MB), 5 tokens x 2 of 8 experts x 1000 x 1056
 // fp16, groups of 32 with zero points 6.8 us, 1 x 512 x 2048 4.3; two waves instead of four 9.4, 7.6, 4.5, eight 8.6, 12.4, 6.1.
-template <int T, int GROUPS, bool ZEROS, int MT, int NT, int DEPTH>
-__global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
-  extern __shared__ float part[];  // [waves][MT][NT][256]
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+constexpr int kW4Depth = 4;
+
+template <int T, int GROUPS, bool ZEROS>
+__global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_kernel(const W4Args p) {
+  __shared__ float part[kW4Waves][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int quarter = lane >> 4, l16 = lane & 15;
   constexpr uint32_t kNowhere = 0x80000000u;  // every buffer is shorter
   int64_t expert = 0;
-  int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT, row_end = min(p.rows, row0 + 16 * MT);
+  int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16, row_end = min(p.rows, row0 + 16);
   if (p.row_start) {
     const int e = nth_expert(p, blockIdx.y, lane);
     if (e < 0) return;
@@ -185,15 +188,13 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
   }
   const int blocks = (p.K + 127) / 128;
   const uint32_t half = p.K / 2;  // bytes of a row
-  const int n0 = static_cast<int>(blockIdx.x) * 16 * NT;
-  const int cols = min(16 * NT, p.N - n0);
+  const int n0 = static_cast<int>(blockIdx.x) * 16;
+  const int cols = min(16, p.N - n0);
   const uint8_t* w_ptr = p.q + expert * p.q_es + static_cast<int64_t>(n0) * half;
   const int64_t s0 = expert * p.s_es + static_cast<int64_t>(n0) * p.G;
   const uint8_t *s_ptr = static_cast<const uint8_t*>(p.s) + 2 * s0, *z_ptr = ZEROS ? p.z + s0 : p.q;
   const uint32_t w_bytes = cols * half, s_count = cols * p.G;
-  uint32_t w_off[NT], s_off[NT];  // of rows past the matrix: past the end
-#pragma unroll
-  for (int n = 0; n < NT; ++n) w_off[n] = (16 * n + l16) * half + 16 * quarter, s_off[n] = (16 * n + l16) * p.G + quarter * GROUPS / 4;
+  const uint32_t w_off = l16 * half + 16 * quarter, s_off = l16 * p.G + quarter * GROUPS / 4;  // of rows past the matrix: past the end
   // in registers, where one v_and_or_b32 takes both
   int mask = T == kInBf16 ? 0x00780078 : 0x03c003c0, bits = T == kInBf16 ? 0x41804180 : 0x4c004c00;
   asm("" : "+s"(mask));
@@ -202,127 +203,87 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) ones[i] = T == kInBf16 ? 0x3f803f80 : 0x3c003c00;
 
-  for (; row0 < row_end; row0 += 16 * MT) {
-    const int rows = static_cast<int>(min(row_end - row0, static_cast<int64_t>(16 * MT)));
+  for (; row0 < row_end; row0 += 16) {
+    const int rows = static_cast<int>(min(row_end - row0, int64_t{16}));
     const uint32_t x_row = static_cast<uint32_t>(p.x_rs) * 2;
     const uint8_t* x_ptr = static_cast<const uint8_t*>(p.x) + row0 * p.x_rs * 2;
     const uint32_t x_bytes = (rows - 1) * x_row + 2u * p.K;
-    uint32_t x_off[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) x_off[m] = 16 * m + l16 < rows ? (16 * m + l16) * x_row + 16 * quarter : kNowhere;
-    v4f acc[MT][NT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    const uint32_t x_off = l16 < rows ? l16 * x_row + 16 * quarter : kNowhere;
+    v4f acc{0.f, 0.f, 0.f, 0.f};
     // The place of a block travels in the scalar offset, so a load costs no vector instruction; past the last block the buffers are
     // empty.  A lane past the last column of a row
     // reads the next row's codes, which then meet zeros of x; the scale of such a group is replaced in multiply().
-    auto load = [&](int kb, W4Block<MT, NT>& b) {
+    auto load = [&](int kb, W4Block& b) {
       const bool in = kb < blocks;
       const uint32_t at = in ? kb : 0;
       const auto w_src = make_rsrc(w_ptr, in ? w_bytes : 0), s_src = make_rsrc(s_ptr, in ? 2 * s_count : 0), z_src = make_rsrc(z_ptr, ZEROS && in ? s_count : 0);
       const auto x_src = make_rsrc(x_ptr, in ? x_bytes : 0);
+      b.w = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(w_src, w_off, 64 * at, 2));
+      b.s = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * s_off, 2 * GROUPS * at, 0);
+      if (ZEROS) b.z = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off, GROUPS * at, 0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        b.w[n] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(w_src, w_off[n], 64 * at, 2));
-        b.s[n] = __builtin_amdgcn_raw_buffer_load_b16(s_src, 2 * s_off[n], 2 * GROUPS * at, 0);
-        if (ZEROS) b.z[n] = __builtin_amdgcn_raw_buffer_load_b8(z_src, s_off[n], GROUPS * at, 0);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b.x[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, x_off[m] + 64 * i, 256 * at, 0));
+      for (int i = 0; i < 4; ++i) b.x[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, x_off + 64 * i, 256 * at, 0));
     };
-    auto multiply = [&](int kb, W4Block<MT, NT>& b) {
-      float sc[NT][GROUPS], coef[NT][GROUPS];
+    auto multiply = [&](int kb, W4Block& b) {
+      float sc[GROUPS], coef[GROUPS];
+      transpose_quarters(b.w);
+      float s = p.s_type == kInBf16 ? __uint_as_float(b.s << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s)));
+      if (ZEROS && b.z > kMaxZero) s = __builtin_nanf("");
+      if (GROUPS > 1 && kb * GROUPS + quarter * GROUPS / 4 >= p.G) s = 0.f;
+      spread_quarters(s, sc);
+      if (ZEROS)
+        spread_quarters(-16.f - static_cast<float>(b.z), coef);
+      else
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        transpose_quarters(b.w[n]);
-        float s = p.s_type == kInBf16 ? __uint_as_float(b.s[n] << 16) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b.s[n])));
-        if (ZEROS && b.z[n] > kMaxZero) s = __builtin_nanf("");
-        if (GROUPS > 1 && kb * GROUPS + quarter * GROUPS / 4 >= p.G) s = 0.f;
-        spread_quarters(s, sc[n]);
-        if (ZEROS)
-          spread_quarters(-16.f - static_cast<float>(b.z[n]), coef[n]);
-        else
-#pragma unroll
-          for (int g = 0; g < GROUPS; ++g) coef[n][g] = -24.f;
-      }
+        for (int g = 0; g < GROUPS; ++g) coef[g] = -24.f;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
-        v4f sum[MT][NT], xs[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          xs[m] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) sum[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
-        }
+        v4f sum{0.f, 0.f, 0.f, 0.f}, xs{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
           // columns past the end: what was read there is the next row, and selecting byte 12 gives zero
           const bool in = kb * 128 + 32 * i < p.K;
           const uint32_t low = in ? 0x05040100u : 0x0c0c0c0cu, high = in ? 0x07060302u : 0x0c0c0c0cu;
-          v4i xf[MT];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const v4i v = b.x[m][i];
-            xf[m][0] = __builtin_amdgcn_perm(v[2], v[0], low);
-            xf[m][1] = __builtin_amdgcn_perm(v[2], v[0], high);
-            xf[m][2] = __builtin_amdgcn_perm(v[3], v[1], low);
-            xf[m][3] = __builtin_amdgcn_perm(v[3], v[1], high);
-          }
-#pragma unroll
-          for (int m = 0; m < MT; ++m) xs[m] = mfma_16x16x32<T>(xf[m], ones, xs[m]);
+          const v4i v = b.x[i];
+          const v4i xf{static_cast<int>(__builtin_amdgcn_perm(v[2], v[0], low)), static_cast<int>(__builtin_amdgcn_perm(v[2], v[0], high)),
+                       static_cast<int>(__builtin_amdgcn_perm(v[3], v[1], low)), static_cast<int>(__builtin_amdgcn_perm(v[3], v[1], high))};
+          xs = mfma_16x16x32<T>(xf, ones, xs);
           constexpr int kUp = T == kInBf16 ? 3 : 6;
+          const int word = b.w[i];
+          v4i codes;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int word = b.w[n][i];
-            v4i v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & mask) | bits;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) sum[m][n] = mfma_16x16x32<T>(xf[m], v, sum[m][n]);
-          }
+          for (int j = 0; j < 4; ++j) codes[j] = ((4 * j < kUp ? word << (kUp - 4 * j) : word >> (4 * j - kUp)) & mask) | bits;
+          sum = mfma_16x16x32<T>(xf, codes, sum);
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(sc[n][g], fmaf(coef[n][g], xs[m][r], sum[m][n][r]), acc[m][n][r]);
+        for (int r = 0; r < 4; ++r) acc[r] = fmaf(sc[g], fmaf(coef[g], xs[r], sum[r]), acc[r]);
       }
     };
-    W4Block<MT, NT> on_way[DEPTH];
+    W4Block on_way[kW4Depth];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      load(wave + d * waves, on_way[d]);
+    for (int d = 0; d < kW4Depth; ++d) {
+      load(wave + d * kW4Waves, on_way[d]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    for (int kb = wave; kb < blocks; kb += DEPTH * waves) {
+    for (int kb = wave; kb < blocks; kb += kW4Depth * kW4Waves) {
       // whole turns: blocks past the last one multiply zeros; the order of loads and products stays as it is written
 #pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
-        multiply(kb + d * waves, on_way[d]);
+      for (int d = 0; d < kW4Depth; ++d) {
+        multiply(kb + d * kW4Waves, on_way[d]);
         __builtin_amdgcn_sched_barrier(0);
-        load(kb + (DEPTH + d) * waves, on_way[d]);
+        load(kb + (kW4Depth + d) * kW4Waves, on_way[d]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // lane l holds rows 4 (l / 16) + r, column l % 16 of a tile
+    // lane l holds rows 4 (l / 16) + r, column l % 16 of the tile
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) part[((wave * MT + m) * NT + n) * 256 + (4 * quarter + r) * 16 + l16] = acc[m][n][r];
+    for (int r = 0; r < 4; ++r) part[wave][(4 * quarter + r) * 16 + l16] = acc[r];
     __syncthreads();
-    for (int i = tid; i < MT * NT * 256; i += blockDim.x) {
-      const int m = i / (NT * 256), n = i / 256 % NT, e = i % 256;
-      const int row = 16 * m + e / 16, col = 16 * n + e % 16;
-      float sum = 0.f;
-      for (int w = 0; w < waves; ++w) sum += part[w * MT * NT * 256 + i];
-      if (row >= rows || col >= cols) continue;
+    const int row = tid / 16, col = tid % 16;  // a thread an element
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kW4Waves; ++w) sum += part[w][tid];
+    if (row < rows && col < cols) {
       const int64_t at = (row0 + row) * p.y_rs + n0 + col;
       if (T == kInBf16)
         static_cast<__bf16*>(p.y)[at] = static_cast<__bf16>(sum);
@@ -342,7 +303,6 @@ __global__ void __launch_bounds__(512) w4_gemm_kernel(const W4Args p) {
 // sums, instructions of the few waves per SIMD and the start of the stream; 64 x 7168 x 18432 47 us, where a SIMD has 13 us of products and 15
 // of other vector instructions to issue and its one or two waves overlap them badly (a third of their time each waiting for issue, waiting for
 // LDS and memory, issuing).  Two chunks on their way instead of one 28 and 49 us, three 30 and 52.
-constexpr int kW4Waves = 4;
 constexpr int kW4Unit = 256;  // columns
 
 // PIECES = 16-byte pieces of x a thread moves per chunk: all rows of a tile take 2 MT UNITS, one is enough for 8 / UNITS rows (1 x 7168 x
