@@ -196,6 +196,8 @@ def moe_unpermute(rows: torch.Tensor, permutation: Union[MoePermutation, torch.T
     if torch.is_grad_enabled() and (rows.requires_grad or (topk_weights is not None and topk_weights.requires_grad)):
         if not whole:
             raise ValueError('the gradients need the MoePermutation of moe_permute: a table of rows may name a row twice')
+        if permutation.source.dtype != torch.int32:
+            raise TypeError(f'the permutation holds int32 tables, got a source of {permutation.source.dtype}')
         if tuple(permutation.source.shape) != (rows.size(0), ):
             raise ValueError(f'the permutation is one of {permutation.source.numel()} rows, got {rows.size(0)}')
         if rows.size(1) > _decoder.NORM_MAX_COLUMNS:
