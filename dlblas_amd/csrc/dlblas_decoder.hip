@@ -158,7 +158,7 @@ int w4_chunk(int mt) { return mt == 1 ? 2 * kW4Unit : kW4Unit; }           // co
 // above 8 rows per expert too, because experts have more than the mean.  Below, whichever of the two kernels is estimated faster, in us:
 //   shared x   a chunk of a workgroup alone on its CU is about one; rounds over the chip x chunks, which go in pairs.  Workgroups beside
 //              each other on a CU overlap, the more the less they have to compute.  With slices a second launch and the sums' way through
-//              memory at 5 TB/s.  Slices that this picks, and others: 1 x 7168 x 18432 nine 20.6, two 24.0, four 21.2; 16 rows nine 24.7, two
+//              memory at 5 TB/s.  Slices that this picks, and others, in one run: 1 x 7168 x 18432 nine 20.6, two 24.0, four 21.2; 16 rows nine 24.7, two
 //              25.0, four 26.0; 1 x 7168 x 7168 four 11.6, one 16.1, seven 12.5; 64 x 36864 x 7168 two 87, one 92, seven 99.
 //   K over the waves   a launch, the columns of K, each the longer the more rows there are, further rounds, at most 2.4 TB/s.
 // Measured, K over the waves / shared: 1 x 512 x 2048 4.3 / 5.9, 16 x 512 x 2048 5.6 / 6.9, 1 x 2112 x 7168 7.6 / 7.6, 16 x 2112 x 7168 11.8 / 8.4,

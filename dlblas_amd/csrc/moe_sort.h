@@ -341,8 +341,8 @@ struct UnpermuteArgs {
 
 // One wave per token and stretch of 512 columns (a chunk a lane); the slots' rows and weights come in one load each, a lane a slot.  The
 // chunks of kUnpermuteRows rows are on their way at a time, behind the last row that one again.  4096 tokens x 8 rows of 7168 bf16, 528 MB:
-// 131 us, 4.0 TB/s, which is what reading 2 GiB in order reaches here too; the stretches of a token next to each other in the grid, or two
-// and seven of them by one wave, took 133, 130 and 130.  1001 x 4096, two thirds of 6 slots here: 8.9 us.
+// 131 us, 4.0 TB/s (streams in order reach 6.0 here, with the non-temporal bit 7.0; these loads do not have it); the stretches of a token next
+// to each other in the grid, or two and seven of them by one wave, took 133, 130 and 130.  1001 x 4096, two thirds of 6 slots here: 8.9 us.
 constexpr int kUnpermuteRows = 4;
 
 template <int T, bool WHOLE>

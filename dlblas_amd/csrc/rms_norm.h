@@ -5,7 +5,8 @@
 //   gradient:    dh = r (w dy) - h r^3 / H sum(w dy h) + dsum,   dw = sum over the rows of dy h r
 //
 // h is rounded before the norm reads it: it is what the next layer adds to and what the gradient starts from, so both see the same
-// rows.  Everything else is held in fp32 and rounded once at the store.
+// rows.  Everything else is held in fp32 and rounded once at the store.  That holds for the sum of squares too: of a row whose sum passes
+// 2^128 r is 0.
 //
 // All of it is bound by memory: a row is read once into registers (8 elements a chunk, CH chunks a thread), the sums cross the
 // workgroup once, and the results leave from the registers.  Chunks are consecutive over the lanes, so 16 lanes hold a group of
@@ -228,8 +229,9 @@ __global__ void __launch_bounds__(kNormMaxThreads) rms_norm_kernel(const NormArg
       store_raw8<T, WHOLE>(p.y, row * p.y_rs, 8 * i, pack_raw8<T>(y), p.H - 8 * i);
       continue;
     }
-    // y / s = 448 h w / max |h w|: r cancels, and for 16-bit rows and weights the operands of that quotient are exact, so a value half way
-    // between two codes stays there (with y rounded first 1 of 10^4 codes of bf16 rows differed, with these operands none of 3 10^6).
+    // y / s = 448 h w / max |h w|: r cancels, and for bf16 rows and weights (8 + 8 + 3 bits) the operands of that quotient are exact, so a
+    // value half way between two codes stays there (with y rounded first 1 of 10^4 codes differed, with these operands none of 3 10^6).  fp16
+    // rows take 25 bits, one rounding of fp32, and fp32 weights under 16-bit rows two.
     // Rows of fp32 take y, as the quantiser does that reads it from memory, and so do groups whose h w is close to the ends of fp32.
     constexpr bool kExact = T != kInF32;
     float num[8], den;

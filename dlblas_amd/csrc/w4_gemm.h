@@ -6,10 +6,10 @@
 // Bound by the weights' bytes while the rows are few, so every weight byte goes from memory to a register once and straight into
 // v_mfma_f32_16x16x32: a lane's 16 bytes are 32 weights of one row of the matrix, four MFMA steps.  There is no conversion: a code
 // moved to the top of the significand of the float 16 is 16 + q exactly (bf16: bits 3 to 6, fp16: bits 6 to 9), a shift and an
-// and-or for two weights, and the 16 leaves through the sum of x over the group, which one more MFMA with a matrix of ones gives for
-// all tiles of a wave:
+// and-or for two weights, and the 16 leaves through the sum of x over the group:
 //   sum x (q - z) = sum x (16 + q) - (16 + z) sum x
-// in fp32; the scale multiplies that once per group.  What this costs is rounding of the fp32 sums of terms up to 31 |x| instead of
+// in fp32; the scale multiplies that once per group.  The kernel whose waves split K has sum x from an MFMA with a matrix of ones and takes
+// (16 + z) times it off; the one whose tiles share x adds -(16 + z) x through an MFMA of its own, which is half of the products it issues.  What this costs is rounding of the fp32 sums of terms up to 31 |x| instead of
 // |q - z| |x|: the unit adds the 8 products of a quarter cut off 2^-24 below the largest of them and rounds after each quarter
 // (measured with ladders of powers of two), so a group's sum is off by at most 24 * 2^-24 * 62 sum |x|.
 // A word's eight codes come out as the pairs (0, 4), (1, 5), (2, 6), (3, 7); x is put into the same order.
@@ -299,8 +299,9 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_gemm_kernel(const W4Args p) 
 // A lane reads 32 bytes of a unit's 128 bytes of a row in two loads, so a load touches whole cache lines: 64 columns a quarter.
 // Eight steps of 32 columns follow, of one group each: for groups of 128 the halves of the wave exchange words, for smaller ones the
 // quarters.  Slices of K (gridDim.z) go to workgroups of their own, whose fp32 sums w4_sum_kernel adds in slice order.
-// 32 experts x 4 rows x 4096 x 7168, 482 MB: 102 us, 4.7 TB/s, the memory's; 16 x 7168 x 18432, 69 MB in nine slices: 20 us and 4 for the
-// sums, instructions of the few waves per SIMD and the start of the stream; 64 x 7168 x 18432 47 us, where a SIMD has 13 us of products and 15
+// 32 experts x 4 rows x 4096 x 7168, 482 MB: 100 us call after call on three sets of weights, of which the cache keeps some, 119 on weights
+// from memory, 4.1 TB/s where streams of weights with the non-temporal bit, which these loads do not have, reach 6.9; 16 x 7168 x 18432, 69 MB
+// in nine slices: 20 us and 4 for the sums from memory, instructions of the few waves per SIMD and the start of the stream; 64 x 7168 x 18432 47 us, where a SIMD has 13 us of products and 15
 // of other vector instructions to issue and its one or two waves overlap them badly (a third of their time each waiting for issue, waiting for
 // LDS and memory, issuing).  Two chunks on their way instead of one 28 and 49 us, three 30 and 52.
 constexpr int kW4Unit = 256;  // columns
@@ -605,7 +606,8 @@ __device__ __forceinline__ float round_to_type(float v) {
   return static_cast<float>(static_cast<_Float16>(v));
 }
 
-// A group's lanes hold eight columns each.  Run once per weight: 4096 x 7168 28 us, 2.6 TB/s, its divisions.
+// A group's lanes hold eight columns each.  Run once per weight: 4096 x 7168 29 us, 2.6 TB/s, with a division for each weight, where one
+// reciprocal a group would do.
 template <int T>
 __global__ void __launch_bounds__(256) w4_quant_kernel(const W4QuantArgs p) {
   const int lanes = p.group / 8;  // of a group: 4, 8 or 16

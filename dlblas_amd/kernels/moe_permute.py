@@ -13,7 +13,8 @@ from .. import _decoder, _fast, _lib
 
 
 class MoePermutation(NamedTuple):
-    """Which slot lies where (all int32): a slot is a (token, j) of topk_ids."""
+    """Which slot lies where (all int32): a slot is a (token, j) of topk_ids.  The tables may lie behind each other in one allocation, on 4
+    bytes each: keeping one keeps all of them."""
     row_index: torch.Tensor  # [T, topk] row of every slot, -1 where it has none
     source: torch.Tensor     # [rows] slot t * topk + j of every row, -1 where it holds none
     m_indices: torch.Tensor  # [rows] expert of every row of a span, -1 past the last span

@@ -4,7 +4,8 @@ block-scaled products, for serving.  The reference has the norms as dlblas/kerne
     h = x + residual, rounded to the type of x          (without a residual h = x)
     y = h / sqrt(mean(h^2) + eps) * weight              in fp32, rounded once
 
-``h`` is rounded before the norm reads it, because it is what the next layer adds to and what the gradient starts from.
+``h`` is rounded before the norm reads it, because it is what the next layer adds to and what the gradient starts from.  The sum of
+squares is held in fp32: rows whose sum passes 2^128 give zeros.
 """
 from typing import Optional
 

@@ -1,4 +1,6 @@
-"""Products of a few rows with 4-bit weights: the decode side of a layer whose weights are kept at half the bytes of e4m3.
+"""Products of a few rows with 4-bit weights: the decode side of a layer whose weights are kept at half the bytes of e4m3.  That is what
+they are for: against ``fp8_gemm`` they are faster where few rows meet many weights (1 x 7168 x 18432 22 and 24 us, 32 experts x 4 rows x
+4096 x 7168 119 and 147) and slower elsewhere (1 x 2112 x 7168 7.6 and 6.3 us, 32 x 7168 x 7168 18 and 14, 64 x 7168 x 18432 48 and 39).
 
     y[m, n] = sum over the groups g of w_s[n, g] * sum_{k in g} x[m, k] * (w_q[n, k] - w_z[n, g])
 

@@ -28,7 +28,8 @@ extern "C" {
 
 /*
  * h = x + residual rounded to the element type (h = x without a residual), y = h * w / sqrt(mean(h^2) + eps); fp32 inside, one
- * rounding at the store.
+ * rounding at the store.  The sum of squares is fp32 as well: rows whose sum passes 2^128 (|h| about 10^17 throughout) give y = 0, or
+ * NaN where they hold an infinity.
  *
  *   x, residual, y, sum  [rows, H]  one element type (dtype); residual NULL: none, and sum is not written
  *   weight               [H]        the same type, or fp32 (weight_dtype)
