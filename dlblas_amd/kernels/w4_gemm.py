@@ -96,7 +96,7 @@ def w4_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, w_z: Optional
 def w4_gemm_grouped(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, row_start: torch.Tensor, row_end: torch.Tensor,
                     w_z: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``w4_gemm`` by expert: the rows [row_start[e], row_end[e]) of ``x`` [R, K] times the weights of expert e, w_q [E, N, K / 2] and so on.
-    The ranges (int32 [E] on the device, clamped to 0 ... R) are those of ``moe_permute``; rows of no expert are not written.  For a decode
+    The ranges (int32 [E] on the device, clamped to 0 ... R, no row in two of them) are those of ``moe_permute``; rows of no expert are not written.  For a decode
     step: an expert's weights are read once per 16 or 32 of its rows, and those of experts without a row not at all."""
     if not torch.compiler.is_compiling():
         y = _fast.w4_gemm_grouped(x, w_q, w_s, row_start, row_end, w_z)
