@@ -12,7 +12,7 @@ SOURCES = ['dlblas_fp8_gemm.hip', 'dlblas_fp8_moe.hip', 'dlblas_decoder.hip']
 
 # packed fp32 VALU forms are switched off for every device compile of this library
 HIPCC_FLAGS = [
-    '-O3', '-std=c++17', '--offload-arch=gfx950', '-shared', '-fPIC', '-Xclang', '-target-feature', '-Xclang',
+    '-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-Xclang', '-target-feature', '-Xclang',
     '-packed-fp32-ops', '-mllvm', '-amdgpu-mfma-vgpr-form=1', '-Wall', '-Wno-unused-function'
 ]
 
@@ -27,11 +27,24 @@ def find_hipcc() -> str:
 def build_library(verbose: bool = False, defines=(), out_path: str = LIB_PATH) -> str:
     """Compile csrc/*.hip into libdlblas_fp8_gemm.so; always recompiles. Returns the library path.
     `defines` / `out_path`: builds kept apart from the library, loaded through the DLBLAS_AMD_LIB environment variable."""
-    cmd = [find_hipcc()] + HIPCC_FLAGS + [f'-D{d}' for d in defines] + ['-o', out_path] + [os.path.join(CSRC_DIR, s) for s in SOURCES]
-    res = subprocess.run(cmd, cwd=CSRC_DIR, capture_output=True, text=True)
-    log = '\n'.join(line for line in (res.stdout + res.stderr).splitlines() if 'packed-fp32-ops' not in line)
-    if res.returncode != 0:
-        raise RuntimeError(f'hipcc failed ({res.returncode}):\n{log}')
+    import tempfile
+    from concurrent.futures import ThreadPoolExecutor
+    hipcc = find_hipcc()
+
+    def run(cmd):
+        res = subprocess.run(cmd, cwd=CSRC_DIR, capture_output=True, text=True)
+        log = '\n'.join(line for line in (res.stdout + res.stderr).splitlines() if 'packed-fp32-ops' not in line)
+        if res.returncode != 0:
+            raise RuntimeError(f'hipcc failed ({res.returncode}):\n{log}')
+        return log
+
+    # the sources beside each other: one of them takes minutes
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(len(SOURCES)) as pool:
+        objs = [os.path.join(objects, s + '.o') for s in SOURCES]
+        logs = list(pool.map(lambda so: run([hipcc] + HIPCC_FLAGS + [f'-D{d}' for d in defines] + ['-c', '-o', so[1], os.path.join(CSRC_DIR, so[0])]),
+                             zip(SOURCES, objs)))
+        logs.append(run([hipcc, '-shared'] + HIPCC_FLAGS + ['-o', out_path] + objs))
+    log = '\n'.join(line for line in logs if line.strip())
     if verbose and log.strip():
         print(log)
     return out_path
