@@ -70,6 +70,26 @@ def rms_norm_backward(dy, dsum, h, weight, dx, dw, eps):
                                         IN_CODES[weight.dtype], _ptr(dx), _rs(dx), _ptr(dw), rows, H, float(eps), _ptr(ws), need, _stream(h)))
 
 
+def layer_norm(x, weight, bias, residual, y, summed, stats, eps):
+    _require_one_gpu(*_present(x, weight, bias, residual, y, summed, stats))
+    with torch.cuda.device(x.device):
+        check(load().dlb_layer_norm(_ptr(x), _rs(x), _ptr(residual), _rs(residual), IN_CODES[x.dtype], _ptr(weight), _ptr(bias), IN_CODES[weight.dtype],
+                                    _ptr(y), _rs(y), _ptr(summed), _rs(summed), _ptr(stats), x.size(0), x.size(1), float(eps), _stream(x)))
+
+
+def layer_norm_backward(dy, dsum, h, weight, stats, dx, dw, db):
+    _require_one_gpu(*_present(dy, dsum, h, weight, stats, dx, dw, db))
+    lib = load()
+    with torch.cuda.device(h.device):
+        rows, H = h.shape
+        # scratch of its own, so that two captured graphs never share it
+        need = lib.dlb_layer_norm_backward_workspace_bytes(rows, H, db is not None) if dw is not None else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+        check(lib.dlb_layer_norm_backward(_ptr(dy), _rs(dy), _ptr(dsum), _rs(dsum), _ptr(h), _rs(h), IN_CODES[h.dtype], _ptr(weight),
+                                          IN_CODES[weight.dtype], _ptr(stats), _ptr(dx), _rs(dx), _ptr(dw), _ptr(db), rows, H, _ptr(ws), need,
+                                          _stream(h)))
+
+
 def moe_permute(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s, alignment):
     _require_one_gpu(*_present(ids, x, x_s, row_index, source, m_indices, row_start, row_end, rows, rows_s))
     code = ROWS_E4M3 if x.dtype == torch.float8_e4m3fn else IN_CODES[x.dtype]

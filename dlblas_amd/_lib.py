@@ -96,6 +96,11 @@ DECODER_SYMBOLS = {
     'dlb_rms_norm_backward_workspace_bytes': (_c_sz, [_c_i64] * 2),
     'dlb_rms_norm_backward':
     (ctypes.c_int, [_c_vp, _c_i64] * 3 + [ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, ctypes.c_float, _c_vp, _c_sz, _c_vp]),
+    'dlb_layer_norm':
+    (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp, ctypes.c_int] + [_c_vp, _c_i64] * 2 + [_c_vp] + [_c_i64] * 2 + [ctypes.c_float, _c_vp]),
+    'dlb_layer_norm_backward_workspace_bytes': (_c_sz, [_c_i64] * 2 + [ctypes.c_int]),
+    'dlb_layer_norm_backward':
+    (ctypes.c_int, [_c_vp, _c_i64] * 3 + [ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 2 + [_c_vp, _c_sz, _c_vp]),
     'dlb_moe_permute_workspace_bytes': (_c_sz, [_c_i64] * 3),
     'dlb_moe_permute': (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64, _c_vp, _c_i64, ctypes.c_int, _c_vp, _c_i64, _c_i64] + [_c_vp] * 7 + [_c_i64] * 6 +
                         [_c_vp, _c_sz, _c_vp]),

@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "host_common.h"
+#include "layer_norm.h"
 #include "moe_sort.h"
 #include "rms_norm.h"
 #include "w4_gemm.h"
@@ -301,9 +302,99 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
     if (int rc = finish("rms_norm_backward")) return rc;
   }
   if (!dw) return DLB_OK;
-  const NormDwArgs d{static_cast<const float*>(workspace), dw, shares, static_cast<int>(H), weight_dtype};
+  const NormDwArgs d{static_cast<const float*>(workspace), dw, nullptr, shares, static_cast<int>(H), static_cast<int>(H), weight_dtype};
   hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(H, 64))), dim3(64 * kDwWaves), 0, st, d);
   return finish("rms_norm_backward (dw)");
+}
+
+int dlb_layer_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, int dtype,
+                   const void* weight, const void* bias, int weight_dtype, void* y, int64_t y_row_stride, void* sum,
+                   int64_t sum_row_stride, float* stats, int64_t rows, int64_t H, float eps, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (int rc = check_norm(x, residual, dtype, weight, weight_dtype, sum, rows, H)) return rc;
+  if (rows == 0 || H == 0) return DLB_OK;
+  if (!y) return fail(DLB_ERR_NULL_POINTER, "y is NULL");
+  if (off_elements(y, dtype) || off_elements(bias, weight_dtype) || misaligned(stats, 4)) return fail(DLB_ERR_ALIGNMENT, "y, bias or stats is not aligned to its elements");
+  if (y_row_stride < H || (residual && sum_row_stride < H)) return fail(DLB_ERR_BAD_STRIDE, "a row stride of the outputs is smaller than H=%lld", (long long)H);
+  if (x_row_stride < 0 || residual_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  LayerNormArgs a{};
+  a.x = x, a.res = residual, a.w = weight, a.b = bias, a.y = y, a.sum = sum, a.stats = stats;
+  a.rows = rows, a.x_rs = x_row_stride, a.res_rs = residual_row_stride, a.y_rs = y_row_stride, a.sum_rs = sum_row_stride;
+  a.H = static_cast<int>(H), a.w_f32 = weight_dtype == kInF32, a.eps = eps;
+  const auto launch = [&](auto t, auto res, auto whole, auto c, auto lanes, int threads, int beside) {
+    hipLaunchKernelGGL((layer_norm_kernel<t(), res(), whole(), c(), lanes()>), row_grid(ceil_div(rows, beside)), dim3(threads, beside), 0,
+                       static_cast<hipStream_t>(stream), a);
+  };
+  with_type(dtype, [&](auto t) {
+    with_flag(residual != nullptr, [&](auto res) {
+      if (H % 8 == 0) {
+        constexpr std::true_type whole;
+        if (with_lanes(H, [&](auto lanes) { launch(t, res, whole, kOne, lanes, lanes(), kNarrowThreads / lanes()); })) return;
+      }
+      const RowShape shape = row_shape(H, 2);
+      with_flag(H % 8 == 0, [&](auto whole) {
+        with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, res, whole, c, kWave, shape.threads, 1); });
+      });
+    });
+  });
+  return finish("layer_norm");
+}
+
+size_t dlb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H, int with_bias) {
+  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::norm_grad_shares(rows, H)) * H * (with_bias ? 2 : 1) * sizeof(float) : 0;
+}
+
+int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
+                            int64_t h_row_stride, int dtype, const void* weight, int weight_dtype, const float* stats, void* dx,
+                            int64_t dx_row_stride, void* dw, void* db, int64_t rows, int64_t H, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (int rc = check_norm(h, dsum, dtype, weight, weight_dtype, dsum, rows, H)) return rc;
+  if (db && !dw) return fail(DLB_ERR_NULL_POINTER, "db without dw");
+  if (H == 0 || (rows == 0 && !dw)) return DLB_OK;
+  if (off_elements(dw, weight_dtype) || off_elements(db, weight_dtype)) return fail(DLB_ERR_ALIGNMENT, "dw or db is not aligned to its elements");
+  if (rows > 0) {
+    if (!dy || !dx || !stats) return fail(DLB_ERR_NULL_POINTER, "dy, dx or stats is NULL");
+    if (off_elements(dy, dtype) || off_elements(dx, dtype) || misaligned(stats, 4)) return fail(DLB_ERR_ALIGNMENT, "a tensor is not aligned to its elements");
+    if (dx_row_stride < H) return fail(DLB_ERR_BAD_STRIDE, "row stride %lld of dx is smaller than H=%lld", (long long)dx_row_stride, (long long)H);
+    if (dy_row_stride < 0 || dsum_row_stride < 0 || h_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+    const size_t need = dlb_layer_norm_backward_workspace_bytes(rows, H, db != nullptr);
+    if (dw && (!workspace || workspace_bytes < need))
+      return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (dw && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int shares = rows > 0 ? norm_grad_shares(rows, H) : 0, columns = static_cast<int>(db ? 2 * H : H);
+  if (rows > 0) {
+    LayerNormGradArgs a{};
+    a.dy = dy, a.dsum = dsum, a.h = h, a.w = weight, a.stats = stats, a.dx = dx, a.part = dw ? static_cast<float*>(workspace) : nullptr;
+    a.rows = rows, a.dy_rs = dy_row_stride, a.dsum_rs = dsum_row_stride, a.h_rs = h_row_stride, a.dx_rs = dx_row_stride;
+    a.H = static_cast<int>(H), a.columns = columns, a.w_f32 = weight_dtype == kInF32;
+    const auto launch = [&](auto t, auto ds, auto bias, auto whole, auto c, auto lanes, int grid, int threads, int beside) {
+      hipLaunchKernelGGL((layer_norm_backward_kernel<t(), ds(), bias(), whole(), c(), lanes()>), dim3(grid), dim3(threads, beside), 0, st, a);
+    };
+    with_type(dtype, [&](auto t) {
+      with_flag(dsum != nullptr, [&](auto ds) {
+        with_flag(db != nullptr, [&](auto bias) {
+          if (H % 8 == 0) {
+            constexpr std::true_type whole;
+            if (with_lanes(H, [&](auto lanes) { launch(t, ds, bias, whole, kOne, lanes, shares / (kNarrowThreads / 64), lanes(), kNarrowThreads / lanes()); })) return;
+          }
+          const RowShape shape = row_shape(H, dtype != kInF32 && H > 4096 ? 2 : 1);
+          with_flag(H % 8 == 0, [&](auto whole) {
+            with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, ds, bias, whole, c, kWave, shares, shape.threads, 1); });
+          });
+        });
+      });
+    });
+    if (int rc = finish("layer_norm_backward")) return rc;
+  }
+  if (!dw) return DLB_OK;
+  const NormDwArgs d{static_cast<const float*>(workspace), dw, db, shares, static_cast<int>(H), columns, weight_dtype};
+  hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(static_cast<unsigned>(ceil_div(columns, 64))), dim3(64 * kDwWaves), 0, st, d);
+  return finish("layer_norm_backward (dw)");
 }
 
 size_t dlb_moe_permute_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts) {

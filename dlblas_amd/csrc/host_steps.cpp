@@ -26,6 +26,9 @@ struct StepAbi {
   decltype(&dlb_moe_unpermute) unpermute;
   decltype(&dlb_w4_gemm_workspace_bytes) w4_ws;
   decltype(&dlb_w4_gemm) w4;
+  decltype(&dlb_layer_norm) layer_norm;
+  decltype(&dlb_layer_norm_backward_workspace_bytes) layer_norm_backward_ws;
+  decltype(&dlb_layer_norm_backward) layer_norm_backward;
 } abi;
 
 constexpr int64_t kMaxTopk = 64, kMaxExperts = DLB_SORT_MAX_EXPERTS;
@@ -176,6 +179,58 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
+// {y} or {y, h}; *stats, where wanted: for the gradient
+variable_list layer_norm_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor* b, const at::Tensor* res, double eps, at::Tensor* stats) {
+  const int64_t H = x.size(-1), rows = x.numel() / H;
+  at::Tensor y = empty(x.sizes(), x.scalar_type(), x), sum;
+  if (res) sum = empty(x.sizes(), x.scalar_type(), x);
+  if (stats) *stats = empty({rows, 2}, at::kFloat, x);
+  must(abi.layer_norm(ptr(x), row_stride(x), optr(res), res ? row_stride(*res) : 0, in_code(x.scalar_type()), ptr(w), optr(b), in_code(w.scalar_type()), ptr(y), H,
+                      res ? ptr(sum) : nullptr, H, stats ? fptr(*stats) : nullptr, rows, H, static_cast<float>(eps), stream_of(x)));
+  return res ? variable_list{y, sum} : variable_list{y};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& b,
+                               const std::optional<at::Tensor>& res, double eps) {
+    at::Tensor stats;
+    variable_list out = layer_norm_forward(x, w, b ? &*b : nullptr, res ? &*res : nullptr, eps, &stats);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["bias"] = b.has_value();
+    ctx->saved_data["res"] = res.has_value();
+    ctx->save_for_backward({res ? out[1] : x, w, stats});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const bool with_res = ctx->saved_data["res"].toBool();
+    const at::Tensor dsum_given = with_res ? grads[1] : at::Tensor();
+    no_tangent(grads[0]), no_tangent(dsum_given);
+    if (!grads[0].defined()) return once({dsum_given, {}, {}, with_res ? dsum_given : at::Tensor(), {}});  // only the sum went on, or nothing
+    const at::Tensor& g = grads[0];
+    DeviceScope scope(g);
+    const int64_t H = g.size(-1), rows = g.numel() / H;
+    const at::Tensor h = whole_columns(given_back(saved[0], g.scalar_type(), g.sizes(), g));
+    const at::Tensor w = given_back(saved[1], is_f32(saved[1]) ? at::kFloat : g.scalar_type(), {H}, g).contiguous();
+    const at::Tensor stats = given_back(saved[2], at::kFloat, {rows, 2}, g).contiguous();
+    const at::Tensor dy = whole_columns(g), dsum = dsum_given.defined() ? whole_columns(dsum_given) : dsum_given;
+    // the inputs that are there are numbered: without a bias the residual would be the third
+    const bool want_w = ctx->needs_input_grad(1), want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    at::Tensor dx = empty(h.sizes(), h.scalar_type(), h), dw, db, shares;
+    size_t need = 0;
+    if (want_w || want_b) {
+      dw = empty(w.sizes(), w.scalar_type(), w);
+      if (want_b) db = empty(w.sizes(), w.scalar_type(), w);
+      need = abi.layer_norm_backward_ws(rows, H, want_b);
+      shares = empty({static_cast<int64_t>(need)}, at::kByte, h);
+    }
+    must(abi.layer_norm_backward(ptr(dy), row_stride(dy), dsum.defined() ? ptr(dsum) : nullptr, dsum.defined() ? row_stride(dsum) : 0, ptr(h), row_stride(h),
+                                 in_code(h.scalar_type()), ptr(w), in_code(w.scalar_type()), fptr(stats), ptr(dx), H, dw.defined() ? ptr(dw) : nullptr,
+                                 want_b ? ptr(db) : nullptr, rows, H, need > 0 ? ptr(shares) : nullptr, need, stream_of(h)));
+    return once({dx, want_w ? dw : at::Tensor(), db, with_res ? dx : at::Tensor(), {}});
+  }
+};
+
 // A view of `size` ints from the offset-th on, without a trip through the dispatcher.
 at::Tensor part_of(const at::Tensor& base, int64_t* offset, at::IntArrayRef size) {
   at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), base.dtype());
@@ -284,6 +339,31 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     const NoGil nogil;
     out = grad ? RmsNorm::apply(x, w, optional_of(res), eps) : norm_forward(x, w, res, eps);
+  }
+  return res ? tuple_of({&out[0], &out[1]}) : THPVariable_Wrap(std::move(out[0]));
+  DECLINE_FAILED
+  HANDLE_EXCEPTIONS_END
+}
+
+// layer_norm(x, weight, bias, eps, residual) -> y, or (y, h)
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_EXCEPTIONS_BEGIN
+  if (n != 5 || !PyFloat_CheckExact(args[3])) NOT_PLAIN;
+  PyObject* const given[] = {args[0], args[1], args[2], args[4]};
+  const at::Tensor* t[4];
+  bool grad = false;
+  if (!take(given, t, 12, &grad)) NOT_PLAIN;
+  const at::Tensor &x = *t[0], &w = *t[1];
+  const at::Tensor *b = t[2], *res = t[3];
+  const double eps = PyFloat_AS_DOUBLE(args[3]);
+  if (!norm_operands(x, w, res) || !(eps >= 0)) NOT_PLAIN;
+  if (b && (b->scalar_type() != w.scalar_type() || b->sizes() != w.sizes() || !b->is_contiguous())) NOT_PLAIN;
+  const OpRecord record("dlblas::layer_norm", t);
+  DeviceScope scope(x);
+  variable_list out;
+  {
+    const NoGil nogil;
+    out = grad ? LayerNorm::apply(x, w, optional_of(b), optional_of(res), eps) : layer_norm_forward(x, w, b, res, eps, nullptr);
   }
   return res ? tuple_of({&out[0], &out[1]}) : THPVariable_Wrap(std::move(out[0]));
   DECLINE_FAILED
@@ -477,5 +557,5 @@ PyObject* init_steps(PyObject*, PyObject* list) {
 }  // namespace
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped),
+PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(layer_norm), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped),
                                    {"init_steps", init_steps, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};

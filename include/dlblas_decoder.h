@@ -1,6 +1,6 @@
 /*
  * C ABI of the steps around the products of a decoder block (MI355X / gfx950): RMS norm with the residual's addition and the
- * 1 x 128 quantiser, tokens sorted by expert and back with their gradients, products of a few rows with 4-bit weights.
+ * 1 x 128 quantiser, layer norm, tokens sorted by expert and back with their gradients, products of a few rows with 4-bit weights.
  * Same library (libdlblas_fp8_gemm.so), same conventions as include/dlblas_fp8_gemm.h: device pointers and sizes only, nothing is
  * allocated or synchronised, work is enqueued on `stream`, 0 = enqueued, negative DLB_ERR_* = rejected with a reason in
  * dlb_last_error() and nothing enqueued.  Every launch is a kernel, so all of them can be captured into a HIP graph.  No call keeps
@@ -63,6 +63,36 @@ size_t dlb_rms_norm_backward_workspace_bytes(int64_t rows, int64_t H);
 int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
                           int64_t h_row_stride, int dtype, const void* weight, int weight_dtype, void* dx, int64_t dx_row_stride,
                           void* dw, int64_t rows, int64_t H, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Layer norm: h = x + residual rounded to the element type (h = x without a residual), m = mean(h), r = 1 / sqrt(mean((h - m)^2) + eps),
+ * y = (h - m) r w + b; fp32 inside, one rounding at the store.  The sum of squares is fp32 as well: rows whose sum passes 2^128
+ * (|h - m| about 10^17 throughout) give y = b, or NaN where they hold an infinity.
+ *
+ *   x, residual, y, sum  [rows, H]  one element type (dtype); residual NULL: none, and sum is not written
+ *   weight, bias         [H]        the same type, or fp32 (weight_dtype, of both); bias NULL: none
+ *   stats                [rows, 2]  fp32, OUT: m and r of every row, for dlb_layer_norm_backward; NULL: not wanted
+ */
+int dlb_layer_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, int dtype,
+                   const void* weight, const void* bias, int weight_dtype, void* y, int64_t y_row_stride, void* sum,
+                   int64_t sum_row_stride, float* stats, int64_t rows, int64_t H, float eps, void* stream);
+
+/* Bytes of scratch dlb_layer_norm_backward needs for dw, and with_bias for db (none otherwise). */
+size_t dlb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H, int with_bias);
+
+/*
+ * The gradients of dlb_layer_norm from its h and stats, n = (h - m) r, t = w dy:  dx = r (t - mean(t) - n mean(t n)) + dsum,
+ * dw = sum over the rows of dy n, db = sum over the rows of dy.  dx is the gradient of x and of the residual alike.  The order of all
+ * sums is fixed.
+ *
+ *   dy, dsum, h, dx  [rows, H]  dtype; dsum (gradient of sum) may be NULL
+ *   dw, db           [H]        weight_dtype; db NULL: not wanted, both NULL: neither
+ *   workspace        4-byte aligned, dlb_layer_norm_backward_workspace_bytes(rows, H, db ? 1 : 0), no initialisation
+ */
+int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
+                            int64_t h_row_stride, int dtype, const void* weight, int weight_dtype, const float* stats, void* dx,
+                            int64_t dx_row_stride, void* dw, void* db, int64_t rows, int64_t H, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* Bytes of scratch dlb_moe_permute needs. */
 size_t dlb_moe_permute_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts);
