@@ -8,7 +8,7 @@ CSRC_DIR = os.path.join(PKG_DIR, 'csrc')
 LIB_NAME = 'libdlblas_fp8_gemm.so'
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 HOST_PATH = os.path.join(PKG_DIR, '_host.so')
-SOURCES = ['dlblas_fp8_gemm.hip', 'dlblas_fp8_moe.hip', 'dlblas_decoder.hip']
+SOURCES = ['dlblas_fp8_gemm.hip', 'dlblas_fp8_moe.hip', 'dlblas_decoder.hip', 'dlblas_mxfp4.hip']
 
 # packed fp32 VALU forms are switched off for every device compile of this library
 HIPCC_FLAGS = [

@@ -1,4 +1,5 @@
-"""ctypes binding of libdlblas_fp8_gemm.so (the C ABI declared in include/dlblas_fp8_gemm.h, dlblas_fp8_moe.h and dlblas_decoder.h).
+"""ctypes binding of libdlblas_fp8_gemm.so (the C ABI declared in include/dlblas_fp8_gemm.h, dlblas_fp8_moe.h,
+dlblas_decoder.h and dlblas_mxfp4.h).
 
 The library is the only implementation: when it has not been built, every op raises ImportError.  There is no
 PyTorch or CPU fallback.  The calling convention (``c_void_p(tensor.data_ptr())`` operands, the stream handle as
@@ -113,6 +114,13 @@ DECODER_SYMBOLS = {
     'dlb_w4_quant': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 3 + [_c_i64] * 3 + [_c_vp]),
 }
 
+# the same for dlblas_mxfp4.h; the calls are in _mxfp4.py
+MXFP4_SYMBOLS = {
+    'dlb_mxfp4_quant': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp] + [_c_i64] * 2 + [_c_vp]),
+    'dlb_mxfp4_gemm_workspace_bytes': (_c_sz, [_c_i64] * 3),
+    'dlb_mxfp4_gemm': (ctypes.c_int, [_c_vp] * 5 + [_c_i64] * 3 + [ctypes.c_int, _c_vp, _c_sz, _c_vp]),
+}
+
 _lock = threading.Lock()
 _lib = None
 _workspaces = {}
@@ -143,7 +151,7 @@ def load() -> ctypes.CDLL:
             lib = ctypes.CDLL(path)
         except OSError as exc:
             raise ImportError(f'cannot load {path}: {exc}') from exc
-        for name, (restype, argtypes) in (SYMBOLS | DECODER_SYMBOLS).items():
+        for name, (restype, argtypes) in (SYMBOLS | DECODER_SYMBOLS | MXFP4_SYMBOLS).items():
             try:
                 fn = getattr(lib, name)
             except AttributeError:

@@ -3,9 +3,8 @@
 #include "../../include/dlblas_decoder.h"
 
 #include <algorithm>
-#include <type_traits>
 
-#include "host_common.h"
+#include "dispatch.h"
 #include "layer_norm.h"
 #include "moe_sort.h"
 #include "rms_norm.h"
@@ -13,35 +12,6 @@
 
 namespace dlb {
 namespace {
-
-int finish(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(DLB_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
-  return DLB_OK;
-}
-
-bool bad_dtype(int d) { return d < kInBf16 || d > kInF32; }
-int64_t size_of(int d) { return d == kInF32 ? 4 : 2; }
-bool off_elements(const void* p, int dtype) { return misaligned(p, size_of(dtype)); }
-
-// Calls f with the type as a constant.
-template <typename F>
-void with_type(int dtype, F f) {
-  if (dtype == kInBf16)
-    f(std::integral_constant<int, kInBf16>());
-  else if (dtype == kInF16)
-    f(std::integral_constant<int, kInF16>());
-  else
-    f(std::integral_constant<int, kInF32>());
-}
-template <typename F>
-void with_flag(bool flag, F f) {
-  flag ? f(std::true_type()) : f(std::false_type());
-}
-template <int... C, typename F>
-void with_chunks(int chunks, F f) {
-  (void)((chunks == C && (f(std::integral_constant<int, C>()), true)) || ...);
-}
 
 // ---- norms ------------------------------------------------------------------------------------------------------------
 
@@ -66,12 +36,6 @@ bool with_lanes(int64_t H, F f) {
   if (H > 256) return false;
   H <= 128 ? f(std::integral_constant<int, 16>()) : f(std::integral_constant<int, 32>());
   return true;
-}
-
-// A grid of `blocks` workgroups in two dimensions.
-dim3 row_grid(int64_t blocks) {
-  constexpr int64_t kMost = 1 << 21;  // of up to 1024 threads, of which one dimension holds fewer than 2^32
-  return dim3(static_cast<unsigned>(std::min(blocks, kMost)), static_cast<unsigned>(ceil_div(blocks, kMost)));
 }
 
 int check_norm(const void* x, const void* residual, int dtype, const void* weight, int weight_dtype, const void* sum, int64_t rows,

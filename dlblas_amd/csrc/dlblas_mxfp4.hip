@@ -1,0 +1,106 @@
+// C ABI of microscaled 4-bit floating point and of the experts for a few tokens: argument validation and launches.
+// The declarations and the contract of every entry point are in include/dlblas_mxfp4.h.
+#include "../../include/dlblas_mxfp4.h"
+
+#include "dispatch.h"
+#include "mxfp4.h"
+
+namespace dlb {
+namespace {
+
+int check_columns(int64_t K) {
+  if (K % kMxGroup != 0) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is not a multiple of 32, the columns of a scale", (long long)K);
+  if (K > DLB_MXFP4_MAX_COLUMNS) return fail(DLB_ERR_BAD_SHAPE, "K=%lld is beyond %d", (long long)K, DLB_MXFP4_MAX_COLUMNS);
+  return DLB_OK;
+}
+
+// How a product runs: few rows, K split over waves, or tiles.
+struct MxPlan {
+  int mt;    // few rows: tiles of 16 of them in a workgroup; 0: tiles through LDS
+  bool pad;  // tiles read the scales of four groups at a time: rows of another number of them are laid out anew
+};
+MxPlan mx_plan(int64_t M, int64_t, int64_t K) {
+  if (M <= 16) return {1, false};
+  if (M <= 32) return {2, false};
+  if (M <= 64) return {4, false};
+  return {0, K / kMxGroup % 4 != 0};
+}
+int64_t padded(int64_t G) { return ceil_div(G, 4) * 4; }
+
+template <class Tile>
+int launch_tiles(MxArgs a, hipStream_t st) {
+  const int64_t tiles_m = ceil_div(a.M, Tile::BM), tiles_n = ceil_div(a.N, Tile::BN);
+  if (tiles_m * tiles_n > (1ll << 30)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld x N=%d beyond the supported range", (long long)a.M, a.N);
+  a.tiles_m = static_cast<int>(tiles_m), a.tiles_n = static_cast<int>(tiles_n), a.group_m = static_cast<int>(std::min<int64_t>(tiles_m, 8));
+  hipLaunchKernelGGL(mxfp4_tile_kernel<Tile>, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * Tile::WAVES), Tile::LDS, st, a);
+  return finish("mxfp4_gemm");
+}
+
+}  // namespace
+}  // namespace dlb
+
+extern "C" {
+
+int dlb_mxfp4_quant(const void* x, int64_t x_row_stride, int dtype, void* q, void* s, int64_t rows, int64_t K, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (bad_dtype(dtype)) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16 / F32", dtype);
+  if (rows < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (rows=%lld K=%lld)", (long long)rows, (long long)K);
+  if (int rc = check_columns(K)) return rc;
+  if (rows > (1ll << 31) - 1) return fail(DLB_ERR_BAD_SHAPE, "rows=%lld beyond the supported range", (long long)rows);
+  if (rows == 0 || K == 0) return DLB_OK;
+  if (!x || !q || !s) return fail(DLB_ERR_NULL_POINTER, "x, q or s is NULL");
+  if (x_row_stride < 0) return fail(DLB_ERR_BAD_STRIDE, "negative row stride");
+  if (off_elements(x, dtype) || misaligned(q, 4)) return fail(DLB_ERR_ALIGNMENT, "x must be aligned to its elements, q to 4 bytes");
+  const MxQuantArgs a{x, static_cast<uint32_t*>(q), static_cast<uint8_t*>(s), rows, x_row_stride, static_cast<int>(K)};
+  with_type(dtype, [&](auto t) { hipLaunchKernelGGL(mxfp4_quant_kernel<t()>, row_grid(ceil_div(rows * (K / 8), 256)), dim3(256), 0, static_cast<hipStream_t>(stream), a); });
+  return finish("mxfp4_quant");
+}
+
+size_t dlb_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || !dlb::mx_plan(M, N, K).pad) return 0;
+  return static_cast<size_t>(M + N) * dlb::padded(K / dlb::kMxGroup);
+}
+
+int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_s, void* c, int64_t M, int64_t N, int64_t K, int out_dtype,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (bad_dtype(out_dtype)) return fail(DLB_ERR_BAD_DTYPE, "out_dtype %d is not DLB_IN_BF16 / F16 / F32", out_dtype);
+  if (M < 0 || N < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
+  if (int rc = check_columns(K)) return rc;
+  if (M > (1ll << 31) - 1 || N > (1 << 27)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld / N=%lld beyond the supported range", (long long)M, (long long)N);
+  if (M == 0 || N == 0) return DLB_OK;
+  if (K == 0) return fail(DLB_ERR_BAD_SHAPE, "K=0: there is no product");
+  if (!a || !b || !a_s || !b_s || !c) return fail(DLB_ERR_NULL_POINTER, "a, b, a_s, b_s or c is NULL");
+  if (misaligned(a, 16) || misaligned(b, 16) || misaligned(a_s, 4) || misaligned(b_s, 4) || off_elements(c, out_dtype))
+    return fail(DLB_ERR_ALIGNMENT, "codes must be 16-byte, scales 4-byte aligned, c to its elements");
+  const MxPlan plan = mx_plan(M, N, K);
+  const size_t need = dlb_mxfp4_gemm_workspace_bytes(M, N, K);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+  if (need > 0 && misaligned(workspace, 16)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MxArgs p{};
+  p.a = static_cast<const uint8_t*>(a), p.b = static_cast<const uint8_t*>(b), p.a_s = static_cast<const uint8_t*>(a_s), p.b_s = static_cast<const uint8_t*>(b_s);
+  p.c = c, p.M = M, p.N = static_cast<int>(N), p.K = static_cast<int>(K), p.G = static_cast<int>(K / kMxGroup), p.pitch = p.G, p.out = out_dtype;
+  if (plan.mt > 0) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(N, 16)), static_cast<unsigned>(ceil_div(M, 16 * plan.mt)));
+    with_chunks<1, 2, 4>(plan.mt, [&](auto mt) {
+      with_flag(p.G % 4 == 0, [&](auto dwords) { hipLaunchKernelGGL((mxfp4_few_kernel<mt(), dwords()>), grid, dim3(64 * kMxFewWaves), 0, st, p); });
+    });
+    return finish("mxfp4_gemm");
+  }
+  if (plan.pad) {
+    const int words = static_cast<int>(padded(p.G) / 4);
+    uint32_t* const to = static_cast<uint32_t*>(workspace);
+    const MxPadArgs pad{p.a_s, p.b_s, to, to + M * words, M, N, p.G, words};
+    hipLaunchKernelGGL(mxfp4_pad_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div((M + N) * words, 256), 2048))), dim3(256), 0, st, pad);
+    if (int rc = finish("mxfp4_gemm (scales)")) return rc;
+    p.a_s = reinterpret_cast<const uint8_t*>(to), p.b_s = reinterpret_cast<const uint8_t*>(to + M * words), p.pitch = 4 * words;
+  }
+  if (ceil_div(M, 256) * ceil_div(N, 256) >= 128) return launch_tiles<MxTile<2, 4, 8, 4>>(p, st);
+  return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
+}
+
+}  // extern "C"

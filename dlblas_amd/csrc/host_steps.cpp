@@ -29,6 +29,9 @@ struct StepAbi {
   decltype(&dlb_layer_norm) layer_norm;
   decltype(&dlb_layer_norm_backward_workspace_bytes) layer_norm_backward_ws;
   decltype(&dlb_layer_norm_backward) layer_norm_backward;
+  decltype(&dlb_mxfp4_quant) mx_quant;
+  decltype(&dlb_mxfp4_gemm_workspace_bytes) mx_ws;
+  decltype(&dlb_mxfp4_gemm) mx;
 } abi;
 
 constexpr int64_t kMaxTopk = 64, kMaxExperts = DLB_SORT_MAX_EXPERTS;
@@ -541,6 +544,80 @@ PyObject* w4_gemm_grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_EXCEPTIONS_END
 }
 
+// ---- 4-bit floating point ---------------------------------------------------------------------------------------------
+
+constexpr int64_t kMxGroup = 32;
+
+// Columns of codes and scales that make an operand, 0: not a plain one.
+int64_t mx_columns(const at::Tensor& q, const at::Tensor& s, int64_t codes_align) {
+  if (q.scalar_type() != at::kByte || s.scalar_type() != at::kByte || q.dim() < 1 || q.dim() != s.dim() || q.numel() == 0 || !q.is_contiguous() || !s.is_contiguous()) return 0;
+  for (int64_t d = 0; d + 1 < q.dim(); ++d)
+    if (q.size(d) != s.size(d)) return 0;
+  const int64_t K = 2 * q.size(-1);
+  if (K % kMxGroup != 0 || K > DLB_MXFP4_MAX_COLUMNS || s.size(-1) != K / kMxGroup) return 0;
+  return reinterpret_cast<uintptr_t>(q.data_ptr()) % codes_align == 0 && reinterpret_cast<uintptr_t>(s.data_ptr()) % 4 == 0 ? K : 0;
+}
+
+// per_group_quant_mxfp4(x) -> (q, s)
+PyObject* per_group_quant_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_EXCEPTIONS_BEGIN
+  const at::Tensor* t[1];
+  if (n != 1 || !take(args, t, 0)) NOT_PLAIN;
+  const at::Tensor& x = *t[0];
+  if (in_code(x.scalar_type()) < 0 || x.dim() < 1 || x.numel() == 0 || row_stride(x) < 0 || x.size(-1) % kMxGroup != 0 || x.size(-1) > DLB_MXFP4_MAX_COLUMNS) NOT_PLAIN;
+  const OpRecord record("dlblas::per_group_quant_mxfp4", t);
+  const int64_t K = x.size(-1);
+  DeviceScope scope(x);
+  at::Tensor q, s;
+  at::DimVector size(x.sizes());
+  int rc;
+  {
+    const NoGil nogil;
+    size.back() = K / 2;
+    q = empty(size, at::kByte, x);
+    size.back() = K / kMxGroup;
+    s = empty(size, at::kByte, x);
+    rc = abi.mx_quant(ptr(x), row_stride(x), in_code(x.scalar_type()), ptr(q), ptr(s), x.numel() / K, K, stream_of(x));
+  }
+  if (rc != DLB_OK) NOT_PLAIN;
+  return tuple_of({&q, &s});
+  HANDLE_EXCEPTIONS_END
+}
+
+// mxfp4_gemm(a, b, a_s, b_s, out_dtype or None) -> c
+PyObject* mxfp4_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_EXCEPTIONS_BEGIN
+  const at::Tensor* t[4];
+  if (n != 5 || !take(args, t, 0)) NOT_PLAIN;
+  const at::Tensor &a = *t[0], &b = *t[1], &a_s = *t[2], &b_s = *t[3];
+  at::ScalarType out;
+  if (args[4] == Py_None)
+    out = c10::get_default_dtype_as_scalartype();
+  else if (THPDtype_Check(args[4]))
+    out = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+  else
+    NOT_PLAIN;
+  const int64_t K = mx_columns(b, b_s, 16);
+  if (in_code(out) < 0 || K == 0 || b.dim() != 2 || mx_columns(a, a_s, 16) != K) NOT_PLAIN;
+  const OpRecord record("dlblas::mxfp4_gemm", t);
+  const int64_t M = a.numel() / (K / 2), N = b.size(0);
+  at::DimVector size(a.sizes());
+  size.back() = N;
+  DeviceScope scope(a);
+  at::Tensor c, scratch;
+  int rc;
+  {
+    const NoGil nogil;
+    c = empty(size, out, a);
+    const size_t need = abi.mx_ws(M, N, K);
+    if (need > 0) scratch = empty({static_cast<int64_t>(need)}, at::kByte, a);
+    rc = abi.mx(ptr(a), ptr(b), ptr(a_s), ptr(b_s), ptr(c), M, N, K, in_code(out), need > 0 ? ptr(scratch) : nullptr, need, stream_of(a));
+  }
+  if (rc != DLB_OK) NOT_PLAIN;
+  return THPVariable_Wrap(std::move(c));
+  HANDLE_EXCEPTIONS_END
+}
+
 // init_steps(addresses): in the order of StepAbi's members
 PyObject* init_steps(PyObject*, PyObject* list) {
   void* slots[sizeof(StepAbi) / sizeof(void*)];
@@ -557,5 +634,5 @@ PyObject* init_steps(PyObject*, PyObject* list) {
 }  // namespace
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(layer_norm), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped),
+PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(layer_norm), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped), FAST(per_group_quant_mxfp4), FAST(mxfp4_gemm),
                                    {"init_steps", init_steps, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};

@@ -28,6 +28,7 @@
 #include "../../include/dlblas_decoder.h"
 #include "../../include/dlblas_fp8_gemm.h"
 #include "../../include/dlblas_fp8_moe.h"
+#include "../../include/dlblas_mxfp4.h"
 
 namespace {
 

@@ -1,0 +1,378 @@
+// Microscaled 4-bit floating point for gfx950: the quantiser and the products of two quantised operands.
+//
+//   groups of 32 columns of a row share the scale 2^(s - 127), s a byte, 255 = NaN; an element is e2m1, 0 .5 1 1.5 2 3 4 6 with a sign
+//   quantising:  s = max(floor(log2 max |x|) - 2, -127) + 127,  q = x 2^(127 - s) to nearest, ties to even, at most 6
+//   product:     y[m, n] = sum over the groups g of 2^(a_s[m, g] + b_s[n, g] - 254) sum_{k in g} a[m, k] b[n, k]
+//
+// (The OCP microscaling formats, version 1.0, name both.)  v_mfma_scale_f32_..._f8f6f4 takes 32 elements and their scale byte from each lane,
+// so a group is what one lane holds of one MFMA: 16 bytes of codes, one byte of scales, and which of a chunk's groups goes to which
+// lane and step is free as long as both operands agree.  Every kernel here gives a lane neighbouring groups, whose scales are one dword
+// and are picked by the instruction's byte selector.  Products of two codes and sums of a group are exact in fp32 (at most 32 x 36 in steps of a
+// quarter); the sum over groups is rounded as the unit does it.
+#pragma once
+
+#include "rows.h"
+
+namespace dlb {
+
+constexpr int kMxGroup = 32;                // columns
+constexpr uint32_t kNowhere = 0x80000000u;  // past the end of every buffer: such a load costs no traffic and gives zero
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+
+// ---- quantiser --------------------------------------------------------------------------------------------------------
+
+struct MxQuantArgs {
+  const void* x;
+  uint32_t* q;   // [rows][K / 2], eight codes a word
+  uint8_t* s;    // [rows][K / 32]
+  int64_t rows, x_rs;
+  int K;
+};
+
+// Eight columns a lane, four lanes a group.
+template <int T>
+__global__ void __launch_bounds__(256) mxfp4_quant_kernel(const MxQuantArgs p) {
+  const int64_t per_row = p.K / 8, total = p.rows * per_row;
+  const int64_t i = static_cast<int64_t>(blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;  // whole groups
+  const int64_t row = i / per_row;
+  const int col = static_cast<int>(i - row * per_row) * 8;
+  float v[8];
+  quant_unpack8<T>(load_raw8<T, true>(p.x, row * p.x_rs, col, 8), v);
+  uint32_t top = 0;  // the largest magnitude as bits, which put infinity above all numbers and NaN above infinity
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+  const int exponent = static_cast<int>(top >> 23);  // floor(log2) + 127; 0 of a subnormal number, whose group takes the smallest scale
+  const int s = exponent == 255 ? 255 : max(exponent - 2, 0);
+  const float up = __uint_as_float(static_cast<uint32_t>(254 - min(s, 253)) << 23);
+  uint32_t word = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // the largest is below 8 here; what lies above 6 is 6
+    const float a = __builtin_amdgcn_fmed3f(v[2 * k] * up, -6.f, 6.f), b = __builtin_amdgcn_fmed3f(v[2 * k + 1] * up, -6.f, 6.f);
+    word |= (__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, a, b, 1.0f, 0) & 0xffu) << (8 * k);
+  }
+  p.q[i] = s == 255 ? 0 : word;
+  if ((threadIdx.x & 3) == 0) p.s[i / 4] = static_cast<uint8_t>(s);
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------------
+
+// 16 x 16 outputs, 128 columns: lane l supplies row l % 16 of each operand, 32 consecutive codes, and receives D[4 (l / 16) + r][l % 16] in
+// component r.  STEP: byte of the scale words.
+template <int STEP>
+__device__ __forceinline__ v4f mfma_mx(const v4i& a, uint32_t a_s, const v4i& b, uint32_t b_s, const v4f& c) {
+  const v8i aw{a.x, a.y, a.z, a.w, 0, 0, 0, 0}, bw{b.x, b.y, b.z, b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aw, bw, c, 4, 4, STEP, static_cast<int>(a_s), STEP, static_cast<int>(b_s));
+}
+
+struct MxArgs {
+  const uint8_t* a;    // [M][K / 2]
+  const uint8_t* b;    // [N][K / 2]
+  const uint8_t* a_s;  // [M][a_pitch]
+  const uint8_t* b_s;  // [N][b_pitch]
+  void* c;             // [M][N]
+  int64_t M;
+  int N, K, G;         // G = K / 32
+  int pitch;           // bytes of a row of scales: G, or of scales that were laid out anew
+  int out;             // DLB_IN_*
+  int tiles_m, tiles_n, group_m;
+};
+
+// Four consecutive columns of one row of c.
+__device__ __forceinline__ void store4(void* c, int type, int64_t at, const v4f& v, int left) {
+  typedef _Float16 v4h_t __attribute__((ext_vector_type(4)));
+  if (type == kInF32) {
+    float* to = static_cast<float*>(c) + at;
+    if (left >= 4) {
+      *reinterpret_cast<v4f_el*>(to) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) to[i] = v[i];
+    }
+    return;
+  }
+  uint16_t* to = static_cast<uint16_t*>(c) + at;
+  const v2i h = type == kInBf16 ? __builtin_bit_cast(v2i, __builtin_convertvector(v, v4bf)) : __builtin_bit_cast(v2i, __builtin_convertvector(v, v4h_t));
+  typedef v2i v2i_el __attribute__((aligned(2)));
+  if (left >= 4) {
+    *reinterpret_cast<v2i_el*>(to) = h;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < left) to[i] = static_cast<uint16_t>(static_cast<uint32_t>(h[i / 2]) >> (16 * (i & 1)));
+  }
+}
+
+constexpr int kMxFewWaves = 8;
+
+// Few rows: bound by the weights' bytes, which go from memory to registers once.  The waves of a workgroup take chunks of 512 columns of 16 rows of
+// b in turn (a lane 64 bytes, four groups, in four loads, and their scales in one), and add their sums through LDS in wave order.
+// DWORDS: rows of scales are a multiple of four groups; otherwise a lane reads its scales one by one.
+template <int MT, bool DWORDS>
+__global__ void __launch_bounds__(64 * kMxFewWaves) mxfp4_few_kernel(const MxArgs p) {
+  __shared__ v4f part[kMxFewWaves][MT][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  const int n0 = blockIdx.x * 16;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  const int cols = min(16, p.N - n0), rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(16 * MT)));
+  const uint32_t half = p.K / 2;
+  const auto b_src = make_rsrc(p.b + static_cast<int64_t>(n0) * half, cols * half);
+  const auto bs_src = make_rsrc(p.b_s + static_cast<int64_t>(n0) * p.pitch, cols * p.pitch);
+  const auto a_src = make_rsrc(p.a + m0 * half, rows * half);
+  const auto as_src = make_rsrc(p.a_s + m0 * p.pitch, rows * p.pitch);
+  struct Chunk {
+    v4i b[4], a[MT][4];
+    uint32_t b_s, a_s[MT];
+  };
+  const auto scales = [&](auto src, bool there, uint32_t row, int g) {
+    if (DWORDS) return __builtin_amdgcn_raw_buffer_load_b32(src, there && g < p.G ? row * p.pitch + g : kNowhere, 0, 0);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b8(src, there && g + i < p.G ? row * p.pitch + g + i : kNowhere, 0, 0)) << (8 * i);
+    return w;
+  };
+  auto load = [&](int c, Chunk& k) {
+    const int g = 16 * c + 4 * q;  // the lane's first group
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = g + i < p.G ? static_cast<uint32_t>(g + i) * 16 : kNowhere;
+      k.b[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(b_src, l16 < cols && at != kNowhere ? l16 * half + at : kNowhere, 0, 2));
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        k.a[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(a_src, 16 * m + l16 < rows && at != kNowhere ? (16 * m + l16) * half + at : kNowhere, 0, 0));
+    }
+    k.b_s = scales(bs_src, l16 < cols, l16, g);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) k.a_s[m] = scales(as_src, 16 * m + l16 < rows, 16 * m + l16, g);
+  };
+  v4f acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Chunk& k) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      acc[m] = mfma_mx<0>(k.b[0], k.b_s, k.a[m][0], k.a_s[m], acc[m]);
+      acc[m] = mfma_mx<1>(k.b[1], k.b_s, k.a[m][1], k.a_s[m], acc[m]);
+      acc[m] = mfma_mx<2>(k.b[2], k.b_s, k.a[m][2], k.a_s[m], acc[m]);
+      acc[m] = mfma_mx<3>(k.b[3], k.b_s, k.a[m][3], k.a_s[m], acc[m]);
+    }
+  };
+  const int chunks = (p.G + 15) / 16;
+  Chunk even, odd;
+  load(wave, even);
+  for (int c = wave; c < chunks; c += 2 * kMxFewWaves) {
+    load(c + kMxFewWaves, odd);
+    multiply(even);
+    load(c + 2 * kMxFewWaves, even);
+    multiply(odd);
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) part[wave][m][lane] = acc[m];
+  __syncthreads();
+  // wave m adds up tile m
+  for (int m = wave; m < MT; m += kMxFewWaves) {
+    v4f sum = part[0][m][lane];
+#pragma unroll
+    for (int w = 1; w < kMxFewWaves; ++w) sum += part[w][m][lane];
+    const int row = 16 * m + l16, col = 4 * q;
+    if (row < rows && col < cols) store4(p.c, p.out, (m0 + row) * p.N + n0 + col, sum, cols - col);
+  }
+}
+
+// Scales of rows whose groups are no multiple of four, with zeros behind the last: both operands' in one launch.
+struct MxPadArgs {
+  const uint8_t *a_s, *b_s;
+  uint32_t *a_to, *b_to;
+  int64_t M, N;
+  int G, words;
+};
+__global__ void __launch_bounds__(256) mxfp4_pad_kernel(const MxPadArgs p) {
+  const int64_t total = (p.M + p.N) * p.words;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / p.words;
+    const int g = static_cast<int>(i - row * p.words) * 4;
+    const uint8_t* from = (row < p.M ? p.a_s + row * p.G : p.b_s + (row - p.M) * p.G) + g;
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (g + k < p.G) w |= static_cast<uint32_t>(from[k]) << (8 * k);
+    (row < p.M ? p.a_to + row * p.words : p.b_to + (row - p.M) * p.words)[g / 4] = w;
+  }
+}
+
+// Many rows: tiles of BM x BN through LDS.  A step is 128 columns, 64 bytes of every row, in a ring of four; the scales of four steps lie in a table of 16
+// bytes a row, two of them in turn.  WGM x WGN waves, each with MF x NF fragments of 16 x 16 outputs (both even).
+template <int WGM_, int WGN_, int MF_, int NF_>
+struct MxTile {
+  static constexpr int WGM = WGM_, WGN = WGN_, MF = MF_, NF = NF_, STAGES = 4;
+  static constexpr int WAVES = WGM * WGN, BM = WGM * MF * 16, BN = WGN * NF * 16;
+  static constexpr int A_INST = BM / 16 / WAVES, B_INST = BN / 16 / WAVES;  // an instruction moves 16 rows
+  static constexpr int S_INST = (BM + BN) / 64 / WAVES;                      // ... or the scales of 64
+  static constexpr int STAGE = (BM + BN) * 64, TABLE = (BM + BN) * 16;
+  static constexpr int LDS = STAGES * STAGE + 2 * TABLE;
+  static_assert(BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0 && (BM + BN) % (64 * WAVES) == 0 && BM % 64 == 0 && LDS <= 160 * 1024, "whole instructions");
+};
+
+// Row of a wave's operand that lane or result index i (0 .. 15) of fragment f stands for: two results of a pair of fragments are 8
+// consecutive rows, which are 8 consecutive columns of c.
+__device__ __forceinline__ int mx_row(int f, int i) { return (f >> 1) * 32 + (f & 1) * 4 + (i >> 2) * 8 + (i & 3); }
+// A row's 16-byte chunk c lies at c ^ mx_swizzle(row).  A ds_read_b128 goes through the banks in turns of 16 lanes, lanes 0-3, 12-15 and 20-27 in
+// the first, the rest of 0-31 in the second: rows of a fragment's runs g = 0, 3 with one chunk and g = 1, 2 with the next.  Rows are 64
+// bytes, so four neighbours fill the banks and what the runs have to differ in is the chunk: (0, 2, 3, 1) does for both turns.
+__device__ __forceinline__ int mx_swizzle(int row) {
+  const int g = (row >> 3) & 3;
+  return (((g ^ (g >> 1)) & 1) << 1) | (g >> 1);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | (((N >> 4) & 0x3) << 14) | (0x7 << 4) | (0xF << 8));
+}
+
+// Behind it every wave's LDS reads have returned; loads into LDS stay on their way.
+__device__ __forceinline__ void mx_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+typedef __attribute__((address_space(3))) void* mx_lds_ptr;
+typedef __attribute__((address_space(3))) uint8_t* mx_lds_bytes;
+
+// Lane i moves 16 bytes to `to` + 16 i.
+template <class LdsPtr>
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t src, LdsPtr to, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (mx_lds_ptr)to, 16, voff, soff, 0, 0);
+}
+
+template <class Tile>
+__global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxArgs p) {
+  constexpr int BM = Tile::BM, BN = Tile::BN, MF = Tile::MF, NF = Tile::NF;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const mx_lds_bytes lds = (mx_lds_bytes)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  // neighbouring tiles on one XCD, patches of group_m row tiles
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int per = tiles / 8, over = tiles % 8, xcd = blockIdx.x % 8;
+  const int id = xcd * per + min(xcd, over) + blockIdx.x / 8;
+  const int width = p.group_m * p.tiles_n, patch = id / width, first_m = patch * p.group_m;
+  const int high = min(p.tiles_m - first_m, p.group_m), in_patch = id - patch * width;
+  const int64_t m0 = static_cast<int64_t>(first_m + in_patch % high) * BM;
+  const int n0 = (in_patch / high) * BN;
+  const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(BM))), cols = min(BN, p.N - n0);
+  const uint32_t half = p.K / 2;
+  const int steps = (p.G + 3) / 4;
+
+  // 16-byte chunk (lane % 4) of row (lane / 4) of an instruction's 16: where it goes decides what it takes
+  const uint8_t *const a_base = p.a + m0 * half, *const b_base = p.b + static_cast<int64_t>(n0) * half;
+  uint32_t a_off[Tile::A_INST], b_off[Tile::B_INST], chunk_col;
+  {
+    const int r = wave * 16 + (lane >> 2);  // of every instruction mod 32: WAVES is even
+    chunk_col = static_cast<uint32_t>((lane & 3) ^ mx_swizzle(r)) * 16;
+#pragma unroll
+    for (int j = 0; j < Tile::A_INST; ++j) a_off[j] = (j * Tile::WAVES * 16 + r) * half + chunk_col;
+#pragma unroll
+    for (int j = 0; j < Tile::B_INST; ++j) b_off[j] = (j * Tile::WAVES * 16 + r) * half + chunk_col;
+  }
+  const bool tail = p.G % 4 != 0;  // the last step is short
+  auto load_stage = [&](int k) {
+    const bool in = k < steps;
+    const uint32_t at = in ? static_cast<uint32_t>(k) * 64 : 0;
+    const auto a_src = make_rsrc(a_base, in ? rows * half : 0), b_src = make_rsrc(b_base, in ? cols * half : 0);
+    const bool past = tail && at + chunk_col >= half;
+    const mx_lds_bytes to = lds + (k & 3) * Tile::STAGE;
+#pragma unroll
+    for (int j = 0; j < Tile::A_INST; ++j)
+      load_to_lds(a_src, to + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : a_off[j], at);
+#pragma unroll
+    for (int j = 0; j < Tile::B_INST; ++j)
+      load_to_lds(b_src, to + BM * 64 + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : b_off[j], at);
+  };
+  // the scales of window w, 16 groups: those of the tile's rows, behind them those of its columns
+  auto load_scales = [&](int w) {
+    const mx_lds_bytes to = lds + Tile::STAGES * Tile::STAGE + (w & 1) * Tile::TABLE;
+    const bool in = 4 * w < steps;
+#pragma unroll
+    for (int j = 0; j < Tile::S_INST; ++j) {
+      const int first = (j * Tile::WAVES + wave) * 64;
+      const bool of_a = first < BM;
+      const auto src = make_rsrc(of_a ? p.a_s + m0 * p.pitch : p.b_s + static_cast<int64_t>(n0) * p.pitch, in ? (of_a ? rows : cols) * p.pitch : 0);
+      load_to_lds(src, to + first * 16, ((of_a ? first : first - BM) + lane) * static_cast<uint32_t>(p.pitch), in ? 16 * w : 0);
+    }
+  };
+
+  const int wm = (wave / Tile::WGN) * MF * 16, wn = (wave % Tile::WGN) * NF * 16;
+  // a lane's chunk of its row of a fragment; fragments of a pair are 4 rows apart, pairs 32
+  const int r0 = mx_row(0, l16);
+  const int frag = r0 * 64 + ((q ^ mx_swizzle(r0)) * 16);
+  v4f acc[MF][NF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  load_scales(0);
+  load_stage(0), load_stage(1), load_stage(2);
+  constexpr int kGroup = Tile::A_INST + Tile::B_INST;
+  for (int k0 = 0; k0 < steps; k0 += 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j;
+      if (k >= steps) break;
+      // in order: what is behind stage k is two stages, and the next scales if they were asked for in between
+      if (j == 1 || j == 2)
+        wait_loads<2 * kGroup + Tile::S_INST>();
+      else
+        wait_loads<2 * kGroup>();
+      mx_barrier();
+      if (j == 0) load_scales(k / 4 + 1);
+      load_stage(k + 3);
+      const uint8_t* const stage = smem + (k & 3) * Tile::STAGE;
+      const uint8_t* const table = smem + Tile::STAGES * Tile::STAGE + ((k >> 2) & 1) * Tile::TABLE;
+      v4i af[MF], bf[NF];
+      uint32_t as[MF], bs[NF];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const int f = wm + (i >> 1) * 32 + (i & 1) * 4;
+        af[i] = *reinterpret_cast<const v4i*>(stage + f * 64 + frag);
+        as[i] = *reinterpret_cast<const uint8_t*>(table + (f + r0) * 16 + 4 * j + q);
+      }
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const int f = BM + wn + (i >> 1) * 32 + (i & 1) * 4;
+        bf[i] = *reinterpret_cast<const v4i*>(stage + f * 64 + frag);
+        bs[i] = *reinterpret_cast<const uint8_t*>(table + (f + r0) * 16 + 4 * j + q);
+      }
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) acc[i][n] = mfma_mx<0>(bf[n], bs[n], af[i], as[i], acc[i][n]);
+    }
+  }
+  wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    const int row = wm + mx_row(i, l16);
+    if (row >= rows) continue;
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+      const int col = wn + (n >> 1) * 32 + (n & 1) * 4 + 8 * q;
+      if (col < cols) store4(p.c, p.out, (m0 + row) * p.N + n0 + col, acc[i][n], cols - col);
+    }
+  }
+}
+
+}  // namespace dlb
