@@ -21,8 +21,10 @@ _FUNCTIONS = ('fp8_gemm', 'quant', 'grouped_contiguous', 'grouped_masked', 'low_
 # the same for the StepAbi struct and the functions of csrc/host_steps.cpp
 _STEP_ABI = ('dlb_last_error', 'dlb_rms_norm_backward_workspace_bytes', 'dlb_rms_norm_backward', 'dlb_moe_unpermute_backward', 'dlb_rms_norm', 'dlb_rms_norm_quant', 'dlb_moe_permute_workspace_bytes', 'dlb_moe_permute', 'dlb_moe_unpermute', 'dlb_w4_gemm_workspace_bytes',
              'dlb_w4_gemm', 'dlb_layer_norm', 'dlb_layer_norm_backward_workspace_bytes', 'dlb_layer_norm_backward',
-             'dlb_mxfp4_quant', 'dlb_mxfp4_gemm_workspace_bytes', 'dlb_mxfp4_gemm')
-_STEP_FUNCTIONS = ('rms_norm', 'rms_norm_quant', 'layer_norm', 'moe_permute', 'moe_unpermute', 'w4_gemm', 'w4_gemm_grouped', 'per_group_quant_mxfp4', 'mxfp4_gemm')
+             'dlb_mxfp4_quant', 'dlb_mxfp4_gemm_workspace_bytes', 'dlb_mxfp4_gemm',
+             'dlb_mxfp4_weight_gemm', 'dlb_few_token_experts_workspace_bytes', 'dlb_few_token_experts')
+_STEP_FUNCTIONS = ('rms_norm', 'rms_norm_quant', 'layer_norm', 'moe_permute', 'moe_unpermute', 'w4_gemm', 'w4_gemm_grouped', 'per_group_quant_mxfp4', 'mxfp4_gemm', 'mxfp4_weight_gemm',
+                   'few_token_experts')
 
 
 def _declined(*args):

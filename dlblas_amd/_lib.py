@@ -119,6 +119,10 @@ MXFP4_SYMBOLS = {
     'dlb_mxfp4_quant': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, _c_vp] + [_c_i64] * 2 + [_c_vp]),
     'dlb_mxfp4_gemm_workspace_bytes': (_c_sz, [_c_i64] * 3),
     'dlb_mxfp4_gemm': (ctypes.c_int, [_c_vp] * 5 + [_c_i64] * 3 + [ctypes.c_int, _c_vp, _c_sz, _c_vp]),
+    'dlb_mxfp4_weight_gemm': (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int] + [_c_vp] * 3 + [_c_i64] * 3 + [_c_vp]),
+    'dlb_few_token_experts_workspace_bytes': (_c_sz, [_c_i64] * 3),
+    'dlb_few_token_experts':
+    (ctypes.c_int, [_c_vp, _c_i64, ctypes.c_int, _c_vp, ctypes.c_int, _c_i64, _c_i64, _c_vp, ctypes.c_int] + [_c_vp] * 5 + [_c_i64] * 5 + [_c_vp, _c_sz, _c_vp]),
 }
 
 _lock = threading.Lock()

@@ -3,6 +3,7 @@
 #include "../../include/dlblas_mxfp4.h"
 
 #include "dispatch.h"
+#include "few_rows.h"
 #include "mxfp4.h"
 
 namespace dlb {
@@ -101,6 +102,96 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
   }
   if (ceil_div(M, 256) * ceil_div(N, 256) >= 128) return launch_tiles<MxTile<2, 4, 8, 4>>(p, st);
   return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
+}
+
+int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, void* y, int64_t M, int64_t N, int64_t K,
+                          void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16", dtype);
+  if (M < 0 || N < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
+  if (int rc = check_columns(K)) return rc;
+  if (M > 32 * 65535 || N > (1 << 27)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld / N=%lld beyond the supported range", (long long)M, (long long)N);
+  if (M == 0 || N == 0) return DLB_OK;
+  if (K == 0) return fail(DLB_ERR_BAD_SHAPE, "K=0: there is no product");
+  if (!x || !q || !s || !y) return fail(DLB_ERR_NULL_POINTER, "x, q, s or y is NULL");
+  if (x_row_stride < 0 || x_row_stride > (1 << 23)) return fail(DLB_ERR_BAD_STRIDE, "x row stride %lld is not 0 ... 2^23", (long long)x_row_stride);
+  if (misaligned(q, 16) || misaligned(x, 4) || x_row_stride % 2 != 0 || off_elements(y, dtype))
+    return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte, rows of x 4-byte aligned, y to its elements");
+  const FewArgs a{x, y, M, x_row_stride, Matrix{static_cast<const uint8_t*>(q), s, static_cast<int>(N), static_cast<int>(K)}};
+  const int mt = M <= 16 ? 1 : 2, nt = N >= 6400 ? 2 : 1;
+  const dim3 grid(static_cast<unsigned>(ceil_div(N, 16 * nt)), static_cast<unsigned>(ceil_div(M, 16 * mt)));
+  with_flag(dtype == kInBf16, [&](auto bf16) {
+    with_chunks<1, 2>(mt, [&](auto m) {
+      with_chunks<1, 2>(nt, [&](auto n) {
+        hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, m(), n()>), grid, dim3(64 * kFewWaves), 0, static_cast<hipStream_t>(stream), a);
+      });
+    });
+  });
+  return finish("mxfp4_weight_gemm");
+}
+
+size_t dlb_few_token_experts_workspace_bytes(int64_t tokens, int64_t topk, int64_t I) {
+  return tokens > 0 && topk > 0 && I > 0 ? static_cast<size_t>(tokens) * topk * I * 2 * sizeof(uint16_t) : 0;
+}
+
+int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k,
+                          const float* weights, int weight_type, const void* up_q, const void* up_s, const void* down_q, const void* down_s, void* out,
+                          int64_t tokens, int64_t topk, int64_t experts, int64_t H, int64_t I, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dlb;
+  clear_error();
+  if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16", dtype);
+  if (ids_dtype != DLB_IDX_I32 && ids_dtype != DLB_IDX_I64) return fail(DLB_ERR_BAD_DTYPE, "ids_dtype %d is not DLB_IDX_I32 / I64", ids_dtype);
+  if (weight_type != DLB_WEIGHTS_E4M3 && weight_type != DLB_WEIGHTS_MXFP4) return fail(DLB_ERR_BAD_DTYPE, "weight_type %d is not DLB_WEIGHTS_E4M3 / MXFP4", weight_type);
+  const bool f4 = weight_type == DLB_WEIGHTS_MXFP4;
+  const int64_t unit = f4 ? kMxGroup : kScaleBlock;
+  if (tokens < 0 || topk < 0 || experts < 0 || H < 0 || I < 0)
+    return fail(DLB_ERR_BAD_SHAPE, "negative dimension (tokens=%lld topk=%lld experts=%lld H=%lld I=%lld)", (long long)tokens, (long long)topk, (long long)experts,
+                (long long)H, (long long)I);
+  if (tokens > kFewTokens || topk < 1 || topk > kFewTopk || experts < 1 || experts > kFewExperts)
+    return fail(DLB_ERR_BAD_SHAPE, "tokens=%lld, topk=%lld, experts=%lld: at most %d, 1 ... %d, 1 ... %d", (long long)tokens, (long long)topk, (long long)experts, kFewTokens,
+                kFewTopk, kFewExperts);
+  if (H % unit != 0 || I % unit != 0 || I == 0 || H > (1 << 20) || I > (1 << 20))
+    return fail(DLB_ERR_BAD_SHAPE, "H=%lld, I=%lld must be multiples of %lld, I at least that, both at most 2^20", (long long)H, (long long)I, (long long)unit);
+  if (tokens * topk * I > (1 << 29)) return fail(DLB_ERR_BAD_SHAPE, "tokens * topk * I=%lld is beyond 2^29", (long long)(tokens * topk * I));
+  if (tokens == 0 || H == 0) return DLB_OK;
+  if (!x || !ids || !weights || !up_q || !up_s || !down_q || !down_s || !out) return fail(DLB_ERR_NULL_POINTER, "a tensor pointer is NULL");
+  if (x_row_stride < 0 || x_row_stride > (1 << 23)) return fail(DLB_ERR_BAD_STRIDE, "x row stride %lld is not 0 ... 2^23", (long long)x_row_stride);
+  if (ids_stride_m < 0 || ids_stride_k < 0) return fail(DLB_ERR_BAD_STRIDE, "negative stride");
+  if (misaligned(x, 4) || x_row_stride % 2 != 0 || misaligned(ids, ids_dtype == DLB_IDX_I64 ? 8 : 4) || misaligned(weights, 4) || misaligned(up_q, 16) ||
+      misaligned(down_q, 16) || (!f4 && (misaligned(up_s, 4) || misaligned(down_s, 4))) || off_elements(out, dtype))
+    return fail(DLB_ERR_ALIGNMENT, "weights must be 16-byte, rows of x 4-byte aligned, the others to their elements");
+  const size_t need = dlb_few_token_experts_workspace_bytes(tokens, topk, I);
+  if (!workspace || workspace_bytes < need) return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+  if (misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  ExpertArgs a{};
+  a.x = x, a.ids = ids, a.weights = weights, a.act = static_cast<uint16_t*>(workspace), a.out = out;
+  a.up = Matrix{static_cast<const uint8_t*>(up_q), up_s, static_cast<int>(2 * I), static_cast<int>(H)};
+  a.down = Matrix{static_cast<const uint8_t*>(down_q), down_s, static_cast<int>(H), static_cast<int>(I)};
+  a.up_q = a.down_q = 0;
+  if (f4) {
+    a.up_q = I * H, a.up_s = 2 * I * (H / kMxGroup), a.down_q = H * (I / 2), a.down_s = H * (I / kMxGroup);
+  } else {
+    a.up_q = 2 * I * H, a.up_s = ceil_div(2 * I, 128) * (H / 128) * 4, a.down_q = H * I, a.down_s = (H / 128) * (I / 128) * 4;
+  }
+  a.x_rs = x_row_stride, a.ids_s0 = ids_stride_m, a.ids_s1 = ids_stride_k;
+  a.T = static_cast<int>(tokens), a.topk = static_cast<int>(topk), a.E = static_cast<int>(experts), a.H = static_cast<int>(H), a.I = static_cast<int>(I);
+  a.ids_is64 = ids_dtype == DLB_IDX_I64;
+  const int64_t slots = tokens * topk;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(H / 16));
+  const int up_mt = tokens > 16 && slots / experts >= 8 ? 2 : 1, down_mt = tokens > 8 && slots / experts > 4 ? 2 : 1;
+  with_flag(f4, [&](auto four) {
+    constexpr int kW = four() ? kE2m1 : kE4m3;
+    with_flag(dtype == kInBf16, [&](auto bf16) {
+      constexpr int kT = bf16() ? kInBf16 : kInF16;
+      with_chunks<1, 2>(up_mt, [&](auto m) { hipLaunchKernelGGL((experts_up_kernel<kT, kW, m()>), up_grid, dim3(64 * kFewWaves), 0, st, a); });
+      with_chunks<1, 2>(down_mt, [&](auto m) {
+        hipLaunchKernelGGL((experts_down_kernel<kT, kW, m()>), down_grid, dim3(64 * kFewWaves), static_cast<size_t>(kFewWaves) * tokens * 16 * sizeof(float), st, a);
+      });
+    });
+  });
+  return finish("few_token_experts");
 }
 
 }  // extern "C"

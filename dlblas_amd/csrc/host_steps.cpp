@@ -32,6 +32,9 @@ struct StepAbi {
   decltype(&dlb_mxfp4_quant) mx_quant;
   decltype(&dlb_mxfp4_gemm_workspace_bytes) mx_ws;
   decltype(&dlb_mxfp4_gemm) mx;
+  decltype(&dlb_mxfp4_weight_gemm) mx_weight;
+  decltype(&dlb_few_token_experts_workspace_bytes) experts_ws;
+  decltype(&dlb_few_token_experts) experts;
 } abi;
 
 constexpr int64_t kMaxTopk = 64, kMaxExperts = DLB_SORT_MAX_EXPERTS;
@@ -618,6 +621,79 @@ PyObject* mxfp4_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_EXCEPTIONS_END
 }
 
+// Rows as the kernels of a few rows read them.
+bool on_dwords(const at::Tensor& x) {
+  const int64_t stride = row_stride(x);
+  return stride >= 0 && stride % 2 == 0 && stride <= (1 << 23) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 4 == 0;
+}
+bool is_16_bit(const at::Tensor& x) { return x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf; }
+
+// mxfp4_weight_gemm(x, w_q, w_s) -> y
+PyObject* mxfp4_weight_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_EXCEPTIONS_BEGIN
+  const at::Tensor* t[3];
+  if (n != 3 || !take(args, t, 0)) NOT_PLAIN;
+  const at::Tensor &x = *t[0], &q = *t[1], &s = *t[2];
+  const int64_t K = mx_columns(q, s, 16);
+  if (!is_16_bit(x) || x.dim() < 1 || x.numel() == 0 || K == 0 || q.dim() != 2 || x.size(-1) != K || !on_dwords(x)) NOT_PLAIN;
+  const OpRecord record("dlblas::mxfp4_weight_gemm", t);
+  const int64_t M = x.numel() / K, N = q.size(0);
+  at::DimVector size(x.sizes());
+  size.back() = N;
+  DeviceScope scope(x);
+  at::Tensor y;
+  int rc;
+  {
+    const NoGil nogil;
+    y = empty(size, x.scalar_type(), x);
+    rc = abi.mx_weight(ptr(x), row_stride(x), in_code(x.scalar_type()), ptr(q), ptr(s), ptr(y), M, N, K, stream_of(x));
+  }
+  if (rc != DLB_OK) NOT_PLAIN;
+  return THPVariable_Wrap(std::move(y));
+  HANDLE_EXCEPTIONS_END
+}
+
+// few_token_experts(x, ids, weights, (w13, its scales), (w2, its scales)) -> out
+PyObject* few_token_experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_EXCEPTIONS_BEGIN
+  if (n != 5 || !PyTuple_CheckExact(args[3]) || !PyTuple_CheckExact(args[4]) || PyTuple_GET_SIZE(args[3]) != 2 || PyTuple_GET_SIZE(args[4]) != 2) NOT_PLAIN;
+  PyObject* const given[] = {args[0], args[1], args[2], PyTuple_GET_ITEM(args[3], 0), PyTuple_GET_ITEM(args[3], 1), PyTuple_GET_ITEM(args[4], 0), PyTuple_GET_ITEM(args[4], 1)};
+  const at::Tensor* t[7];
+  if (!take(given, t, 0)) NOT_PLAIN;
+  const at::Tensor &x = *t[0], &ids = *t[1], &w = *t[2], &up = *t[3], &up_s = *t[4], &down = *t[5], &down_s = *t[6];
+  if (!is_16_bit(x) || x.dim() != 2 || x.numel() == 0 || !on_dwords(x) || ids.dim() != 2 || idx_code(ids.scalar_type()) < 0 || ids.numel() == 0 || ids.size(0) != x.size(0)) NOT_PLAIN;
+  if (!is_f32(w) || w.sizes() != ids.sizes() || !w.is_contiguous() || up.dim() != 3 || down.dim() != 3 || up.scalar_type() != down.scalar_type()) NOT_PLAIN;
+  const bool f4 = up.scalar_type() == at::kByte;
+  if (!f4 && !is_f8(up)) NOT_PLAIN;
+  const int64_t T = x.size(0), H = x.size(1), topk = ids.size(1), E = up.size(0), I = up.size(1) / 2, part = f4 ? 2 : 1;
+  if (up.size(1) != 2 * I || up.size(2) * part != H || down.size(0) != E || down.size(1) != H || down.size(2) * part != I || I == 0 || E == 0) NOT_PLAIN;
+  if (f4) {
+    if (mx_columns(up, up_s, 16) == 0 || mx_columns(down, down_s, 16) == 0) NOT_PLAIN;
+  } else {
+    if (H % kBlock != 0 || I % kBlock != 0 || !is_f32(up_s) || !is_f32(down_s) || up_s.sizes() != at::IntArrayRef({E, ceil_div(2 * I, kBlock), H / kBlock}) ||
+        down_s.sizes() != at::IntArrayRef({E, H / kBlock, I / kBlock}))
+      NOT_PLAIN;
+    for (const at::Tensor* m : {&up, &up_s, &down, &down_s})
+      if (!m->is_contiguous()) NOT_PLAIN;
+    if (reinterpret_cast<uintptr_t>(up.data_ptr()) % 16 != 0 || reinterpret_cast<uintptr_t>(down.data_ptr()) % 16 != 0) NOT_PLAIN;
+  }
+  const OpRecord record("dlblas::few_token_experts", t);
+  DeviceScope scope(x);
+  at::Tensor out, scratch;
+  int rc;
+  {
+    const NoGil nogil;
+    out = empty({T, H}, x.scalar_type(), x);
+    const size_t need = abi.experts_ws(T, topk, I);
+    scratch = empty({static_cast<int64_t>(need)}, at::kByte, x);
+    rc = abi.experts(ptr(x), row_stride(x), in_code(x.scalar_type()), ptr(ids), idx_code(ids.scalar_type()), ids.stride(0), ids.stride(1), fptr(w),
+                     f4 ? DLB_WEIGHTS_MXFP4 : DLB_WEIGHTS_E4M3, ptr(up), ptr(up_s), ptr(down), ptr(down_s), ptr(out), T, topk, E, H, I, ptr(scratch), need, stream_of(x));
+  }
+  if (rc != DLB_OK) NOT_PLAIN;
+  return THPVariable_Wrap(std::move(out));
+  HANDLE_EXCEPTIONS_END
+}
+
 // init_steps(addresses): in the order of StepAbi's members
 PyObject* init_steps(PyObject*, PyObject* list) {
   void* slots[sizeof(StepAbi) / sizeof(void*)];
@@ -634,5 +710,5 @@ PyObject* init_steps(PyObject*, PyObject* list) {
 }  // namespace
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(layer_norm), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped), FAST(per_group_quant_mxfp4), FAST(mxfp4_gemm),
+PyMethodDef host_step_methods[] = {FAST(rms_norm), FAST(rms_norm_quant), FAST(layer_norm), FAST(moe_permute), FAST(moe_unpermute), FAST(w4_gemm), FAST(w4_gemm_grouped), FAST(per_group_quant_mxfp4), FAST(mxfp4_gemm), FAST(mxfp4_weight_gemm), FAST(few_token_experts),
                                    {"init_steps", init_steps, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};

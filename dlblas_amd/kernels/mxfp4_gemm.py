@@ -29,6 +29,11 @@ def _gemm_op(a: torch.Tensor, b: torch.Tensor, a_s: torch.Tensor, b_s: torch.Ten
     _mxfp4.gemm(a, b, a_s, b_s, c)
 
 
+@torch.library.custom_op('dlblas::mxfp4_weight_gemm', mutates_args=('y', ), device_types='cuda')
+def _weight_op(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, y: torch.Tensor) -> None:
+    _mxfp4.weight_gemm(x, w_q, w_s, y)
+
+
 def _check_columns(K):
     if K % GROUP != 0:
         raise ValueError(f'the last dimension {K} must be divisible by {GROUP}, the columns of a scale')
@@ -108,10 +113,39 @@ def mxfp4_gemm(a: torch.Tensor, b: torch.Tensor, a_s: torch.Tensor, b_s: torch.T
     return c
 
 
+def mxfp4_weight_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor) -> torch.Tensor:
+    """``x`` [..., K] (bf16 / fp16) times weights in 4-bit floating point, ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / 32] uint8 as
+    ``per_group_quant_mxfp4`` makes them: [..., N] in the type of x; fp32 sums, one rounding.
+
+    For up to a few dozen rows, which stay unquantised: the weights are read once per 32 of them.  Beside bf16 rows weights below 2^-126 in
+    magnitude may count as zero.
+    """
+    if not torch.compiler.is_compiling():
+        y = _fast.mxfp4_weight_gemm(x, w_q, w_s)
+        if y is not None:
+            return y
+    _decoder.no_tangents(x)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f'x must be bfloat16 or float16, got {x.dtype}')
+    K = _check_operand(w_q, w_s, 'w', 2)
+    if x.dim() < 1 or x.size(-1) != K:
+        raise ValueError(f'x must be [..., {K}], got {list(x.shape)}')
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise NotImplementedError('products with 4-bit weights have no gradient: call them under torch.no_grad()')
+    N = w_q.size(0)
+    y = torch.empty(x.shape[:-1] + (N, ), dtype=x.dtype, device=x.device)
+    if y.numel() > 0:
+        _weight_op(x if x.dim() == 2 else x.reshape(-1, K), w_q, w_s, y.view(-1, N))
+    return y
+
+
 def _register():
-    m, n, k, g = (SymVar(s) for s in 'm n k g'.split())
+    m, n, k, kh, g = (SymVar(s) for s in 'm n k kh g'.split())
     u8 = lambda *size: Tensor(size, dtype=torch.uint8, device='cuda')
-    register_dlblas_op('mxfp4_gemm', None, (u8(m, k), u8(n, k), u8(m, g), u8(n, g)), mxfp4_gemm, _bench(mxfp4_gemm), mxfp4_gemm)
+    register_dlblas_op('mxfp4_gemm', None, (u8(m, kh), u8(n, kh), u8(m, g), u8(n, g)), mxfp4_gemm, _bench(mxfp4_gemm), mxfp4_gemm)
+    for dt in (torch.bfloat16, torch.float16):
+        register_dlblas_op('mxfp4_weight_gemm', None, (Tensor((m, k), dtype=dt, device='cuda'), u8(n, kh), u8(n, g)), mxfp4_weight_gemm, _bench(mxfp4_weight_gemm),
+                           mxfp4_weight_gemm)
     for dt in (torch.bfloat16, torch.float16, torch.float32):
         register_dlblas_op('per_group_quant_mxfp4', None, (Tensor((m, k), dtype=dt, device='cuda'), ), per_group_quant_mxfp4, _bench(per_group_quant_mxfp4),
                            per_group_quant_mxfp4)

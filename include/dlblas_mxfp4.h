@@ -45,6 +45,51 @@ size_t dlb_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_s, void* c, int64_t M, int64_t N, int64_t K, int out_dtype,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * y[m, n] = sum over the groups g of 2^(s[n, g] - 127) sum_{k in g} x[m, k] q[n, k]; fp32 sums, one rounding at the end.  Beside bf16 rows weights
+ * below 2^-126 in magnitude may count as zero.  Meant for up to a few dozen rows: the weights are read once per 32 of them.
+ *
+ *   x [M, K]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
+ *   q [N, K/2]   codes, 16-byte aligned;  s [N, K/32] scales
+ *   y [M, N]     dtype, contiguous
+ *
+ * K % 32 == 0, at most DLB_MXFP4_MAX_COLUMNS.
+ */
+int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, void* y, int64_t M, int64_t N, int64_t K,
+                          void* stream);
+
+/* what dlb_few_token_experts takes at most */
+#define DLB_FEW_TOKENS 64
+#define DLB_FEW_TOPK 16
+#define DLB_FEW_EXPERTS 1024
+/* weight types of dlb_few_token_experts: e4m3fn with fp32 scales of 128 x 128, or the 4-bit format above */
+#define DLB_WEIGHTS_E4M3 0
+#define DLB_WEIGHTS_MXFP4 1
+
+/* Bytes of scratch dlb_few_token_experts needs. */
+size_t dlb_few_token_experts_workspace_bytes(int64_t tokens, int64_t topk, int64_t I);
+
+/*
+ * A layer of experts for a few tokens:
+ *   out[t] = sum over the slots j with 0 <= ids[t, j] < experts of weights[t, j] Down[e] (silu(Gate[e] x[t]) * (Up[e] x[t])),  e = ids[t, j]
+ * Products and sums in fp32; what lies between the products is held in 16 bits of significand, the result rounded once.  Zeros for a token
+ * without an expert here; slots that name one expert twice count both weights.  The order of all sums depends on the routing and the sizes alone.
+ * Beside bf16 rows, and in Down, weights below 2^-126 in magnitude may count as zero.
+ *
+ *   x       [tokens, H]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
+ *   ids     [tokens, topk]  int32 / int64 (ids_dtype, DLB_IDX_*) through two strides;  weights [tokens, topk] fp32, contiguous
+ *   up_q    [experts, 2 I, H], rows of Gate, then rows of Up;  down_q [experts, H, I]: e4m3fn, or codes of half that width, 16-byte aligned
+ *   up_s, down_s            scales: [experts, ceil(rows / 128), columns / 128] fp32, or [experts, rows, columns / 32] bytes
+ *   out     [tokens, H]     dtype, contiguous
+ *   workspace               4-byte aligned, dlb_few_token_experts_workspace_bytes(tokens, topk, I), no initialisation; calls that can overlap need
+ *                           their own
+ *
+ * tokens at most 64, topk 16, experts 1024; H and I multiples of 128 with e4m3 weights, of 32 with 4-bit ones, at most 2^20.
+ */
+int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k,
+                          const float* weights, int weight_type, const void* up_q, const void* up_s, const void* down_q, const void* down_s, void* out,
+                          int64_t tokens, int64_t topk, int64_t experts, int64_t H, int64_t I, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,3 +38,34 @@ def gemm(a, a_s, b, b_s):
     """(product, sum of the magnitudes of its terms)."""
     x, w = values(a, a_s), values(b, b_s)
     return x @ w.t(), x.abs() @ w.abs().t()
+
+
+def e4m3_values(q, s):
+    """[E, N, K] numbers of e4m3 weights with a scale per 128 x 128."""
+    wide = s.double().repeat_interleave(128, 1)[:, :q.shape[1]].repeat_interleave(128, 2)
+    return q.double() * wide
+
+
+def experts(x, ids, weights, w13, w2):
+    """(out, bound of an evaluation with fp32 sums and 16 bits between the products), from the numbers of the weights [E, 2 I, H], [E, H, I].
+
+    A sum of n terms is off by at most (n + 8) 2^-23 of its magnitudes (the unit cuts off where it does not round).  silu(g) u: g and u as far off as that,
+    |silu'| <= 1.1, the exponential off by (2 + |g|) 2^-23 of itself, silu then by as much of itself, and four roundings; then the two bf16 hold
+    2^-16 of it."""
+    T, H = x.shape
+    I = w13.shape[1] // 2
+    x, out, bound = x.double(), torch.zeros(T, H, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    for t in range(T):
+        for e, w in zip(ids[t].tolist(), weights[t].double().tolist()):
+            if not 0 <= e < w13.shape[0]:
+                continue
+            both, mag = w13[e] @ x[t], w13[e].abs() @ x[t].abs()
+            off = (H + 8) * 2 * FP32 * mag
+            (g, u), (g_off, u_off) = both.split(I), off.split(I)
+            silu = g / (1 + torch.exp(-g))
+            act = silu * u
+            act_off = 1.1 * g_off * (u.abs() + u_off) + silu.abs() * u_off + act.abs() * ((6 + g.abs()) * 2 * FP32 + 2.0**-16)
+            out[t] += w * (w2[e] @ act)
+            terms = abs(w) * (w2[e].abs() @ act.abs())
+            bound[t] += abs(w) * (w2[e].abs() @ act_off) + (I + 40) * 2 * FP32 * terms
+    return out, bound
