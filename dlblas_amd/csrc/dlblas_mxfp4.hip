@@ -119,12 +119,16 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (misaligned(q, 16) || misaligned(x, 4) || x_row_stride % 2 != 0 || off_elements(y, dtype))
     return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte, rows of x 4-byte aligned, y to its elements");
   const FewArgs a{x, y, M, x_row_stride, Matrix{static_cast<const uint8_t*>(q), s, static_cast<int>(N), static_cast<int>(K)}};
-  const int mt = M <= 16 ? 1 : 2, nt = N >= 6400 ? 2 : 1;
-  const dim3 grid(static_cast<unsigned>(ceil_div(N, 16 * nt)), static_cast<unsigned>(ceil_div(M, 16 * mt)));
+  const int rows = M <= 4 ? 4 : M <= 8 ? 8 : M <= 16 ? 16 : 32, nt = N >= 6400 ? 2 : 1;
+  const dim3 grid(static_cast<unsigned>(ceil_div(N, 16 * nt)), static_cast<unsigned>(ceil_div(M, rows)));
   with_flag(dtype == kInBf16, [&](auto bf16) {
-    with_chunks<1, 2>(mt, [&](auto m) {
-      with_chunks<1, 2>(nt, [&](auto n) {
-        hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, m(), n()>), grid, dim3(64 * kFewWaves), 0, static_cast<hipStream_t>(stream), a);
+    with_flag(K % 128 != 0, [&](auto ragged) {
+      with_chunks<4, 8, 16, 32>(rows, [&](auto r) {
+        with_chunks<1, 2>(nt, [&](auto n) {
+          typedef FewShape<kE2m1, r(), n()> Shape;
+          hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n(), ragged()>), grid, dim3(64 * Shape::kWaves), Shape::kLds,
+                             static_cast<hipStream_t>(stream), a);
+        });
       });
     });
   });
@@ -180,16 +184,23 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   const int64_t slots = tokens * topk;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(H / 16));
-  const int up_mt = tokens > 16 && slots / experts >= 8 ? 2 : 1, down_mt = tokens > 8 && slots / experts > 4 ? 2 : 1;
-  with_flag(f4, [&](auto four) {
-    constexpr int kW = four() ? kE2m1 : kE4m3;
-    with_flag(dtype == kInBf16, [&](auto bf16) {
-      constexpr int kT = bf16() ? kInBf16 : kInF16;
-      with_chunks<1, 2>(up_mt, [&](auto m) { hipLaunchKernelGGL((experts_up_kernel<kT, kW, m()>), up_grid, dim3(64 * kFewWaves), 0, st, a); });
-      with_chunks<1, 2>(down_mt, [&](auto m) {
-        hipLaunchKernelGGL((experts_down_kernel<kT, kW, m()>), down_grid, dim3(64 * kFewWaves), static_cast<size_t>(kFewWaves) * tokens * 16 * sizeof(float), st, a);
-      });
+  // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches.
+  const int64_t mean = slots / std::min(experts, slots);
+  const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16, down_tokens = tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
+  const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
+    with_chunks<4, 8, 16>(up_rows, [&](auto r) {
+      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), up_grid, dim3(64 * kExpertWaves), (ExpertShape<kw(), r(), 2>::kRing), st, a);
     });
+    with_chunks<2, 4, 8>(down_tokens, [&](auto t) {
+      const int64_t lds = experts_down_lds(ExpertShape<kw(), 2 * t(), 1>::kRing, tokens, topk, experts, t());
+      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), ragged_down()>), down_grid, dim3(64 * kExpertWaves), static_cast<size_t>(lds), st, a);
+    });
+  };
+  with_flag(dtype == kInBf16, [&](auto bf16) {
+    constexpr std::integral_constant<int, bf16() ? kInBf16 : kInF16> kt;
+    constexpr std::false_type whole;
+    if (!f4) return launch(kt, std::integral_constant<int, kE4m3>(), whole, whole);
+    with_flag(H % 128 != 0, [&](auto up) { with_flag(I % 128 != 0, [&](auto down) { launch(kt, std::integral_constant<int, kE2m1>(), up, down); }); });
   });
   return finish("few_token_experts");
 }

@@ -1,13 +1,10 @@
 // Few 16-bit rows times quantised weights for gfx950, and what is built of it: a product with 4-bit weights and a layer of experts in two kernels.
 //
-// Bound by the weights' bytes: each goes from memory to a register once, is converted there and meets the rows in v_mfma_f32_16x16x32.  A lane
-// holds 32 bytes of one of 16 rows of a matrix, so that a wave reads whole 128-byte lines; which columns a lane's words are is free as long as the
-// lanes with the rows take the same.  Weights are
+// Bound by the weights' bytes: each comes from memory once, is converted in registers and meets the rows in v_mfma_f32_16x16x32.  Weights are
 //   e4m3   with one fp32 scale per 128 x 128: exact in 16 bits, sums of 128 columns times the scale in fp32
 //   e2m1   with a power of two per 32 columns.  Beside bf16 rows the scale goes into the conversion: e2m1 has two bits of significand and bf16 the
-//          range of the scales, so the products stay exact (scales below 2^-124, whose weights are subnormal numbers of bf16, may count as 0).  fp16 has not
-//          that range: there the words change places between the quarters of the wave, so that a step is one group, and the group's sum meets its
-//          scale in fp32.
+//          range of the scales, so the products stay exact (weights below 2^-126, which are subnormal numbers of bf16, may count as 0).  fp16 has not
+//          that range: there a group's sum meets its scale in fp32.
 // The waves of a workgroup split K and add their sums through LDS in wave order.
 #pragma once
 
@@ -26,15 +23,6 @@ __device__ __forceinline__ v4f mfma_16x16x32(const v4i& a, const v4i& b, const v
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Words i of the four quarters of the wave change places with quarters i of the words: quarter q of word i then holds what
-// quarter i held in word q.
-__device__ __forceinline__ void transpose_quarters(v4i& v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v[0]), static_cast<unsigned>(v[2]), false, false);
-  const auto b = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v[1]), static_cast<unsigned>(v[3]), false, false);
-  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-  const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-  v = v4i{static_cast<int>(c[0]), static_cast<int>(c[1]), static_cast<int>(d[0]), static_cast<int>(d[1])};
-}
 // The value of each quarter in all quarters.
 __device__ __forceinline__ void spread_quarters(uint32_t v, uint32_t (&out)[4]) {
   const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
@@ -68,6 +56,14 @@ __device__ __forceinline__ v4i from_e2m1(int word, float scale) {
              __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
 }
 
+// What is the same for the lanes of a wave, in scalar registers: a buffer that the compiler cannot see to be that costs a loop over the lanes a load.
+__device__ __forceinline__ uint32_t in_scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const uint8_t* in_scalar(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = in_scalar(static_cast<uint32_t>(v)), hi = in_scalar(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const uint8_t*>(hi << 32 | lo);
+}
+
 // A matrix of weights [N][K].  e4m3: q has K bytes a row, s is [ceil(N / 128)][K / 128] fp32; e2m1: K / 2, and [N][K / 32] bytes.
 struct Matrix {
   const uint8_t* q;
@@ -75,30 +71,34 @@ struct Matrix {
   int N, K;
 };
 
-// What a wave reads of a matrix: a chunk is 128 bytes of each of 16 rows.
-template <int T, int W>
-struct Few {
-  static constexpr int kCols = W == kE2m1 ? 256 : 128;  // of a chunk
-  static constexpr int kSteps = kCols / 32;             // MFMA steps
-  static constexpr bool kByGroup = W == kE2m1 && T == kInF16;
+// A wave's own stream: chunks of 128 columns of NT tiles of 16 weight rows and of R rows of x come into a ring of DEPTH chunks in LDS that no other
+// wave reads, so nothing but the wave's own counter of loads is waited for.  They go through LDS because of the order of the lanes: an MFMA wants
+// neighbouring rows in neighbouring lanes, and loaded that way every lane touches a cache line of its own, 64 a load, which held 32 experts x 4
+// rows x 4096 x 7168 e4m3 at 250 us however much was on its way.  Here four to sixteen lanes share a row.
+//
+// A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of e4m3
+// piece ^ (row / 2), of e2m1 piece ^ (row / 4).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a
+// word of its 16 bytes a quarter.  RAGGED: e2m1, K is no multiple of 128.
+constexpr int stream_tile(int weights) { return (weights == kE4m3 ? 2048 : 1024) + 256; }
+constexpr int stream_loads(int weights, int R, int NT, bool ragged) { return NT * ((weights == kE4m3 ? 2 : 1) + (ragged ? 0 : 1)) + R / 4; }
+constexpr int stream_bytes(int weights, int R, int NT) { return NT * stream_tile(weights) + R * 256; }
 
-  // First column of the eight that quarter q of the rows' lanes takes in step i.
-  static __device__ __forceinline__ int column(int q, int i) {
-    if (W == kE4m3) return 32 * q + 8 * i;
-    return kByGroup ? 64 * (i & 3) + 32 * (i >> 2) + 8 * q : 64 * q + 8 * i;
-  }
-
-  struct Weights {
-    v4i w[2];
-    uint32_t s;  // e2m1: the scales of a lane's two groups; e4m3: the scale's bits
-  };
+template <int T, int W, int R, int NT, int DEPTH, bool RAGGED>
+struct Stream {
+  static constexpr int kCols = 128, kMT = (R + 15) / 16;
+  static constexpr int kTile = stream_tile(W), kX = R * 256;  // bytes of a chunk; a tile's scales are behind its codes
+  static constexpr int kChunk = NT * kTile + kX, kBytes = DEPTH * kChunk;
+  static constexpr int kXLoads = R / 4;
+  // Loads of a chunk into LDS, which is what is counted.  RAGGED scales come to registers, a byte a load: the compiler may issue those later than
+  // they are written, and a wait that counted them would end too early.
+  static constexpr int kLoads = stream_loads(W, R, NT, RAGGED);
+  static_assert((R == 4 || R == 8 || R == 16 || R == 32) && (DEPTH - 1) * kLoads < 64 && !(RAGGED && W == kE4m3), "whole loads of x, a counter of six bits");
 
   // 16 rows of a matrix, from row n0 on.
   struct Tile {
-    const uint8_t* q;
-    const uint8_t* s;
+    const uint8_t *q, *s;
     uint32_t q_bytes, s_bytes;
-    __device__ __forceinline__ Tile(const Matrix& m, int n0) {
+    __device__ __forceinline__ void point_at(const Matrix& m, int n0) {
       const int rows = max(0, min(16, m.N - n0));
       const uint32_t q_pitch = W == kE2m1 ? m.K / 2 : m.K;
       q = m.q + static_cast<int64_t>(n0) * q_pitch, q_bytes = rows * q_pitch;
@@ -106,81 +106,169 @@ struct Few {
         s = static_cast<const uint8_t*>(m.s) + static_cast<int64_t>(n0) * (m.K / kMxGroup), s_bytes = rows * (m.K / kMxGroup);
       else
         s = reinterpret_cast<const uint8_t*>(static_cast<const float*>(m.s) + static_cast<int64_t>(n0 / 128) * (m.K / 128)), s_bytes = rows > 0 ? m.K / 32 : 0;
+      q = in_scalar(q), s = in_scalar(s), q_bytes = in_scalar(q_bytes), s_bytes = in_scalar(s_bytes);
     }
   };
 
-  // Chunk c; `in` (the same for the wave) false: nothing.  Loads are issued either way, none stands behind a branch.
-  static __device__ __forceinline__ void load(const Tile& t, int K, int c, bool in, int q, int l16, Weights& o) {
-    const uint32_t at = in ? static_cast<uint32_t>(c) * 128 : 0;
-    const auto src = make_rsrc(t.q, in ? t.q_bytes : 0);
+  const uint8_t* ring;  // this wave's
+  mx_lds_bytes ring_to;
+  int K, chunks;
+  const uint8_t* x;
+  uint32_t x_bytes;
+  uint32_t w_at, s_at;  // where a lane starts in a tile, and in its scales
+  int w_from, x_from;   // where it reads in a chunk
+  int q, l16;
+  uint32_t x_at[kXLoads];  // its row of x of each load with its piece; past the end of every buffer: none
+  Tile tile[NT];
+  uint32_t scales[RAGGED ? DEPTH : 1][NT][4];  // RAGGED
+  v4f acc[NT][kMT];
+
+  __device__ __forceinline__ Stream(uint8_t* lds, int wave, int lane, int columns, const void* x_base, uint32_t bytes)
+      : ring(lds + wave * kBytes), ring_to((mx_lds_bytes)lds + wave * kBytes), K(columns), chunks((columns + kCols - 1) / kCols),
+        x(in_scalar(static_cast<const uint8_t*>(x_base))), x_bytes(in_scalar(bytes)), q(lane >> 4), l16(lane & 15) {
     if (W == kE4m3) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) o.w[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, l16 * static_cast<uint32_t>(K) + 32 * q + 16 * i, at, 2));
-      o.s = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(t.s, in ? t.s_bytes : 0), 0, in ? 4 * c : 0, 0);
-      return;
+      const int row = lane >> 3;
+      w_at = row * K + ((lane & 7) ^ (row >> 1)) * 16, s_at = 0;
+      w_from = l16 * 128 + ((q ^ (l16 >> 1)) & 7) * 16;
+      x_from = (2 * q) * 16;
+    } else {
+      const int row = lane >> 2;
+      w_at = row * (K / 2) + ((lane & 3) ^ (row >> 2)) * 16;
+      s_at = q == 0 ? l16 * (K / kMxGroup) : kNowhere;  // one quarter asks
+      w_from = l16 * 64 + (l16 >> 2) * 16 + 4 * q;
+      x_from = q * 16;
     }
-    const int G = K / kMxGroup, g = 8 * c + 2 * q;  // the lane's first group of its row
-    const auto s_src = make_rsrc(t.s, in ? t.s_bytes : 0);
+    x_from = (l16 & (R - 1)) * 256 + (x_from ^ (l16 & (R - 1) & 15) * 16);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool there = g + i < G;  // else it would be the next row's
-      o.w[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, there ? l16 * static_cast<uint32_t>(K / 2) + 32 * q + 16 * i : kNowhere, at, 2));
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  // Row of x that load j brings for a lane, and the lane's column there.
+  static __device__ __forceinline__ int x_row(int lane, int j) { return 4 * j + (lane >> 4); }
+  static __device__ __forceinline__ int x_column(int lane, int j) { return ((lane & 15) ^ (x_row(lane, j) & 15)) * 8; }
+  // at: byte of that row, kNowhere: none
+  __device__ __forceinline__ void set_row(int lane, int j, uint32_t at) { x_at[j] = at == kNowhere ? kNowhere : at + 2 * x_column(lane, j); }
+
+  // Chunk c into place d; `in` false (the same for the wave): nothing is brought.  Loads are issued either way.
+  __device__ __forceinline__ void load(int d, int lane, int c, bool in) {
+    const mx_lds_bytes to = ring_to + d * kChunk;
+    const uint32_t at = in ? static_cast<uint32_t>(c) * (W == kE4m3 ? 128 : 64) : 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // Past the end of a row of e2m1 a lane brings the next one's codes, which meet zeros of x; the scales there are zeros too, which are numbers.
+      const auto src = make_rsrc(tile[n].q, in ? tile[n].q_bytes : 0);
+      load_to_lds<2>(src, to + n * kTile, w_at, at);
+      // eight rows further on row / 2 has another third bit: the other half of the row
+      if (W == kE4m3) load_to_lds<2>(src, to + n * kTile + 1024, (w_at ^ 64) + 8 * K, at);
+      if (!RAGGED) {
+        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kTile + kTile - 256, s_at, in ? 4 * c : 0);
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        scales[d][n][i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(tile[n].s, in && 4 * c + i < K / kMxGroup ? tile[n].s_bytes : 0), s_at + i, in ? 4 * c : 0, 0);
     }
-    const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b8(s_src, g < G ? l16 * static_cast<uint32_t>(G) + 2 * q : kNowhere, at / 16, 0);
-    const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b8(s_src, g + 1 < G ? l16 * static_cast<uint32_t>(G) + 2 * q + 1 : kNowhere, at / 16, 0);
-    o.s = lo | hi << 8;
+#pragma unroll
+    for (int j = 0; j < kXLoads; ++j) {
+      const bool there = !RAGGED || c * kCols + x_column(lane, j) < K;
+      load_to_lds<0>(make_rsrc(x, in ? x_bytes : 0), to + NT * kTile + j * 1024, there ? x_at[j] : kNowhere, in ? static_cast<uint32_t>(c) * (2 * kCols) : 0);
+    }
   }
 
-  // acc[m] += rows m times the chunk; lane l receives D[4 (l / 16) + r][l % 16], rows by matrix rows.
-  template <int MT>
-  static __device__ __forceinline__ void multiply(Weights& w, const v4i (&x)[MT][kSteps], v4f (&acc)[MT]) {
-    if (W == kE4m3) {
-      v4f sum[MT];
+  // The chunk in place d, behind which there are DEPTH - 1 others, times its rows: lane l of acc[n][m] has rows 4 (l / 16) + r, column l % 16.
+  __device__ __forceinline__ void multiply(int d) {
+    wait_loads<(DEPTH - 1) * kLoads>();  // in order
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* const from = ring + d * kChunk;
+    v4i xf[kMT][4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) sum[m] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < kMT; ++m)
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const v4i f = from_e4m3<T>(w.w[i >> 1][2 * (i & 1)], w.w[i >> 1][2 * (i & 1) + 1]);
+      for (int i = 0; i < 4; ++i) xf[m][i] = *reinterpret_cast<const v4i*>(from + NT * kTile + m * 4096 + (x_from ^ (W == kE4m3 ? 128 * (i >> 1) + 16 * (i & 1) : 64 * i)));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) sum[m] = mfma_16x16x32<T>(x[m][i], f, sum[m]);
+    for (int n = 0; n < NT; ++n) {
+      if (W == kE4m3) {
+        v4f sum[kMT];
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) sum[m] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const v4i v = *reinterpret_cast<const v4i*>(from + n * kTile + (w_from ^ 64 * u));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const v4i f = from_e4m3<T>(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+            for (int m = 0; m < kMT; ++m) sum[m] = mfma_16x16x32<T>(xf[m][2 * u + i], f, sum[m]);
+          }
+        }
+        const float s = *reinterpret_cast<const float*>(from + n * kTile + kTile - 256);
+#pragma unroll
+        for (int m = 0; m < kMT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s, sum[m][r], acc[n][m][r]);
+        continue;
       }
-      const float s = __uint_as_float(w.s);
+      // each quarter makes one of the four scales of its rows, for all of them
+      uint32_t four, by_group[4];
+      if (RAGGED) {
+        four = scales[d][n][0];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(s, sum[m][r], acc[m][r]);
-      return;
-    }
-    const float scale[2] = {mx_scale(w.s & 0xffu), mx_scale(w.s >> 8)};
-    if (!kByGroup) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const v4i f = from_e2m1<T>(w.w[i >> 2][i & 3], scale[i >> 2]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = mfma_16x16x32<T>(x[m][i], f, acc[m]);
+        for (int i = 1; i < 4; ++i) four |= scales[d][n][i] << (8 * i);
+        spread_quarters(four, by_group);
+        four = by_group[0];
+      } else {
+        four = *reinterpret_cast<const uint32_t*>(from + n * kTile + kTile - 256 + 4 * l16);
       }
-      return;
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t by_group[4];  // of groups 2 i + u
-      spread_quarters(__float_as_uint(scale[u]), by_group);
-      transpose_quarters(w.w[u]);
+      spread_quarters(__float_as_uint(mx_scale(four >> (8 * q) & 0xffu)), by_group);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const v4i f = from_e2m1<T>(w.w[u][i], 1.0f);
+        const float scale = __uint_as_float(by_group[i]);
+        const v4i f = from_e2m1<T>(*reinterpret_cast<const int*>(from + n * kTile + (w_from ^ 16 * i)), T == kInBf16 ? scale : 1.0f);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const v4f sum = mfma_16x16x32<T>(x[m][4 * u + i], f, v4f{0.f, 0.f, 0.f, 0.f});
+        for (int m = 0; m < kMT; ++m) {
+          if (T == kInBf16) {
+            acc[n][m] = mfma_16x16x32<T>(xf[m][i], f, acc[n][m]);
+            continue;
+          }
+          const v4f sum = mfma_16x16x32<T>(xf[m][i], f, v4f{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(__uint_as_float(by_group[i]), sum[r], acc[m][r]);
+          for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(scale, sum[r], acc[n][m][r]);
         }
       }
     }
+    // what is read of this place has arrived before its next chunk is asked for
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // Chunks wave, wave + waves, ... of K.
+  __device__ __forceinline__ void split_k(int lane, int wave, int waves) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      load(d, lane, wave + d * waves, wave + d * waves < chunks);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int c = wave; c < chunks; c += DEPTH * waves) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        multiply(d);
+        const int next = c + (DEPTH + d) * waves;
+        load(d, lane, next, next < chunks);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_loads<0>();  // nothing is on its way into LDS any more
   }
 };
 
-constexpr int kFewWaves = 8;
+// Chunks in a wave's ring: as many as leave room for `groups` workgroups on a CU.
+constexpr int stream_depth(int weights, int R, int NT, int waves, int groups) {
+  const int depth = (160 * 1024 / groups - 8192) / (waves * stream_bytes(weights, R, NT));
+  return depth > 6 ? 6 : depth;
+}
 
 __device__ __forceinline__ void store1(void* to, int type, int64_t at, float v) {
   if (type == kInBf16)
@@ -189,46 +277,6 @@ __device__ __forceinline__ void store1(void* to, int type, int64_t at, float v) 
     static_cast<_Float16*>(to)[at] = static_cast<_Float16>(v);
   else
     static_cast<float*>(to)[at] = v;
-}
-
-// Chunks wave, wave + 8, ... of K: the next one is asked for before this one is multiplied.  x_off: of a lane's row m, kNowhere: none.
-template <int T, int W, int MT, int NT>
-__device__ __forceinline__ void split_k(const typename Few<T, W>::Tile (&tile)[NT], int K, __amdgpu_buffer_rsrc_t x_src, const uint32_t (&x_off)[MT], int wave, int q, int l16,
-                                        v4f (&acc)[NT][MT]) {
-  typedef Few<T, W> F;
-  struct Chunk {
-    typename F::Weights w[NT];
-    v4i x[MT][F::kSteps];
-  };
-  const int chunks = (K + F::kCols - 1) / F::kCols;
-  auto load = [&](int c, Chunk& k) {
-    const bool in = c < chunks;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) F::load(tile[n], K, c, in, q, l16, k.w[n]);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < F::kSteps; ++i) {
-        const int col = c * F::kCols + F::column(q, i);
-        k.x[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, x_off[m] != kNowhere && col < K ? x_off[m] + 2 * col : kNowhere, 0, 0));
-      }
-  };
-  auto multiply = [&](Chunk& k) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) F::template multiply<MT>(k.w[n], k.x, acc[n]);
-  };
-  Chunk even, odd;
-  load(wave, even);
-  for (int c = wave; c < chunks; c += 2 * kFewWaves) {
-    load(c + kFewWaves, odd);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(even);
-    __builtin_amdgcn_sched_barrier(0);
-    load(c + 2 * kFewWaves, even);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(odd);
-    __builtin_amdgcn_sched_barrier(0);
-  }
 }
 
 // ---- one matrix -------------------------------------------------------------------------------------------------------
@@ -240,42 +288,45 @@ struct FewArgs {
   Matrix w;
 };
 
-template <int T, int W, int MT, int NT>
-__global__ void __launch_bounds__(64 * kFewWaves) few_rows_kernel(const FewArgs p) {
-  __shared__ v4f part[kFewWaves][NT * MT][64];
+template <int W, int R, int NT>
+struct FewShape {
+  static constexpr int kWaves = R == 32 ? 4 : 8, kDepth = stream_depth(W, R, NT, kWaves, 1);
+  static constexpr int kRing = kWaves * kDepth * stream_bytes(W, R, NT);
+  static constexpr int kParts = kWaves * NT * ((R + 15) / 16) * 1024;
+  static constexpr int kLds = kRing > kParts ? kRing : kParts;
+};
+
+// R rows of x against 16 NT rows of the matrix.
+template <int T, int W, int R, int NT, bool RAGGED>
+__global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_kernel(const FewArgs p) {
+  typedef FewShape<W, R, NT> Shape;
+  typedef Stream<T, W, R, NT, Shape::kDepth, RAGGED> S;
+  constexpr int kWaves = Shape::kWaves, kMT = S::kMT;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int n0 = blockIdx.x * 16 * NT;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
-  const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(16 * MT)));
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * R;
+  const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(R)));
   const uint32_t pitch = static_cast<uint32_t>(p.x_rs) * 2;
-  const auto x_src = make_rsrc(static_cast<const uint8_t*>(p.x) + m0 * p.x_rs * 2, (rows - 1) * pitch + 2 * p.w.K);
-  uint32_t x_off[MT];
+  S s(lds, wave, lane, p.w.K, static_cast<const uint8_t*>(p.x) + m0 * p.x_rs * 2, (rows - 1) * pitch + 2 * p.w.K);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) x_off[m] = 16 * m + l16 < rows ? (16 * m + l16) * pitch : kNowhere;
-  typedef typename Few<T, W>::Tile Tile;
-  v4f acc[NT][MT];
+  for (int n = 0; n < NT; ++n) s.tile[n].point_at(p.w, n0 + 16 * n);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
-  if constexpr (NT == 1) {
-    const Tile tile[1] = {Tile(p.w, n0)};
-    split_k<T, W, MT, 1>(tile, p.w.K, x_src, x_off, wave, q, l16, acc);
-  } else {
-    const Tile tile[2] = {Tile(p.w, n0), Tile(p.w, n0 + 16)};
-    split_k<T, W, MT, 2>(tile, p.w.K, x_src, x_off, wave, q, l16, acc);
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) part[wave][n * MT + m][lane] = acc[n][m];
+  for (int j = 0; j < S::kXLoads; ++j) s.set_row(lane, j, S::x_row(lane, j) < rows ? S::x_row(lane, j) * pitch : kNowhere);
+  s.split_k(lane, wave, kWaves);
   __syncthreads();
-  for (int i = wave; i < NT * MT; i += kFewWaves) {
-    v4f sum = part[0][i][lane];
+  v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][NT kMT][64]
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) sum += part[w][i][lane];
-    const int n = i / MT, m = i - n * MT, col = n0 + 16 * n + l16;
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) part[(wave * NT * kMT + n * kMT + m) * 64 + lane] = s.acc[n][m];
+  __syncthreads();
+  for (int i = wave; i < NT * kMT; i += kWaves) {
+    v4f sum = part[i * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += part[(w * NT * kMT + i) * 64 + lane];
+    const int n = i / kMT, m = i - n * kMT, col = n0 + 16 * n + l16;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 16 * m + 4 * q + r;
@@ -290,7 +341,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) few_rows_kernel(const FewArgs 
 //
 // The first kernel leaves w silu(g) u of every slot, the second reads it against the experts' second matrices.  No sort in front: there are at most 64
 // tokens, a lane of a wave each, so the tokens of an expert are a ballot.  In between the numbers are held as the sum of two bf16, 16 bits of
-// significand, which the second kernel's rows take one beside the other: eight tokens and their rests are the 16 rows of an MFMA.  An
+// significand, which the second kernel takes one beside the other: eight tokens and their rests are the 16 rows of an MFMA.  An
 // expert that a token names twice counts with the sum of both weights.
 
 constexpr int kFewTokens = 64, kFewTopk = 16, kFewExperts = 1024;
@@ -312,10 +363,12 @@ __device__ __forceinline__ Matrix of_expert(const Matrix& m, int64_t q, int64_t 
   return Matrix{m.q + e * q, static_cast<const uint8_t*>(m.s) + e * s, m.N, m.K};
 }
 
+// The expert of a slot, -1: none of these.  Both widths by words, without a branch between the loads of several slots.
 __device__ __forceinline__ int expert_of(const ExpertArgs& p, int t, int j) {
-  const int64_t at = t * p.ids_s0 + j * p.ids_s1;
-  const int64_t e = p.ids_is64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at];
-  return e >= 0 && e < p.E ? static_cast<int>(e) : -1;
+  const int64_t at = (t * p.ids_s0 + j * p.ids_s1) << p.ids_is64;
+  const int32_t* const words = static_cast<const int32_t*>(p.ids);
+  const int low = words[at], high = words[at + p.ids_is64];
+  return low >= 0 && low < p.E && (p.ids_is64 == 0 || high == 0) ? low : -1;
 }
 
 // Lane i of the result: the lane of the i-th bit of the mask.
@@ -329,11 +382,21 @@ __device__ __forceinline__ int nth_lane(uint64_t mask, int lane) {
 // silu(g) u
 __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
+constexpr int kExpertWaves = 4;
+
+template <int W, int R, int NT>
+struct ExpertShape {
+  static constexpr int kDepth = stream_depth(W, R, NT, kExpertWaves, 2);
+  static constexpr int kRing = kExpertWaves * kDepth * stream_bytes(W, R, NT);
+};
+
 // A workgroup takes 16 rows of Gate and the same of Up, of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
-// it is the first to name it.
-template <int T, int W, int MT>
-__global__ void __launch_bounds__(64 * kFewWaves) experts_up_kernel(const ExpertArgs p) {
-  __shared__ v4f part[kFewWaves][2 * MT][64];
+// it is the first to name it; R of its tokens at a time.
+template <int T, int W, int R, bool RAGGED>
+__global__ void __launch_bounds__(64 * kExpertWaves) experts_up_kernel(const ExpertArgs p) {
+  typedef Stream<T, W, R, 2, ExpertShape<W, R, 2>::kDepth, RAGGED> S;
+  static_assert(S::kMT == 1, "the sums of a pass are a tile of Gate and one of Up");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int slots = p.T * p.topk, y = blockIdx.y;
@@ -353,52 +416,44 @@ __global__ void __launch_bounds__(64 * kFewWaves) experts_up_kernel(const Expert
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (lane >= p.T || j0 + i >= p.topk || named[i] != e) continue;
-      if (first < 0) first = token * p.topk + j0 + i;
-      weight += w[i];
+      const bool names = lane < p.T && j0 + i < p.topk && named[i] == e;
+      first = names && first < 0 ? token * p.topk + j0 + i : first;
+      weight += names ? w[i] : 0.f;
     }
   }
   const uint64_t mask = __ballot(first >= 0);
   if (mask == 0) return;
   if (by_slot && __shfl(first, __builtin_ctzll(mask)) != y) return;
   const int rows = __popcll(mask), token_of = nth_lane(mask, lane);
-  typedef typename Few<T, W>::Tile Tile;
   const Matrix up = of_expert(p.up, p.up_q, p.up_s, e);
   const int n0 = blockIdx.x * 16;
-  const Tile tile[2] = {Tile(up, n0), Tile(up, p.I + n0)};
-  const auto x_src = make_rsrc(p.x, static_cast<uint32_t>((p.T - 1) * p.x_rs + p.H) * 2);
   const int64_t rest = static_cast<int64_t>(slots) * p.I;
-  for (int b = 0; b < rows; b += 16 * MT) {
-    uint32_t x_off[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int i = b + 16 * m + l16;
-      const int token = __shfl(token_of, i & 63);
-      x_off[m] = i < rows ? static_cast<uint32_t>(token * p.x_rs) * 2 : kNowhere;
-    }
-    v4f acc[2][MT];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
-    split_k<T, W, MT, 2>(tile, p.H, x_src, x_off, wave, q, l16, acc);
+  v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][2][64]
+  for (int b = 0; b < rows; b += R) {
     if (b > 0) __syncthreads();
+    S s(lds, wave, lane, p.H, p.x, static_cast<uint32_t>((p.T - 1) * p.x_rs + p.H) * 2);
+    s.tile[0].point_at(up, n0), s.tile[1].point_at(up, p.I + n0);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) part[wave][n * MT + m][lane] = acc[n][m];
+    for (int j = 0; j < S::kXLoads; ++j) {
+      const int i = b + S::x_row(lane, j);
+      const int t = __shfl(token_of, i & 63);
+      s.set_row(lane, j, i < rows ? static_cast<uint32_t>(t * p.x_rs) * 2 : kNowhere);
+    }
+    s.split_k(lane, wave, kExpertWaves);
     __syncthreads();
-    if (wave >= MT) continue;
-    v4f g = part[0][wave][lane], u = part[0][MT + wave][lane];
+    part[(2 * wave) * 64 + lane] = s.acc[0][0], part[(2 * wave + 1) * 64 + lane] = s.acc[1][0];
+    __syncthreads();
+    if (wave != 0) continue;
+    v4f g = part[lane], u = part[64 + lane];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) g += part[w][wave][lane], u += part[w][MT + wave][lane];
+    for (int w = 1; w < kExpertWaves; ++w) g += part[2 * w * 64 + lane], u += part[(2 * w + 1) * 64 + lane];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = b + 16 * wave + 4 * q + r;
-      const int token = __shfl(token_of, i & 63);
-      const int slot = __shfl(first, token);
-      const float v = gated(g[r], u[r]) * __shfl(weight, token);
-      if (i >= rows) continue;
+      const int i = b + 4 * q + r;
+      const int t = __shfl(token_of, i & 63);
+      const int slot = __shfl(first, t);
+      const float v = gated(g[r], u[r]) * __shfl(weight, t);
+      if (4 * q + r >= R || i >= rows) continue;
       const __bf16 hi = static_cast<__bf16>(v);
       const float f = static_cast<float>(hi);
       const __bf16 lo = static_cast<__bf16>(fabsf(f) == __builtin_inff() ? 0.f : v - f);
@@ -408,12 +463,15 @@ __global__ void __launch_bounds__(64 * kFewWaves) experts_up_kernel(const Expert
   }
 }
 
-// A workgroup takes 16 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than 8 MT tokens, by chunks
-// of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
-template <int TO, int W, int MT>
-__global__ void __launch_bounds__(64 * kFewWaves) experts_down_kernel(const ExpertArgs p) {
-  typedef Few<kInBf16, W> F;
-  extern __shared__ __attribute__((aligned(16))) char dynamic[];  // [waves][T][16] sums
+// A workgroup takes 16 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
+// chunks of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
+// The 2 TOKENS rows of x are the numbers of the tokens and behind them their rests.
+template <int TO, int W, int TOKENS, bool RAGGED>
+__global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const ExpertArgs p) {
+  constexpr int R = 2 * TOKENS;
+  typedef ExpertShape<W, R, 1> Shape;
+  typedef Stream<kInBf16, W, R, 1, Shape::kDepth, RAGGED> S;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // the rings, behind them [waves][T][16] sums, behind those the slots of the entries' rows
   __shared__ int count[kFewExperts];
   __shared__ int16_t ids[kFewTopk][kFewTokens];
   __shared__ int32_t entry[kFewTokens * kFewTopk];  // expert, pass << 16
@@ -421,9 +479,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) experts_down_kernel(const Expe
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int slots = p.T * p.topk;
-  constexpr int kThreads = 64 * kFewWaves;
+  constexpr int kThreads = 64 * kExpertWaves;
+  float* const all = reinterpret_cast<float*>(lds + Shape::kRing);
+  float* const sums = all + wave * p.T * 16;
+  int16_t* const row_slot = reinterpret_cast<int16_t*>(all + kExpertWaves * p.T * 16);  // [entries][TOKENS], -1: none
   for (int i = tid; i < p.E; i += kThreads) count[i] = 0;
-  float* const sums = reinterpret_cast<float*>(dynamic) + wave * p.T * 16;
   for (int i = lane; i < p.T * 16; i += 64) sums[i] = 0.f;
   __syncthreads();
   for (int s = tid; s < slots; s += kThreads) {
@@ -436,7 +496,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) experts_down_kernel(const Expe
     // a token that names an expert twice counts twice here: at most an entry without rows
     int before = 0;
     for (int e0 = 0; e0 < p.E; e0 += 64) {
-      const int passes = e0 + lane < p.E ? (count[e0 + lane] + 8 * MT - 1) / (8 * MT) : 0;
+      const int passes = e0 + lane < p.E ? (count[e0 + lane] + TOKENS - 1) / TOKENS : 0;
       int upto = passes;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
@@ -449,107 +509,103 @@ __global__ void __launch_bounds__(64 * kFewWaves) experts_down_kernel(const Expe
     if (lane == 0) entries = before;
   }
   __syncthreads();
-  const int n0 = blockIdx.x * 16;
-  const int chunks = (p.I + F::kCols - 1) / F::kCols;
-  const int total = __builtin_amdgcn_readfirstlane(entries) * chunks;
-  const int each = (total + kFewWaves - 1) / kFewWaves;
-  const int start = min(total, wave * each), end = min(total, start + each);
-  const uint32_t rest = static_cast<uint32_t>(slots) * p.I * 2;
-  const auto x_src = make_rsrc(p.act, 2 * rest);
-
-  struct Chunk {
-    typename F::Weights w[1];
-    v4i x[MT][F::kSteps];
-  };
-  v4f acc[1][MT];
+  // the rows of every entry, by the waves in turn
+  const int count_of_entries = __builtin_amdgcn_readfirstlane(entries);
+  for (int i = wave; i < count_of_entries; i += kExpertWaves) {
+    const int en = __builtin_amdgcn_readfirstlane(entry[i]), e = en & 0xffff;
+    int slot = -1;
+    for (int j0 = 0; j0 < p.topk; j0 += 8) {
+      int named[8];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[0][m] = v4f{0.f, 0.f, 0.f, 0.f};
-  // the rows of the entry whose chunks are being asked for
-  uint32_t x_off[MT];
-  const uint8_t *w_q = p.down.q, *w_s = static_cast<const uint8_t*>(p.down.s);
-  auto tokens_of = [&](int en, int& slot_of) {  // the lane's token's slot; the tokens' mask
-    const int e = en & 0xffff;
-    slot_of = -1;
-    for (int j = p.topk - 1; j >= 0; --j)
-      if (lane < p.T && ids[j][lane] == e) slot_of = lane * p.topk + j;
-    return __ballot(slot_of >= 0);
-  };
-  auto point_at = [&](int i) {
-    const int en = __builtin_amdgcn_readfirstlane(entry[i]);
-    int slot_of;
-    const uint64_t mask = tokens_of(en, slot_of);
-    const int rows = __popcll(mask), token_of = nth_lane(mask, lane), first = (en >> 16) * 8 * MT;
+      for (int j = 0; j < 8; ++j) named[j] = ids[min(j0 + j, p.topk - 1)][lane];
+      int at = -1;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int r = first + 8 * m + (l16 & 7);
-      const int slot = __shfl(slot_of, __shfl(token_of, r & 63));
-      x_off[m] = r < rows ? static_cast<uint32_t>(slot) * p.I * 2 + (l16 >> 3) * rest : kNowhere;
+      for (int j = 7; j >= 0; --j) at = named[j] == e && j0 + j < p.topk ? j0 + j : at;
+      if (slot < 0 && at >= 0) slot = lane * p.topk + at;
     }
-    w_q = p.down.q + (en & 0xffff) * p.down_q, w_s = static_cast<const uint8_t*>(p.down.s) + (en & 0xffff) * p.down_s;
-  };
-  int l_entry = start / max(chunks, 1), l_chunk = start - l_entry * chunks, l_left = end - start;
-  if (l_left > 0) point_at(l_entry);
-  auto load_next = [&](Chunk& k) {
-    const bool in = l_left > 0;
-    const typename F::Tile tile(Matrix{w_q, w_s, p.H, p.I}, n0);
-    F::load(tile, p.I, l_chunk, in, q, l16, k.w[0]);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < F::kSteps; ++i) {
-        const int col = l_chunk * F::kCols + F::column(q, i);
-        k.x[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(x_src, in && x_off[m] != kNowhere && col < p.I ? x_off[m] + 2 * col : kNowhere, 0, 0));
-      }
-    if (--l_left > 0 && ++l_chunk == chunks) l_chunk = 0, point_at(++l_entry);
-  };
-  int m_entry = l_entry, m_chunk = l_chunk, m_left = l_left;
-  // the sums of an entry's rows go to their tokens
-  auto leave = [&](int i) {
-    const int en = __builtin_amdgcn_readfirstlane(entry[i]);
-    int slot_of;
-    const uint64_t mask = tokens_of(en, slot_of);
-    const int rows = __popcll(mask), token_of = nth_lane(mask, lane), first = (en >> 16) * 8 * MT;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = acc[0][m][r] + __shfl_xor(acc[0][m][r], 32);  // a token's numbers and what they left
-        const int i = first + 8 * m + (4 * q + r & 7);
-        const int token = __shfl(token_of, i & 63);
-        if (q < 2 && i < rows) sums[token * 16 + l16] += v;
-        acc[0][m][r] = 0.f;
-      }
-  };
-  auto multiply = [&](Chunk& k) {
-    F::template multiply<MT>(k.w[0], k.x, acc[0]);
-    if (m_left > 0 && (--m_left == 0 || ++m_chunk == chunks)) {
-      leave(m_entry);
-      m_chunk = 0, ++m_entry;
-    }
-  };
-  if (start < end) {
-    Chunk even, odd;
-    load_next(even);
-    for (int i = start; i < end; i += 2) {
-      load_next(odd);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(even);
-      __builtin_amdgcn_sched_barrier(0);
-      load_next(even);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(odd);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    if (lane >= p.T) slot = -1;
+    const uint64_t mask = __ballot(slot >= 0);
+    // row of the lane's token in this pass; rows without one behind the last
+    const int row = __popcll(mask & ((uint64_t{1} << lane) - 1)) - (en >> 16) * TOKENS, rows = __popcll(mask) - (en >> 16) * TOKENS;
+    if (slot >= 0 && row >= 0 && row < TOKENS) row_slot[i * TOKENS + row] = static_cast<int16_t>(slot);
+    if (lane < TOKENS && lane >= rows) row_slot[i * TOKENS + lane] = -1;
   }
   __syncthreads();
-  const float* const all = reinterpret_cast<const float*>(dynamic);
+  const int n0 = blockIdx.x * 16;
+  const uint32_t rest = static_cast<uint32_t>(slots) * p.I * 2;
+  S s(lds, wave, lane, p.I, p.act, 2 * rest);
+  const int total = count_of_entries * s.chunks, each = (total + kExpertWaves - 1) / kExpertWaves;
+  const int start = min(total, wave * each), end = min(total, start + each);
+  auto point_at = [&](int i) {
+    const int e = __builtin_amdgcn_readfirstlane(entry[i]) & 0xffff;
+#pragma unroll
+    for (int j = 0; j < S::kXLoads; ++j) {
+      const int r = S::x_row(lane, j), slot = row_slot[i * TOKENS + r % TOKENS];
+      s.set_row(lane, j, slot >= 0 ? static_cast<uint32_t>(slot) * p.I * 2 + (r / TOKENS) * rest : kNowhere);
+    }
+    s.tile[0].point_at(of_expert(p.down, p.down_q, p.down_s, e), n0);
+  };
+  // the chunk that is asked for next, and the one that is multiplied next
+  int l_entry = start / s.chunks, l_chunk = start - l_entry * s.chunks, l_left = end - start;
+  int m_entry = l_entry, m_chunk = l_chunk, m_left = l_left;
+  auto load_next = [&](int d) {
+    s.load(d, lane, l_chunk, l_left > 0);
+    if (--l_left > 0 && ++l_chunk == s.chunks) l_chunk = 0, point_at(++l_entry);
+  };
+  // the sums of an entry's rows go to their tokens
+  auto leave = [&](int i) {
+    v4f& a = s.acc[0][0];
+    const int at = i * TOKENS;
+    if (TOKENS == 2) {
+      if (q == 0)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (row_slot[at + r] >= 0) sums[row_slot[at + r] / p.topk * 16 + l16] += a[r] + a[r + 2];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = a[r] + __shfl_xor(a[r], TOKENS == 4 ? 16 : 32);  // a token's number and what it left
+        const int row = 4 * q + r;
+        if (row < TOKENS && row_slot[at + row] >= 0) sums[row_slot[at + row] / p.topk * 16 + l16] += v;
+      }
+    }
+    a = v4f{0.f, 0.f, 0.f, 0.f};
+  };
+  if (start < end) {
+    point_at(l_entry);
+#pragma unroll
+    for (int d = 0; d < Shape::kDepth; ++d) {
+      load_next(d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int i = start; i < end; i += Shape::kDepth) {
+#pragma unroll
+      for (int d = 0; d < Shape::kDepth; ++d) {
+        s.multiply(d);
+        if (m_left > 0 && (--m_left == 0 || ++m_chunk == s.chunks)) {
+          leave(m_entry);
+          m_chunk = 0, ++m_entry;
+        }
+        load_next(d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends
+  }
+  __syncthreads();
   for (int i = tid; i < p.T * 16; i += kThreads) {
     float v = all[i];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) v += all[w * p.T * 16 + i];
+    for (int w = 1; w < kExpertWaves; ++w) v += all[w * p.T * 16 + i];
     const int t = i >> 4, col = n0 + (i & 15);
     if (col < p.H) store1(p.out, TO, static_cast<int64_t>(t) * p.H + col, v);
   }
+}
+
+// LDS of experts_down_kernel: an expert's tokens over TOKENS, rounded up, adds up to no more entries than slots, and than experts and a TOKENS-th of them.
+constexpr int64_t experts_down_lds(int64_t ring, int64_t tokens, int64_t topk, int64_t experts, int64_t a_pass) {
+  const int64_t slots = tokens * topk, most = experts + slots / a_pass, entries = slots < most ? slots : most;
+  return ring + kExpertWaves * tokens * 16 * 4 + entries * a_pass * 2;
 }
 
 }  // namespace dlb

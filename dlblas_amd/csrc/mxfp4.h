@@ -252,9 +252,14 @@ typedef __attribute__((address_space(3))) void* mx_lds_ptr;
 typedef __attribute__((address_space(3))) uint8_t* mx_lds_bytes;
 
 // Lane i moves 16 bytes to `to` + 16 i.
-template <class LdsPtr>
+template <int POLICY, class LdsPtr>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t src, LdsPtr to, uint32_t voff, uint32_t soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (mx_lds_ptr)to, 16, voff, soff, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (mx_lds_ptr)to, 16, voff, soff, 0, POLICY);
+}
+// ... 4 bytes to `to` + 4 i.
+template <class LdsPtr>
+__device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t src, LdsPtr to, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (mx_lds_ptr)to, 4, voff, soff, 0, 0);
 }
 
 template <class Tile>
@@ -296,10 +301,10 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
     const mx_lds_bytes to = lds + (k & 3) * Tile::STAGE;
 #pragma unroll
     for (int j = 0; j < Tile::A_INST; ++j)
-      load_to_lds(a_src, to + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : a_off[j], at);
+      load_to_lds<0>(a_src, to + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : a_off[j], at);
 #pragma unroll
     for (int j = 0; j < Tile::B_INST; ++j)
-      load_to_lds(b_src, to + BM * 64 + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : b_off[j], at);
+      load_to_lds<0>(b_src, to + BM * 64 + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : b_off[j], at);
   };
   // the scales of window w, 16 groups: those of the tile's rows, behind them those of its columns
   auto load_scales = [&](int w) {
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
       const int first = (j * Tile::WAVES + wave) * 64;
       const bool of_a = first < BM;
       const auto src = make_rsrc(of_a ? p.a_s + m0 * p.pitch : p.b_s + static_cast<int64_t>(n0) * p.pitch, in ? (of_a ? rows : cols) * p.pitch : 0);
-      load_to_lds(src, to + first * 16, ((of_a ? first : first - BM) + lane) * static_cast<uint32_t>(p.pitch), in ? 16 * w : 0);
+      load_to_lds<0>(src, to + first * 16, ((of_a ? first : first - BM) + lane) * static_cast<uint32_t>(p.pitch), in ? 16 * w : 0);
     }
   };
 
