@@ -111,7 +111,7 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (dtype != kInBf16 && dtype != kInF16) return fail(DLB_ERR_BAD_DTYPE, "dtype %d is not DLB_IN_BF16 / F16", dtype);
   if (M < 0 || N < 0 || K < 0) return fail(DLB_ERR_BAD_SHAPE, "negative dimension (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
   if (int rc = check_columns(K)) return rc;
-  if (M > 32 * 65535 || N > (1 << 27)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld / N=%lld beyond the supported range", (long long)M, (long long)N);
+  if (M > (1 << 21) || N > (1 << 23)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld / N=%lld beyond the supported range", (long long)M, (long long)N);
   if (M == 0 || N == 0) return DLB_OK;
   if (K == 0) return fail(DLB_ERR_BAD_SHAPE, "K=0: there is no product");
   if (!x || !q || !s || !y) return fail(DLB_ERR_NULL_POINTER, "x, q, s or y is NULL");
@@ -119,11 +119,13 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (misaligned(q, 16) || misaligned(x, 4) || x_row_stride % 2 != 0 || off_elements(y, dtype))
     return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte, rows of x 4-byte aligned, y to its elements");
   const FewArgs a{x, y, M, x_row_stride, Matrix{static_cast<const uint8_t*>(q), s, static_cast<int>(N), static_cast<int>(K)}};
-  const int rows = M <= 4 ? 4 : M <= 8 ? 8 : M <= 16 ? 16 : 32, nt = N >= 6400 ? 2 : 1;
-  const dim3 grid(static_cast<unsigned>(ceil_div(N, 16 * nt)), static_cast<unsigned>(ceil_div(M, rows)));
+  const int rows = M <= 4 ? 4 : M <= 8 ? 8 : 16, nt = N >= 6400 ? 2 : 1;
+  const int64_t tiles = ceil_div(N, 16 * nt);
+  if (ceil_div(tiles, 8) > 65535) return fail(DLB_ERR_BAD_SHAPE, "N=%lld beyond the supported range", (long long)N);
+  const dim3 grid(static_cast<unsigned>(8 * ceil_div(M, rows)), static_cast<unsigned>(ceil_div(tiles, 8)));
   with_flag(dtype == kInBf16, [&](auto bf16) {
     with_flag(K % 128 != 0, [&](auto ragged) {
-      with_chunks<4, 8, 16, 32>(rows, [&](auto r) {
+      with_chunks<4, 8, 16>(rows, [&](auto r) {
         with_chunks<1, 2>(nt, [&](auto n) {
           typedef FewShape<kE2m1, r(), n()> Shape;
           hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n(), ragged()>), grid, dim3(64 * Shape::kWaves), Shape::kLds,
@@ -183,17 +185,17 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   a.ids_is64 = ids_dtype == DLB_IDX_I64;
   const int64_t slots = tokens * topk;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(H / 16));
+  const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(ceil_div(H, 16 * kDownTiles)));
   // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches.
   const int64_t mean = slots / std::min(experts, slots);
   const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16, down_tokens = tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
   const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
-      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), up_grid, dim3(64 * kExpertWaves), (ExpertShape<kw(), r(), 2>::kRing), st, a);
+      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), up_grid, dim3(64 * kUpWaves), (UpShape<kw(), r()>::kLds), st, a);
     });
     with_chunks<2, 4, 8>(down_tokens, [&](auto t) {
-      const int64_t lds = experts_down_lds(ExpertShape<kw(), 2 * t(), 1>::kRing, tokens, topk, experts, t());
-      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), ragged_down()>), down_grid, dim3(64 * kExpertWaves), static_cast<size_t>(lds), st, a);
+      const int64_t lds = experts_down_lds<kw(), t()>(tokens, topk, experts);
+      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), ragged_down()>), down_grid, dim3(64 * (DownShape<kw(), t()>::kWaves)), static_cast<size_t>(lds), st, a);
     });
   };
   with_flag(dtype == kInBf16, [&](auto bf16) {

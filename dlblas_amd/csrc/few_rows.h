@@ -71,28 +71,34 @@ struct Matrix {
   int N, K;
 };
 
-// A wave's own stream: chunks of 128 columns of NT tiles of 16 weight rows and of R rows of x come into a ring of DEPTH chunks in LDS that no other
-// wave reads, so nothing but the wave's own counter of loads is waited for.  They go through LDS because of the order of the lanes: an MFMA wants
-// neighbouring rows in neighbouring lanes, and loaded that way every lane touches a cache line of its own, 64 a load, which held 32 experts x 4
-// rows x 4096 x 7168 e4m3 at 250 us however much was on its way.  Here four to sixteen lanes share a row.
+// A wave's own stream: chunks of 128 bytes of each row of NT tiles of 16 weight rows, and of R rows of x, come into a ring of DEPTH chunks in LDS that
+// no other wave reads, so nothing but the wave's own counter of loads is waited for.  They go through LDS because of the order of the lanes: an MFMA
+// wants neighbouring rows in neighbouring lanes, and loaded that way every lane touches a cache line of its own, 64 a load, which held 32 experts x 4
+// rows x 4096 x 7168 e4m3 at 250 us however much was on its way.  Here eight lanes share a line, and all of it is asked for at once: chunks of half a line
+// of e2m1 150 us, and the products themselves cost nothing of that.
 //
-// A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of e4m3
-// piece ^ (row / 2), of e2m1 piece ^ (row / 4).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a
-// word of its 16 bytes a quarter.  RAGGED: e2m1, K is no multiple of 128.
-constexpr int stream_tile(int weights) { return (weights == kE4m3 ? 2048 : 1024) + 256; }
-constexpr int stream_loads(int weights, int R, int NT, bool ragged) { return NT * ((weights == kE4m3 ? 2 : 1) + (ragged ? 0 : 1)) + R / 4; }
-constexpr int stream_bytes(int weights, int R, int NT) { return NT * stream_tile(weights) + R * 256; }
+// A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of weights
+// piece ^ (row / 2).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a word of its 16 bytes a
+// quarter.  RAGGED: e2m1, K is no multiple of 128.
+constexpr int stream_columns(int weights) { return weights == kE4m3 ? 128 : 256; }
+constexpr int kStreamTile = 2048 + 256;  // bytes of a tile's chunk: codes, and behind them scales
+constexpr int stream_x_loads(int weights, int R) { return R * stream_columns(weights) / 512; }
+constexpr int stream_bytes(int weights, int R, int NT) { return NT * kStreamTile + R * stream_columns(weights) * 2; }
+// Chunks of a ring of `waves` waves in `bytes` of LDS.
+constexpr int stream_depth(int weights, int R, int NT, int waves, int bytes) {
+  const int depth = bytes / (waves * stream_bytes(weights, R, NT));
+  return depth > 6 ? 6 : depth;
+}
 
 template <int T, int W, int R, int NT, int DEPTH, bool RAGGED>
 struct Stream {
-  static constexpr int kCols = 128, kMT = (R + 15) / 16;
-  static constexpr int kTile = stream_tile(W), kX = R * 256;  // bytes of a chunk; a tile's scales are behind its codes
-  static constexpr int kChunk = NT * kTile + kX, kBytes = DEPTH * kChunk;
-  static constexpr int kXLoads = R / 4;
+  static constexpr int kCols = stream_columns(W), kSteps = kCols / 32;
+  static constexpr int kXPitch = 2 * kCols, kXLoads = stream_x_loads(W, R), kXLanes = kXPitch / 16;  // lanes of a load that share a row of x
+  static constexpr int kChunk = stream_bytes(W, R, NT), kBytes = DEPTH * kChunk;
   // Loads of a chunk into LDS, which is what is counted.  RAGGED scales come to registers, a byte a load: the compiler may issue those later than
   // they are written, and a wait that counted them would end too early.
-  static constexpr int kLoads = stream_loads(W, R, NT, RAGGED);
-  static_assert((R == 4 || R == 8 || R == 16 || R == 32) && (DEPTH - 1) * kLoads < 64 && !(RAGGED && W == kE4m3), "whole loads of x, a counter of six bits");
+  static constexpr int kLoads = NT * (RAGGED ? 2 : 3) + kXLoads;
+  static_assert((R == 4 || R == 8 || R == 16) && DEPTH >= 2 && (DEPTH - 1) * kLoads < 64 && !(RAGGED && W == kE4m3), "whole loads of x, a counter of six bits");
 
   // 16 rows of a matrix, from row n0 on.
   struct Tile {
@@ -112,7 +118,7 @@ struct Stream {
 
   const uint8_t* ring;  // this wave's
   mx_lds_bytes ring_to;
-  int K, chunks;
+  int K, chunks, row_bytes;
   const uint8_t* x;
   uint32_t x_bytes;
   uint32_t w_at, s_at;  // where a lane starts in a tile, and in its scales
@@ -120,122 +126,105 @@ struct Stream {
   int q, l16;
   uint32_t x_at[kXLoads];  // its row of x of each load with its piece; past the end of every buffer: none
   Tile tile[NT];
-  uint32_t scales[RAGGED ? DEPTH : 1][NT][4];  // RAGGED
-  v4f acc[NT][kMT];
+  uint32_t scales[RAGGED ? DEPTH : 1][NT][2];  // RAGGED
+  v4f acc[NT];
 
   __device__ __forceinline__ Stream(uint8_t* lds, int wave, int lane, int columns, const void* x_base, uint32_t bytes)
-      : ring(lds + wave * kBytes), ring_to((mx_lds_bytes)lds + wave * kBytes), K(columns), chunks((columns + kCols - 1) / kCols),
+      : ring(lds + wave * kBytes), ring_to((mx_lds_bytes)lds + wave * kBytes), K(columns), chunks((columns + kCols - 1) / kCols), row_bytes(W == kE4m3 ? columns : columns / 2),
         x(in_scalar(static_cast<const uint8_t*>(x_base))), x_bytes(in_scalar(bytes)), q(lane >> 4), l16(lane & 15) {
-    if (W == kE4m3) {
-      const int row = lane >> 3;
-      w_at = row * K + ((lane & 7) ^ (row >> 1)) * 16, s_at = 0;
-      w_from = l16 * 128 + ((q ^ (l16 >> 1)) & 7) * 16;
-      x_from = (2 * q) * 16;
-    } else {
-      const int row = lane >> 2;
-      w_at = row * (K / 2) + ((lane & 3) ^ (row >> 2)) * 16;
-      s_at = q == 0 ? l16 * (K / kMxGroup) : kNowhere;  // one quarter asks
-      w_from = l16 * 64 + (l16 >> 2) * 16 + 4 * q;
-      x_from = q * 16;
-    }
-    x_from = (l16 & (R - 1)) * 256 + (x_from ^ (l16 & (R - 1) & 15) * 16);
+    const int row = lane >> 3, x_row16 = l16 & (R - 1);
+    w_at = row * row_bytes + ((lane & 7) ^ (row >> 1)) * 16;
+    w_from = l16 * 128 + (W == kE4m3 ? ((q ^ (l16 >> 1)) & 7) * 16 : (l16 >> 1) * 16 + 4 * q);
+    x_from = x_row16 * kXPitch + ((W == kE4m3 ? 2 * q : q) ^ x_row16) * 16;
+    if (W == kE4m3)
+      s_at = 0;
+    else if (RAGGED)
+      s_at = l16 * (K / kMxGroup) + 2 * q;
+    else
+      s_at = lane < 32 ? (lane >> 1) * (K / kMxGroup) + 4 * (lane & 1) : kNowhere;  // eight scales a row
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int m = 0; m < kMT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   // Row of x that load j brings for a lane, and the lane's column there.
-  static __device__ __forceinline__ int x_row(int lane, int j) { return 4 * j + (lane >> 4); }
-  static __device__ __forceinline__ int x_column(int lane, int j) { return ((lane & 15) ^ (x_row(lane, j) & 15)) * 8; }
+  static __device__ __forceinline__ int x_row(int lane, int j) { return 64 / kXLanes * j + lane / kXLanes; }
+  static __device__ __forceinline__ int x_column(int lane, int j) { return (lane % kXLanes ^ (x_row(lane, j) & 15)) * 8; }
   // at: byte of that row, kNowhere: none
   __device__ __forceinline__ void set_row(int lane, int j, uint32_t at) { x_at[j] = at == kNowhere ? kNowhere : at + 2 * x_column(lane, j); }
 
   // Chunk c into place d; `in` false (the same for the wave): nothing is brought.  Loads are issued either way.
   __device__ __forceinline__ void load(int d, int lane, int c, bool in) {
     const mx_lds_bytes to = ring_to + d * kChunk;
-    const uint32_t at = in ? static_cast<uint32_t>(c) * (W == kE4m3 ? 128 : 64) : 0;
+    const uint32_t at = in ? static_cast<uint32_t>(c) * 128 : 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       // Past the end of a row of e2m1 a lane brings the next one's codes, which meet zeros of x; the scales there are zeros too, which are numbers.
       const auto src = make_rsrc(tile[n].q, in ? tile[n].q_bytes : 0);
-      load_to_lds<2>(src, to + n * kTile, w_at, at);
-      // eight rows further on row / 2 has another third bit: the other half of the row
-      if (W == kE4m3) load_to_lds<2>(src, to + n * kTile + 1024, (w_at ^ 64) + 8 * K, at);
-      if (!RAGGED) {
-        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kTile + kTile - 256, s_at, in ? 4 * c : 0);
-        continue;
-      }
+      load_to_lds<2>(src, to + n * kStreamTile, w_at, at);
+      // eight rows further on row / 2 has another third bit: the other half of the chunk
+      const uint32_t half = ((lane & 7) ^ (lane >> 4)) < 4 ? 64u : -64u;
+      load_to_lds<2>(src, to + n * kStreamTile + 1024, w_at + half + 8 * row_bytes, at);
+      if (W == kE4m3) {
+        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kStreamTile + 2048, s_at, in ? 4 * c : 0);
+      } else if (!RAGGED) {
+        const bool there = 8 * c + 4 * (lane & 1) < K / kMxGroup;
+        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kStreamTile + 2048, there ? s_at : kNowhere, in ? 8 * c : 0);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        scales[d][n][i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(tile[n].s, in && 4 * c + i < K / kMxGroup ? tile[n].s_bytes : 0), s_at + i, in ? 4 * c : 0, 0);
+        for (int i = 0; i < 2; ++i) {
+          const bool there = 8 * c + 2 * q + i < K / kMxGroup;
+          scales[d][n][i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), there ? s_at + i : kNowhere, in ? 8 * c : 0, 0);
+        }
+      }
     }
 #pragma unroll
     for (int j = 0; j < kXLoads; ++j) {
-      const bool there = !RAGGED || c * kCols + x_column(lane, j) < K;
-      load_to_lds<0>(make_rsrc(x, in ? x_bytes : 0), to + NT * kTile + j * 1024, there ? x_at[j] : kNowhere, in ? static_cast<uint32_t>(c) * (2 * kCols) : 0);
+      const bool there = W == kE4m3 || c * kCols + x_column(lane, j) < K;
+      load_to_lds<0>(make_rsrc(x, in ? x_bytes : 0), to + NT * kStreamTile + j * 1024, there ? x_at[j] : kNowhere, in ? static_cast<uint32_t>(c) * kXPitch : 0);
     }
   }
 
-  // The chunk in place d, behind which there are DEPTH - 1 others, times its rows: lane l of acc[n][m] has rows 4 (l / 16) + r, column l % 16.
+  // The chunk in place d, behind which there are DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16.
   __device__ __forceinline__ void multiply(int d) {
     wait_loads<(DEPTH - 1) * kLoads>();  // in order
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const uint8_t* const from = ring + d * kChunk;
-    v4i xf[kMT][4];
+    const uint8_t* const from = ring + d * kChunk;  // what is ^ed below is within what a row has of a chunk
+    v4i xf[kSteps];
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xf[m][i] = *reinterpret_cast<const v4i*>(from + NT * kTile + m * 4096 + (x_from ^ (W == kE4m3 ? 128 * (i >> 1) + 16 * (i & 1) : 64 * i)));
+    for (int i = 0; i < kSteps; ++i) xf[i] = *reinterpret_cast<const v4i*>(from + NT * kStreamTile + (x_from ^ (W == kE4m3 ? 128 * (i >> 1) + 16 * (i & 1) : 64 * i)));
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      const uint8_t* const codes = from + n * kStreamTile;
       if (W == kE4m3) {
-        v4f sum[kMT];
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) sum[m] = v4f{0.f, 0.f, 0.f, 0.f};
+        v4f sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const v4i v = *reinterpret_cast<const v4i*>(from + n * kTile + (w_from ^ 64 * u));
+          const v4i v = *reinterpret_cast<const v4i*>(codes + (w_from ^ 64 * u));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const v4i f = from_e4m3<T>(v[2 * i], v[2 * i + 1]);
-#pragma unroll
-            for (int m = 0; m < kMT; ++m) sum[m] = mfma_16x16x32<T>(xf[m][2 * u + i], f, sum[m]);
-          }
+          for (int i = 0; i < 2; ++i) sum = mfma_16x16x32<T>(xf[2 * u + i], from_e4m3<T>(v[2 * i], v[2 * i + 1]), sum);
         }
-        const float s = *reinterpret_cast<const float*>(from + n * kTile + kTile - 256);
+        const float s = *reinterpret_cast<const float*>(codes + 2048);
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s, sum[m][r], acc[n][m][r]);
+        for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, sum[r], acc[n][r]);
         continue;
       }
-      // each quarter makes one of the four scales of its rows, for all of them
-      uint32_t four, by_group[4];
-      if (RAGGED) {
-        four = scales[d][n][0];
+      // each quarter makes two of the eight scales of its rows, for all of them: groups 2 i + u
+      uint32_t by_group[2][4];
+      const uint32_t two = RAGGED ? 0u : *reinterpret_cast<const uint16_t*>(codes + 2048 + 8 * l16 + 2 * q);
 #pragma unroll
-        for (int i = 1; i < 4; ++i) four |= scales[d][n][i] << (8 * i);
-        spread_quarters(four, by_group);
-        four = by_group[0];
-      } else {
-        four = *reinterpret_cast<const uint32_t*>(from + n * kTile + kTile - 256 + 4 * l16);
-      }
-      spread_quarters(__float_as_uint(mx_scale(four >> (8 * q) & 0xffu)), by_group);
+      for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(RAGGED ? scales[d][n][u] : u == 0 ? two & 0xffu : two >> 8)), by_group[u]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float scale = __uint_as_float(by_group[i]);
-        const v4i f = from_e2m1<T>(*reinterpret_cast<const int*>(from + n * kTile + (w_from ^ 16 * i)), T == kInBf16 ? scale : 1.0f);
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          if (T == kInBf16) {
-            acc[n][m] = mfma_16x16x32<T>(xf[m][i], f, acc[n][m]);
-            continue;
-          }
-          const v4f sum = mfma_16x16x32<T>(xf[m][i], f, v4f{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(scale, sum[r], acc[n][m][r]);
+      for (int i = 0; i < kSteps; ++i) {
+        const float scale = __uint_as_float(by_group[i & 1][i >> 1 & 3]);
+        const v4i f = from_e2m1<T>(*reinterpret_cast<const int*>(codes + (w_from ^ 16 * i)), T == kInBf16 ? scale : 1.0f);
+        if (T == kInBf16) {
+          acc[n] = mfma_16x16x32<T>(xf[i], f, acc[n]);
+          continue;
         }
+        const v4f sum = mfma_16x16x32<T>(xf[i], f, v4f{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(scale, sum[r], acc[n][r]);
+        __builtin_amdgcn_sched_barrier(0);  // the sums of all steps would not fit the registers
       }
     }
     // what is read of this place has arrived before its next chunk is asked for
@@ -264,12 +253,6 @@ struct Stream {
   }
 };
 
-// Chunks in a wave's ring: as many as leave room for `groups` workgroups on a CU.
-constexpr int stream_depth(int weights, int R, int NT, int waves, int groups) {
-  const int depth = (160 * 1024 / groups - 8192) / (waves * stream_bytes(weights, R, NT));
-  return depth > 6 ? 6 : depth;
-}
-
 __device__ __forceinline__ void store1(void* to, int type, int64_t at, float v) {
   if (type == kInBf16)
     static_cast<__bf16*>(to)[at] = static_cast<__bf16>(v);
@@ -290,23 +273,24 @@ struct FewArgs {
 
 template <int W, int R, int NT>
 struct FewShape {
-  static constexpr int kWaves = R == 32 ? 4 : 8, kDepth = stream_depth(W, R, NT, kWaves, 1);
-  static constexpr int kRing = kWaves * kDepth * stream_bytes(W, R, NT);
-  static constexpr int kParts = kWaves * NT * ((R + 15) / 16) * 1024;
-  static constexpr int kLds = kRing > kParts ? kRing : kParts;
+  static constexpr int kBudget = 156 * 1024, kWaves = 8 * 2 * stream_bytes(W, R, NT) <= kBudget ? 8 : 4, kDepth = stream_depth(W, R, NT, kWaves, kBudget);
+  static constexpr int kLds = kWaves * kDepth * stream_bytes(W, R, NT);
+  static_assert(kLds >= kWaves * NT * 1024, "room for the waves' sums");
 };
 
-// R rows of x against 16 NT rows of the matrix.
+// R rows of x against 16 NT rows of the matrix.  blockIdx.y: eight column tiles, one for each XCD, blockIdx.x: those tiles by the blocks of R rows, so that the
+// workgroups that share weights run beside each other on one XCD.
 template <int T, int W, int R, int NT, bool RAGGED>
 __global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_kernel(const FewArgs p) {
   typedef FewShape<W, R, NT> Shape;
   typedef Stream<T, W, R, NT, Shape::kDepth, RAGGED> S;
-  constexpr int kWaves = Shape::kWaves, kMT = S::kMT;
+  constexpr int kWaves = Shape::kWaves;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
-  const int n0 = blockIdx.x * 16 * NT;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * R;
+  const int n0 = (blockIdx.y * 8 + blockIdx.x % 8) * 16 * NT;
+  if (n0 >= p.w.N) return;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.x / 8) * R;
   const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(R)));
   const uint32_t pitch = static_cast<uint32_t>(p.x_rs) * 2;
   S s(lds, wave, lane, p.w.K, static_cast<const uint8_t*>(p.x) + m0 * p.x_rs * 2, (rows - 1) * pitch + 2 * p.w.K);
@@ -316,22 +300,19 @@ __global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_ke
   for (int j = 0; j < S::kXLoads; ++j) s.set_row(lane, j, S::x_row(lane, j) < rows ? S::x_row(lane, j) * pitch : kNowhere);
   s.split_k(lane, wave, kWaves);
   __syncthreads();
-  v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][NT kMT][64]
+  v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][NT][64]
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int m = 0; m < kMT; ++m) part[(wave * NT * kMT + n * kMT + m) * 64 + lane] = s.acc[n][m];
+  for (int n = 0; n < NT; ++n) part[(wave * NT + n) * 64 + lane] = s.acc[n];
   __syncthreads();
-  for (int i = wave; i < NT * kMT; i += kWaves) {
-    v4f sum = part[i * 64 + lane];
+  if (wave >= NT) return;
+  v4f sum = part[wave * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += part[(w * NT * kMT + i) * 64 + lane];
-    const int n = i / kMT, m = i - n * kMT, col = n0 + 16 * n + l16;
+  for (int w = 1; w < kWaves; ++w) sum += part[(w * NT + wave) * 64 + lane];
+  const int col = n0 + 16 * wave + l16;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * m + 4 * q + r;
-      if (row < rows && col < p.w.N) store1(p.y, T, (m0 + row) * p.w.N + col, sum[r]);
-    }
+  for (int r = 0; r < 4; ++r) {
+    const int row = 4 * q + r;
+    if (row < rows && col < p.w.N) store1(p.y, T, (m0 + row) * p.w.N + col, sum[r]);
   }
 }
 
@@ -382,20 +363,25 @@ __device__ __forceinline__ int nth_lane(uint64_t mask, int lane) {
 // silu(g) u
 __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
-constexpr int kExpertWaves = 4;
+constexpr int kUpWaves = 4;
+template <int W, int R>
+struct UpShape {
+  static constexpr int kBudget = 2 * kUpWaves * stream_bytes(W, R, 2) <= 76 * 1024 ? 76 * 1024 : 152 * 1024;  // two workgroups a CU, or one
+  static constexpr int kDepth = stream_depth(W, R, 2, kUpWaves, kBudget), kLds = kUpWaves * kDepth * stream_bytes(W, R, 2);
+};
 
-template <int W, int R, int NT>
-struct ExpertShape {
-  static constexpr int kDepth = stream_depth(W, R, NT, kExpertWaves, 2);
-  static constexpr int kRing = kExpertWaves * kDepth * stream_bytes(W, R, NT);
+constexpr int kDownTiles = 2;
+template <int W, int TOKENS>
+struct DownShape {
+  static constexpr int kBudget = (TOKENS <= 4 ? 140 : 108) * 1024, kWaves = TOKENS <= 4 ? 8 : 4;  // beside it the sums of up to 64 tokens have to fit, of more than four by four waves
+  static constexpr int kDepth = stream_depth(W, 2 * TOKENS, kDownTiles, kWaves, kBudget), kRing = kWaves * kDepth * stream_bytes(W, 2 * TOKENS, kDownTiles);
 };
 
 // A workgroup takes 16 rows of Gate and the same of Up, of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
 // it is the first to name it; R of its tokens at a time.
 template <int T, int W, int R, bool RAGGED>
-__global__ void __launch_bounds__(64 * kExpertWaves) experts_up_kernel(const ExpertArgs p) {
-  typedef Stream<T, W, R, 2, ExpertShape<W, R, 2>::kDepth, RAGGED> S;
-  static_assert(S::kMT == 1, "the sums of a pass are a tile of Gate and one of Up");
+__global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertArgs p) {
+  typedef Stream<T, W, R, 2, UpShape<W, R>::kDepth, RAGGED> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
@@ -439,14 +425,14 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_up_kernel(const Exp
       const int t = __shfl(token_of, i & 63);
       s.set_row(lane, j, i < rows ? static_cast<uint32_t>(t * p.x_rs) * 2 : kNowhere);
     }
-    s.split_k(lane, wave, kExpertWaves);
+    s.split_k(lane, wave, kUpWaves);
     __syncthreads();
-    part[(2 * wave) * 64 + lane] = s.acc[0][0], part[(2 * wave + 1) * 64 + lane] = s.acc[1][0];
+    part[(2 * wave) * 64 + lane] = s.acc[0], part[(2 * wave + 1) * 64 + lane] = s.acc[1];
     __syncthreads();
     if (wave != 0) continue;
     v4f g = part[lane], u = part[64 + lane];
 #pragma unroll
-    for (int w = 1; w < kExpertWaves; ++w) g += part[2 * w * 64 + lane], u += part[(2 * w + 1) * 64 + lane];
+    for (int w = 1; w < kUpWaves; ++w) g += part[2 * w * 64 + lane], u += part[(2 * w + 1) * 64 + lane];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = b + 4 * q + r;
@@ -463,15 +449,16 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_up_kernel(const Exp
   }
 }
 
-// A workgroup takes 16 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
+// A workgroup takes 32 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
 // chunks of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
 // The 2 TOKENS rows of x are the numbers of the tokens and behind them their rests.
 template <int TO, int W, int TOKENS, bool RAGGED>
-__global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const ExpertArgs p) {
+__global__ void __launch_bounds__(64 * (DownShape<W, TOKENS>::kWaves)) experts_down_kernel(const ExpertArgs p) {
   constexpr int R = 2 * TOKENS;
-  typedef ExpertShape<W, R, 1> Shape;
-  typedef Stream<kInBf16, W, R, 1, Shape::kDepth, RAGGED> S;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // the rings, behind them [waves][T][16] sums, behind those the slots of the entries' rows
+  typedef DownShape<W, TOKENS> Shape;
+  typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth, RAGGED> S;
+  constexpr int kWaves = Shape::kWaves, kWide = 16 * kDownTiles;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // the rings, behind them [waves][T][kWide] sums, behind those the slots of the entries' rows
   __shared__ int count[kFewExperts];
   __shared__ int16_t ids[kFewTopk][kFewTokens];
   __shared__ int32_t entry[kFewTokens * kFewTopk];  // expert, pass << 16
@@ -479,12 +466,12 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int slots = p.T * p.topk;
-  constexpr int kThreads = 64 * kExpertWaves;
+  constexpr int kThreads = 64 * kWaves;
   float* const all = reinterpret_cast<float*>(lds + Shape::kRing);
-  float* const sums = all + wave * p.T * 16;
-  int16_t* const row_slot = reinterpret_cast<int16_t*>(all + kExpertWaves * p.T * 16);  // [entries][TOKENS], -1: none
+  float* const sums = all + wave * p.T * kWide;
+  int16_t* const row_slot = reinterpret_cast<int16_t*>(all + kWaves * p.T * kWide);  // [entries][TOKENS], -1: none
   for (int i = tid; i < p.E; i += kThreads) count[i] = 0;
-  for (int i = lane; i < p.T * 16; i += 64) sums[i] = 0.f;
+  for (int i = lane; i < p.T * kWide; i += 64) sums[i] = 0.f;
   __syncthreads();
   for (int s = tid; s < slots; s += kThreads) {
     const int t = s / p.topk, j = s - t * p.topk, e = expert_of(p, t, j);
@@ -511,7 +498,7 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
   __syncthreads();
   // the rows of every entry, by the waves in turn
   const int count_of_entries = __builtin_amdgcn_readfirstlane(entries);
-  for (int i = wave; i < count_of_entries; i += kExpertWaves) {
+  for (int i = wave; i < count_of_entries; i += kWaves) {
     const int en = __builtin_amdgcn_readfirstlane(entry[i]), e = en & 0xffff;
     int slot = -1;
     for (int j0 = 0; j0 < p.topk; j0 += 8) {
@@ -531,10 +518,10 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
     if (lane < TOKENS && lane >= rows) row_slot[i * TOKENS + lane] = -1;
   }
   __syncthreads();
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * kWide;
   const uint32_t rest = static_cast<uint32_t>(slots) * p.I * 2;
   S s(lds, wave, lane, p.I, p.act, 2 * rest);
-  const int total = count_of_entries * s.chunks, each = (total + kExpertWaves - 1) / kExpertWaves;
+  const int total = count_of_entries * s.chunks, each = (total + kWaves - 1) / kWaves;
   const int start = min(total, wave * each), end = min(total, start + each);
   auto point_at = [&](int i) {
     const int e = __builtin_amdgcn_readfirstlane(entry[i]) & 0xffff;
@@ -543,7 +530,8 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
       const int r = S::x_row(lane, j), slot = row_slot[i * TOKENS + r % TOKENS];
       s.set_row(lane, j, slot >= 0 ? static_cast<uint32_t>(slot) * p.I * 2 + (r / TOKENS) * rest : kNowhere);
     }
-    s.tile[0].point_at(of_expert(p.down, p.down_q, p.down_s, e), n0);
+#pragma unroll
+    for (int n = 0; n < kDownTiles; ++n) s.tile[n].point_at(of_expert(p.down, p.down_q, p.down_s, e), n0 + 16 * n);
   };
   // the chunk that is asked for next, and the one that is multiplied next
   int l_entry = start / s.chunks, l_chunk = start - l_entry * s.chunks, l_left = end - start;
@@ -554,22 +542,19 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
   };
   // the sums of an entry's rows go to their tokens
   auto leave = [&](int i) {
-    v4f& a = s.acc[0][0];
-    const int at = i * TOKENS;
-    if (TOKENS == 2) {
-      if (q == 0)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (row_slot[at + r] >= 0) sums[row_slot[at + r] / p.topk * 16 + l16] += a[r] + a[r + 2];
-    } else {
+    for (int n = 0; n < kDownTiles; ++n) {
+      v4f& a = s.acc[n];
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = a[r] + (TOKENS == 2 ? a[(r + 2) & 3] : __shfl_xor(a[r], TOKENS == 4 ? 16 : 32));  // a token's number and what it left
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float v = a[r] + __shfl_xor(a[r], TOKENS == 4 ? 16 : 32);  // a token's number and what it left
-        const int row = 4 * q + r;
-        if (row < TOKENS && row_slot[at + row] >= 0) sums[row_slot[at + row] / p.topk * 16 + l16] += v;
+        const int row = 4 * q + r, slot = row < TOKENS ? row_slot[i * TOKENS + row] : -1;
+        if (slot >= 0) sums[slot / p.topk * kWide + 16 * n + l16] += v[r];
       }
+      a = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    a = v4f{0.f, 0.f, 0.f, 0.f};
   };
   if (start < end) {
     point_at(l_entry);
@@ -593,19 +578,20 @@ __global__ void __launch_bounds__(64 * kExpertWaves) experts_down_kernel(const E
     wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends
   }
   __syncthreads();
-  for (int i = tid; i < p.T * 16; i += kThreads) {
+  for (int i = tid; i < p.T * kWide; i += kThreads) {
     float v = all[i];
 #pragma unroll
-    for (int w = 1; w < kExpertWaves; ++w) v += all[w * p.T * 16 + i];
-    const int t = i >> 4, col = n0 + (i & 15);
+    for (int w = 1; w < kWaves; ++w) v += all[w * p.T * kWide + i];
+    const int t = i / kWide, col = n0 + i % kWide;
     if (col < p.H) store1(p.out, TO, static_cast<int64_t>(t) * p.H + col, v);
   }
 }
 
 // LDS of experts_down_kernel: an expert's tokens over TOKENS, rounded up, adds up to no more entries than slots, and than experts and a TOKENS-th of them.
-constexpr int64_t experts_down_lds(int64_t ring, int64_t tokens, int64_t topk, int64_t experts, int64_t a_pass) {
-  const int64_t slots = tokens * topk, most = experts + slots / a_pass, entries = slots < most ? slots : most;
-  return ring + kExpertWaves * tokens * 16 * 4 + entries * a_pass * 2;
+template <int W, int TOKENS>
+int64_t experts_down_lds(int64_t tokens, int64_t topk, int64_t experts) {
+  const int64_t slots = tokens * topk, most = experts + slots / TOKENS, entries = slots < most ? slots : most;
+  return DownShape<W, TOKENS>::kRing + DownShape<W, TOKENS>::kWaves * tokens * 16 * kDownTiles * 4 + entries * TOKENS * 2;
 }
 
 }  // namespace dlb

@@ -47,7 +47,8 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
 
 /*
  * y[m, n] = sum over the groups g of 2^(s[n, g] - 127) sum_{k in g} x[m, k] q[n, k]; fp32 sums, one rounding at the end.  Beside bf16 rows weights
- * below 2^-126 in magnitude may count as zero.  Meant for up to a few dozen rows: the weights are read once per 32 of them.
+ * below 2^-126 in magnitude may count as zero.  Meant for up to a few dozen rows: the weights are read once per 16 of them,
+ * beside each other.
  *
  *   x [M, K]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
  *   q [N, K/2]   codes, 16-byte aligned;  s [N, K/32] scales
