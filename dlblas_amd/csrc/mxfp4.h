@@ -71,6 +71,11 @@ __device__ __forceinline__ v4f mfma_mx(const v4i& a, uint32_t a_s, const v4i& b,
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aw, bw, c, 4, 4, STEP, static_cast<int>(a_s), STEP, static_cast<int>(b_s));
 }
 
+// The same for a step that unrolling makes a constant.
+__device__ __forceinline__ v4f mfma_mx_step(int step, const v4i& a, uint32_t a_s, const v4i& b, uint32_t b_s, const v4f& c) {
+  return step == 0 ? mfma_mx<0>(a, a_s, b, b_s, c) : step == 1 ? mfma_mx<1>(a, a_s, b, b_s, c) : step == 2 ? mfma_mx<2>(a, a_s, b, b_s, c) : mfma_mx<3>(a, a_s, b, b_s, c);
+}
+
 struct MxArgs {
   const uint8_t* a;    // [M][K / 2]
   const uint8_t* b;    // [N][K / 2]
@@ -329,6 +334,15 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
+  // The scales of a row's 16 groups; a quarter's lane keeps those of its group of each of the four steps, a byte a step.
+  const uint32_t pick = 0x04000400u + 0x00010001u * (0x100u * q + q);  // bytes q, 4 + q
+  auto own_scales = [&](const uint8_t* row) {
+    const v4i v = *reinterpret_cast<const v4i*>(row);
+    const uint32_t low = __builtin_amdgcn_perm(v[1], v[0], pick), high = __builtin_amdgcn_perm(v[3], v[2], pick);
+    return __builtin_amdgcn_perm(high, low, 0x05040100u);
+  };
+  uint32_t as[MF], bs[NF];
+
   load_scales(0);
   load_stage(0), load_stage(1), load_stage(2);
   constexpr int kGroup = Tile::A_INST + Tile::B_INST;
@@ -347,24 +361,21 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
       load_stage(k + 3);
       const uint8_t* const stage = smem + (k & 3) * Tile::STAGE;
       const uint8_t* const table = smem + Tile::STAGES * Tile::STAGE + ((k >> 2) & 1) * Tile::TABLE;
+      if (j == 0) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i) as[i] = own_scales(table + (wm + (i >> 1) * 32 + (i & 1) * 4 + r0) * 16);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) bs[i] = own_scales(table + (BM + wn + (i >> 1) * 32 + (i & 1) * 4 + r0) * 16);
+      }
       v4i af[MF], bf[NF];
-      uint32_t as[MF], bs[NF];
 #pragma unroll
-      for (int i = 0; i < MF; ++i) {
-        const int f = wm + (i >> 1) * 32 + (i & 1) * 4;
-        af[i] = *reinterpret_cast<const v4i*>(stage + f * 64 + frag);
-        as[i] = *reinterpret_cast<const uint8_t*>(table + (f + r0) * 16 + 4 * j + q);
-      }
+      for (int i = 0; i < NF; ++i) bf[i] = *reinterpret_cast<const v4i*>(stage + (BM + wn + (i >> 1) * 32 + (i & 1) * 4) * 64 + frag);
 #pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        const int f = BM + wn + (i >> 1) * 32 + (i & 1) * 4;
-        bf[i] = *reinterpret_cast<const v4i*>(stage + f * 64 + frag);
-        bs[i] = *reinterpret_cast<const uint8_t*>(table + (f + r0) * 16 + 4 * j + q);
-      }
+      for (int i = 0; i < MF; ++i) af[i] = *reinterpret_cast<const v4i*>(stage + (wm + (i >> 1) * 32 + (i & 1) * 4) * 64 + frag);
 #pragma unroll
       for (int i = 0; i < MF; ++i)
 #pragma unroll
-        for (int n = 0; n < NF; ++n) acc[i][n] = mfma_mx<0>(bf[n], bs[n], af[i], as[i], acc[i][n]);
+        for (int n = 0; n < NF; ++n) acc[i][n] = mfma_mx_step(j, bf[n], bs[n], af[i], as[i], acc[i][n]);
     }
   }
   wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends
