@@ -100,7 +100,15 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
     if (int rc = finish("mxfp4_gemm (scales)")) return rc;
     p.a_s = reinterpret_cast<const uint8_t*>(to), p.b_s = reinterpret_cast<const uint8_t*>(to + M * words), p.pitch = 4 * words;
   }
-  if (ceil_div(M, 256) * ceil_div(N, 256) >= 128) return launch_tiles<MxTile<2, 4, 8, 4>>(p, st);
+  if (ceil_div(M, 256) * ceil_div(N, 256) >= 128) {
+    const int64_t tiles_m = ceil_div(M, 256), tiles_n = ceil_div(N, 256);
+    if (tiles_m * tiles_n > (1ll << 30)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld x N=%lld beyond the supported range", (long long)M, (long long)N);
+    p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group_m = static_cast<int>(std::min<int64_t>(tiles_m, 8));
+    with_type(out_dtype, [&](auto t) {
+      hipLaunchKernelGGL(mxfp4_ring_kernel<t()>, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * MxRing::kWaves), MxRing::kLds, st, p);
+    });
+    return finish("mxfp4_gemm");
+  }
   return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
 }
 

@@ -391,4 +391,169 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
   }
 }
 
+// Large products: 256 x 256 outputs in eight waves of 128 x 64, steps of 256 columns, 128 bytes of every row, in a ring of two.  Bound by what moves: the MFMAs
+// of a step take 2048 cycles (a loop of nothing else reaches 6.3 to 7.3 PFLOP/s on random codes, for its power), its 64 KB come in whole cache lines
+// (with steps of half a line, 64-byte requests to the L2, moving them took 280 us of 4096 x 7168 x 18432 without any MFMA).
+// LDS is handed over at two points of a step, so that a byte is on its way for one and a half: at Y every wave has read its columns and its first four
+// fragments of rows (part one), at X of the next step the other four (part two).  The reads behind a point are covered by the MFMAs of the fragment read
+// in front of it.
+//   ... X(k): part two of step k + 1 is asked for, fragments 0 to 3 | Y(k): part one of step k + 2, fragments 4 to 7 | X(k + 1) ...
+struct MxRing {
+  static constexpr int kWaves = 8, kTile = 256, kStage = 2 * kTile * 128, kTable = 2 * kTile * 16, kLds = 2 * kStage + 2 * kTable;
+};
+
+// A row's 16-byte piece c lies at c ^ this: as mx_swizzle, of rows of 128 bytes.  Row bit 1 parts neighbours of one parity, and the four runs of a fragment, two of
+// which read the next piece in the same turn, take 0, 4, 5, 1.
+__device__ __forceinline__ int mx_ring_swizzle(int row) {
+  const int g = (row >> 3) & 3;
+  return (row & 2) | (((g ^ (g >> 1)) & 1) << 2) | (g >> 1);
+}
+
+template <int OUT>
+__global__ void __launch_bounds__(64 * MxRing::kWaves) mxfp4_ring_kernel(const MxArgs p) {
+  constexpr int kTile = MxRing::kTile;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const mx_lds_bytes lds = (mx_lds_bytes)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  // neighbouring tiles on one XCD, patches of group_m row tiles
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int per = tiles / 8, over = tiles % 8, xcd = blockIdx.x % 8;
+  const int id = xcd * per + min(xcd, over) + blockIdx.x / 8;
+  const int width = p.group_m * p.tiles_n, patch = id / width, first_m = patch * p.group_m;
+  const int high = min(p.tiles_m - first_m, p.group_m), in_patch = id - patch * width;
+  const int64_t m0 = static_cast<int64_t>(first_m + in_patch % high) * kTile;
+  const int n0 = (in_patch / high) * kTile;
+  const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(kTile))), cols = min(kTile, p.N - n0);
+  const uint32_t half = p.K / 2;
+  const int steps = (p.G + 7) / 8;
+
+  // An instruction moves 8 rows, number 8 j + wave of an operand; of the rows, which come in two parts, numbers 0-7 and 16-23, then the others.  All numbers of a
+  // wave agree mod 4, which makes the lane's piece the same.
+  const uint8_t *const a_base = p.a + m0 * half, *const b_base = p.b + static_cast<int64_t>(n0) * half;
+  const uint32_t piece = static_cast<uint32_t>((lane & 7) ^ mx_ring_swizzle(8 * wave + (lane >> 3))) * 16;
+  uint32_t a_off[4], b_off[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    b_off[j] = (64 * j + 8 * wave + (lane >> 3)) * half + piece;
+    a_off[j] = (128 * (j & 1) + 64 * (j >> 1) + 8 * wave + (lane >> 3)) * half + piece;
+  }
+  const bool tail = p.G % 8 != 0;  // the last step is short
+  const auto load = [&](bool part_one, int k) {
+    const bool in = k < steps;
+    const uint32_t at = in ? static_cast<uint32_t>(k) * 128 : 0;
+    const bool past = tail && at + piece >= half;
+    const auto a_src = make_rsrc(a_base, in ? rows * half : 0), b_src = make_rsrc(b_base, in ? cols * half : 0);
+    const mx_lds_bytes to = lds + (k & 1) * MxRing::kStage;
+    if (part_one) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load_to_lds<0>(b_src, to + kTile * 128 + (8 * j + wave) * 1024, past ? kNowhere : b_off[j], at);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = part_one ? j : 2 + j;
+      load_to_lds<0>(a_src, to + (16 * j + (part_one ? 0 : 8) + wave) * 1024, past ? kNowhere : a_off[i], at);
+    }
+  };
+  // the scales of window w, 16 groups, two steps: those of the tile's rows, behind them those of its columns
+  const auto load_scales = [&](int w) {
+    const bool in = 2 * w < steps, of_a = wave < 4;
+    const auto src = make_rsrc(of_a ? p.a_s + m0 * p.pitch : p.b_s + static_cast<int64_t>(n0) * p.pitch, in ? (of_a ? rows : cols) * p.pitch : 0);
+    load_to_lds<0>(src, lds + 2 * MxRing::kStage + (w & 1) * MxRing::kTable + wave * 1024, ((wave & 3) * 64 + lane) * static_cast<uint32_t>(p.pitch), in ? 16 * w : 0);
+  };
+
+  const int wm = (wave / 4) * 128, wn = (wave % 4) * 64;
+  const int r0 = mx_row(0, l16);
+  const int from_a = (wm + r0) * 128 + (q ^ mx_ring_swizzle(r0)) * 16, from_b = (kTile + wn + r0) * 128 + (q ^ mx_ring_swizzle(r0)) * 16;
+  struct Fragment {
+    v4i half[2];
+  };
+  const auto fragment = [&](int k, int from, int i) {
+    const uint8_t* const at = smem + (k & 1) * MxRing::kStage + ((i >> 1) * 32 + (i & 1) * 4) * 128;
+    return Fragment{{*reinterpret_cast<const v4i*>(at + from), *reinterpret_cast<const v4i*>(at + (from ^ 64))}};
+  };
+  const uint32_t pick = 0x04000400u + 0x00010001u * (0x100u * q + q);  // bytes q, 4 + q
+  const auto own_scales = [&](int w, int row) {
+    const v4i v = *reinterpret_cast<const v4i*>(smem + 2 * MxRing::kStage + (w & 1) * MxRing::kTable + row * 16);
+    const uint32_t low = __builtin_amdgcn_perm(v[1], v[0], pick), high = __builtin_amdgcn_perm(v[3], v[2], pick);
+    // groups past the end: what lies there are the next row's, which need not be numbers
+    const int bytes = (p.G - 16 * w + 3) / 4;
+    return __builtin_amdgcn_perm(high, low, 0x05040100u) & (bytes >= 4 ? ~0u : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1);
+  };
+  v4f acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[i][n] = v4f{0.f, 0.f, 0.f, 0.f};
+  uint32_t as[8], bs[4];
+  Fragment b[2][4], a[8];
+
+  const auto products = [&](int parity, int i) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[i][n] = mfma_mx_step(2 * parity + t, b[parity][n].half[t], bs[n], a[i].half[t], as[i], acc[i][n]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  load_scales(0), load(true, 0), load(false, 0), load(true, 1);
+  wait_loads<8>();
+  mx_barrier();
+  load(false, 1);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) b[0][n] = fragment(0, from_b, n), bs[n] = own_scales(0, kTile + wn + mx_row(n, 0) + r0);
+  a[0] = fragment(0, from_a, 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) as[i] = own_scales(0, wm + mx_row(i, 0) + r0);
+  for (int k0 = 0; k0 < steps; k0 += 2) {
+#pragma unroll
+    for (int parity = 0; parity < 2; ++parity) {
+      const int k = k0 + parity;
+      if (k >= steps) break;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) a[i + 1] = fragment(k, from_a, i + 1), products(parity, i);
+      // Y: part two of this step was asked for at X of the last but one; behind it came one part one, with scales where that step was even, and one part two
+      if (parity == 0)
+        wait_loads<8>();
+      else
+        wait_loads<9>();
+      mx_barrier();
+      if (parity == 0) load_scales(k / 2 + 1);
+      load(true, k + 2);
+#pragma unroll
+      for (int i = 3; i < 7; ++i) a[i + 1] = fragment(k, from_a, i + 1), products(parity, i);
+      // X of the next step
+      if (parity == 0)
+        wait_loads<9>();
+      else
+        wait_loads<8>();
+      mx_barrier();
+      load(false, k + 2);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) b[1 - parity][n] = fragment(k + 1, from_b, n);
+      a[0] = fragment(k + 1, from_a, 0);
+      products(parity, 7);
+      if (parity == 1) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) bs[n] = own_scales(k / 2 + 1, kTile + wn + mx_row(n, 0) + r0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) as[i] = own_scales(k / 2 + 1, wm + mx_row(i, 0) + r0);
+      }
+    }
+  }
+  wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = wm + mx_row(i, l16);
+    if (row >= rows) continue;
+#pragma unroll
+    for (int n = 0; n < 4; n += 2) {
+      const int col = wn + (n >> 1) * 32 + 8 * q;
+      if (col >= cols) continue;
+      const float v[8] = {acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3], acc[i][n + 1][0], acc[i][n + 1][1], acc[i][n + 1][2], acc[i][n + 1][3]};
+      store_raw8<OUT>(p.c, (m0 + row) * p.N + n0, col, pack_raw8<OUT>(v), cols - col);
+    }
+  }
+}
+
 }  // namespace dlb
