@@ -194,17 +194,28 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   const int64_t slots = tokens * topk;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(ceil_div(H, 16 * kDownTiles)));
-  // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches.
-  const int64_t mean = slots / std::min(experts, slots);
-  const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16, down_tokens = tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
+  // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches.  The second product's
+  // rows share the LDS with what is on its way of the weights: few rows and eight waves while an expert has about three tokens or fewer (8 tokens, 8 of 32 experts,
+  // 7168 x 2048: e4m3 79 us, e2m1 59 us, with eight rows 103 and 75 us); more tokens leave no room for eight waves' sums, or, of e2m1, are no faster by them (16 tokens: 88 us with either).
+  const int64_t named = std::min(experts, slots), mean = slots / named;
+  const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16;
   const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
       hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), up_grid, dim3(64 * kUpWaves), (UpShape<kw(), r()>::kLds), st, a);
     });
-    with_chunks<2, 4, 8>(down_tokens, [&](auto t) {
-      const int64_t lds = experts_down_lds<kw(), t()>(tokens, topk, experts);
-      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), ragged_down()>), down_grid, dim3(64 * (DownShape<kw(), t()>::kWaves)), static_cast<size_t>(lds), st, a);
-    });
+    const auto down = [&](auto t, auto waves) {
+      const int64_t lds = experts_down_lds<kw(), t(), waves()>(tokens, topk, experts);
+      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), waves(), ragged_down()>), down_grid, dim3(64 * waves()), static_cast<size_t>(lds), st, a);
+    };
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
+    if (tokens <= 2) return down(two, eight);
+    if (tokens <= 4 || (tokens <= kDownWideTokens && slots <= 3 * named)) return down(four, eight);
+    if constexpr (kw() == kE4m3) {
+      if (tokens <= kDownWideTokens) return down(eight, eight);
+    }
+    down(eight, four);
   };
   with_flag(dtype == kInBf16, [&](auto bf16) {
     constexpr std::integral_constant<int, bf16() ? kInBf16 : kInF16> kt;

@@ -371,10 +371,13 @@ struct UpShape {
 };
 
 constexpr int kDownTiles = 2;
-template <int W, int TOKENS>
+// An expert's tokens over those of a pass, rounded up, adds up to no more than the slots, and than the experts and the slots over those of a pass.
+__host__ __device__ constexpr int64_t down_entries(int64_t slots, int64_t experts, int64_t a_pass) { return slots < experts + slots / a_pass ? slots : experts + slots / a_pass; }
+constexpr int kDownWideTokens = 16;  // as many as eight waves have room for the sums of
+template <int W, int TOKENS, int WAVES>
 struct DownShape {
-  static constexpr int kBudget = (TOKENS <= 4 ? 140 : 108) * 1024, kWaves = TOKENS <= 4 ? 8 : 4;  // beside it the sums of up to 64 tokens have to fit, of more than four by four waves
-  static constexpr int kDepth = stream_depth(W, 2 * TOKENS, kDownTiles, kWaves, kBudget), kRing = kWaves * kDepth * stream_bytes(W, 2 * TOKENS, kDownTiles);
+  static constexpr int kBudget = (WAVES == 8 ? 138 : 108) * 1024;  // the tables of the tokens have to fit beside it
+  static constexpr int kDepth = stream_depth(W, 2 * TOKENS, kDownTiles, WAVES, kBudget), kRing = WAVES * kDepth * stream_bytes(W, 2 * TOKENS, kDownTiles);
 };
 
 // A workgroup takes 16 rows of Gate and the same of Up, of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
@@ -452,24 +455,27 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
 // A workgroup takes 32 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
 // chunks of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
 // The 2 TOKENS rows of x are the numbers of the tokens and behind them their rests.
-template <int TO, int W, int TOKENS, bool RAGGED>
-__global__ void __launch_bounds__(64 * (DownShape<W, TOKENS>::kWaves)) experts_down_kernel(const ExpertArgs p) {
+template <int TO, int W, int TOKENS, int kWaves, bool RAGGED>
+__global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertArgs p) {
   constexpr int R = 2 * TOKENS;
-  typedef DownShape<W, TOKENS> Shape;
+  typedef DownShape<W, TOKENS, kWaves> Shape;
   typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth, RAGGED> S;
-  constexpr int kWaves = Shape::kWaves, kWide = 16 * kDownTiles;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // the rings, behind them [waves][T][kWide] sums, behind those the slots of the entries' rows
-  __shared__ int count[kFewExperts];
-  __shared__ int16_t ids[kFewTopk][kFewTokens];
-  __shared__ int32_t entry[kFewTokens * kFewTopk];  // expert, pass << 16
+  constexpr int kWide = 16 * kDownTiles;
+  // The rings; behind them [waves][T][kWide] sums, the entries (expert, pass << 16), the slots of their rows ([TOKENS], -1: none).  What the list of entries is made
+  // from lies where the rings are later.
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int entries;
+  int* const count = reinterpret_cast<int*>(lds);                                             // [E]
+  int16_t(*const ids)[kFewTokens] = reinterpret_cast<int16_t(*)[kFewTokens]>(lds + kFewExperts * 4);  // [topk]
+  static_assert(Shape::kRing >= kFewExperts * 4 + kFewTopk * kFewTokens * 2, "room for them");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int slots = p.T * p.topk;
   constexpr int kThreads = 64 * kWaves;
   float* const all = reinterpret_cast<float*>(lds + Shape::kRing);
   float* const sums = all + wave * p.T * kWide;
-  int16_t* const row_slot = reinterpret_cast<int16_t*>(all + kWaves * p.T * kWide);  // [entries][TOKENS], -1: none
+  int32_t* const entry = reinterpret_cast<int32_t*>(all + kWaves * p.T * kWide);
+  int16_t* const row_slot = reinterpret_cast<int16_t*>(entry + down_entries(p.T * p.topk, p.E, TOKENS));
   for (int i = tid; i < p.E; i += kThreads) count[i] = 0;
   for (int i = lane; i < p.T * kWide; i += 64) sums[i] = 0.f;
   __syncthreads();
@@ -587,11 +593,12 @@ __global__ void __launch_bounds__(64 * (DownShape<W, TOKENS>::kWaves)) experts_d
   }
 }
 
-// LDS of experts_down_kernel: an expert's tokens over TOKENS, rounded up, adds up to no more entries than slots, and than experts and a TOKENS-th of them.
-template <int W, int TOKENS>
+template <int W, int TOKENS, int WAVES>
 int64_t experts_down_lds(int64_t tokens, int64_t topk, int64_t experts) {
-  const int64_t slots = tokens * topk, most = experts + slots / TOKENS, entries = slots < most ? slots : most;
-  return DownShape<W, TOKENS>::kRing + DownShape<W, TOKENS>::kWaves * tokens * 16 * kDownTiles * 4 + entries * TOKENS * 2;
+  typedef DownShape<W, TOKENS, WAVES> Shape;
+  constexpr int kMostTokens = WAVES == 8 ? kDownWideTokens : kFewTokens, kMostSlots = kMostTokens * kFewTopk;
+  static_assert(Shape::kRing + WAVES * kMostTokens * 16 * kDownTiles * 4 + kMostSlots * (4 + TOKENS * 2) + 64 <= 160 * 1024, "what a CU has, for the most tokens and slots");
+  return Shape::kRing + WAVES * tokens * 16 * kDownTiles * 4 + down_entries(tokens * topk, experts, TOKENS) * (4 + TOKENS * 2);
 }
 
 }  // namespace dlb
