@@ -28,6 +28,9 @@ MxPlan mx_plan(int64_t M, int64_t, int64_t K) {
 }
 int64_t padded(int64_t G) { return ceil_div(G, 4) * 4; }
 
+// Rows of scales that do not start on four bytes: kernels of a few rows load them byte by byte.
+bool bytes_apart(const void* s, int64_t K) { return K / kMxGroup % 4 != 0 || misaligned(s, 4); }
+
 template <class Tile>
 int launch_tiles(MxArgs a, hipStream_t st) {
   const int64_t tiles_m = ceil_div(a.M, Tile::BM), tiles_n = ceil_div(a.N, Tile::BN);
@@ -132,7 +135,7 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (ceil_div(tiles, 8) > 65535) return fail(DLB_ERR_BAD_SHAPE, "N=%lld beyond the supported range", (long long)N);
   const dim3 grid(static_cast<unsigned>(8 * ceil_div(M, rows)), static_cast<unsigned>(ceil_div(tiles, 8)));
   with_flag(dtype == kInBf16, [&](auto bf16) {
-    with_flag(K % 128 != 0, [&](auto ragged) {
+    with_flag(bytes_apart(s, K), [&](auto ragged) {
       with_chunks<4, 8, 16>(rows, [&](auto r) {
         with_chunks<1, 2>(nt, [&](auto n) {
           typedef FewShape<kE2m1, r(), n()> Shape;
@@ -221,7 +224,7 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
     constexpr std::integral_constant<int, bf16() ? kInBf16 : kInF16> kt;
     constexpr std::false_type whole;
     if (!f4) return launch(kt, std::integral_constant<int, kE4m3>(), whole, whole);
-    with_flag(H % 128 != 0, [&](auto up) { with_flag(I % 128 != 0, [&](auto down) { launch(kt, std::integral_constant<int, kE2m1>(), up, down); }); });
+    with_flag(bytes_apart(up_s, H), [&](auto up) { with_flag(bytes_apart(down_s, I), [&](auto down) { launch(kt, std::integral_constant<int, kE2m1>(), up, down); }); });
   });
   return finish("few_token_experts");
 }
