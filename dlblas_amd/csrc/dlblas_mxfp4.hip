@@ -15,28 +15,49 @@ int check_columns(int64_t K) {
   return DLB_OK;
 }
 
-// How a product runs: few rows, K split over waves, or tiles.
-struct MxPlan {
-  int mt;    // few rows: tiles of 16 of them in a workgroup; 0: tiles through LDS
-  bool pad;  // tiles read the scales of four groups at a time: rows of another number of them are laid out anew
-};
-MxPlan mx_plan(int64_t M, int64_t, int64_t K) {
-  if (M <= 16) return {1, false};
-  if (M <= 32) return {2, false};
-  if (M <= 64) return {4, false};
-  return {0, K / kMxGroup % 4 != 0};
+// How a product runs.  us of M x N x K, one side of a border and the other:
+//   16 x 2112 x 7168    split 1 x 1: 6.3, 1 x 2: 7.5        16 x 7168 x 18432: 23.0, 16.4
+//   17 x 7168 x 18432   split 1 x 2: 29,  2 x 2: 18
+//   65 x 2112 x 7168    split 2 x 2: 8.1, 64 tiles: 14.7    128 x 2112 x 7168 (264 workgroups): 13.8, 14.8   65 x 7168 x 18432: 49, 33
+//   64 x 7168 x 18432   split 4 x 2: 28,  64 tiles: 32      65: 50, 33
+//   256 x 7168 x 18432  64 tiles: 48, 128 tiles: 56         512: 93, 60;  1024 x 2112 x 7168: 28, 26
+//   1024 x 7168 x 18432 128 tiles: 104, 256 tiles: 115      2048: 205, 130;  2048 x 2112 x 7168: 39, 50;  4096: 66, 52
+enum class MxWay { kSplit11, kSplit12, kSplit22, kSplit42, kTiles64, kTiles128, kTiles256 };
+MxWay mx_way(int64_t M, int64_t N) {
+  const auto tiles = [&](int m, int n) { return ceil_div(M, m) * ceil_div(N, n); };
+  if (M <= 16) return N <= 4096 ? MxWay::kSplit11 : MxWay::kSplit12;
+  if (M <= 32 || tiles(32, 32) <= 256) return MxWay::kSplit22;  // workgroups for every CU
+  if (M <= 64) return MxWay::kSplit42;
+  if (tiles(64, 64) <= 512) return MxWay::kTiles64;  // two a CU
+  return tiles(256, 256) >= 128 ? MxWay::kTiles256 : MxWay::kTiles128;
 }
+// Tiles read the scales of four groups at a time: rows of another number of them are laid out anew.
+bool mx_pads(int64_t M, int64_t N, int64_t K) { return mx_way(M, N) >= MxWay::kTiles64 && K / kMxGroup % 4 != 0; }
 int64_t padded(int64_t G) { return ceil_div(G, 4) * 4; }
 
 // Rows of scales that do not start on four bytes: kernels of a few rows load them byte by byte.
 bool bytes_apart(const void* s, int64_t K) { return K / kMxGroup % 4 != 0 || misaligned(s, 4); }
 
+// Tiles of BM x BN; at most as many workgroups as a launch has threads for.
+int mx_tiles(MxArgs& a, int BM, int BN, int threads) {
+  const int64_t tiles_m = ceil_div(a.M, BM), tiles_n = ceil_div(a.N, BN);
+  if (tiles_m * (tiles_n + 7) > ((1ll << 32) - 1) / threads) return fail(DLB_ERR_BAD_SHAPE, "M=%lld x N=%d beyond the supported range", (long long)a.M, a.N);
+  a.tiles_m = static_cast<int>(tiles_m), a.tiles_n = static_cast<int>(tiles_n), a.group_m = static_cast<int>(std::min<int64_t>(tiles_m, 8));
+  return DLB_OK;
+}
+
+template <class Split>
+int launch_split(MxArgs a, hipStream_t st) {
+  if (int rc = mx_tiles(a, 16 * Split::MT, 16 * Split::NT, 64 * Split::WAVES)) return rc;
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.tiles_n, 8) * 8 * a.tiles_m));
+  with_flag(a.G % 4 == 0, [&](auto dwords) { hipLaunchKernelGGL((mxfp4_split_kernel<Split, dwords()>), grid, dim3(64 * Split::WAVES), Split::LDS, st, a); });
+  return finish("mxfp4_gemm");
+}
+
 template <class Tile>
 int launch_tiles(MxArgs a, hipStream_t st) {
-  const int64_t tiles_m = ceil_div(a.M, Tile::BM), tiles_n = ceil_div(a.N, Tile::BN);
-  if (tiles_m * tiles_n > (1ll << 30)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld x N=%d beyond the supported range", (long long)a.M, a.N);
-  a.tiles_m = static_cast<int>(tiles_m), a.tiles_n = static_cast<int>(tiles_n), a.group_m = static_cast<int>(std::min<int64_t>(tiles_m, 8));
-  hipLaunchKernelGGL(mxfp4_tile_kernel<Tile>, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * Tile::WAVES), Tile::LDS, st, a);
+  if (int rc = mx_tiles(a, Tile::BM, Tile::BN, 64 * Tile::WAVES)) return rc;
+  hipLaunchKernelGGL(mxfp4_tile_kernel<Tile>, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n)), dim3(64 * Tile::WAVES), Tile::LDS, st, a);
   return finish("mxfp4_gemm");
 }
 
@@ -62,7 +83,7 @@ int dlb_mxfp4_quant(const void* x, int64_t x_row_stride, int dtype, void* q, voi
 }
 
 size_t dlb_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || !dlb::mx_plan(M, N, K).pad) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !dlb::mx_pads(M, N, K)) return 0;
   return static_cast<size_t>(M + N) * dlb::padded(K / dlb::kMxGroup);
 }
 
@@ -79,7 +100,6 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
   if (!a || !b || !a_s || !b_s || !c) return fail(DLB_ERR_NULL_POINTER, "a, b, a_s, b_s or c is NULL");
   if (misaligned(a, 16) || misaligned(b, 16) || misaligned(a_s, 4) || misaligned(b_s, 4) || off_elements(c, out_dtype))
     return fail(DLB_ERR_ALIGNMENT, "codes must be 16-byte, scales 4-byte aligned, c to its elements");
-  const MxPlan plan = mx_plan(M, N, K);
   const size_t need = dlb_mxfp4_gemm_workspace_bytes(M, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
@@ -88,14 +108,14 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
   MxArgs p{};
   p.a = static_cast<const uint8_t*>(a), p.b = static_cast<const uint8_t*>(b), p.a_s = static_cast<const uint8_t*>(a_s), p.b_s = static_cast<const uint8_t*>(b_s);
   p.c = c, p.M = M, p.N = static_cast<int>(N), p.K = static_cast<int>(K), p.G = static_cast<int>(K / kMxGroup), p.pitch = p.G, p.out = out_dtype;
-  if (plan.mt > 0) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(N, 16)), static_cast<unsigned>(ceil_div(M, 16 * plan.mt)));
-    with_chunks<1, 2, 4>(plan.mt, [&](auto mt) {
-      with_flag(p.G % 4 == 0, [&](auto dwords) { hipLaunchKernelGGL((mxfp4_few_kernel<mt(), dwords()>), grid, dim3(64 * kMxFewWaves), 0, st, p); });
-    });
-    return finish("mxfp4_gemm");
+  switch (mx_way(M, N)) {
+    case MxWay::kSplit11: return launch_split<MxSplit<1, 1, 8>>(p, st);
+    case MxWay::kSplit12: return launch_split<MxSplit<1, 2, 4>>(p, st);
+    case MxWay::kSplit22: return launch_split<MxSplit<2, 2, 8>>(p, st);
+    case MxWay::kSplit42: return launch_split<MxSplit<4, 2, 4>>(p, st);
+    default: break;
   }
-  if (plan.pad) {
+  if (need > 0) {
     const int words = static_cast<int>(padded(p.G) / 4);
     uint32_t* const to = static_cast<uint32_t*>(workspace);
     const MxPadArgs pad{p.a_s, p.b_s, to, to + M * words, M, N, p.G, words};
@@ -103,16 +123,13 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
     if (int rc = finish("mxfp4_gemm (scales)")) return rc;
     p.a_s = reinterpret_cast<const uint8_t*>(to), p.b_s = reinterpret_cast<const uint8_t*>(to + M * words), p.pitch = 4 * words;
   }
-  if (ceil_div(M, 256) * ceil_div(N, 256) >= 128) {
-    const int64_t tiles_m = ceil_div(M, 256), tiles_n = ceil_div(N, 256);
-    if (tiles_m * tiles_n > (1ll << 30)) return fail(DLB_ERR_BAD_SHAPE, "M=%lld x N=%lld beyond the supported range", (long long)M, (long long)N);
-    p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group_m = static_cast<int>(std::min<int64_t>(tiles_m, 8));
-    with_type(out_dtype, [&](auto t) {
-      hipLaunchKernelGGL(mxfp4_ring_kernel<t()>, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * MxRing::kWaves), MxRing::kLds, st, p);
-    });
-    return finish("mxfp4_gemm");
-  }
-  return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
+  if (mx_way(M, N) == MxWay::kTiles64) return launch_tiles<MxTile<2, 1, 2, 4>>(p, st);
+  if (mx_way(M, N) == MxWay::kTiles128) return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
+  if (int rc = mx_tiles(p, MxRing::kTile, MxRing::kTile, 64 * MxRing::kWaves)) return rc;
+  with_type(out_dtype, [&](auto t) {
+    hipLaunchKernelGGL(mxfp4_ring_kernel<t()>, dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n)), dim3(64 * MxRing::kWaves), MxRing::kLds, st, p);
+  });
+  return finish("mxfp4_gemm");
 }
 
 int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const void* q, const void* s, void* y, int64_t M, int64_t N, int64_t K,

@@ -115,84 +115,6 @@ __device__ __forceinline__ void store4(void* c, int type, int64_t at, const v4f&
   }
 }
 
-constexpr int kMxFewWaves = 8;
-
-// Few rows: bound by the weights' bytes, which go from memory to registers once.  The waves of a workgroup take chunks of 512 columns of 16 rows of
-// b in turn (a lane 64 bytes, four groups, in four loads, and their scales in one), and add their sums through LDS in wave order.
-// DWORDS: rows of scales are a multiple of four groups; otherwise a lane reads its scales one by one.
-template <int MT, bool DWORDS>
-__global__ void __launch_bounds__(64 * kMxFewWaves) mxfp4_few_kernel(const MxArgs p) {
-  __shared__ v4f part[kMxFewWaves][MT][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int q = lane >> 4, l16 = lane & 15;
-  const int n0 = blockIdx.x * 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
-  const int cols = min(16, p.N - n0), rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(16 * MT)));
-  const uint32_t half = p.K / 2;
-  const auto b_src = make_rsrc(p.b + static_cast<int64_t>(n0) * half, cols * half);
-  const auto bs_src = make_rsrc(p.b_s + static_cast<int64_t>(n0) * p.pitch, cols * p.pitch);
-  const auto a_src = make_rsrc(p.a + m0 * half, rows * half);
-  const auto as_src = make_rsrc(p.a_s + m0 * p.pitch, rows * p.pitch);
-  struct Chunk {
-    v4i b[4], a[MT][4];
-    uint32_t b_s, a_s[MT];
-  };
-  const auto scales = [&](auto src, bool there, uint32_t row, int g) {
-    if (DWORDS) return __builtin_amdgcn_raw_buffer_load_b32(src, there && g < p.G ? row * p.pitch + g : kNowhere, 0, 0);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b8(src, there && g + i < p.G ? row * p.pitch + g + i : kNowhere, 0, 0)) << (8 * i);
-    return w;
-  };
-  auto load = [&](int c, Chunk& k) {
-    const int g = 16 * c + 4 * q;  // the lane's first group
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = g + i < p.G ? static_cast<uint32_t>(g + i) * 16 : kNowhere;
-      k.b[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(b_src, l16 < cols && at != kNowhere ? l16 * half + at : kNowhere, 0, 2));
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        k.a[m][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(a_src, 16 * m + l16 < rows && at != kNowhere ? (16 * m + l16) * half + at : kNowhere, 0, 0));
-    }
-    k.b_s = scales(bs_src, l16 < cols, l16, g);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) k.a_s[m] = scales(as_src, 16 * m + l16 < rows, 16 * m + l16, g);
-  };
-  v4f acc[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = v4f{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const Chunk& k) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      acc[m] = mfma_mx<0>(k.b[0], k.b_s, k.a[m][0], k.a_s[m], acc[m]);
-      acc[m] = mfma_mx<1>(k.b[1], k.b_s, k.a[m][1], k.a_s[m], acc[m]);
-      acc[m] = mfma_mx<2>(k.b[2], k.b_s, k.a[m][2], k.a_s[m], acc[m]);
-      acc[m] = mfma_mx<3>(k.b[3], k.b_s, k.a[m][3], k.a_s[m], acc[m]);
-    }
-  };
-  const int chunks = (p.G + 15) / 16;
-  Chunk even, odd;
-  load(wave, even);
-  for (int c = wave; c < chunks; c += 2 * kMxFewWaves) {
-    load(c + kMxFewWaves, odd);
-    multiply(even);
-    load(c + 2 * kMxFewWaves, even);
-    multiply(odd);
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m) part[wave][m][lane] = acc[m];
-  __syncthreads();
-  // wave m adds up tile m
-  for (int m = wave; m < MT; m += kMxFewWaves) {
-    v4f sum = part[0][m][lane];
-#pragma unroll
-    for (int w = 1; w < kMxFewWaves; ++w) sum += part[w][m][lane];
-    const int row = 16 * m + l16, col = 4 * q;
-    if (row < rows && col < cols) store4(p.c, p.out, (m0 + row) * p.N + n0 + col, sum, cols - col);
-  }
-}
-
 // Scales of rows whose groups are no multiple of four, with zeros behind the last: both operands' in one launch.
 struct MxPadArgs {
   const uint8_t *a_s, *b_s;
@@ -214,8 +136,9 @@ __global__ void __launch_bounds__(256) mxfp4_pad_kernel(const MxPadArgs p) {
   }
 }
 
-// Many rows: tiles of BM x BN through LDS.  A step is 128 columns, 64 bytes of every row, in a ring of four; the scales of four steps lie in a table of 16
-// bytes a row, two of them in turn.  WGM x WGN waves, each with MF x NF fragments of 16 x 16 outputs (both even).
+// Tiles of BM x BN through LDS.  A step is 128 columns, 64 bytes of every row, in a ring of four; the scales of four steps lie in a table of 16
+// bytes a row, two of them in turn.  WGM x WGN waves, each with MF x NF fragments of 16 x 16 outputs (both even).  Bound by what a CU brings into its LDS, about
+// 32 KB a microsecond with one or two workgroups on it; a ring of eight takes as long.
 template <int WGM_, int WGN_, int MF_, int NF_>
 struct MxTile {
   static constexpr int WGM = WGM_, WGN = WGN_, MF = MF_, NF = NF_, STAGES = 4;
@@ -388,6 +311,134 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
       const int col = wn + (n >> 1) * 32 + (n & 1) * 4 + 8 * q;
       if (col < cols) store4(p.c, p.out, (m0 + row) * p.N + n0 + col, acc[i][n], cols - col);
     }
+  }
+}
+
+// Few rows, or few tiles: 16 MT x 16 NT outputs in a workgroup whose waves split K, a chunk of 256 columns, 128 bytes of every row, each in turn, and add
+// their sums through LDS in wave order.  What a wave takes comes through a ring of its own in LDS, so that whole cache lines are asked for and no wave waits for another.
+template <int MT_, int NT_, int WAVES_>
+struct MxSplit {
+  static constexpr int MT = MT_, NT = NT_, WAVES = WAVES_, FRAGS = MT + NT;
+  static constexpr int STAGE = FRAGS * 16 * (128 + 8), MOST = 156 * 1024 / (WAVES * STAGE), DEPTH = MOST > 4 ? 4 : MOST;
+  static constexpr int SUMS = WAVES * MT * NT * 1024, RING = WAVES * DEPTH * STAGE, LDS = SUMS > RING ? SUMS : RING;
+  static_assert(DEPTH >= 1 && LDS <= 160 * 1024, "what a CU has");
+};
+
+// A row's 16-byte piece c lies at c ^ this, as in mx_ring_swizzle, for lanes that read pieces 2 (lane / 16) + step of row lane % 16.
+__device__ __forceinline__ int mx_split_swizzle(int row) {
+  const int i = row >> 1;
+  return (i & 4) | (i & 1) << 1 | (((i >> 1) ^ (i >> 2)) & 1);
+}
+
+// DWORDS: rows of scales are whole words; otherwise a lane reads its scales one by one.
+template <class Split, bool DWORDS>
+__global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const MxArgs p) {
+  constexpr int MT = Split::MT, NT = Split::NT, FRAGS = Split::FRAGS, WAVES = Split::WAVES, DEPTH = Split::DEPTH;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  // eight column tiles, one for each XCD, by the blocks of rows
+  const uint32_t beside = 8 * p.tiles_m, group = blockIdx.x / beside, in_group = blockIdx.x - group * beside;
+  const int n0 = static_cast<int>(group * 8 + in_group % 8) * 16 * NT;
+  const int64_t m0 = static_cast<int64_t>(in_group / 8) * 16 * MT;
+  if (n0 >= p.N) return;
+  const int cols = min(16 * NT, p.N - n0), rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(16 * MT)));
+  const uint32_t half = p.K / 2, pitch = p.pitch;
+  const uint8_t *const a = p.a + m0 * half, *const b = p.b + static_cast<int64_t>(n0) * half;
+  const uint8_t *const a_s = p.a_s + m0 * pitch, *const b_s = p.b_s + static_cast<int64_t>(n0) * pitch;
+  const int chunks = (p.G + 7) / 8;
+
+  // Fragments of a first, then those of b; an instruction moves eight rows, half of one, and the scales of a whole one, eight a row, are another's.
+  const int r8 = lane >> 3;
+  const uint32_t piece[2] = {static_cast<uint32_t>((lane & 7) ^ mx_split_swizzle(r8)) * 16, static_cast<uint32_t>((lane & 7) ^ mx_split_swizzle(8 + r8)) * 16};
+  uint32_t from[2 * FRAGS];
+#pragma unroll
+  for (int j = 0; j < 2 * FRAGS; ++j) from[j] = (8 * (j < 2 * MT ? j : j - 2 * MT) + r8) * half + piece[j & 1];
+  const mx_lds_bytes ring_to = (mx_lds_bytes)smem + wave * DEPTH * Split::STAGE;
+  uint32_t bytes[DEPTH][FRAGS][2];  // without DWORDS: this lane's two scales
+  constexpr int kLoads = FRAGS * (DWORDS ? 3 : 4);
+  const auto load = [&](int d, int c) {
+    const bool in = c < chunks;
+    const uint32_t at = in ? static_cast<uint32_t>(c) * 128 : 0, at_s = in ? static_cast<uint32_t>(c) * 8 : 0;
+    const auto a_src = make_rsrc(a, in ? rows * half : 0), b_src = make_rsrc(b, in ? cols * half : 0);
+    const auto as_src = make_rsrc(a_s, in ? rows * pitch : 0), bs_src = make_rsrc(b_s, in ? cols * pitch : 0);
+    const mx_lds_bytes to = ring_to + d * Split::STAGE;
+    const bool past[2] = {at + piece[0] >= half, at + piece[1] >= half};  // in a short last chunk
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j) load_to_lds<0>(a_src, to + j * 1024, past[j & 1] ? kNowhere : from[j], at);
+#pragma unroll
+    for (int j = 2 * MT; j < 2 * FRAGS; ++j) load_to_lds<2>(b_src, to + j * 1024, past[j & 1] ? kNowhere : from[j], at);
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f) {
+      const uint32_t first = 16 * (f < MT ? f : f - MT);
+      if (DWORDS) {
+        const uint32_t its = (first + (lane >> 1)) * pitch + 4 * (lane & 1);
+        if (lane < 32) load4_to_lds(f < MT ? as_src : bs_src, to + FRAGS * 2048 + f * 128, at_s + 4 * (lane & 1) < p.G ? its : kNowhere, at_s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          bytes[d][f][i] = __builtin_amdgcn_raw_buffer_load_b8(f < MT ? as_src : bs_src, static_cast<int>(at_s) + 2 * q + i < p.G ? (first + l16) * pitch + 2 * q + i : kNowhere, at_s, 0);
+      }
+    }
+  };
+
+  v4f acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+  const uint8_t* const mine = smem + wave * DEPTH * Split::STAGE + l16 * 128;
+  const int at[2] = {((2 * q) ^ mx_split_swizzle(l16)) * 16, ((2 * q + 1) ^ mx_split_swizzle(l16)) * 16};
+  auto multiply = [&](int d) {
+    wait_loads<(DEPTH - 1) * kLoads>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* const stage = mine + d * Split::STAGE;
+    v4i v[FRAGS][2];
+    uint32_t s[FRAGS];
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f) {
+      if (!DWORDS) asm volatile("" : "+v"(bytes[d][f][0]), "+v"(bytes[d][f][1]));  // not before: they would be waited for where they are loaded
+      s[f] = DWORDS ? *reinterpret_cast<const uint16_t*>(stage - l16 * 128 + FRAGS * 2048 + f * 128 + l16 * 8 + 2 * q) : bytes[d][f][0] | bytes[d][f][1] << 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[f][h] = *reinterpret_cast<const v4i*>(stage + f * 2048 + at[h]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[m][n] = mfma_mx<0>(v[MT + n][0], s[MT + n], v[m][0], s[m], acc[m][n]);
+        acc[m][n] = mfma_mx<1>(v[MT + n][1], s[MT + n], v[m][1], s[m], acc[m][n]);
+      }
+    // what is read of this place has arrived before its next chunk is asked for
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) load(d, wave + d * WAVES);
+  for (int c = wave; c < chunks; c += DEPTH * WAVES) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      multiply(d);  // zeros past the last chunk
+      load(d, c + (DEPTH + d) * WAVES);
+    }
+  }
+  wait_loads<0>();  // nothing is on its way into LDS any more
+  __syncthreads();
+  v4f* const part = reinterpret_cast<v4f*>(smem);  // [waves][MT][NT][64]
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) part[((wave * MT + m) * NT + n) * 64 + lane] = acc[m][n];
+  __syncthreads();
+#pragma unroll
+  for (int t = wave; t < MT * NT; t += WAVES) {
+    v4f sum = part[t * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum += part[(w * MT * NT + t) * 64 + lane];
+    const int row = 16 * (t / NT) + l16, col = 16 * (t % NT) + 4 * q;
+    if (row < rows && col < cols) store4(p.c, p.out, (m0 + row) * p.N + n0 + col, sum, cols - col);
   }
 }
 
