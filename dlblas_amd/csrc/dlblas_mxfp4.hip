@@ -31,8 +31,8 @@ MxWay mx_way(int64_t M, int64_t N) {
   if (tiles(64, 64) <= 512) return MxWay::kTiles64;  // two a CU
   return tiles(256, 256) >= 128 ? MxWay::kTiles256 : MxWay::kTiles128;
 }
-// Tiles read the scales of four groups at a time: rows of another number of them are laid out anew.
-bool mx_pads(int64_t M, int64_t N, int64_t K) { return mx_way(M, N) >= MxWay::kTiles64 && K / kMxGroup % 4 != 0; }
+// The largest tiles read the scales of four groups at a time: rows of another number of them are laid out anew.
+bool mx_pads(int64_t M, int64_t N, int64_t K) { return mx_way(M, N) == MxWay::kTiles256 && K / kMxGroup % 4 != 0; }
 int64_t padded(int64_t G) { return ceil_div(G, 4) * 4; }
 
 // Rows of scales that do not start on four bytes: kernels of a few rows load them byte by byte.
@@ -57,7 +57,9 @@ int launch_split(MxArgs a, hipStream_t st) {
 template <class Tile>
 int launch_tiles(MxArgs a, hipStream_t st) {
   if (int rc = mx_tiles(a, Tile::BM, Tile::BN, 64 * Tile::WAVES)) return rc;
-  hipLaunchKernelGGL(mxfp4_tile_kernel<Tile>, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n)), dim3(64 * Tile::WAVES), Tile::LDS, st, a);
+  with_flag(a.G % 4 != 0, [&](auto ragged) {
+    hipLaunchKernelGGL((mxfp4_tile_kernel<Tile, ragged()>), dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n)), dim3(64 * Tile::WAVES), Tile::LDS, st, a);
+  });
   return finish("mxfp4_gemm");
 }
 
@@ -113,7 +115,9 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
     case MxWay::kSplit12: return launch_split<MxSplit<1, 2, 4>>(p, st);
     case MxWay::kSplit22: return launch_split<MxSplit<2, 2, 8>>(p, st);
     case MxWay::kSplit42: return launch_split<MxSplit<4, 2, 4>>(p, st);
-    default: break;
+    case MxWay::kTiles64: return launch_tiles<MxTile<2, 1, 2, 4>>(p, st);
+    case MxWay::kTiles128: return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
+    case MxWay::kTiles256: break;
   }
   if (need > 0) {
     const int words = static_cast<int>(padded(p.G) / 4);
@@ -123,8 +127,6 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
     if (int rc = finish("mxfp4_gemm (scales)")) return rc;
     p.a_s = reinterpret_cast<const uint8_t*>(to), p.b_s = reinterpret_cast<const uint8_t*>(to + M * words), p.pitch = 4 * words;
   }
-  if (mx_way(M, N) == MxWay::kTiles64) return launch_tiles<MxTile<2, 1, 2, 4>>(p, st);
-  if (mx_way(M, N) == MxWay::kTiles128) return launch_tiles<MxTile<2, 2, 4, 4>>(p, st);
   if (int rc = mx_tiles(p, MxRing::kTile, MxRing::kTile, 64 * MxRing::kWaves)) return rc;
   with_type(out_dtype, [&](auto t) {
     hipLaunchKernelGGL(mxfp4_ring_kernel<t()>, dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n)), dim3(64 * MxRing::kWaves), MxRing::kLds, st, p);

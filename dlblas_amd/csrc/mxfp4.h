@@ -190,7 +190,9 @@ __device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t src, LdsPtr 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (mx_lds_ptr)to, 4, voff, soff, 0, 0);
 }
 
-template <class Tile>
+// RAGGED: rows of scales are no whole words.  They go through registers on their way into the table, shifted and with zeros behind the last, instead of being
+// laid out anew by a launch of its own.
+template <class Tile, bool RAGGED>
 __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxArgs p) {
   constexpr int BM = Tile::BM, BN = Tile::BN, MF = Tile::MF, NF = Tile::NF;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -235,15 +237,55 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
       load_to_lds<0>(b_src, to + BM * 64 + (j * Tile::WAVES + wave) * 1024, past ? kNowhere : b_off[j], at);
   };
   // the scales of window w, 16 groups: those of the tile's rows, behind them those of its columns
+  uint32_t words[Tile::S_INST][5];
+  // RAGGED: of a wave's j-th 64 rows of scales, the word where the operand's start, and from there the lane's row and the end
+  struct ScaleRows {
+    const uint8_t* base;
+    uint32_t at, bytes;
+  };
+  const auto scale_rows = [&](int j) {
+    const int first = (j * Tile::WAVES + wave) * 64;
+    const bool of_a = first < BM;
+    const uint8_t* const base = of_a ? p.a_s + m0 * p.G : p.b_s + static_cast<int64_t>(n0) * p.G;
+    const uint32_t over = reinterpret_cast<uintptr_t>(base) & 3;
+    return ScaleRows{base - over, over + (static_cast<uint32_t>(of_a ? first : first - BM) + lane) * p.G, over + static_cast<uint32_t>(of_a ? rows : cols) * p.G};
+  };
   auto load_scales = [&](int w) {
-    const mx_lds_bytes to = lds + Tile::STAGES * Tile::STAGE + (w & 1) * Tile::TABLE;
     const bool in = 4 * w < steps;
+    if (RAGGED) {
+#pragma unroll
+      for (int j = 0; j < Tile::S_INST; ++j) {
+        const ScaleRows r = scale_rows(j);
+        const auto src = make_rsrc(r.base, in ? (r.bytes + 3) & ~3u : 0);  // whole words, the last with up to three bytes of something else
+        const uint32_t from = (r.at + 16 * w) & ~3u;
+        const v4i four = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, from, 0, 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) words[j][i] = four[i];
+        words[j][4] = __builtin_amdgcn_raw_buffer_load_b32(src, from + 16, 0, 0);
+      }
+      return;
+    }
+    const mx_lds_bytes to = lds + Tile::STAGES * Tile::STAGE + (w & 1) * Tile::TABLE;
 #pragma unroll
     for (int j = 0; j < Tile::S_INST; ++j) {
       const int first = (j * Tile::WAVES + wave) * 64;
       const bool of_a = first < BM;
       const auto src = make_rsrc(of_a ? p.a_s + m0 * p.pitch : p.b_s + static_cast<int64_t>(n0) * p.pitch, in ? (of_a ? rows : cols) * p.pitch : 0);
       load_to_lds<0>(src, to + first * 16, ((of_a ? first : first - BM) + lane) * static_cast<uint32_t>(p.pitch), in ? 16 * w : 0);
+    }
+  };
+
+  auto store_scales = [&](int w) {
+#pragma unroll
+    for (int j = 0; j < Tile::S_INST; ++j) {
+      const uint32_t shift = scale_rows(j).at & 3;
+      v4i v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int left = p.G - 16 * w - 4 * i;
+        v[i] = __builtin_amdgcn_alignbyte(words[j][i + 1], words[j][i], shift) & (left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1);
+      }
+      *reinterpret_cast<v4i*>(smem + Tile::STAGES * Tile::STAGE + (w & 1) * Tile::TABLE + ((j * Tile::WAVES + wave) * 64 + lane) * 16) = v;
     }
   };
 
@@ -267,6 +309,7 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
   uint32_t as[MF], bs[NF];
 
   load_scales(0);
+  if (RAGGED) store_scales(0);
   load_stage(0), load_stage(1), load_stage(2);
   constexpr int kGroup = Tile::A_INST + Tile::B_INST;
   for (int k0 = 0; k0 < steps; k0 += 4) {
@@ -274,8 +317,8 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
     for (int j = 0; j < 4; ++j) {
       const int k = k0 + j;
       if (k >= steps) break;
-      // in order: what is behind stage k is two stages, and the next scales if they were asked for in between
-      if (j == 1 || j == 2)
+      // in order: what is behind stage k is two stages, and the next scales if they were asked for in between (RAGGED: wherever the compiler put those)
+      if (!RAGGED && (j == 1 || j == 2))
         wait_loads<2 * kGroup + Tile::S_INST>();
       else
         wait_loads<2 * kGroup>();
@@ -299,6 +342,7 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
       for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int n = 0; n < NF; ++n) acc[i][n] = mfma_mx_step(j, bf[n], bs[n], af[i], as[i], acc[i][n]);
+      if (RAGGED && j == 3) store_scales(k / 4 + 1);  // the other table, which was read for the last time a window ago
     }
   }
   wait_loads<0>();  // nothing is on its way into LDS when the workgroup ends

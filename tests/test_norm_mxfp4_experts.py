@@ -80,9 +80,9 @@ def test_mxfp4_entry_points_refuse():
         (dict(M=1 << 31), SHAPE), (dict(N=(1 << 27) + 1), SHAPE), (dict(a=null), NULL), (dict(b=null), NULL), (dict(a_s=null), NULL), (dict(b_s=null), NULL), (dict(c=null), NULL),
         (dict(a=at(4104)), ALIGN), (dict(b=at(4104)), ALIGN), (dict(a_s=at(4098)), ALIGN), (dict(b_s=at(4098)), ALIGN), (dict(c=at(4097)), ALIGN), (dict(dt=2, c=at(4098)), ALIGN),
         (dict(M=0, a=null), OK), (dict(N=0, c=null), OK)])
-    need = lib.dlb_mxfp4_gemm_workspace_bytes(1000, 1000, 96)
-    assert need > 0 and lib.dlb_mxfp4_gemm_workspace_bytes(1000, 1000, 256) == 0 == lib.dlb_mxfp4_gemm_workspace_bytes(4, 64, 96) and lib.dlb_mxfp4_gemm_workspace_bytes(0, 64, 96) == 0 == lib.dlb_mxfp4_gemm_workspace_bytes(-1, 64, 96)
-    refused('dlb_mxfp4_gemm', dict(good, M=1000, N=1000, K=96, ws=fake, wsb=need), [(dict(ws=null), WORKSPACE), (dict(wsb=need - 1), WORKSPACE), (dict(ws=at(4104)), ALIGN)])
+    need = lib.dlb_mxfp4_gemm_workspace_bytes(4096, 4096, 96)
+    assert need > 0 and lib.dlb_mxfp4_gemm_workspace_bytes(4096, 4096, 256) == 0 == lib.dlb_mxfp4_gemm_workspace_bytes(4, 64, 96) and lib.dlb_mxfp4_gemm_workspace_bytes(0, 64, 96) == 0 == lib.dlb_mxfp4_gemm_workspace_bytes(-1, 64, 96)
+    refused('dlb_mxfp4_gemm', dict(good, M=4096, N=4096, K=96, ws=fake, wsb=need), [(dict(ws=null), WORKSPACE), (dict(wsb=need - 1), WORKSPACE), (dict(ws=at(4104)), ALIGN)])
     good = dict(x=fake, x_rs=256, dt=0, q=fake, s=fake, y=fake, M=4, N=64, K=256, st=null)
     refused('dlb_mxfp4_weight_gemm', good, [
         (dict(dt=2), DTYPE), (dict(M=-1), SHAPE), (dict(N=-1), SHAPE), (dict(K=0), SHAPE), (dict(K=100), SHAPE), (dict(K=(1 << 22) + 32), SHAPE), (dict(M=(1 << 21) + 1), SHAPE),

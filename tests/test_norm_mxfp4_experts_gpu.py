@@ -170,7 +170,7 @@ def test_two_graphs_in_flight_at_once(dev, which):
             args = (torch.randn(16, 1024, generator=g).to(bf16).to(dev), torch.randint(0, 8, (16, 4), generator=g).to(dev), torch.rand(16, 4, generator=g).to(dev), up, down)
             calls.append(lambda args=args: few_token_experts(*args))
         else:
-            a, b = (tuple(t.to(dev) for t in codes((n, ), 1056, g)) for n in (700, 900))
+            a, b = (tuple(t.to(dev) for t in codes((n, ), 1056, g)) for n in (3000, 2900))
             calls.append(lambda a=a, b=b: mxfp4_gemm(a[0], b[0], a[1], b[1], bf16))
     want = [call() for call in calls]
     graphs, held = [], []
@@ -472,6 +472,27 @@ def test_scales_off_their_words(dev, columns):
     for n in (1, 2, 3):
         assert torch.equal(mxfp4_gemm(moved(a, n), moved(b, n), moved(a_s, n), moved(b_s, n), f32), want)
         assert torch.equal(mxfp4_weight_gemm(x, b, moved(b_s, n)), few)
+
+
+# few rows against many columns, blocks of rows that still fill no card, small and large tiles; whole words of scales and others
+WAYS = [(9, 4130, 544), (16, 5000, 768), (32, 9000, 96), (20, 4200, 1280), (40, 4200, 544), (64, 5000, 1024), (70, 200, 1056), (130, 900, 640), (300, 1000, 640), (257, 1030, 1056),
+        (1500, 1600, 640), (1411, 1633, 288), (1500, 1601, 1056)]
+
+
+@pytest.mark.parametrize('M,N,K', WAYS)
+def test_products_of_every_size(dev, M, N, K):
+    """One row and one column have a first scale that is no number: their results alone are none, also where a row's scales end inside a word."""
+    print(f'case {M}x{N}x{K}', flush=True)
+    g = torch.Generator().manual_seed(M + N + K)
+    (a, a_s), (b, b_s) = codes((M, ), K, g), codes((N, ), K, g)
+    a_s[M // 2, 0] = b_s[N // 3, 0] = 255
+    got = mxfp4_gemm(*(t.to(dev) for t in (a, b, a_s, b_s)), f32).cpu()
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[M // 2], nan[:, N // 3] = True, True
+    assert torch.equal(got.isnan(), nan)
+    a_s[M // 2, 0] = b_s[N // 3, 0] = 122
+    want, mag = orc.gemm(a, a_s, b, b_s)
+    inside(got[~nan], want[~nan], product_bound(K, mag)[~nan], f'{M}x{N}x{K}')
 
 
 def test_the_widest_rows(dev):
