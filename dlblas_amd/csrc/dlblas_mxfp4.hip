@@ -215,15 +215,19 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   a.ids_is64 = ids_dtype == DLB_IDX_I64;
   const int64_t slots = tokens * topk;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 up_grid(static_cast<unsigned>(I / 16), static_cast<unsigned>(std::min(experts, slots))), down_grid(static_cast<unsigned>(ceil_div(H, 16 * kDownTiles)));
-  // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches.  The second product's
-  // rows share the LDS with what is on its way of the weights: few rows and eight waves while an expert has about three tokens or fewer (8 tokens, 8 of 32 experts,
-  // 7168 x 2048: e4m3 79 us, e2m1 59 us, with eight rows 103 and 75 us); more tokens leave no room for eight waves' sums, or, of e2m1, are no faster by them (16 tokens: 88 us with either).
+  const dim3 down_grid(static_cast<unsigned>(ceil_div(H, 16 * kDownTiles)));
+  // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches, and x for rows without a token is
+  // not read.  8 of 32 experts, 4096 x 7168, us e4m3 / e2m1: 8 tokens by four 148 / 100, by eight 131 / 110; 16 tokens by eight 146 / 121, by sixteen 163 / 147;
+  // 32 tokens by eight 224 / 181, by sixteen 174 / 154.
+  // The second product's rows share the LDS with what is on its way of the weights: four tokens a pass and eight waves while an expert has three or fewer (7168 x 2048,
+  // 8 tokens: 79 / 59, by eight 103 / 75); eight waves as long as there is room for their sums (16 tokens e4m3: 96, four waves 113; e2m1 is no faster by them, 88).
   const int64_t named = std::min(experts, slots), mean = slots / named;
   const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16;
   const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
-      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), up_grid, dim3(64 * kUpWaves), (UpShape<kw(), r()>::kLds), st, a);
+      typedef UpShape<kw(), r()> Shape;
+      const dim3 grid(static_cast<unsigned>(I / (16 * Shape::kPairs)), static_cast<unsigned>(named));
+      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
     });
     const auto down = [&](auto t, auto waves) {
       const int64_t lds = experts_down_lds<kw(), t(), waves()>(tokens, topk, experts);
