@@ -149,19 +149,24 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (misaligned(q, 16) || misaligned(x, 4) || x_row_stride % 2 != 0 || off_elements(y, dtype))
     return fail(DLB_ERR_ALIGNMENT, "q must be 16-byte, rows of x 4-byte aligned, y to its elements");
   const FewArgs a{x, y, M, x_row_stride, Matrix{static_cast<const uint8_t*>(q), s, static_cast<int>(N), static_cast<int>(K)}};
-  const int rows = M <= 4 ? 4 : M <= 8 ? 8 : 16, nt = N >= 6400 ? 2 : 1;
+  // As few tiles of columns a workgroup as leave one for each CU: more of them share the rows, whose copies are most of what comes into LDS, and of up to eight rows
+  // two are enough.  us with 1, 2, 4 tiles: 16 x 4096 x 7168 9.3, 12.0, 16.5;  16 x 7168 x 18432 30, 23, 33;  32 x 4096 x 7168 16.5, 11.9, 16.2;
+  // 64 x 7168 x 18432 94, 71, 57;  8 x 18432 x 7168 31, 26, 32.  Rows: 4 x 7168 x 18432 by four 16.7, by eight 17.4;  8 by eight 19.3, by sixteen 19.5;  8 x 18432 x 7168 26, 31.
+  const int rows = M <= 4 ? 4 : M <= 8 ? 8 : 16;
+  const auto groups = [&](int tiles) { return ceil_div(M, rows) * ceil_div(N, 16 * tiles); };
+  const int nt = groups(1) <= 256 ? 1 : groups(2) <= 256 || rows < 16 ? 2 : 4;
   const int64_t tiles = ceil_div(N, 16 * nt);
   if (ceil_div(tiles, 8) > 65535) return fail(DLB_ERR_BAD_SHAPE, "N=%lld beyond the supported range", (long long)N);
   const dim3 grid(static_cast<unsigned>(8 * ceil_div(M, rows)), static_cast<unsigned>(ceil_div(tiles, 8)));
   with_flag(dtype == kInBf16, [&](auto bf16) {
     with_flag(bytes_apart(s, K), [&](auto ragged) {
-      with_chunks<4, 8, 16>(rows, [&](auto r) {
-        with_chunks<1, 2>(nt, [&](auto n) {
-          typedef FewShape<kE2m1, r(), n()> Shape;
-          hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n(), ragged()>), grid, dim3(64 * Shape::kWaves), Shape::kLds,
-                             static_cast<hipStream_t>(stream), a);
-        });
-      });
+      const auto launch = [&](auto r, auto n) {
+        typedef FewShape<kE2m1, r(), n()> Shape;
+        hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n(), ragged()>), grid, dim3(64 * Shape::kWaves), Shape::kLds,
+                           static_cast<hipStream_t>(stream), a);
+      };
+      if (rows == 16) return with_chunks<1, 2, 4>(nt, [&](auto n) { launch(std::integral_constant<int, 16>(), n); });
+      with_chunks<4, 8>(rows, [&](auto r) { with_chunks<1, 2>(nt, [&](auto n) { launch(r, n); }); });
     });
   });
   return finish("mxfp4_weight_gemm");

@@ -495,6 +495,15 @@ def test_products_of_every_size(dev, M, N, K):
     inside(got[~nan], want[~nan], product_bound(K, mag)[~nan], f'{M}x{N}x{K}')
 
 
+@pytest.mark.parametrize('M,N,K', [(3, 4200, 1024), (7, 4200, 544), (16, 4200, 256), (9, 9000, 1056), (16, 8210, 768), (40, 5000, 1024), (64, 4100, 160)])
+def test_few_rows_of_every_size(dev, M, N, K):
+    print(f'case {M}x{N}x{K}', flush=True)
+    g = torch.Generator().manual_seed(M + N + K)
+    x, (q, s) = torch.randn(M, K, generator=g).to(bf16), codes((N, ), K, g)
+    w, rows = orc.values(q, s), x.double()
+    inside(mxfp4_weight_gemm(*(t.to(dev) for t in (x, q, s))), rows @ w.t(), (K + 16) * 2 * orc.FP32 * (rows.abs() @ w.abs().t()), f'{M}x{N}x{K}')
+
+
 def test_the_widest_rows(dev):
     K = 1 << 22
     g = torch.Generator().manual_seed(9)
@@ -557,7 +566,7 @@ def test_weights_whose_offsets_pass_32_bits(dev):
     assert q.numel() > 2**32
     x = torch.randn(9, K, device=dev, generator=g).to(bf16)
     y = mxfp4_weight_gemm(x, q, s)
-    for at in (slice(0, 6400), slice(N - 6400, N)):  # as many as make the tiles as wide
+    for at in (slice(0, 20000), slice(N - 20000, N)):  # as many as make the tiles as wide
         assert torch.equal(y[:, at], mxfp4_weight_gemm(x, q[at].clone(), s[at].clone()))
     del q, s
     H, I = 2048, 2048
