@@ -89,6 +89,14 @@ int norm_grad_shares(int64_t rows, int64_t H) {
   return static_cast<int>(std::min<int64_t>(ceil_div(rows, rows_each), 512) * (kNarrowThreads / 64));
 }
 
+// Those of the layer norm, 16 waves a CU: a second bias's worth of shares makes them dearer, and with a row's eight columns to a lane and its weights in registers one wide
+// workgroup has as many loads on its way as two (4096 x 7168 with residual and bias: 256 of them 41 us, 512 47).
+int layer_norm_grad_shares(int64_t rows, int64_t H) {
+  if (H % 8 == 0 && H <= 256) return norm_grad_shares(rows, H);
+  const int64_t waves = ceil_div(H, 512);
+  return static_cast<int>(std::min(rows, std::max<int64_t>(waves > 8 ? 256 : 512, std::min(256 * std::max<int64_t>(1, 16 / waves), rows / 8))));
+}
+
 // ---- tokens by expert -------------------------------------------------------------------------------------------------
 
 int check_rows(int64_t tokens, int64_t H, int64_t topk, int64_t num_rows) {
@@ -306,7 +314,7 @@ int dlb_layer_norm(const void* x, int64_t x_row_stride, const void* residual, in
 }
 
 size_t dlb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H, int with_bias) {
-  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::norm_grad_shares(rows, H)) * H * (with_bias ? 2 : 1) * sizeof(float) : 0;
+  return rows > 0 && H > 0 ? static_cast<size_t>(dlb::layer_norm_grad_shares(rows, H)) * H * (with_bias ? 2 : 1) * sizeof(float) : 0;
 }
 
 int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
@@ -330,7 +338,7 @@ int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* d
     if (dw && misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int shares = rows > 0 ? norm_grad_shares(rows, H) : 0, columns = static_cast<int>(db ? 2 * H : H);
+  const int shares = rows > 0 ? layer_norm_grad_shares(rows, H) : 0, columns = static_cast<int>(db ? 2 * H : H);
   if (rows > 0) {
     LayerNormGradArgs a{};
     a.dy = dy, a.dsum = dsum, a.h = h, a.w = weight, a.stats = stats, a.dx = dx, a.part = dw ? static_cast<float*>(workspace) : nullptr;
@@ -346,7 +354,7 @@ int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* d
             constexpr std::true_type whole;
             if (with_lanes(H, [&](auto lanes) { launch(t, ds, bias, whole, kOne, lanes, shares / (kNarrowThreads / 64), lanes(), kNarrowThreads / lanes()); })) return;
           }
-          const RowShape shape = row_shape(H, dtype != kInF32 && H > 4096 ? 2 : 1);
+          const RowShape shape = row_shape(H, 1);
           with_flag(H % 8 == 0, [&](auto whole) {
             with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, ds, bias, whole, c, kWave, shares, shape.threads, 1); });
           });

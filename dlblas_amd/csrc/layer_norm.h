@@ -162,6 +162,17 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       if (DSUM && CH < 4) r.ds[c] = load_raw8<T, WHOLE>(p.dsum, row * p.dsum_rs, col, p.H - col);
     }
   };
+  // The weights stay in registers where rows are asked for ahead: loads return in order, so a weight that is loaded behind the next row waits for that row.
+  float kept[kAhead ? CH : 1][8];
+  if (kAhead) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], kept[c]);
+  }
+  const auto weights = [&](int c, float(&w)[8]) {
+    if (!kAhead) return load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = kept[c][k];
+  };
   Row now, next;
   if (kAhead) load(min(static_cast<int64_t>(worker), p.rows - 1), now);
   int turn = 0;
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       float hv[8], g[8], w[8], s = 0.f, d = 0.f;
       quant_unpack8<T>(now.h[c], hv);
       quant_unpack8<T>(now.dy[c], g);
-      load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], w);
+      weights(c, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {  // elements past the end: g is zero
         const float t = g[k] * w[k];
@@ -202,7 +213,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       float hv[8], g[8], w[8];
       quant_unpack8<T>(now.h[c], hv);
       quant_unpack8<T>(now.dy[c], g);
-      load_weight8<T, WHOLE>(p.w, p.w_f32, 8 * at[c], p.H - 8 * at[c], w);
+      weights(c, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float n = (hv[k] - mean) * r;
