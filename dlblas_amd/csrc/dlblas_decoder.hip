@@ -301,12 +301,14 @@ int dlb_layer_norm(const void* x, int64_t x_row_stride, const void* residual, in
   with_type(dtype, [&](auto t) {
     with_flag(residual != nullptr, [&](auto res) {
       if (H % 8 == 0) {
-        constexpr std::true_type whole;
+        constexpr std::integral_constant<Edge, kOnChunk> whole;
         if (with_lanes(H, [&](auto lanes) { launch(t, res, whole, kOne, lanes, lanes(), kNarrowThreads / lanes()); })) return;
       }
       const RowShape shape = row_shape(H, 2);
+      if (H < 8) return launch(t, res, std::integral_constant<Edge, kBelowChunk>(), kOne, kWave, 64, 1);
       with_flag(H % 8 == 0, [&](auto whole) {
-        with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, res, whole, c, kWave, shape.threads, 1); });
+        constexpr std::integral_constant<Edge, whole() ? kOnChunk : kInChunk> edge;
+        with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, res, edge, c, kWave, shape.threads, 1); });
       });
     });
   });
@@ -351,12 +353,14 @@ int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* d
       with_flag(dsum != nullptr, [&](auto ds) {
         with_flag(db != nullptr, [&](auto bias) {
           if (H % 8 == 0) {
-            constexpr std::true_type whole;
+            constexpr std::integral_constant<Edge, kOnChunk> whole;
             if (with_lanes(H, [&](auto lanes) { launch(t, ds, bias, whole, kOne, lanes, shares / (kNarrowThreads / 64), lanes(), kNarrowThreads / lanes()); })) return;
           }
           const RowShape shape = row_shape(H, 1);
+          if (H < 8) return launch(t, ds, bias, std::integral_constant<Edge, kBelowChunk>(), kOne, kWave, shares, 64, 1);
           with_flag(H % 8 == 0, [&](auto whole) {
-            with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, ds, bias, whole, c, kWave, shares, shape.threads, 1); });
+            constexpr std::integral_constant<Edge, whole() ? kOnChunk : kInChunk> edge;
+            with_chunks<1, 2, 4>(shape.chunks, [&](auto c) { launch(t, ds, bias, edge, c, kWave, shares, shape.threads, 1); });
           });
         });
       });

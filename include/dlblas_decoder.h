@@ -72,6 +72,7 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
  *   x, residual, y, sum  [rows, H]  one element type (dtype); residual NULL: none, and sum is not written
  *   weight, bias         [H]        the same type, or fp32 (weight_dtype, of both); bias NULL: none
  *   stats                [rows, 2]  fp32, OUT: m and r of every row, for dlb_layer_norm_backward; NULL: not wanted
+ * No output overlaps an input.
  */
 int dlb_layer_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, int dtype,
                    const void* weight, const void* bias, int weight_dtype, void* y, int64_t y_row_stride, void* sum,
@@ -86,7 +87,7 @@ size_t dlb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H, int with
  * sums is fixed.
  *
  *   dy, dsum, h, dx  [rows, H]  dtype; dsum (gradient of sum) may be NULL
- *   dw, db           [H]        weight_dtype; db NULL: not wanted, both NULL: neither
+ *   dw, db           [H]        weight_dtype; db NULL: not wanted, both NULL: neither.  No output overlaps an input.
  *   workspace        4-byte aligned, dlb_layer_norm_backward_workspace_bytes(rows, H, db ? 1 : 0), no initialisation
  */
 int dlb_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsum, int64_t dsum_row_stride, const void* h,
