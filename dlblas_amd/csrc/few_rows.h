@@ -100,18 +100,19 @@ struct Stream {
   static constexpr int kLoads = NT * (RAGGED ? 2 : 3) + kXLoads;
   static_assert((R == 4 || R == 8 || R == 16) && DEPTH >= 2 && (DEPTH - 1) * kLoads < 64 && !(RAGGED && W == kE4m3), "whole loads of x, a counter of six bits");
 
-  // 16 rows of a matrix, from row n0 on.
+  // 16 rows of a matrix, from row n0 on; past its end the last that it has (a buffer of no bytes would not do: its end is compared with what a chunk's offset leaves of it).
   struct Tile {
     const uint8_t *q, *s;
     uint32_t q_bytes, s_bytes;
     __device__ __forceinline__ void point_at(const Matrix& m, int n0) {
-      const int rows = max(0, min(16, m.N - n0));
+      n0 = min(n0, (m.N - 1) / 16 * 16);
+      const int rows = min(16, m.N - n0);
       const uint32_t q_pitch = W == kE2m1 ? m.K / 2 : m.K;
       q = m.q + static_cast<int64_t>(n0) * q_pitch, q_bytes = rows * q_pitch;
       if (W == kE2m1)
         s = static_cast<const uint8_t*>(m.s) + static_cast<int64_t>(n0) * (m.K / kMxGroup), s_bytes = rows * (m.K / kMxGroup);
       else
-        s = reinterpret_cast<const uint8_t*>(static_cast<const float*>(m.s) + static_cast<int64_t>(n0 / 128) * (m.K / 128)), s_bytes = rows > 0 ? m.K / 32 : 0;
+        s = reinterpret_cast<const uint8_t*>(static_cast<const float*>(m.s) + static_cast<int64_t>(n0 / 128) * (m.K / 128)), s_bytes = m.K / 32;
       q = in_scalar(q), s = in_scalar(s), q_bytes = in_scalar(q_bytes), s_bytes = in_scalar(s_bytes);
     }
   };
