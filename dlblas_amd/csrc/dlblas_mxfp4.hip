@@ -222,17 +222,26 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 down_grid(static_cast<unsigned>(ceil_div(H, 16 * kDownTiles)));
   // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches, and x for rows without a token is
-  // not read.  8 of 32 experts, 4096 x 7168, us e4m3 / e2m1: 8 tokens by four 148 / 100, by eight 131 / 110; 16 tokens by eight 146 / 121, by sixteen 163 / 147;
-  // 32 tokens by eight 224 / 181, by sixteen 174 / 154.
+  // not read.  8 of 32 experts, 4096 x 7168, us e4m3 / e2m1 (with four waves to K): 8 tokens by four 148 / 100, by eight 131 / 110; 16 tokens by eight 146 / 121, by sixteen
+  // 163 / 147; 32 tokens by eight 224 / 181, by sixteen 174 / 154.
   // The second product's rows share the LDS with what is on its way of the weights: four tokens a pass and eight waves while an expert has three or fewer (7168 x 2048,
   // 8 tokens: 79 / 59, by eight 103 / 75); eight waves as long as there is room for their sums (16 tokens e4m3: 96, four waves 113; e2m1 is no faster by them, 88).
   const int64_t named = std::min(experts, slots), mean = slots / named;
   const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16;
   const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
+    const auto up = [&](auto r, auto split) {
+      typedef UpShape<kw(), r(), split()> Shape;
+      const dim3 grid(static_cast<unsigned>(ceil_div(I, Shape::kColumns)), static_cast<unsigned>(named));
+      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), split(), ragged_up()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
+    };
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
-      typedef UpShape<kw(), r()> Shape;
-      const dim3 grid(static_cast<unsigned>(I / (16 * Shape::kPairs)), static_cast<unsigned>(named));
-      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), ragged_up()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
+      // Two waves to K, whose runs are then long against their start and end; four where K is short, or an e4m3 expert has few rows.  e2m1 / e4m3 us, 8 of 32 experts,
+      // 4096 x 7168: 8 tokens two 96 / 133, four 109 / 130;  16 tokens 104 / 144, 122 / 149;  64 tokens 194 / 230, 228 / 250;  5 tokens, 1088 x 1056: 12.3, four 9.0.
+      if constexpr (kw() == kE2m1) {
+        with_flag(H >= 4096, [&](auto two) { up(r, std::integral_constant<int, two() ? 2 : 4>()); });
+      } else {
+        up(r, std::integral_constant<int, r() == 16 ? 2 : 4>());
+      }
     });
     const auto down = [&](auto t, auto waves) {
       const int64_t lds = experts_down_lds<kw(), t(), waves()>(tokens, topk, experts);

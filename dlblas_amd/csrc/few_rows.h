@@ -5,7 +5,7 @@
 //   e2m1   with a power of two per 32 columns.  Beside bf16 rows the scale goes into the conversion: e2m1 has two bits of significand and bf16 the
 //          range of the scales, so the products stay exact (weights below 2^-126, which are subnormal numbers of bf16, may count as 0).  fp16 has not
 //          that range: there a group's sum meets its scale in fp32.
-// The waves of a workgroup split K and add their sums through LDS in wave order.
+// Waves split K and add their sums through LDS in wave order.
 #pragma once
 
 #include "mxfp4.h"
@@ -366,10 +366,11 @@ __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + __
 
 constexpr int kUpWaves = 4;
 // Pairs of tiles of Gate and Up that share the rows of x, which are most of what comes into LDS where there are 16 of them (64 tokens, 8 of 32 experts, 4096 x 7168:
-// two pairs 226 us e2m1, 251 us e4m3, one 306 and 280 us; eight rows, 16 tokens: 131 and 169 us, one 121 and 146 us).
-template <int W, int R>
+// two pairs 226 us e2m1, 251 us e4m3, one 306 and 280 us; eight rows, 16 tokens: 131 and 169 us, one 121 and 146 us; all with four waves to K).
+template <int W, int R, int SPLIT>
 struct UpShape {
-  static constexpr int kPairs = R == 16 ? 2 : 1, kTiles = 2 * kPairs, kBudget = 2 * kUpWaves * stream_bytes(W, R, kTiles) <= 76 * 1024 ? 76 * 1024 : 152 * 1024;  // two workgroups a CU, or one
+  static constexpr int kPairs = R == 16 ? 2 : 1, kColumns = 16 * kPairs * kUpWaves / SPLIT;  // of a workgroup
+  static constexpr int kTiles = 2 * kPairs, kBudget = 2 * kUpWaves * stream_bytes(W, R, kTiles) <= 76 * 1024 ? 76 * 1024 : 152 * 1024;  // two workgroups a CU, or one
   static constexpr int kDepth = stream_depth(W, R, kTiles, kUpWaves, kBudget), kLds = kUpWaves * kDepth * stream_bytes(W, R, kTiles);
 };
 
@@ -383,11 +384,11 @@ struct DownShape {
   static constexpr int kDepth = stream_depth(W, 2 * TOKENS, kDownTiles, WAVES, kBudget), kRing = WAVES * kDepth * stream_bytes(W, 2 * TOKENS, kDownTiles);
 };
 
-// A workgroup takes the rows of its pairs of Gate and Up, of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
+// A workgroup takes kColumns rows of Gate and the same of Up, SPLIT waves share K; of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
 // it is the first to name it; R of its tokens at a time.
-template <int T, int W, int R, bool RAGGED>
+template <int T, int W, int R, int SPLIT, bool RAGGED>
 __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertArgs p) {
-  typedef UpShape<W, R> Shape;
+  typedef UpShape<W, R, SPLIT> Shape;
   constexpr int kPairs = Shape::kPairs, kTiles = Shape::kTiles;
   typedef Stream<T, W, R, kTiles, Shape::kDepth, RAGGED> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
   if (by_slot && __shfl(first, __builtin_ctzll(mask)) != y) return;
   const int rows = __popcll(mask), token_of = nth_lane(mask, lane);
   const Matrix up = of_expert(p.up, p.up_q, p.up_s, e);
-  const int n0 = blockIdx.x * 16 * kPairs;
+  const int of = wave % SPLIT, n0 = blockIdx.x * Shape::kColumns + wave / SPLIT * 16 * kPairs;  // past the end: nothing is stored
   const int64_t rest = static_cast<int64_t>(slots) * p.I;
   v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][tiles][64]
   for (int b = 0; b < rows; b += R) {
@@ -434,15 +435,17 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
       const int t = __shfl(token_of, i & 63);
       s.set_row(lane, j, i < rows ? static_cast<uint32_t>(t * p.x_rs) * 2 : kNowhere);
     }
-    s.split_k(lane, wave, kUpWaves);
+    s.split_k(lane, of, SPLIT);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) part[(kTiles * wave + n) * 64 + lane] = s.acc[n];
     __syncthreads();
-    if (wave >= kPairs) continue;
-    v4f g = part[2 * wave * 64 + lane], u = part[(2 * wave + 1) * 64 + lane];
+    static_assert(kPairs <= SPLIT, "a wave for each");
+    if (of >= kPairs || n0 + 16 * of >= p.I) continue;
+    const v4f* const mine = part + (kTiles * (wave - of) + 2 * of) * 64;
+    v4f g = mine[lane], u = mine[64 + lane];
 #pragma unroll
-    for (int w = 1; w < kUpWaves; ++w) g += part[(kTiles * w + 2 * wave) * 64 + lane], u += part[(kTiles * w + 2 * wave + 1) * 64 + lane];
+    for (int w = 1; w < SPLIT; ++w) g += mine[kTiles * w * 64 + lane], u += mine[(kTiles * w + 1) * 64 + lane];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = b + 4 * q + r;
@@ -453,7 +456,7 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
       const __bf16 hi = static_cast<__bf16>(v);
       const float f = static_cast<float>(hi);
       const __bf16 lo = static_cast<__bf16>(fabsf(f) == __builtin_inff() ? 0.f : v - f);
-      uint16_t* const to = p.act + static_cast<int64_t>(slot) * p.I + n0 + 16 * wave + l16;
+      uint16_t* const to = p.act + static_cast<int64_t>(slot) * p.I + n0 + 16 * of + l16;
       to[0] = __builtin_bit_cast(uint16_t, hi), to[rest] = __builtin_bit_cast(uint16_t, lo);
     }
   }

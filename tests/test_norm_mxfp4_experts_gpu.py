@@ -440,6 +440,23 @@ def test_the_largest_tables_of_routing(dev, T, E, topk, kind):
         inside(out, *orc.experts(x, ids, weights, w13, w2), f'{T} tokens')
 
 
+@pytest.mark.parametrize('kind', ['f8', 'f4'])
+@pytest.mark.parametrize('T,dtype', [(1, f16), (6, bf16), (40, bf16), (40, f16)])
+def test_long_rows(dev, T, dtype, kind):
+    """Columns of x that two waves share, and halves of a workgroup's columns that an expert does not have."""
+    g = torch.Generator().manual_seed(T)
+    E, topk, H, I = 3, 2, 4224, 128 if kind == 'f8' else 96
+    x, weights, ids = torch.randn(T, H, generator=g).to(dtype), torch.rand(T, topk, generator=g), torch.randint(0, E, (T, topk), generator=g)
+    if kind == 'f4':
+        up, down = codes((E, 2 * I), H, g, 118), codes((E, H), I, g, 118)
+        w13, w2 = orc.values(*up), orc.values(*down)
+    else:
+        up, down = ((torch.randn(E, n, k, generator=g).to(f8), 0.01 * (1 + torch.rand(E, n // 128, k // 128, generator=g))) for n, k in ((2 * I, H), (H, I)))
+        w13, w2 = orc.e4m3_values(*up), orc.e4m3_values(*down)
+    on = lambda pair: tuple(t.to(dev) for t in pair)
+    inside(few_token_experts(x.to(dev), ids.to(dev), weights.to(dev), on(up), on(down)), *orc.experts(x, ids, weights, w13, w2), f'{T} tokens')
+
+
 def test_rows_and_ids_that_are_broadcast_and_weights_of_nobody(dev):
     g = torch.Generator().manual_seed(7)
     up, down = (tuple(t.to(dev) for t in codes((4, n), k, g)) for n, k in ((192, 160), (160, 96)))
