@@ -257,10 +257,8 @@ struct Stream {
 __device__ __forceinline__ void store1(void* to, int type, int64_t at, float v) {
   if (type == kInBf16)
     static_cast<__bf16*>(to)[at] = static_cast<__bf16>(v);
-  else if (type == kInF16)
-    static_cast<_Float16*>(to)[at] = static_cast<_Float16>(v);
   else
-    static_cast<float*>(to)[at] = v;
+    static_cast<_Float16*>(to)[at] = static_cast<_Float16>(v);
 }
 
 // ---- one matrix -------------------------------------------------------------------------------------------------------

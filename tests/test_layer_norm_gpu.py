@@ -1,6 +1,6 @@
 """Layer norm and its gradients against the definitions in 64 bits; the bounds are those of oracle/layer_norm.py plus half a step of the stored
-type.  dw, db: a workgroup adds rows / 512 terms, a lane of the second kernel an eighth of a sixteenth of up to 4096 shares, and their sums
-are added in 3 + 4 steps: below rows / 512 + 128 + 60 roundings of the sum of magnitudes, as for the RMS norm."""
+type.  dw, db: a workgroup adds at most rows / 256 + 1 terms, a lane of the second kernel an eighth of a sixteenth of up to 4096 shares, and their sums
+are added in 3 + 4 steps: below rows / 256 + 128 + 60 roundings of the sum of magnitudes, as for the RMS norm."""
 import pytest
 import torch
 
@@ -155,7 +155,7 @@ def test_gradients(dev, rows, H, residual, bias, dtype):
     inside(got['x'], dx, dx_off, 'dx')
     if residual:
         assert torch.equal(got['res'], got['x'])
-    adds = -(-rows // 512) + 128 + 60
+    adds = -(-rows // 256) + 128 + 60
     inside(got['w'], dw, n_off + adds * orc.FP32 * dw_mag, 'dw')
     if bias:
         inside(got['b'], db, adds * orc.FP32 * db_mag, 'db')
