@@ -35,9 +35,6 @@ MxWay mx_way(int64_t M, int64_t N) {
 bool mx_pads(int64_t M, int64_t N, int64_t K) { return mx_way(M, N) == MxWay::kTiles256 && K / kMxGroup % 4 != 0; }
 int64_t padded(int64_t G) { return ceil_div(G, 4) * 4; }
 
-// Rows of scales that do not start on four bytes: kernels of a few rows load them byte by byte.
-bool bytes_apart(const void* s, int64_t K) { return K / kMxGroup % 4 != 0 || misaligned(s, 4); }
-
 // Tiles of BM x BN; at most as many workgroups as a launch has threads for.
 int mx_tiles(MxArgs& a, int BM, int BN, int threads) {
   const int64_t tiles_m = ceil_div(a.M, BM), tiles_n = ceil_div(a.N, BN);
@@ -50,7 +47,7 @@ template <class Split>
 int launch_split(MxArgs a, hipStream_t st) {
   if (int rc = mx_tiles(a, 16 * Split::MT, 16 * Split::NT, 64 * Split::WAVES)) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(a.tiles_n, 8) * 8 * a.tiles_m));
-  with_flag(a.G % 4 == 0, [&](auto dwords) { hipLaunchKernelGGL((mxfp4_split_kernel<Split, dwords()>), grid, dim3(64 * Split::WAVES), Split::LDS, st, a); });
+  hipLaunchKernelGGL(mxfp4_split_kernel<Split>, grid, dim3(64 * Split::WAVES), Split::LDS, st, a);
   return finish("mxfp4_gemm");
 }
 
@@ -159,15 +156,12 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
   if (ceil_div(tiles, 8) > 65535) return fail(DLB_ERR_BAD_SHAPE, "N=%lld beyond the supported range", (long long)N);
   const dim3 grid(static_cast<unsigned>(8 * ceil_div(M, rows)), static_cast<unsigned>(ceil_div(tiles, 8)));
   with_flag(dtype == kInBf16, [&](auto bf16) {
-    with_flag(bytes_apart(s, K), [&](auto ragged) {
-      const auto launch = [&](auto r, auto n) {
-        typedef FewShape<kE2m1, r(), n()> Shape;
-        hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n(), ragged()>), grid, dim3(64 * Shape::kWaves), Shape::kLds,
-                           static_cast<hipStream_t>(stream), a);
-      };
-      if (rows == 16) return with_chunks<1, 2, 4>(nt, [&](auto n) { launch(std::integral_constant<int, 16>(), n); });
-      with_chunks<4, 8>(rows, [&](auto r) { with_chunks<1, 2>(nt, [&](auto n) { launch(r, n); }); });
-    });
+    const auto launch = [&](auto r, auto n) {
+      typedef FewShape<kE2m1, r(), n()> Shape;
+      hipLaunchKernelGGL((few_rows_kernel<bf16() ? kInBf16 : kInF16, kE2m1, r(), n()>), grid, dim3(64 * Shape::kWaves), Shape::kLds, static_cast<hipStream_t>(stream), a);
+    };
+    if (rows == 16) return with_chunks<1, 2, 4>(nt, [&](auto n) { launch(std::integral_constant<int, 16>(), n); });
+    with_chunks<4, 8>(rows, [&](auto r) { with_chunks<1, 2>(nt, [&](auto n) { launch(r, n); }); });
   });
   return finish("mxfp4_weight_gemm");
 }
@@ -228,11 +222,11 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   // 8 tokens: 79 / 59, by eight 103 / 75); eight waves as long as there is room for their sums (16 tokens e4m3: 96, four waves 113; e2m1 is no faster by them, 88).
   const int64_t named = std::min(experts, slots), mean = slots / named;
   const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16;
-  const auto launch = [&](auto kt, auto kw, auto ragged_up, auto ragged_down) {
+  const auto launch = [&](auto kt, auto kw) {
     const auto up = [&](auto r, auto split) {
       typedef UpShape<kw(), r(), split()> Shape;
       const dim3 grid(static_cast<unsigned>(ceil_div(I, Shape::kColumns)), static_cast<unsigned>(named));
-      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), split(), ragged_up()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
+      hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), split()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
     };
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
       // Two waves to K, whose runs are then long against their start and end; four where K is short, or an e4m3 expert has few rows.  e2m1 / e4m3 us, 8 of 32 experts,
@@ -245,7 +239,7 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
     });
     const auto down = [&](auto t, auto waves) {
       const int64_t lds = experts_down_lds<kw(), t(), waves()>(tokens, topk, experts);
-      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), waves(), ragged_down()>), down_grid, dim3(64 * waves()), static_cast<size_t>(lds), st, a);
+      hipLaunchKernelGGL((experts_down_kernel<kt(), kw(), t(), waves()>), down_grid, dim3(64 * waves()), static_cast<size_t>(lds), st, a);
     };
     constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 4> four;
@@ -259,9 +253,10 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   };
   with_flag(dtype == kInBf16, [&](auto bf16) {
     constexpr std::integral_constant<int, bf16() ? kInBf16 : kInF16> kt;
-    constexpr std::false_type whole;
-    if (!f4) return launch(kt, std::integral_constant<int, kE4m3>(), whole, whole);
-    with_flag(bytes_apart(up_s, H), [&](auto up) { with_flag(bytes_apart(down_s, I), [&](auto down) { launch(kt, std::integral_constant<int, kE2m1>(), up, down); }); });
+    if (f4)
+      launch(kt, std::integral_constant<int, kE2m1>());
+    else
+      launch(kt, std::integral_constant<int, kE4m3>());
   });
   return finish("few_token_experts");
 }

@@ -79,7 +79,7 @@ struct Matrix {
 //
 // A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of weights
 // piece ^ (row / 2).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a word of its 16 bytes a
-// quarter.  RAGGED: e2m1, K is no multiple of 128.
+// quarter.  The eight scales of a row's chunk of e2m1 start at any byte: they come as the three words they can lie in.
 constexpr int stream_columns(int weights) { return weights == kE4m3 ? 128 : 256; }
 constexpr int kStreamTile = 2048 + 256;  // bytes of a tile's chunk: codes, and behind them scales
 constexpr int stream_x_loads(int weights, int R) { return R * stream_columns(weights) / 512; }
@@ -90,15 +90,13 @@ constexpr int stream_depth(int weights, int R, int NT, int waves, int bytes) {
   return depth > 6 ? 6 : depth;
 }
 
-template <int T, int W, int R, int NT, int DEPTH, bool RAGGED>
+template <int T, int W, int R, int NT, int DEPTH>
 struct Stream {
   static constexpr int kCols = stream_columns(W), kSteps = kCols / 32;
   static constexpr int kXPitch = 2 * kCols, kXLoads = stream_x_loads(W, R), kXLanes = kXPitch / 16;  // lanes of a load that share a row of x
   static constexpr int kChunk = stream_bytes(W, R, NT), kBytes = DEPTH * kChunk;
-  // Loads of a chunk into LDS, which is what is counted.  RAGGED scales come to registers, a byte a load: the compiler may issue those later than
-  // they are written, and a wait that counted them would end too early.
-  static constexpr int kLoads = NT * (RAGGED ? 2 : 3) + kXLoads;
-  static_assert((R == 4 || R == 8 || R == 16) && DEPTH >= 2 && (DEPTH - 1) * kLoads < 64 && !(RAGGED && W == kE4m3), "whole loads of x, a counter of six bits");
+  static constexpr int kLoads = NT * 3 + kXLoads;  // of a chunk
+  static_assert((R == 4 || R == 8 || R == 16) && DEPTH >= 2 && (DEPTH - 1) * kLoads < 64, "whole loads of x, a counter of six bits");
 
   // 16 rows of a matrix, from row n0 on; past its end the last that it has (a buffer of no bytes would not do: its end is compared with what a chunk's offset leaves of it).
   struct Tile {
@@ -109,10 +107,12 @@ struct Stream {
       const int rows = min(16, m.N - n0);
       const uint32_t q_pitch = W == kE2m1 ? m.K / 2 : m.K;
       q = m.q + static_cast<int64_t>(n0) * q_pitch, q_bytes = rows * q_pitch;
-      if (W == kE2m1)
-        s = static_cast<const uint8_t*>(m.s) + static_cast<int64_t>(n0) * (m.K / kMxGroup), s_bytes = rows * (m.K / kMxGroup);
-      else
+      if (W == kE2m1) {  // 16 rows of scales are whole words, so every tile starts as far into one as the matrix does
+        const uint32_t into = reinterpret_cast<uintptr_t>(m.s) & 3;
+        s = static_cast<const uint8_t*>(m.s) - into + static_cast<int64_t>(n0) * (m.K / kMxGroup), s_bytes = (into + rows * (m.K / kMxGroup) + 3) & ~3u;
+      } else {
         s = reinterpret_cast<const uint8_t*>(static_cast<const float*>(m.s) + static_cast<int64_t>(n0 / 128) * (m.K / 128)), s_bytes = m.K / 32;
+      }
       q = in_scalar(q), s = in_scalar(s), q_bytes = in_scalar(q_bytes), s_bytes = in_scalar(s_bytes);
     }
   };
@@ -123,26 +123,23 @@ struct Stream {
   const uint8_t* x;
   uint32_t x_bytes;
   uint32_t w_at, s_at;  // where a lane starts in a tile, and in its scales
-  int w_from, x_from;   // where it reads in a chunk
+  int w_from, x_from, s_from;   // where it reads in a chunk
   int q, l16;
   uint32_t x_at[kXLoads];  // its row of x of each load with its piece; past the end of every buffer: none
   Tile tile[NT];
-  uint32_t scales[RAGGED ? DEPTH : 1][NT][2];  // RAGGED
   v4f acc[NT];
 
-  __device__ __forceinline__ Stream(uint8_t* lds, int wave, int lane, int columns, const void* x_base, uint32_t bytes)
+  __device__ __forceinline__ Stream(uint8_t* lds, int wave, int lane, int columns, const void* x_base, uint32_t bytes, const void* scales)
       : ring(lds + wave * kBytes), ring_to((mx_lds_bytes)lds + wave * kBytes), K(columns), chunks((columns + kCols - 1) / kCols), row_bytes(W == kE4m3 ? columns : columns / 2),
         x(in_scalar(static_cast<const uint8_t*>(x_base))), x_bytes(in_scalar(bytes)), q(lane >> 4), l16(lane & 15) {
     const int row = lane >> 3, x_row16 = l16 & (R - 1);
     w_at = row * row_bytes + ((lane & 7) ^ (row >> 1)) * 16;
     w_from = l16 * 128 + (W == kE4m3 ? ((q ^ (l16 >> 1)) & 7) * 16 : (l16 >> 1) * 16 + 4 * q);
     x_from = x_row16 * kXPitch + ((W == kE4m3 ? 2 * q : q) ^ x_row16) * 16;
-    if (W == kE4m3)
-      s_at = 0;
-    else if (RAGGED)
-      s_at = l16 * (K / kMxGroup) + 2 * q;
-    else
-      s_at = lane < 32 ? (lane >> 1) * (K / kMxGroup) + 4 * (lane & 1) : kNowhere;  // eight scales a row
+    const uint32_t into = reinterpret_cast<uintptr_t>(scales) & 3, pitch = columns / kMxGroup;
+    const uint32_t its = into + (lane >> 2) * pitch, words = its % 4 == 0 ? 2 : 3;
+    s_at = W == kE4m3 ? 0 : (lane & 3) >= words ? kNowhere : (its & ~3u) + 4 * (lane & 3);
+    s_from = W == kE4m3 ? 2048 : 2048 + 16 * l16 + ((into + l16 * pitch) & 3) + 2 * q;
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -158,24 +155,13 @@ struct Stream {
     const uint32_t at = in ? static_cast<uint32_t>(c) * 128 : 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      // Past the end of a row of e2m1 a lane brings the next one's codes, which meet zeros of x; the scales there are zeros too, which are numbers.
+      // Past the end of a row of e2m1 a lane brings the next one's codes, which meet zeros of x.
       const auto src = make_rsrc(tile[n].q, in ? tile[n].q_bytes : 0);
       load_to_lds<2>(src, to + n * kStreamTile, w_at, at);
       // eight rows further on row / 2 has another third bit: the other half of the chunk
       const uint32_t half = ((lane & 7) ^ (lane >> 4)) < 4 ? 64u : -64u;
       load_to_lds<2>(src, to + n * kStreamTile + 1024, w_at + half + 8 * row_bytes, at);
-      if (W == kE4m3) {
-        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kStreamTile + 2048, s_at, in ? 4 * c : 0);
-      } else if (!RAGGED) {
-        const bool there = 8 * c + 4 * (lane & 1) < K / kMxGroup;
-        load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kStreamTile + 2048, there ? s_at : kNowhere, in ? 8 * c : 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bool there = 8 * c + 2 * q + i < K / kMxGroup;
-          scales[d][n][i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), there ? s_at + i : kNowhere, in ? 8 * c : 0, 0);
-        }
-      }
+      load4_to_lds(make_rsrc(tile[n].s, in ? tile[n].s_bytes : 0), to + n * kStreamTile + 2048, s_at, in ? (W == kE4m3 ? 4 : 8) * c : 0);
     }
 #pragma unroll
     for (int j = 0; j < kXLoads; ++j) {
@@ -184,11 +170,12 @@ struct Stream {
     }
   }
 
-  // The chunk in place d, behind which there are DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16.
-  __device__ __forceinline__ void multiply(int d) {
+  // Chunk c, in place d and behind it DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16.
+  __device__ __forceinline__ void multiply(int d, int c) {
     wait_loads<(DEPTH - 1) * kLoads>();  // in order
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
+    const uint32_t scaled = mx_scales_in_row(K / kMxGroup - 8 * c - 2 * q);
     const uint8_t* const from = ring + d * kChunk;  // what is ^ed below is within what a row has of a chunk
     v4i xf[kSteps];
 #pragma unroll
@@ -204,16 +191,16 @@ struct Stream {
 #pragma unroll
           for (int i = 0; i < 2; ++i) sum = mfma_16x16x32<T>(xf[2 * u + i], from_e4m3<T>(v[2 * i], v[2 * i + 1]), sum);
         }
-        const float s = *reinterpret_cast<const float*>(codes + 2048);
+        const float s = *reinterpret_cast<const float*>(codes + s_from);
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, sum[r], acc[n][r]);
         continue;
       }
       // each quarter makes two of the eight scales of its rows, for all of them: groups 2 i + u
       uint32_t by_group[2][4];
-      const uint32_t two = RAGGED ? 0u : *reinterpret_cast<const uint16_t*>(codes + 2048 + 8 * l16 + 2 * q);
+      const uint32_t two = *reinterpret_cast<const mx_two_bytes*>(codes + s_from) & scaled;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(RAGGED ? scales[d][n][u] : u == 0 ? two & 0xffu : two >> 8)), by_group[u]);
+      for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(two >> 8 * u & 0xff)), by_group[u]);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const float scale = __uint_as_float(by_group[i & 1][i >> 1 & 3]);
@@ -244,7 +231,7 @@ struct Stream {
     for (int c = wave; c < chunks; c += DEPTH * waves) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
-        multiply(d);
+        multiply(d, c + d * waves);
         const int next = c + (DEPTH + d) * waves;
         load(d, lane, next, next < chunks);
         __builtin_amdgcn_sched_barrier(0);
@@ -279,10 +266,10 @@ struct FewShape {
 
 // R rows of x against 16 NT rows of the matrix.  blockIdx.y: eight column tiles, one for each XCD, blockIdx.x: those tiles by the blocks of R rows, so that the
 // workgroups that share weights run beside each other on one XCD.
-template <int T, int W, int R, int NT, bool RAGGED>
+template <int T, int W, int R, int NT>
 __global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_kernel(const FewArgs p) {
   typedef FewShape<W, R, NT> Shape;
-  typedef Stream<T, W, R, NT, Shape::kDepth, RAGGED> S;
+  typedef Stream<T, W, R, NT, Shape::kDepth> S;
   constexpr int kWaves = Shape::kWaves;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -292,7 +279,7 @@ __global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_ke
   const int64_t m0 = static_cast<int64_t>(blockIdx.x / 8) * R;
   const int rows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(R)));
   const uint32_t pitch = static_cast<uint32_t>(p.x_rs) * 2;
-  S s(lds, wave, lane, p.w.K, static_cast<const uint8_t*>(p.x) + m0 * p.x_rs * 2, (rows - 1) * pitch + 2 * p.w.K);
+  S s(lds, wave, lane, p.w.K, static_cast<const uint8_t*>(p.x) + m0 * p.x_rs * 2, (rows - 1) * pitch + 2 * p.w.K, p.w.s);
 #pragma unroll
   for (int n = 0; n < NT; ++n) s.tile[n].point_at(p.w, n0 + 16 * n);
 #pragma unroll
@@ -384,11 +371,11 @@ struct DownShape {
 
 // A workgroup takes kColumns rows of Gate and the same of Up, SPLIT waves share K; of expert blockIdx.y, or where there are more experts than slots of that slot's expert, if
 // it is the first to name it; R of its tokens at a time.
-template <int T, int W, int R, int SPLIT, bool RAGGED>
+template <int T, int W, int R, int SPLIT>
 __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertArgs p) {
   typedef UpShape<W, R, SPLIT> Shape;
   constexpr int kPairs = Shape::kPairs, kTiles = Shape::kTiles;
-  typedef Stream<T, W, R, kTiles, Shape::kDepth, RAGGED> S;
+  typedef Stream<T, W, R, kTiles, Shape::kDepth> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
@@ -424,7 +411,7 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
   v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][tiles][64]
   for (int b = 0; b < rows; b += R) {
     if (b > 0) __syncthreads();
-    S s(lds, wave, lane, p.H, p.x, static_cast<uint32_t>((p.T - 1) * p.x_rs + p.H) * 2);
+    S s(lds, wave, lane, p.H, p.x, static_cast<uint32_t>((p.T - 1) * p.x_rs + p.H) * 2, p.up.s);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) s.tile[2 * i].point_at(up, n0 + 16 * i), s.tile[2 * i + 1].point_at(up, p.I + n0 + 16 * i);
 #pragma unroll
@@ -463,11 +450,11 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
 // A workgroup takes 32 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
 // chunks of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
 // The 2 TOKENS rows of x are the numbers of the tokens and behind them their rests.
-template <int TO, int W, int TOKENS, int kWaves, bool RAGGED>
+template <int TO, int W, int TOKENS, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertArgs p) {
   constexpr int R = 2 * TOKENS;
   typedef DownShape<W, TOKENS, kWaves> Shape;
-  typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth, RAGGED> S;
+  typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth> S;
   constexpr int kWide = 16 * kDownTiles;
   // The rings; behind them [waves][T][kWide] sums, the entries (expert, pass << 16), the slots of their rows ([TOKENS], -1: none).  What the list of entries is made
   // from lies where the rings are later.
@@ -534,7 +521,7 @@ __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertA
   __syncthreads();
   const int n0 = blockIdx.x * kWide;
   const uint32_t rest = static_cast<uint32_t>(slots) * p.I * 2;
-  S s(lds, wave, lane, p.I, p.act, 2 * rest);
+  S s(lds, wave, lane, p.I, p.act, 2 * rest, p.down.s);
   const int total = count_of_entries * s.chunks, each = (total + kWaves - 1) / kWaves;
   const int start = min(total, wave * each), end = min(total, start + each);
   auto point_at = [&](int i) {
@@ -580,7 +567,7 @@ __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertA
     for (int i = start; i < end; i += Shape::kDepth) {
 #pragma unroll
       for (int d = 0; d < Shape::kDepth; ++d) {
-        s.multiply(d);
+        s.multiply(d, m_chunk);
         if (m_left > 0 && (--m_left == 0 || ++m_chunk == s.chunks)) {
           leave(m_entry);
           m_chunk = 0, ++m_entry;

@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(64 * Tile::WAVES) mxfp4_tile_kernel(const MxAr
 template <int MT_, int NT_, int WAVES_>
 struct MxSplit {
   static constexpr int MT = MT_, NT = NT_, WAVES = WAVES_, FRAGS = MT + NT;
-  static constexpr int STAGE = FRAGS * 16 * (128 + 8), MOST = 156 * 1024 / (WAVES * STAGE), DEPTH = MOST > 4 ? 4 : MOST;
+  static constexpr int STAGE = FRAGS * 16 * (128 + 12), MOST = 158 * 1024 / (WAVES * STAGE), DEPTH = MOST > 4 ? 4 : MOST;
   static constexpr int SUMS = WAVES * MT * NT * 1024, RING = WAVES * DEPTH * STAGE, LDS = SUMS > RING ? SUMS : RING;
   static_assert(DEPTH >= 1 && LDS <= 160 * 1024, "what a CU has");
 };
@@ -374,8 +374,12 @@ __device__ __forceinline__ int mx_split_swizzle(int row) {
   return (i & 4) | (i & 1) << 1 | (((i >> 1) ^ (i >> 2)) & 1);
 }
 
-// DWORDS: rows of scales are whole words; otherwise a lane reads its scales one by one.
-template <class Split, bool DWORDS>
+// Two scales, where `left` of a row begin there: past its end are someone else's, of zeros but perhaps no numbers.
+typedef uint16_t mx_two_bytes __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t mx_scales_in_row(int left) { return left >= 2 ? 0xffffu : left == 1 ? 0xffu : 0u; }
+
+// The eight scales of a row's chunk start at any byte: they come as the three words they can lie in.
+template <class Split>
 __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const MxArgs p) {
   constexpr int MT = Split::MT, NT = Split::NT, FRAGS = Split::FRAGS, WAVES = Split::WAVES, DEPTH = Split::DEPTH;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -392,20 +396,19 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
   const uint8_t *const a_s = p.a_s + m0 * pitch, *const b_s = p.b_s + static_cast<int64_t>(n0) * pitch;
   const int chunks = (p.G + 7) / 8;
 
-  // Fragments of a first, then those of b; an instruction moves eight rows, half of one, and the scales of a whole one, eight a row, are another's.
+  // Fragments of a first, then those of b; an instruction moves eight rows, half of one, and the scales of a whole one are another's.
   const int r8 = lane >> 3;
   const uint32_t piece[2] = {static_cast<uint32_t>((lane & 7) ^ mx_split_swizzle(r8)) * 16, static_cast<uint32_t>((lane & 7) ^ mx_split_swizzle(8 + r8)) * 16};
   uint32_t from[2 * FRAGS];
 #pragma unroll
   for (int j = 0; j < 2 * FRAGS; ++j) from[j] = (8 * (j < 2 * MT ? j : j - 2 * MT) + r8) * half + piece[j & 1];
   const mx_lds_bytes ring_to = (mx_lds_bytes)smem + wave * DEPTH * Split::STAGE;
-  uint32_t bytes[DEPTH][FRAGS][2];  // without DWORDS: this lane's two scales
-  constexpr int kLoads = FRAGS * (DWORDS ? 3 : 4);
+  constexpr int kLoads = FRAGS * 3;
   const auto load = [&](int d, int c) {
     const bool in = c < chunks;
     const uint32_t at = in ? static_cast<uint32_t>(c) * 128 : 0, at_s = in ? static_cast<uint32_t>(c) * 8 : 0;
     const auto a_src = make_rsrc(a, in ? rows * half : 0), b_src = make_rsrc(b, in ? cols * half : 0);
-    const auto as_src = make_rsrc(a_s, in ? rows * pitch : 0), bs_src = make_rsrc(b_s, in ? cols * pitch : 0);
+    const auto as_src = make_rsrc(a_s, in ? (rows * pitch + 3) & ~3u : 0), bs_src = make_rsrc(b_s, in ? (cols * pitch + 3) & ~3u : 0);  // whole words
     const mx_lds_bytes to = ring_to + d * Split::STAGE;
     const bool past[2] = {at + piece[0] >= half, at + piece[1] >= half};  // in a short last chunk
 #pragma unroll
@@ -414,15 +417,8 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
     for (int j = 2 * MT; j < 2 * FRAGS; ++j) load_to_lds<2>(b_src, to + j * 1024, past[j & 1] ? kNowhere : from[j], at);
 #pragma unroll
     for (int f = 0; f < FRAGS; ++f) {
-      const uint32_t first = 16 * (f < MT ? f : f - MT);
-      if (DWORDS) {
-        const uint32_t its = (first + (lane >> 1)) * pitch + 4 * (lane & 1);
-        if (lane < 32) load4_to_lds(f < MT ? as_src : bs_src, to + FRAGS * 2048 + f * 128, at_s + 4 * (lane & 1) < p.G ? its : kNowhere, at_s);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          bytes[d][f][i] = __builtin_amdgcn_raw_buffer_load_b8(f < MT ? as_src : bs_src, static_cast<int>(at_s) + 2 * q + i < p.G ? (first + l16) * pitch + 2 * q + i : kNowhere, at_s, 0);
-      }
+      const uint32_t its = (16 * (f < MT ? f : f - MT) + lane / 3) * pitch;
+      if (lane < 48) load4_to_lds(f < MT ? as_src : bs_src, to + FRAGS * 2048 + f * 192, lane % 3 == 2 && its % 4 == 0 ? kNowhere : (its & ~3u) + 4 * (lane % 3), at_s);
     }
   };
 
@@ -433,17 +429,18 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
     for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
   const uint8_t* const mine = smem + wave * DEPTH * Split::STAGE + l16 * 128;
   const int at[2] = {((2 * q) ^ mx_split_swizzle(l16)) * 16, ((2 * q + 1) ^ mx_split_swizzle(l16)) * 16};
-  auto multiply = [&](int d) {
+  const int scales_at = FRAGS * 2048 - l16 * 128 + l16 * 12 + (l16 * pitch & 3) + 2 * q;  // 16 rows of scales are whole words
+  auto multiply = [&](int d, int c) {
     wait_loads<(DEPTH - 1) * kLoads>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     const uint8_t* const stage = mine + d * Split::STAGE;
+    const uint32_t scaled = mx_scales_in_row(p.G - 8 * c - 2 * q);
     v4i v[FRAGS][2];
     uint32_t s[FRAGS];
 #pragma unroll
     for (int f = 0; f < FRAGS; ++f) {
-      if (!DWORDS) asm volatile("" : "+v"(bytes[d][f][0]), "+v"(bytes[d][f][1]));  // not before: they would be waited for where they are loaded
-      s[f] = DWORDS ? *reinterpret_cast<const uint16_t*>(stage - l16 * 128 + FRAGS * 2048 + f * 128 + l16 * 8 + 2 * q) : bytes[d][f][0] | bytes[d][f][1] << 8;
+      s[f] = *reinterpret_cast<const mx_two_bytes*>(stage + scales_at + f * 192) & scaled;
 #pragma unroll
       for (int h = 0; h < 2; ++h) v[f][h] = *reinterpret_cast<const v4i*>(stage + f * 2048 + at[h]);
     }
@@ -464,7 +461,7 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
   for (int c = wave; c < chunks; c += DEPTH * WAVES) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      multiply(d);  // zeros past the last chunk
+      multiply(d, c + d * WAVES);  // zeros past the last chunk
       load(d, c + (DEPTH + d) * WAVES);
     }
   }
