@@ -79,7 +79,7 @@ struct Matrix {
 //
 // A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of weights
 // piece ^ (row / 2).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a word of its 16 bytes a
-// quarter.  The eight scales of a row's chunk of e2m1 start at any byte: they come as the three words they can lie in.
+// quarter.  The eight scales of a row's chunk of e2m1 start at any byte: they come as the two or three words they lie in.
 constexpr int stream_columns(int weights) { return weights == kE4m3 ? 128 : 256; }
 constexpr int kStreamTile = 2048 + 256;  // bytes of a tile's chunk: codes, and behind them scales
 constexpr int stream_x_loads(int weights, int R) { return R * stream_columns(weights) / 512; }
@@ -137,9 +137,10 @@ struct Stream {
     w_from = l16 * 128 + (W == kE4m3 ? ((q ^ (l16 >> 1)) & 7) * 16 : (l16 >> 1) * 16 + 4 * q);
     x_from = x_row16 * kXPitch + ((W == kE4m3 ? 2 * q : q) ^ x_row16) * 16;
     const uint32_t into = reinterpret_cast<uintptr_t>(scales) & 3, pitch = columns / kMxGroup;
-    const uint32_t its = into + (lane >> 2) * pitch, words = its % 4 == 0 ? 2 : 3;
-    s_at = W == kE4m3 ? 0 : (lane & 3) >= words ? kNowhere : (its & ~3u) + 4 * (lane & 3);
-    s_from = W == kE4m3 ? 2048 : 2048 + 16 * l16 + ((into + l16 * pitch) & 3) + 2 * q;
+    const int lanes = (into | pitch % 4) == 0 ? 1 : 2;  // log2 of those of a row: of whole words two, otherwise three of four
+    const uint32_t row_of = lane >> lanes, word = lane & ((1 << lanes) - 1);
+    s_at = W == kE4m3 ? 0 : row_of < 16 && word < 3 ? ((into + row_of * pitch) & ~3u) + 4 * word : kNowhere;
+    s_from = W == kE4m3 ? 2048 : 2048 + (l16 << (lanes + 2)) + ((into + l16 * pitch) & 3) + 2 * q;
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -172,10 +173,10 @@ struct Stream {
 
   // Chunk c, in place d and behind it DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16.
   __device__ __forceinline__ void multiply(int d, int c) {
+    const uint32_t scaled = mx_scales_in_row(K / kMxGroup - 8 * c - 2 * q);
     wait_loads<(DEPTH - 1) * kLoads>();  // in order
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t scaled = mx_scales_in_row(K / kMxGroup - 8 * c - 2 * q);
     const uint8_t* const from = ring + d * kChunk;  // what is ^ed below is within what a row has of a chunk
     v4i xf[kSteps];
 #pragma unroll

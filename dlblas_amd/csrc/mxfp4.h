@@ -378,7 +378,7 @@ __device__ __forceinline__ int mx_split_swizzle(int row) {
 typedef uint16_t mx_two_bytes __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t mx_scales_in_row(int left) { return left >= 2 ? 0xffffu : left == 1 ? 0xffu : 0u; }
 
-// The eight scales of a row's chunk start at any byte: they come as the three words they can lie in.
+// The eight scales of a row's chunk start at any byte: they come as the two or three words they lie in.
 template <class Split>
 __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const MxArgs p) {
   constexpr int MT = Split::MT, NT = Split::NT, FRAGS = Split::FRAGS, WAVES = Split::WAVES, DEPTH = Split::DEPTH;
@@ -403,6 +403,9 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
 #pragma unroll
   for (int j = 0; j < 2 * FRAGS; ++j) from[j] = (8 * (j < 2 * MT ? j : j - 2 * MT) + r8) * half + piece[j & 1];
   const mx_lds_bytes ring_to = (mx_lds_bytes)smem + wave * DEPTH * Split::STAGE;
+  const bool words = pitch % 4 == 0;
+  const uint32_t row_of = words ? lane >> 1 : lane / 3, word = words ? lane & 1 : lane % 3;
+  const uint32_t scales_of = row_of < 16 ? (row_of * pitch & ~3u) + 4 * word : kNowhere;
   constexpr int kLoads = FRAGS * 3;
   const auto load = [&](int d, int c) {
     const bool in = c < chunks;
@@ -417,8 +420,8 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
     for (int j = 2 * MT; j < 2 * FRAGS; ++j) load_to_lds<2>(b_src, to + j * 1024, past[j & 1] ? kNowhere : from[j], at);
 #pragma unroll
     for (int f = 0; f < FRAGS; ++f) {
-      const uint32_t its = (16 * (f < MT ? f : f - MT) + lane / 3) * pitch;
-      if (lane < 48) load4_to_lds(f < MT ? as_src : bs_src, to + FRAGS * 2048 + f * 192, lane % 3 == 2 && its % 4 == 0 ? kNowhere : (its & ~3u) + 4 * (lane % 3), at_s);
+      const uint32_t first = 16 * (f < MT ? f : f - MT) * pitch;  // a whole word
+      if (lane < 48) load4_to_lds(f < MT ? as_src : bs_src, to + FRAGS * 2048 + f * 192, scales_of == kNowhere ? kNowhere : first + scales_of, at_s);
     }
   };
 
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(64 * Split::WAVES) mxfp4_split_kernel(const Mx
     for (int n = 0; n < NT; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
   const uint8_t* const mine = smem + wave * DEPTH * Split::STAGE + l16 * 128;
   const int at[2] = {((2 * q) ^ mx_split_swizzle(l16)) * 16, ((2 * q + 1) ^ mx_split_swizzle(l16)) * 16};
-  const int scales_at = FRAGS * 2048 - l16 * 128 + l16 * 12 + (l16 * pitch & 3) + 2 * q;  // 16 rows of scales are whole words
+  const int scales_at = FRAGS * 2048 - l16 * 128 + l16 * (words ? 8 : 12) + (l16 * pitch & 3) + 2 * q;
   auto multiply = [&](int d, int c) {
     wait_loads<(DEPTH - 1) * kLoads>();
     asm volatile("" ::: "memory");
