@@ -167,7 +167,7 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
 }
 
 size_t dlb_few_token_experts_workspace_bytes(int64_t tokens, int64_t topk, int64_t I) {
-  return tokens > 0 && topk > 0 && I > 0 ? static_cast<size_t>(tokens) * topk * I * 2 * sizeof(uint16_t) : 0;
+  return tokens > 0 && topk > 0 && I > 0 ? static_cast<size_t>(tokens) * topk * I * sizeof(float) : 0;
 }
 
 int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const void* ids, int ids_dtype, int64_t ids_stride_m, int64_t ids_stride_k,
@@ -200,7 +200,7 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   if (!workspace || workspace_bytes < need) return fail(DLB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
   if (misaligned(workspace, 4)) return fail(DLB_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
   ExpertArgs a{};
-  a.x = x, a.ids = ids, a.weights = weights, a.act = static_cast<uint16_t*>(workspace), a.out = out;
+  a.x = x, a.ids = ids, a.weights = weights, a.act = static_cast<float*>(workspace), a.out = out;
   a.up = Matrix{static_cast<const uint8_t*>(up_q), up_s, static_cast<int>(2 * I), static_cast<int>(H)};
   a.down = Matrix{static_cast<const uint8_t*>(down_q), down_s, static_cast<int>(H), static_cast<int>(I)};
   a.up_q = a.down_q = 0;
@@ -218,8 +218,9 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
   // Tokens of an expert that a workgroup takes at a time; one with more reads the expert's weights again, from the caches, and x for rows without a token is
   // not read.  8 of 32 experts, 4096 x 7168, us e4m3 / e2m1 (with four waves to K): 8 tokens by four 148 / 100, by eight 131 / 110; 16 tokens by eight 146 / 121, by sixteen
   // 163 / 147; 32 tokens by eight 224 / 181, by sixteen 174 / 154.
-  // The second product's rows share the LDS with what is on its way of the weights: four tokens a pass and eight waves while an expert has three or fewer (7168 x 2048,
-  // 8 tokens: 79 / 59, by eight 103 / 75); eight waves as long as there is room for their sums (16 tokens e4m3: 96, four waves 113; e2m1 is no faster by them, 88).
+  // The second product's rows share the LDS with what is on its way of the weights, and a wave makes the parts of its rows anew for every chunk.  us, 7168 x 2048, four tokens a
+  // pass on eight waves against eight of them (e4m3 on eight waves, of e2m1 there is room for four): 8 tokens x 8 of 32 experts e4m3 67 / 69, e2m1 61 / 89;  16 tokens of 32
+  // experts 103 / 81, 92 / 102;  of 24 (5.3 tokens each) e2m1 90 / 89;  of 16 86 / 79.
   const int64_t named = std::min(experts, slots), mean = slots / named;
   const int up_rows = tokens <= 4 ? 4 : tokens <= 8 || mean <= 4 ? 8 : 16;
   const auto launch = [&](auto kt, auto kw) {
@@ -245,7 +246,7 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
     constexpr std::integral_constant<int, 4> four;
     constexpr std::integral_constant<int, 8> eight;
     if (tokens <= 2) return down(two, eight);
-    if (tokens <= 4 || (tokens <= kDownWideTokens && slots <= 3 * named)) return down(four, eight);
+    if (tokens <= 4 || (tokens <= kDownWideTokens && slots <= (kw() == kE2m1 ? 4 : 3) * named)) return down(four, eight);
     if constexpr (kw() == kE4m3) {
       if (tokens <= kDownWideTokens) return down(eight, eight);
     }

@@ -77,6 +77,12 @@ struct Matrix {
 // rows x 4096 x 7168 e4m3 at 250 us however much was on its way.  Here eight lanes share a line, and all of it is asked for at once: chunks of half a line
 // of e2m1 150 us, and the products themselves cost nothing of that.
 //
+// Rows of x are 16-bit numbers, or with F32 fp32 ones, R / 2 of them: each is the sum of three bf16, the nearest, the nearest to what that leaves, and the rest, which
+// has six bits at most (parts below 2^-126 may count as 0).  Every part has a product of its own.  A lane makes the parts of eight numbers, those of one step in R / 2 rows of
+// the MFMA and of the next in the R / 2 behind them, so that none makes what another has; a product of one step then fills those rows, and what it leaves in the others is
+// of no use.  (Instructions bound this: with lanes that exchange their parts, first and second in the rows of one product, as long, and with every lane making the parts of both
+// 8 % longer.)  Sums of the first parts stay apart: what an infinity leaves is no number.
+//
 // A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of weights
 // piece ^ (row / 2).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a word of its 16 bytes a
 // quarter.  The eight scales of a row's chunk of e2m1 start at any byte: they come as the two or three words they lie in.
@@ -90,13 +96,14 @@ constexpr int stream_depth(int weights, int R, int NT, int waves, int bytes) {
   return depth > 6 ? 6 : depth;
 }
 
-template <int T, int W, int R, int NT, int DEPTH>
+template <int T, int W, int R, int NT, int DEPTH, bool F32 = false>
 struct Stream {
-  static constexpr int kCols = stream_columns(W), kSteps = kCols / 32;
-  static constexpr int kXPitch = 2 * kCols, kXLoads = stream_x_loads(W, R), kXLanes = kXPitch / 16;  // lanes of a load that share a row of x
+  static constexpr int kCols = stream_columns(W), kSteps = kCols / 32, kXRows = F32 ? R / 2 : R, kXSize = F32 ? 4 : 2;
+  static constexpr int kXPitch = kXSize * kCols, kXLoads = stream_x_loads(W, R), kXLanes = kXPitch / 16;  // lanes of a load that share a row of x
   static constexpr int kChunk = stream_bytes(W, R, NT), kBytes = DEPTH * kChunk;
   static constexpr int kLoads = NT * 3 + kXLoads;  // of a chunk
   static_assert((R == 4 || R == 8 || R == 16) && DEPTH >= 2 && (DEPTH - 1) * kLoads < 64, "whole loads of x, a counter of six bits");
+  static_assert(!F32 || T == kInBf16, "parts of fp32");
 
   // 16 rows of a matrix, from row n0 on; past its end the last that it has (a buffer of no bytes would not do: its end is compared with what a chunk's offset leaves of it).
   struct Tile {
@@ -128,27 +135,42 @@ struct Stream {
   uint32_t x_at[kXLoads];  // its row of x of each load with its piece; past the end of every buffer: none
   Tile tile[NT];
   v4f acc[NT];
+  // With F32, of the steps g + kTurns i: rows kXRows g to kXRows (g + 1) - 1, the others are of no use.
+  static constexpr int kTurns = F32 && W == kE2m1 && R <= 8 ? 4 : 2;
+  struct Sums {
+    v4f first[kTurns], rest[kTurns];  // of the first parts, of the others
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) first[i] = rest[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  Sums sums[F32 ? NT : 1];
 
   __device__ __forceinline__ Stream(uint8_t* lds, int wave, int lane, int columns, const void* x_base, uint32_t bytes, const void* scales)
       : ring(lds + wave * kBytes), ring_to((mx_lds_bytes)lds + wave * kBytes), K(columns), chunks((columns + kCols - 1) / kCols), row_bytes(W == kE4m3 ? columns : columns / 2),
         x(in_scalar(static_cast<const uint8_t*>(x_base))), x_bytes(in_scalar(bytes)), q(lane >> 4), l16(lane & 15) {
-    const int row = lane >> 3, x_row16 = l16 & (R - 1);
+    const int row = lane >> 3, x_row16 = l16 & (kXRows - 1);
     w_at = row * row_bytes + ((lane & 7) ^ (row >> 1)) * 16;
     w_from = l16 * 128 + (W == kE4m3 ? ((q ^ (l16 >> 1)) & 7) * 16 : (l16 >> 1) * 16 + 4 * q);
-    x_from = x_row16 * kXPitch + ((W == kE4m3 ? 2 * q : q) ^ x_row16) * 16;
+    // of fp32 two pieces, in lanes of the next rows those of the step behind
+    const int second = F32 ? (l16 / kXRows & (kTurns - 1)) * (W == kE4m3 ? 2 : 8) : 0;
+    x_from = x_row16 * kXPitch + (((W == kE4m3 ? 2 * q : q) * (F32 ? 2 : 1) + second) ^ x_swizzle(x_row16)) * 16;
     const uint32_t into = reinterpret_cast<uintptr_t>(scales) & 3, pitch = columns / kMxGroup;
     const int lanes = (into | pitch % 4) == 0 ? 1 : 2;  // log2 of those of a row: of whole words two, otherwise three of four
     const uint32_t row_of = lane >> lanes, word = lane & ((1 << lanes) - 1);
     s_at = W == kE4m3 ? 0 : row_of < 16 && word < 3 ? ((into + row_of * pitch) & ~3u) + 4 * word : kNowhere;
     s_from = W == kE4m3 ? 2048 : 2048 + (l16 << (lanes + 2)) + ((into + l16 * pitch) & 3) + 2 * q;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) acc[n] = v4f{0.f, 0.f, 0.f, 0.f}, sums[F32 ? n : 0].clear();
   }
+  // A row's 16-byte piece c of x lies at c ^ this.  Of fp32 a turn of 16 lanes holds every row with two quarters, whose pieces differ in bit 1 (e2m1) or 2 (e4m3), and half of
+  // the rows have a step, which is bit 3 (e2m1) or 1 (e4m3), behind the others: the rows take the other three bits.
+  static __device__ __forceinline__ int x_swizzle(int row) { return !F32 ? row : W == kE4m3 ? (row & 3) | (row & 4) << 1 : (row & 1) | (row & 6) << 1; }
   // Row of x that load j brings for a lane, and the lane's column there.
   static __device__ __forceinline__ int x_row(int lane, int j) { return 64 / kXLanes * j + lane / kXLanes; }
-  static __device__ __forceinline__ int x_column(int lane, int j) { return (lane % kXLanes ^ (x_row(lane, j) & 15)) * 8; }
+  static __device__ __forceinline__ int x_column(int lane, int j) { return (lane % kXLanes ^ x_swizzle(x_row(lane, j) & 15)) * (16 / kXSize); }
   // at: byte of that row, kNowhere: none
-  __device__ __forceinline__ void set_row(int lane, int j, uint32_t at) { x_at[j] = at == kNowhere ? kNowhere : at + 2 * x_column(lane, j); }
+  __device__ __forceinline__ void set_row(int lane, int j, uint32_t at) { x_at[j] = at == kNowhere ? kNowhere : at + kXSize * x_column(lane, j); }
 
   // Chunk c into place d; `in` false (the same for the wave): nothing is brought.  Loads are issued either way.
   __device__ __forceinline__ void load(int d, int lane, int c, bool in) {
@@ -171,13 +193,33 @@ struct Stream {
     }
   }
 
-  // Chunk c, in place d and behind it DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16.
-  __device__ __forceinline__ void multiply(int d, int c) {
-    const uint32_t scaled = mx_scales_in_row(K / kMxGroup - 8 * c - 2 * q);
-    wait_loads<(DEPTH - 1) * kLoads>();  // in order
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    const uint8_t* const from = ring + d * kChunk;  // what is ^ed below is within what a row has of a chunk
+  // Eight fp32 numbers as three parts each.
+  static __device__ __forceinline__ void parts(const v4f (&v)[2], v4i (&part)[3]) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    // -1 beside 0, out of the compiler's sight: it would write the lower one as the constant -1.0 of the instruction, which is that of fp32, the upper one
+    uint32_t lower = 0xbf80u, upper = 0xbf800000u;
+    asm("" : "+s"(lower), "+s"(upper));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v2f f{v[i / 2][2 * (i & 1)], v[i / 2][2 * (i & 1) + 1]};
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const v2bf b = __builtin_convertvector(f, v2bf);
+        part[k][i] = __builtin_bit_cast(int, b);
+        f = v2f{__builtin_amdgcn_fdot2_f32_bf16(b, __builtin_bit_cast(v2bf, lower), f[0], false), __builtin_amdgcn_fdot2_f32_bf16(b, __builtin_bit_cast(v2bf, upper), f[1], false)};
+      }
+    }
+  }
+
+  // Of a tile's chunk of e2m1, the scales of groups 2 i + u of row l16: each quarter makes two of the eight of its rows, for all of them.
+  __device__ __forceinline__ void scales(const uint8_t* codes, uint32_t scaled, uint32_t (&by_group)[2][4]) const {
+    const uint32_t two = *reinterpret_cast<const mx_two_bytes*>(codes + s_from) & scaled;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(two >> 8 * u & 0xff)), by_group[u]);
+  }
+
+  __device__ __forceinline__ void multiply_rows(const uint8_t* from, uint32_t scaled) {
     v4i xf[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) xf[i] = *reinterpret_cast<const v4i*>(from + NT * kStreamTile + (x_from ^ (W == kE4m3 ? 128 * (i >> 1) + 16 * (i & 1) : 64 * i)));
@@ -197,11 +239,8 @@ struct Stream {
         for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, sum[r], acc[n][r]);
         continue;
       }
-      // each quarter makes two of the eight scales of its rows, for all of them: groups 2 i + u
       uint32_t by_group[2][4];
-      const uint32_t two = *reinterpret_cast<const mx_two_bytes*>(codes + s_from) & scaled;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(two >> 8 * u & 0xff)), by_group[u]);
+      scales(codes, scaled, by_group);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const float scale = __uint_as_float(by_group[i & 1][i >> 1 & 3]);
@@ -216,6 +255,73 @@ struct Stream {
         __builtin_amdgcn_sched_barrier(0);  // the sums of all steps would not fit the registers
       }
     }
+  }
+
+  // The same for rows of fp32.
+  __device__ __forceinline__ void multiply_parts(const uint8_t* from, uint32_t scaled) {
+    v4f raw[kSteps / kTurns][2];
+#pragma unroll
+    for (int i = 0; i < kSteps / kTurns; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) raw[i][h] = *reinterpret_cast<const v4f*>(from + NT * kStreamTile + (x_from ^ (128 * kTurns * i + 16 * h)));
+    constexpr int kLoadsOfCodes = W == kE4m3 ? 2 : kSteps;
+    v4i codes[NT][kLoadsOfCodes];  // of e2m1 the first word
+    uint32_t by_group[NT][2][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < kLoadsOfCodes; ++i)
+        if (W == kE4m3)
+          codes[n][i] = *reinterpret_cast<const v4i*>(from + n * kStreamTile + (w_from ^ 64 * i));
+        else
+          codes[n][i][0] = *reinterpret_cast<const int*>(from + n * kStreamTile + (w_from ^ 16 * i));
+      if (W == kE2m1) scales(from + n * kStreamTile, scaled, by_group[n]);
+    }
+    Sums sum[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      if (W == kE2m1)
+        sum[n] = sums[n];
+      else
+        sum[n].clear();
+    v4i part[3];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i % kTurns == 0) parts(raw[i / kTurns], part);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const v4i f = W == kE4m3 ? from_e4m3<T>(codes[n][i >> 1 & (kLoadsOfCodes - 1)][2 * (i & 1)], codes[n][i >> 1 & (kLoadsOfCodes - 1)][2 * (i & 1) + 1])
+                                 : from_e2m1<T>(codes[n][i & (kLoadsOfCodes - 1)][0], __uint_as_float(by_group[n][i & 1][i >> 1 & 3]));
+        const int g = i % kTurns;
+        sum[n].first[g] = mfma_16x16x32<T>(part[0], f, sum[n].first[g]);
+        sum[n].rest[g] = mfma_16x16x32<T>(part[2], f, mfma_16x16x32<T>(part[1], f, sum[n].rest[g]));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (W == kE2m1) {
+        sums[n] = sum[n];
+        continue;
+      }
+      const float s = *reinterpret_cast<const float*>(from + n * kStreamTile + s_from);
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[n].first[i][r] = fmaf(s, sum[n].first[i][r], sums[n].first[i][r]), sums[n].rest[i][r] = fmaf(s, sum[n].rest[i][r], sums[n].rest[i][r]);
+    }
+  }
+
+  // Chunk c, in place d and behind it DEPTH - 1 others, times its rows: lane l of acc[n] has rows 4 (l / 16) + r, column l % 16, with F32 sums[n].
+  __device__ __forceinline__ void multiply(int d, int c) {
+    const uint32_t scaled = mx_scales_in_row(K / kMxGroup - 8 * c - 2 * q);
+    wait_loads<(DEPTH - 1) * kLoads>();  // in order
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* const from = ring + d * kChunk;  // what is ^ed is within what a row has of a chunk
+    if constexpr (F32)
+      multiply_parts(from, scaled);
+    else
+      multiply_rows(from, scaled);
     // what is read of this place has arrived before its next chunk is asked for
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     asm volatile("" ::: "memory");
@@ -308,9 +414,8 @@ __global__ void __launch_bounds__(64 * (FewShape<W, R, NT>::kWaves)) few_rows_ke
 //   out[t] = sum over the slots j with 0 <= ids[t, j] < E of w[t, j] Down[e] (silu(Gate[e] x[t]) * (Up[e] x[t])),   e = ids[t, j]
 //
 // The first kernel leaves w silu(g) u of every slot, the second reads it against the experts' second matrices.  No sort in front: there are at most 64
-// tokens, a lane of a wave each, so the tokens of an expert are a ballot.  In between the numbers are held as the sum of two bf16, 16 bits of
-// significand, which the second kernel takes one beside the other: eight tokens and their rests are the 16 rows of an MFMA.  An
-// expert that a token names twice counts with the sum of both weights.
+// tokens, a lane of a wave each, so the tokens of an expert are a ballot.  In between the numbers are fp32 (Stream, F32).  An expert that a token names twice counts with the sum of
+// both weights.
 
 constexpr int kFewTokens = 64, kFewTopk = 16, kFewExperts = 1024;
 
@@ -318,7 +423,7 @@ struct ExpertArgs {
   const void* x;         // [T][x_rs]
   const void* ids;       // [T][topk], int32 or int64, through two strides
   const float* weights;  // [T][topk]
-  uint16_t* act;         // [2][T topk][I] bf16: the numbers, and what they leave
+  float* act;            // [T topk][I]
   void* out;             // [T][H]
   Matrix up, down;       // of expert 0: [2 I][H], [H][I]
   int64_t up_q, up_s, down_q, down_s;  // bytes to the next expert
@@ -408,7 +513,6 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
   const int rows = __popcll(mask), token_of = nth_lane(mask, lane);
   const Matrix up = of_expert(p.up, p.up_q, p.up_s, e);
   const int of = wave % SPLIT, n0 = blockIdx.x * Shape::kColumns + wave / SPLIT * 16 * kPairs;  // past the end: nothing is stored
-  const int64_t rest = static_cast<int64_t>(slots) * p.I;
   v4f* const part = reinterpret_cast<v4f*>(lds);  // [waves][tiles][64]
   for (int b = 0; b < rows; b += R) {
     if (b > 0) __syncthreads();
@@ -438,24 +542,18 @@ __global__ void __launch_bounds__(64 * kUpWaves) experts_up_kernel(const ExpertA
       const int t = __shfl(token_of, i & 63);
       const int slot = __shfl(first, t);
       const float v = gated(g[r], u[r]) * __shfl(weight, t);
-      if (4 * q + r >= R || i >= rows) continue;
-      const __bf16 hi = static_cast<__bf16>(v);
-      const float f = static_cast<float>(hi);
-      const __bf16 lo = static_cast<__bf16>(fabsf(f) == __builtin_inff() ? 0.f : v - f);
-      uint16_t* const to = p.act + static_cast<int64_t>(slot) * p.I + n0 + 16 * of + l16;
-      to[0] = __builtin_bit_cast(uint16_t, hi), to[rest] = __builtin_bit_cast(uint16_t, lo);
+      if (4 * q + r < R && i < rows) p.act[static_cast<int64_t>(slot) * p.I + n0 + 16 * of + l16] = v;
     }
   }
 }
 
 // A workgroup takes 32 columns of the output of all tokens.  Its work is a list of experts, several times where one has more than TOKENS of them, by
 // chunks of their K = I; each wave takes a run of that and adds its sums up in an LDS table of its own, and the tables are added in wave order.
-// The 2 TOKENS rows of x are the numbers of the tokens and behind them their rests.
 template <int TO, int W, int TOKENS, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertArgs p) {
   constexpr int R = 2 * TOKENS;
   typedef DownShape<W, TOKENS, kWaves> Shape;
-  typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth> S;
+  typedef Stream<kInBf16, W, R, kDownTiles, Shape::kDepth, true> S;
   constexpr int kWide = 16 * kDownTiles;
   // The rings; behind them [waves][T][kWide] sums, the entries (expert, pass << 16), the slots of their rows ([TOKENS], -1: none).  What the list of entries is made
   // from lies where the rings are later.
@@ -521,16 +619,15 @@ __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertA
   }
   __syncthreads();
   const int n0 = blockIdx.x * kWide;
-  const uint32_t rest = static_cast<uint32_t>(slots) * p.I * 2;
-  S s(lds, wave, lane, p.I, p.act, 2 * rest, p.down.s);
+  S s(lds, wave, lane, p.I, p.act, static_cast<uint32_t>(slots) * p.I * 4, p.down.s);
   const int total = count_of_entries * s.chunks, each = (total + kWaves - 1) / kWaves;
   const int start = min(total, wave * each), end = min(total, start + each);
   auto point_at = [&](int i) {
     const int e = __builtin_amdgcn_readfirstlane(entry[i]) & 0xffff;
 #pragma unroll
     for (int j = 0; j < S::kXLoads; ++j) {
-      const int r = S::x_row(lane, j), slot = row_slot[i * TOKENS + r % TOKENS];
-      s.set_row(lane, j, slot >= 0 ? static_cast<uint32_t>(slot) * p.I * 2 + (r / TOKENS) * rest : kNowhere);
+      const int slot = row_slot[i * TOKENS + S::x_row(lane, j)];
+      s.set_row(lane, j, slot >= 0 ? static_cast<uint32_t>(slot) * p.I * 4 : kNowhere);
     }
 #pragma unroll
     for (int n = 0; n < kDownTiles; ++n) s.tile[n].point_at(of_expert(p.down, p.down_q, p.down_s, e), n0 + 16 * n);
@@ -546,16 +643,29 @@ __global__ void __launch_bounds__(64 * kWaves) experts_down_kernel(const ExpertA
   auto leave = [&](int i) {
 #pragma unroll
     for (int n = 0; n < kDownTiles; ++n) {
-      v4f& a = s.acc[n];
+      auto& a = s.sums[n];
       float v[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = a[r] + (TOKENS == 2 ? a[(r + 2) & 3] : __shfl_xor(a[r], TOKENS == 4 ? 16 : 32));  // a token's number and what it left
+      for (int r = 0; r < 4; ++r) {
+        // number r of the first quarter's lanes, from those rows of each turn: row 4 q + r of turn 4 q / TOKENS
+        const auto whole = [&](const v4f (&of)[S::kTurns]) {
+          if (TOKENS == 2) {
+            const float two = of[0][r & 1] + of[1][2 + (r & 1)];
+            return S::kTurns == 2 ? two : two + (__shfl_xor(of[S::kTurns - 2][r & 1], 16) + __shfl_xor(of[S::kTurns - 1][2 + (r & 1)], 16));
+          }
+          if (TOKENS == 8) return of[0][r] + __shfl_xor(of[1][r], 32);
+          const float two = of[0][r] + __shfl_xor(of[1][r], 16);
+          return S::kTurns == 2 ? two : two + (__shfl_xor(of[S::kTurns - 2][r], 32) + __shfl_xor(of[S::kTurns - 1][r], 48));
+        };
+        const float first = whole(a.first), rest = whole(a.rest);
+        v[r] = fabsf(first) < __builtin_inff() ? first + rest : first;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 4 * q + r, slot = row < TOKENS ? row_slot[i * TOKENS + row] : -1;
         if (slot >= 0) sums[slot / p.topk * kWide + 16 * n + l16] += v[r];
       }
-      a = v4f{0.f, 0.f, 0.f, 0.f};
+      a.clear();
     }
   };
   if (start < end) {

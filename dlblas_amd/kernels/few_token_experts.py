@@ -3,8 +3,8 @@
     out[t] = sum over the slots j of topk_weights[t, j] * W2[e] (silu(gate) * up),   gate, up = halves of W13[e] x[t],   e = topk_ids[t, j]
 
 Beside ``fused_moe_v3`` and ``low_latency_experts``, which take quantised tokens that are sorted or laid out by expert, and hold what lies between the
-products in e4m3: here tokens come as they are in 16 bits, routing is read on the device, and between the products 16 bits of significand
-remain.  Weights are those calls' e4m3 ones or the 4-bit ones of ``per_group_quant_mxfp4``.  The reference has no counterpart.
+products in e4m3: here tokens come as they are in 16 bits, routing is read on the device, and what lies between the products is fp32.  Weights are
+those calls' e4m3 ones or the 4-bit ones of ``per_group_quant_mxfp4``.  The reference has no counterpart.
 """
 from typing import Tuple
 

@@ -73,9 +73,10 @@ size_t dlb_few_token_experts_workspace_bytes(int64_t tokens, int64_t topk, int64
 /*
  * A layer of experts for a few tokens:
  *   out[t] = sum over the slots j with 0 <= ids[t, j] < experts of weights[t, j] Down[e] (silu(Gate[e] x[t]) * (Up[e] x[t])),  e = ids[t, j]
- * Products and sums in fp32; what lies between the products is held in 16 bits of significand, the result rounded once.  Zeros for a token
+ * Products, sums and what lies between the products in fp32, the result rounded once.  Zeros for a token
  * without an expert here; slots that name one expert twice count both weights.  The order of all sums depends on the routing and the sizes alone.
- * Beside bf16 rows, and in Down, weights below 2^-126 in magnitude may count as zero.
+ * Beside bf16 rows, and in Down, weights below 2^-126 in magnitude may count as zero, and in Down what lies between the products is exact down to
+ * 2^-126 alone.
  *
  *   x       [tokens, H]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
  *   ids     [tokens, topk]  int32 / int64 (ids_dtype, DLB_IDX_*) through two strides;  weights [tokens, topk] fp32, contiguous
