@@ -452,8 +452,8 @@ __device__ __forceinline__ int nth_lane(uint64_t mask, int lane) {
   return __builtin_amdgcn_ds_permute(to * 4, lane);
 }
 
-// silu(g) u
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+// silu(g) u; the fast exponential is off by as many roundings as |g|
+__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 constexpr int kUpWaves = 4;
 // Pairs of tiles of Gate and Up that share the rows of x, which are most of what comes into LDS where there are 16 of them (64 tokens, 8 of 32 experts, 4096 x 7168:

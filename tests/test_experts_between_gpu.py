@@ -100,3 +100,26 @@ def test_infinities_and_the_largest_numbers(dev, T, kind):
     assert torch.equal(out[T // 2], torch.full((H, ), -math.inf).mul(down[0].sign()).to(bf16))
     others = torch.arange(T) != T // 2
     assert torch.equal(out[others], before[others])
+
+
+def test_gates_far_below_zero(dev):
+    """Of one expert g is -20 ... -84, of the other as near to 0, weighted so that the parts nearly cancel.  exp is off by 2^-23 of itself, whatever its size; the sum with 1, the division, the products
+    with u and the weight by 2^-24 each: 3 2^-23 a slot, and what the sums add, as above, 2^-23 + 2 2^-24: 10 2^-23 M for both."""
+    g = torch.Generator().manual_seed(2)
+    T, H, I = 40, 128, 128
+    x = torch.zeros(T, H)
+    x[:, 0] = -10 - 32 * torch.rand(T, generator=g)
+    x = x.to(bf16)
+    gates = torch.tensor([2.0, 2.0**-7])
+    rows = torch.ones(2, 2 * I)
+    rows[:, :I] = gates[:, None]
+    down = some((1, H), g)
+    both = x[:, :1].double() * gates.double()  # g of both
+    a = both / (1 + torch.exp(-both)) * x[:, :1].double()
+    weights = (torch.tensor([1.0, -(1 - 2.0**-12)], dtype=f64) / a).float()
+    assert bool(weights.isfinite().all())
+    ids = torch.tensor([[0, 1]]).expand(T, 2).contiguous()
+    out = few_token_experts(x.to(dev), ids.to(dev), weights.to(dev), *(tuple(t.to(dev) for t in coded('f8', v)) for v in (one_column(2, 2 * I, H, rows), one_weight(2, H, I, down)))).cpu()
+    want = (a * weights.double()).sum(1, keepdim=True) * down.double()
+    off = (out.double() - want).abs() - 10 * 2 * FP32 * down.double().abs() * (1 + half_step(bf16)) - half_step(bf16) * want.abs()
+    assert float(off.max()) <= 0, f'{float(off.max()):.3e} beyond the bound'
