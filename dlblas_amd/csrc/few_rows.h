@@ -3,8 +3,8 @@
 // Bound by the weights' bytes: each comes from memory once, is converted in registers and meets the rows in v_mfma_f32_16x16x32.  Weights are
 //   e4m3   with one fp32 scale per 128 x 128: exact in 16 bits, sums of 128 columns times the scale in fp32
 //   e2m1   with a power of two per 32 columns.  Beside bf16 rows the scale goes into the conversion: e2m1 has two bits of significand and bf16 the
-//          range of the scales, so the products stay exact (weights below 2^-126, which are subnormal numbers of bf16, may count as 0).  fp16 has not
-//          that range: there a group's sum meets its scale in fp32.
+//          range of the scales but for their ends, so the products stay exact.  A chunk with a scale at one of those scales its groups' sums in fp32, by what
+//          the conversion does not take.  fp16 has not that range: there a group's sum always meets its scale in fp32.
 // Waves split K and add their sums through LDS in wave order.
 #pragma once
 
@@ -212,46 +212,91 @@ struct Stream {
     }
   }
 
-  // Of a tile's chunk of e2m1, the scales of groups 2 i + u of row l16: each quarter makes two of the eight of its rows, for all of them.
-  __device__ __forceinline__ void scales(const uint8_t* codes, uint32_t scaled, uint32_t (&by_group)[2][4]) const {
-    const uint32_t two = *reinterpret_cast<const mx_two_bytes*>(codes + s_from) & scaled;
+  // The scales of e2m1 of row l16 of every tile, of groups 2 q and 2 q + 1 of a chunk; zeros past the end of the row.  Beside bf16: whether there is a weight, in any row of the wave,
+  // that it does not hold.  The first test takes three scales more than the ends, 253 to 255 and 0 to 4 by five bits; a group of zeros, whose scale is 0, passes the second
+  // (64 x 7168 x 18432 with a group of zeros in 63: 76 us, without it 98; with none 58).
+  __device__ __forceinline__ bool scales(const uint8_t* from, uint32_t scaled, uint32_t (&two)[NT]) const {
+    bool beyond = false;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) spread_quarters(__float_as_uint(mx_scale(two >> 8 * u & 0xff)), by_group[u]);
+    for (int n = 0; n < NT; ++n) {
+      const uint32_t of = *reinterpret_cast<const mx_two_bytes*>(from + n * kStreamTile + s_from);
+      two[n] = of & scaled;
+      const uint32_t behind = ((of & scaled) | (0x8080u & ~scaled)) + 0x0303u;  // a carry is one of a byte that is beyond
+      beyond |= (behind & 0xf8u) == 0 || (behind & 0xf800u) == 0;
+    }
+    if (T != kInBf16 || __builtin_amdgcn_ballot_w64(beyond) == 0) return false;
+    bool out = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t s = two[n] >> 8 * u & 0xff, in_row = scaled >> 8 * u & 0xff;
+        const v4i w = *reinterpret_cast<const v4i*>(from + n * kStreamTile + l16 * 128 + ((2 * q + u) ^ (l16 >> 1)) * 16);
+        out |= in_row && (s >= 253 || (s < 2 && ((w[0] | w[1] | w[2] | w[3]) & 0x77777777) != 0));
+      }
+    return __builtin_amdgcn_ballot_w64(out) != 0;
+  }
+  // Those of groups 2 i + u for all quarters, each of which has two: as fp32, for bf16 by the exponent alone.
+  static __device__ __forceinline__ void spread(uint32_t two, uint32_t (&by_group)[2][4]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) spread_quarters(T == kInBf16 ? (two >> 8 * u & 0xff) << 23 : __float_as_uint(mx_scale(two >> 8 * u & 0xff)), by_group[u]);
+  }
+  // A scale as one that bf16 has for every code, 2^-125 ... 2^125, and the rest of it, for sums in fp32: 2^-2 ... 2^2, NaN of NaN.
+  static __device__ __forceinline__ void part_scale(uint32_t scale, float& inner, float& outer) {
+    const uint32_t s = scale >> 23, near = min(max(s, 2u), 252u);
+    inner = __uint_as_float(near << 23), outer = __uint_as_float(s == 255 ? 0x7fc00000u : (127 + s - near) << 23);
   }
 
   __device__ __forceinline__ void multiply_rows(const uint8_t* from, uint32_t scaled) {
+    if constexpr (W == kE4m3)
+      multiply_rows_e4m3(from);
+    else if (uint32_t two[NT]; scales(from, scaled, two))
+      multiply_rows_e2m1<T == kInBf16>(from, two);
+    else
+      multiply_rows_e2m1<false>(from, two);
+  }
+  __device__ __forceinline__ void multiply_rows_e4m3(const uint8_t* from) {
     v4i xf[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) xf[i] = *reinterpret_cast<const v4i*>(from + NT * kStreamTile + (x_from ^ (W == kE4m3 ? 128 * (i >> 1) + 16 * (i & 1) : 64 * i)));
+    for (int i = 0; i < kSteps; ++i) xf[i] = *reinterpret_cast<const v4i*>(from + NT * kStreamTile + (x_from ^ (128 * (i >> 1) + 16 * (i & 1))));
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint8_t* const codes = from + n * kStreamTile;
-      if (W == kE4m3) {
-        v4f sum{0.f, 0.f, 0.f, 0.f};
+      v4f sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const v4i v = *reinterpret_cast<const v4i*>(codes + (w_from ^ 64 * u));
+      for (int u = 0; u < 2; ++u) {
+        const v4i v = *reinterpret_cast<const v4i*>(codes + (w_from ^ 64 * u));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) sum = mfma_16x16x32<T>(xf[2 * u + i], from_e4m3<T>(v[2 * i], v[2 * i + 1]), sum);
-        }
-        const float s = *reinterpret_cast<const float*>(codes + s_from);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, sum[r], acc[n][r]);
-        continue;
+        for (int i = 0; i < 2; ++i) sum = mfma_16x16x32<T>(xf[2 * u + i], from_e4m3<T>(v[2 * i], v[2 * i + 1]), sum);
       }
+      const float s = *reinterpret_cast<const float*>(codes + s_from);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, sum[r], acc[n][r]);
+    }
+  }
+  template <bool BEYOND>
+  __device__ __forceinline__ void multiply_rows_e2m1(const uint8_t* from, const uint32_t (&two)[NT]) {
+    v4i xf[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) xf[i] = *reinterpret_cast<const v4i*>(from + NT * kStreamTile + (x_from ^ 64 * i));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* const codes = from + n * kStreamTile;
       uint32_t by_group[2][4];
-      scales(codes, scaled, by_group);
+      spread(two[n], by_group);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const float scale = __uint_as_float(by_group[i & 1][i >> 1 & 3]);
-        const v4i f = from_e2m1<T>(*reinterpret_cast<const int*>(codes + (w_from ^ 16 * i)), T == kInBf16 ? scale : 1.0f);
-        if (T == kInBf16) {
+        const uint32_t scale = by_group[i & 1][i >> 1 & 3];
+        float inner = T == kInBf16 ? __uint_as_float(scale) : 1.0f, outer = __uint_as_float(scale);
+        if (BEYOND) part_scale(scale, inner, outer);
+        const v4i f = from_e2m1<T>(*reinterpret_cast<const int*>(codes + (w_from ^ 16 * i)), inner);
+        if (T == kInBf16 && !BEYOND) {
           acc[n] = mfma_16x16x32<T>(xf[i], f, acc[n]);
           continue;
         }
         const v4f sum = mfma_16x16x32<T>(xf[i], f, v4f{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(scale, sum[r], acc[n][r]);
+        for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(outer, sum[r], acc[n][r]);
         __builtin_amdgcn_sched_barrier(0);  // the sums of all steps would not fit the registers
       }
     }
@@ -259,55 +304,85 @@ struct Stream {
 
   // The same for rows of fp32.
   __device__ __forceinline__ void multiply_parts(const uint8_t* from, uint32_t scaled) {
-    v4f raw[kSteps / kTurns][2];
+    if constexpr (W == kE4m3)
+      multiply_parts_e4m3(from);
+    else if (uint32_t two[NT]; scales(from, scaled, two))
+      multiply_parts_e2m1<true>(from, two);
+    else
+      multiply_parts_e2m1<false>(from, two);
+  }
+  __device__ __forceinline__ void load_raw(const uint8_t* from, v4f (&raw)[kSteps / kTurns][2]) const {
 #pragma unroll
     for (int i = 0; i < kSteps / kTurns; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) raw[i][h] = *reinterpret_cast<const v4f*>(from + NT * kStreamTile + (x_from ^ (128 * kTurns * i + 16 * h)));
-    constexpr int kLoadsOfCodes = W == kE4m3 ? 2 : kSteps;
-    v4i codes[NT][kLoadsOfCodes];  // of e2m1 the first word
-    uint32_t by_group[NT][2][4];
+  }
+  // sums + the parts times a fragment
+  static __device__ __forceinline__ void add_product(const v4i (&part)[3], const v4i& f, v4f& first, v4f& rest) {
+    first = mfma_16x16x32<T>(part[0], f, first);
+    rest = mfma_16x16x32<T>(part[2], f, mfma_16x16x32<T>(part[1], f, rest));
+  }
+  __device__ __forceinline__ void multiply_parts_e4m3(const uint8_t* from) {
+    v4f raw[kSteps / kTurns][2];
+    load_raw(from, raw);
+    v4i codes[NT][2];
+    Sums sum[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < kLoadsOfCodes; ++i)
-        if (W == kE4m3)
-          codes[n][i] = *reinterpret_cast<const v4i*>(from + n * kStreamTile + (w_from ^ 64 * i));
-        else
-          codes[n][i][0] = *reinterpret_cast<const int*>(from + n * kStreamTile + (w_from ^ 16 * i));
-      if (W == kE2m1) scales(from + n * kStreamTile, scaled, by_group[n]);
+      for (int u = 0; u < 2; ++u) codes[n][u] = *reinterpret_cast<const v4i*>(from + n * kStreamTile + (w_from ^ 64 * u));
+      sum[n].clear();
     }
-    Sums sum[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      if (W == kE2m1)
-        sum[n] = sums[n];
-      else
-        sum[n].clear();
     v4i part[3];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       if (i % kTurns == 0) parts(raw[i / kTurns], part);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const v4i f = W == kE4m3 ? from_e4m3<T>(codes[n][i >> 1 & (kLoadsOfCodes - 1)][2 * (i & 1)], codes[n][i >> 1 & (kLoadsOfCodes - 1)][2 * (i & 1) + 1])
-                                 : from_e2m1<T>(codes[n][i & (kLoadsOfCodes - 1)][0], __uint_as_float(by_group[n][i & 1][i >> 1 & 3]));
-        const int g = i % kTurns;
-        sum[n].first[g] = mfma_16x16x32<T>(part[0], f, sum[n].first[g]);
-        sum[n].rest[g] = mfma_16x16x32<T>(part[2], f, mfma_16x16x32<T>(part[1], f, sum[n].rest[g]));
-      }
+      for (int n = 0; n < NT; ++n)
+        add_product(part, from_e4m3<T>(codes[n][i >> 1][2 * (i & 1)], codes[n][i >> 1][2 * (i & 1) + 1]), sum[n].first[i % kTurns], sum[n].rest[i % kTurns]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (W == kE2m1) {
-        sums[n] = sum[n];
-        continue;
-      }
       const float s = *reinterpret_cast<const float*>(from + n * kStreamTile + s_from);
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i)
+      for (int i = 0; i < kTurns; ++i) add_scaled(sums[n], i, s, sum[n].first[i], sum[n].rest[i]);
+    }
+  }
+  static __device__ __forceinline__ void add_scaled(Sums& to, int turn, float s, const v4f& first, const v4f& rest) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sums[n].first[i][r] = fmaf(s, sum[n].first[i][r], sums[n].first[i][r]), sums[n].rest[i][r] = fmaf(s, sum[n].rest[i][r], sums[n].rest[i][r]);
+    for (int r = 0; r < 4; ++r) to.first[turn][r] = fmaf(s, first[r], to.first[turn][r]), to.rest[turn][r] = fmaf(s, rest[r], to.rest[turn][r]);
+  }
+  template <bool BEYOND>
+  __device__ __forceinline__ void multiply_parts_e2m1(const uint8_t* from, const uint32_t (&two)[NT]) {
+    v4f raw[kSteps / kTurns][2];
+    load_raw(from, raw);
+    int codes[NT][kSteps];
+    uint32_t by_group[NT][2][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) codes[n][i] = *reinterpret_cast<const int*>(from + n * kStreamTile + (w_from ^ 16 * i));
+      spread(two[n], by_group[n]);
+    }
+    v4i part[3];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int turn = i % kTurns;
+      if (turn == 0) parts(raw[i / kTurns], part);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t scale = by_group[n][i & 1][i >> 1 & 3];
+        if (!BEYOND) {
+          add_product(part, from_e2m1<T>(codes[n][i], __uint_as_float(scale)), sums[n].first[turn], sums[n].rest[turn]);
+          continue;
+        }
+        float inner, outer;
+        part_scale(scale, inner, outer);
+        v4f first{0.f, 0.f, 0.f, 0.f}, rest{0.f, 0.f, 0.f, 0.f};
+        add_product(part, from_e2m1<T>(codes[n][i], inner), first, rest);
+        add_scaled(sums[n], turn, outer, first, rest);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 

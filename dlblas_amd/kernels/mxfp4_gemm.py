@@ -117,8 +117,7 @@ def mxfp4_weight_gemm(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor) -> 
     """``x`` [..., K] (bf16 / fp16) times weights in 4-bit floating point, ``w_q`` [N, K / 2] uint8 with scales ``w_s`` [N, K / 32] uint8 as
     ``per_group_quant_mxfp4`` makes them: [..., N] in the type of x; fp32 sums, one rounding.
 
-    For up to a few dozen rows, which stay unquantised: the weights are read once per 16 of them.  Beside bf16 rows weights below 2^-126 in
-    magnitude may count as zero.
+    For up to a few dozen rows, which stay unquantised: the weights are read once per 16 of them.
     """
     if not torch.compiler.is_compiling():
         y = _fast.mxfp4_weight_gemm(x, w_q, w_s)

@@ -46,8 +46,7 @@ int dlb_mxfp4_gemm(const void* a, const void* b, const void* a_s, const void* b_
                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * y[m, n] = sum over the groups g of 2^(s[n, g] - 127) sum_{k in g} x[m, k] q[n, k]; fp32 sums, one rounding at the end.  Beside bf16 rows weights
- * below 2^-126 in magnitude may count as zero.  Meant for up to a few dozen rows: the weights are read once per 16 of them,
+ * y[m, n] = sum over the groups g of 2^(s[n, g] - 127) sum_{k in g} x[m, k] q[n, k]; fp32 sums, one rounding at the end.  Meant for up to a few dozen rows: the weights are read once per 16 of them,
  * beside each other.
  *
  *   x [M, K]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
@@ -75,8 +74,7 @@ size_t dlb_few_token_experts_workspace_bytes(int64_t tokens, int64_t topk, int64
  *   out[t] = sum over the slots j with 0 <= ids[t, j] < experts of weights[t, j] Down[e] (silu(Gate[e] x[t]) * (Up[e] x[t])),  e = ids[t, j]
  * Products, sums and what lies between the products in fp32, the result rounded once.  Zeros for a token
  * without an expert here; slots that name one expert twice count both weights.  The order of all sums depends on the routing and the sizes alone.
- * Beside bf16 rows, and in Down, weights below 2^-126 in magnitude may count as zero, and in Down what lies between the products is exact down to
- * 2^-126 alone.
+ * What lies between the products meets Down exactly down to 2^-126.
  *
  *   x       [tokens, H]     bf16 / fp16 (dtype), row stride x_row_stride (even, at most 2^23), 4-byte aligned
  *   ids     [tokens, topk]  int32 / int64 (ids_dtype, DLB_IDX_*) through two strides;  weights [tokens, topk] fp32, contiguous
