@@ -6,7 +6,7 @@
 //
 // h is rounded before the norm reads it, as in the RMS norm and for the same reason; everything else is fp32 with one rounding at the store.  The
 // squares are those of h - m, from a second sweep over the registers: the difference of mean(h^2) and m^2 would lose a row whose mean is large
-// against its spread.  m and r of every row are kept for the gradient (8 bytes a row), which then needs one pass of sums over the workgroup
+// against its spread.  Sums of h are taken by 2^-16 and h - m by half, both exact, so that neither leaves the range where h is finite.  m and r of every row are kept for the gradient (8 bytes a row), which then needs one pass of sums over the workgroup
 // instead of three.
 //
 // Bound by memory like the RMS norm, and built like it: a row is read once into registers (8 elements a chunk, CH chunks a thread) and the results
@@ -85,10 +85,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_kernel(const Layer
     float v[8], e = 0.f;
     quant_unpack8<T>(h[c], v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e += EDGE == kInChunk && k < again[c] ? 0.f : v[k];  // elements past the end are zero
+    for (int k = 0; k < 8; ++k) e = fmaf(EDGE == kInChunk && k < again[c] ? 0.f : v[k], 0x1p-16f, e);  // elements past the end are zero
     s += c * threads + tid < chunks ? e : 0.f;
   }
-  const float mean = row_sum<LANES>(s, part[0], tid, threads) * inv_h;
+  const float mean = row_sum<LANES>(s, part[0], tid, threads) * (0x1p16f * inv_h), half = 0.5f * mean;
   s = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -96,12 +96,12 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_kernel(const Layer
     quant_unpack8<T>(h[c], v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float d = (EDGE == kInChunk && k < again[c]) || (EDGE == kBelowChunk && k >= p.H) ? 0.f : v[k] - mean;
+      const float d = (EDGE == kInChunk && k < again[c]) || (EDGE == kBelowChunk && k >= p.H) ? 0.f : fmaf(v[k], 0.5f, -half);
       e = fmaf(d, d, e);
     }
     s += c * threads + tid < chunks ? e : 0.f;
   }
-  const float r = 1.0f / sqrtf(row_sum<LANES>(s, part[1], tid, threads) * inv_h + p.eps);
+  const float r = 1.0f / sqrtf(row_sum<LANES>(s, part[1], tid, threads) * (4.0f * inv_h) + p.eps), twice = 2.0f * r;
   if (p.stats && tid == 0) p.stats[2 * row] = mean, p.stats[2 * row + 1] = r;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -112,10 +112,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_kernel(const Layer
     if (p.b) {
       load_weight8<T, WHOLE>(p.b, p.w_f32, at[c], p.H, b);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = fmaf((v[k] - mean) * r, w[k], b[k]);
+      for (int k = 0; k < 8; ++k) v[k] = fmaf(fmaf(v[k], 0.5f, -half) * twice, w[k], b[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (v[k] - mean) * r * w[k];
+      for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], 0.5f, -half) * twice * w[k];
     }
     store_raw8<T, WHOLE>(p.y, row * p.y_rs, at[c], pack_raw8<T>(v), p.H);
   }
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       load(min(row + workers, p.rows - 1), next);  // behind the last row that one again
     else
       load(row, now);
-    const float mean = now.mean, r = now.r;
+    const float half = 0.5f * now.mean, r = now.r, twice = 2.0f * r;
     float sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       for (int k = 0; k < 8; ++k) {  // elements past the end: g is zero
         const float t = EDGE == kInChunk && k < again[c] ? 0.f : g[k] * w[k];
         s += t;
-        d = fmaf(t, (hv[k] - mean) * r, d);
+        d = fmaf(t, fmaf(hv[k], 0.5f, -half) * twice, d);
       }
       const bool live = c * threads + tid < chunks;
       sum += live ? s : 0.f, dot += live ? d : 0.f;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_backward_kernel(co
       weights(c, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float n = (hv[k] - mean) * r;
+        const float n = fmaf(hv[k], 0.5f, -half) * twice;
         dw[c][k] = fmaf(g[k], n, dw[c][k]);
         if (BIAS) db[c][k] += g[k];
         g[k] = r * (fmaf(g[k], w[k], -middle) - n * along);

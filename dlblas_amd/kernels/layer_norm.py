@@ -5,7 +5,7 @@ reference has the norm without a residual under dlblas/kernels/layer_norm/.
     y = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps) * weight + bias in fp32, rounded once
 
 ``h`` is rounded before the norm reads it, because it is what the next layer adds to and what the gradient starts from.  The squares are those
-of the centred row, in fp32: rows whose sum passes 2^128 give the bias.
+of the centred row, in fp32: rows whose sum passes 2^130 give the bias.
 """
 from typing import Optional
 

@@ -66,8 +66,8 @@ int dlb_rms_norm_backward(const void* dy, int64_t dy_row_stride, const void* dsu
 
 /*
  * Layer norm: h = x + residual rounded to the element type (h = x without a residual), m = mean(h), r = 1 / sqrt(mean((h - m)^2) + eps),
- * y = (h - m) r w + b; fp32 inside, one rounding at the store.  The sum of squares is fp32 as well: rows whose sum passes 2^128
- * (|h - m| about 10^17 throughout) give y = b, or NaN where they hold an infinity.
+ * y = (h - m) r w + b; fp32 inside, one rounding at the store.  The sum of squares is fp32 as well: rows whose sum passes 2^130
+ * (|h - m| about 4 * 10^17 at 7168 columns) give y = b and count nothing in the gradients, or NaN where they hold an infinity.
  *
  *   x, residual, y, sum  [rows, H]  one element type (dtype); residual NULL: none, and sum is not written
  *   weight, bias         [H]        the same type, or fp32 (weight_dtype, of both); bias NULL: none
