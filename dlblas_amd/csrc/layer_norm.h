@@ -6,7 +6,8 @@
 //
 // h is rounded before the norm reads it, as in the RMS norm and for the same reason; everything else is fp32 with one rounding at the store.  The
 // squares are those of h - m, from a second sweep over the registers: the difference of mean(h^2) and m^2 would lose a row whose mean is large
-// against its spread.  Sums of h are taken by 2^-16 and h - m by half, both exact, so that neither leaves the range where h is finite.  m and r of every row are kept for the gradient (8 bytes a row), which then needs one pass of sums over the workgroup
+// against its spread.  The same sweep has the sum of h - m, what the rounded mean is off by: corrected by it the mean of a constant row is its value, which the sum's and
+// 1 / H's roundings miss (7168 columns of 1e5 in bf16 by 2^-7, more than sqrt(eps)).  Sums of h are taken by 2^-16 and h - m by half, both exact, so that neither leaves the range where h is finite.  m and r of every row are kept for the gradient (8 bytes a row), which then needs one pass of sums over the workgroup
 // instead of three.
 //
 // Bound by memory like the RMS norm, and built like it: a row is read once into registers (8 elements a chunk, CH chunks a thread) and the results
@@ -48,11 +49,22 @@ __device__ __forceinline__ float row_sum(float v, float* part, int tid, int thre
   return v;
 }
 
+// The same of two.
+template <int LANES>
+__device__ __forceinline__ void row_sums(float& a, float& b, float* part_a, float* part_b, int tid, int threads) {
+  a = wave_sum<LANES>(a), b = wave_sum<LANES>(b);
+  if (LANES < 64 || threads == 64) return;
+  if ((tid & 63) == 0) part_a[tid >> 6] = a, part_b[tid >> 6] = b;
+  lds_barrier();
+  a = b = 0.f;
+  for (int i = 0; i < threads / 64; ++i) a += part_a[i], b += part_b[i];
+}
+
 // One workgroup per row, or blockDim.y narrow rows, as in rms_norm_kernel.
 template <int T, bool RES, Edge EDGE, int CH, int LANES>
 __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_kernel(const LayerNormArgs p) {
   constexpr bool WHOLE = EDGE != kBelowChunk;
-  __shared__ float part[2][kNormMaxWaves];
+  __shared__ float part[3][kNormMaxWaves];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int64_t row = grid_row() * blockDim.y + beside<LANES>();
   if (row >= p.rows) return;  // with rows beside each other in a workgroup there is no barrier
@@ -88,20 +100,25 @@ __global__ void __launch_bounds__(kNormMaxThreads) layer_norm_kernel(const Layer
     for (int k = 0; k < 8; ++k) e = fmaf(EDGE == kInChunk && k < again[c] ? 0.f : v[k], 0x1p-16f, e);  // elements past the end are zero
     s += c * threads + tid < chunks ? e : 0.f;
   }
-  const float mean = row_sum<LANES>(s, part[0], tid, threads) * (0x1p16f * inv_h), half = 0.5f * mean;
+  const float near = row_sum<LANES>(s, part[0], tid, threads) * (0x1p16f * inv_h), rough = 0.5f * near;
   s = 0.f;
+  float left = 0.f;  // of (h - near) / 2, by 2^-16 as above
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    float v[8], e = 0.f;
+    float v[8], e = 0.f, l = 0.f;
     quant_unpack8<T>(h[c], v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float d = (EDGE == kInChunk && k < again[c]) || (EDGE == kBelowChunk && k >= p.H) ? 0.f : fmaf(v[k], 0.5f, -half);
-      e = fmaf(d, d, e);
+      const float d = (EDGE == kInChunk && k < again[c]) || (EDGE == kBelowChunk && k >= p.H) ? 0.f : fmaf(v[k], 0.5f, -rough);
+      e = fmaf(d, d, e), l = fmaf(d, 0x1p-16f, l);
     }
-    s += c * threads + tid < chunks ? e : 0.f;
+    s += c * threads + tid < chunks ? e : 0.f, left += c * threads + tid < chunks ? l : 0.f;
   }
-  const float r = 1.0f / sqrtf(row_sum<LANES>(s, part[1], tid, threads) * (4.0f * inv_h) + p.eps), twice = 2.0f * r;
+  row_sums<LANES>(s, left, part[1], part[2], tid, threads);
+  const float off = left * (0x1p16f * inv_h);  // half of what `near` is off by
+  const float mean = fmaf(2.0f, off, near), half = 0.5f * mean;
+  // (one rounding, so that squares beyond the range stay beyond it; NaN comes back by the mean)
+  const float r = 1.0f / sqrtf(fmaxf(4.0f * fmaf(-off, off, s * inv_h), 0.f) + p.eps), twice = 2.0f * r;
   if (p.stats && tid == 0) p.stats[2 * row] = mean, p.stats[2 * row + 1] = r;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {

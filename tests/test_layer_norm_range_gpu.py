@@ -54,3 +54,37 @@ def test_infinities_still_show(dev):
     x[2, 9] = float('nan')
     w, b = torch.ones(1024), torch.zeros(1024)
     assert bool(layer_norm(*(t.to(dev) for t in (x, w, b))).isnan().all())
+
+
+@pytest.mark.parametrize('dtype', [bf16, torch.float16, f32])
+@pytest.mark.parametrize('residual', [False, True])
+@pytest.mark.parametrize('H', [5, 64, 264, 1000, 2050, 7168, 20001, 32768])
+def test_constant_rows(dev, H, residual, dtype):
+    """The mean of a constant row is its value, whatever 1 / H rounds to: y = b, and nothing for the weight's gradient."""
+    g = torch.Generator().manual_seed(H)
+    values = torch.tensor([0.1, 3.0, -1000.1, 60000.0] + ([] if dtype == torch.float16 else [1e5, -1.2345e9, 7e25]))
+    x = values[:, None].expand(-1, H).to(dtype).contiguous()
+    res = (torch.zeros_like(x) if residual else None)
+    w, b = (1 + 0.2 * torch.randn(H, generator=g)).to(dtype), torch.randn(H, generator=g).to(dtype)
+    leaves = [t.to(dev).requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves, 1e-5, None if res is None else res.to(dev))
+    y = y[0] if residual else y
+    assert torch.equal(y.detach().cpu(), b.expand_as(x))
+    _, dw, _ = torch.autograd.grad([y], leaves, [torch.randn(x.shape, generator=g).to(dtype).to(dev)])
+    assert float(dw.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('H', [264, 1000, 7168])
+@pytest.mark.parametrize('far', [100.0, 1e4, 1e6])
+def test_rows_far_from_zero(dev, H, far):
+    """The mean is corrected by that of h - mean, so what it is off by is its own rounding, 2^-24 of it, and 60 2^-24 of the mean |h - m|; the squares' mean is off by the square of that and 64 roundings
+    (56 of the sum and the correction's), the root by half."""
+    g = torch.Generator().manual_seed(H)
+    x = far + torch.randn(9, H, generator=g)
+    w, b = torch.ones(H), torch.zeros(H)
+    h = x.double()
+    d = h - h.mean(1, keepdim=True)
+    r = 1 / (d.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    off = 2.0**-24 * h.mean(1, keepdim=True).abs() + 60 * 2.0**-24 * d.abs().mean(1, keepdim=True)
+    bound = r * (off + 2.0**-24 * d.abs()) + (d * r).abs() * ((off * r)**2 / 2 + 40 * 2.0**-24)
+    inside(layer_norm(*(t.to(dev) for t in (x, w, b))), d * r, bound, f'{far}')
