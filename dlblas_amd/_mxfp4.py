@@ -7,7 +7,7 @@ from ._lib import IDX_CODES, IN_CODES, _ptr, _stream, check, load
 
 GROUP = 32  # columns that share a scale
 MAX_COLUMNS = 1 << 22
-FEW_TOKENS, FEW_TOPK, FEW_EXPERTS = 64, 16, 1024
+FEW_TOKENS, FEW_TOPK, FEW_EXPERTS, FEW_NUMBERS = 64, 16, 1024, 1 << 29
 WEIGHTS_E4M3, WEIGHTS_MXFP4 = 0, 1
 
 

@@ -188,7 +188,7 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
                 kFewTopk, kFewExperts);
   if (H % unit != 0 || I % unit != 0 || I == 0 || H > (1 << 20) || I > (1 << 20))
     return fail(DLB_ERR_BAD_SHAPE, "H=%lld, I=%lld must be multiples of %lld, I at least that, both at most 2^20", (long long)H, (long long)I, (long long)unit);
-  if (tokens * topk * I > (1 << 29)) return fail(DLB_ERR_BAD_SHAPE, "tokens * topk * I=%lld is beyond 2^29", (long long)(tokens * topk * I));
+  if (tokens * topk * I > DLB_FEW_NUMBERS) return fail(DLB_ERR_BAD_SHAPE, "tokens * topk * I=%lld is beyond 2^29", (long long)(tokens * topk * I));
   if (tokens == 0 || H == 0) return DLB_OK;
   if (!x || !ids || !weights || !up_q || !up_s || !down_q || !down_s || !out) return fail(DLB_ERR_NULL_POINTER, "a tensor pointer is NULL");
   if (x_row_stride < 0 || x_row_stride > (1 << 23)) return fail(DLB_ERR_BAD_STRIDE, "x row stride %lld is not 0 ... 2^23", (long long)x_row_stride);

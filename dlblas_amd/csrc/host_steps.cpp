@@ -666,6 +666,8 @@ PyObject* few_token_experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool f4 = up.scalar_type() == at::kByte;
   if (!f4 && !is_f8(up)) NOT_PLAIN;
   const int64_t T = x.size(0), H = x.size(1), topk = ids.size(1), E = up.size(0), I = up.size(1) / 2, part = f4 ? 2 : 1;
+  // too much for the kernels: refused before anything is allocated for it
+  if (T > DLB_FEW_TOKENS || topk > DLB_FEW_TOPK || E > DLB_FEW_EXPERTS || T * topk * I > DLB_FEW_NUMBERS) NOT_PLAIN;
   if (up.size(1) != 2 * I || up.size(2) * part != H || down.size(0) != E || down.size(1) != H || down.size(2) * part != I || I == 0 || E == 0) NOT_PLAIN;
   if (f4) {
     if (mx_columns(up, up_s, 16) == 0 || mx_columns(down, down_s, 16) == 0) NOT_PLAIN;

@@ -91,6 +91,8 @@ def few_token_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: tor
     _check_weights('w2_weight', w2, w2_s, I)
     if w2.size(0) != E or w2.size(1) != H:
         raise ValueError(f'w2_weight must be [{E}, {H}, {I}], got {list(w2.shape)}')
+    if T * topk_ids.size(1) * I > _mxfp4.FEW_NUMBERS:
+        raise ValueError(f'tokens * topk * I is {T * topk_ids.size(1) * I}, at most {_mxfp4.FEW_NUMBERS} are implemented')
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, topk_weights, w13, w13_s, w2, w2_s)):
         raise NotImplementedError('few_token_experts has no gradient: call it under torch.no_grad()')
     out = torch.empty((T, H), dtype=x.dtype, device=x.device)

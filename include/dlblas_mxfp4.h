@@ -62,6 +62,7 @@ int dlb_mxfp4_weight_gemm(const void* x, int64_t x_row_stride, int dtype, const 
 #define DLB_FEW_TOKENS 64
 #define DLB_FEW_TOPK 16
 #define DLB_FEW_EXPERTS 1024
+#define DLB_FEW_NUMBERS (1 << 29) /* tokens * topk * I */
 /* weight types of dlb_few_token_experts: e4m3fn with fp32 scales of 128 x 128, or the 4-bit format above */
 #define DLB_WEIGHTS_E4M3 0
 #define DLB_WEIGHTS_MXFP4 1
