@@ -57,7 +57,7 @@ def few_token_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: tor
 
     Returns:
         ``[T, H]`` in the type of x; fp32 sums, one rounding; zeros for a token without an expert here.  Not differentiable.  For more tokens:
-        ``fused_moe_v3``.
+        ``fused_moe_v3`` with e4m3 weights; no call takes 4-bit ones by expert for a prompt, which leaves ``mxfp4_gemm`` on the rows of one expert after the other.
     """
     if not torch.compiler.is_compiling():
         out = _fast.few_token_experts(x, topk_ids, topk_weights, w13_weight, w2_weight)
@@ -77,7 +77,8 @@ def few_token_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: tor
         raise ValueError(f'topk_weights must be like topk_ids {list(topk_ids.shape)}, got {list(topk_weights.shape)}')
     T, H = x.shape
     if T > _mxfp4.FEW_TOKENS:
-        raise ValueError(f'at most {_mxfp4.FEW_TOKENS} tokens are implemented, got {T}: fused_moe_v3 takes more')
+        more = 'fused_moe_v3 takes more' if w13.dtype != torch.uint8 else 'of 4-bit experts more go through mxfp4_gemm, expert by expert'
+        raise ValueError(f'at most {_mxfp4.FEW_TOKENS} tokens are implemented, got {T}: {more}')
     if not 1 <= topk_ids.size(1) <= _mxfp4.FEW_TOPK:
         raise ValueError(f'1 to {_mxfp4.FEW_TOPK} experts a token are implemented, got {topk_ids.size(1)}')
     if w13.dtype != w2.dtype:

@@ -22,3 +22,15 @@ def test_too_many_numbers_between_the_products():
     with pytest.raises(ValueError, match='tokens'):
         few_token_experts(meta(T, H, dtype=torch.bfloat16), meta(T, topk, dtype=torch.int32), meta(T, topk, dtype=torch.float32), (meta(1, 2 * I, H // 2, dtype=u8), meta(1, 2 * I, H // 32, dtype=u8)),
                           (meta(1, H, I // 2, dtype=u8), meta(1, H, I // 32, dtype=u8)))
+
+
+@pytest.mark.parametrize('bits', [8, 4])
+def test_a_prompt_is_sent_to_a_call_that_takes_its_weights(bits):
+    T, topk, E, H, I = 65, 2, 4, 256, 128
+    zeros = lambda *size, dtype: torch.zeros(size, dtype=dtype)
+    if bits == 4:
+        w13, w2 = ((zeros(E, n, k // 2, dtype=torch.uint8), zeros(E, n, k // 32, dtype=torch.uint8)) for n, k in ((2 * I, H), (H, I)))
+    else:
+        w13, w2 = ((zeros(E, n, k, dtype=torch.uint8).view(torch.float8_e4m3fn), zeros(E, n // 128, k // 128, dtype=torch.float32)) for n, k in ((2 * I, H), (H, I)))
+    with pytest.raises(ValueError, match='fused_moe_v3' if bits == 8 else 'mxfp4_gemm'):
+        few_token_experts(zeros(T, H, dtype=torch.bfloat16), zeros(T, topk, dtype=torch.int32), zeros(T, topk, dtype=torch.float32), w13, w2)
