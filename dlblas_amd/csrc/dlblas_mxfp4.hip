@@ -230,12 +230,16 @@ int dlb_few_token_experts(const void* x, int64_t x_row_stride, int dtype, const 
       hipLaunchKernelGGL((experts_up_kernel<kt(), kw(), r(), split()>), grid, dim3(64 * kUpWaves), Shape::kLds, st, a);
     };
     with_chunks<4, 8, 16>(up_rows, [&](auto r) {
-      // Two waves to K, whose runs are then long against their start and end; four where K is short, or an e4m3 expert has few rows.  e2m1 / e4m3 us, 8 of 32 experts,
-      // 4096 x 7168: 8 tokens two 96 / 133, four 109 / 130;  16 tokens 104 / 144, 122 / 149;  64 tokens 194 / 230, 228 / 250;  5 tokens, 1088 x 1056: 12.3, four 9.0.
-      if constexpr (kw() == kE2m1) {
-        with_flag(H >= 4096, [&](auto two) { up(r, std::integral_constant<int, two() ? 2 : 4>()); });
+      // Two waves to K, whose runs are then long against their start and end, while that leaves workgroups for three quarters of the CUs; four otherwise, and with e4m3 weights for eight
+      // rows or fewer.  us of both products with two / four, 2 slots a token, 8 experts:
+      //   e2m1, H = 2048: 5 tokens, I = 544 (136 workgroups) 22.0 / 21.0, 768 (192) 21.0 / 21.3, 2048 (512) 28.7 / 32.1;  H = 7168: 29.9 / 26.8, 29.1 / 28.6, 45.3 / 45.2
+      //         64 tokens, H = 2048: I = 1024 (128) 67.9 / 61.4, 1536 (192) 81.9 / 84.8;  16 tokens x 8 of 32 experts, I = 2048: H = 1024 115 / 138, 4096 149 / 163, 7168 189 / 200
+      //   e4m3, 64 tokens: H = 2048: I = 1024 64.9 / 58.9, 1536 77.5 / 79.5, 4096 157 / 164;  5 tokens: H = 2048: I = 2048 30.6 / 31.1;  H = 7168: 52.5 / 49.9
+      if constexpr (kw() == kE2m1 || r() == 16) {
+        const bool enough = ceil_div(I, UpShape<kw(), r(), 2>::kColumns) * named >= 192;
+        with_flag(enough, [&](auto two) { up(r, std::integral_constant<int, two() ? 2 : 4>()); });
       } else {
-        up(r, std::integral_constant<int, r() == 16 ? 2 : 4>());
+        up(r, std::integral_constant<int, 4>());
       }
     });
     const auto down = [&](auto t, auto waves) {
