@@ -16,7 +16,7 @@ int check_columns(int64_t K) {
 }
 
 // How a product runs.  us of M x N x K, one side of a border and the other:
-//   16 x 2112 x 7168    split 1 x 1: 6.3, 1 x 2: 7.5        16 x 7168 x 18432: 23.0, 16.4
+//   16 x 2112 x 7168    split 1 x 1: 5.8, 1 x 2: 7.5        16 x 7168 x 18432: 23.0, 16.4
 //   17 x 7168 x 18432   split 1 x 2: 29,  2 x 2: 18
 //   65 x 2112 x 7168    split 2 x 2: 8.1, 64 tiles: 14.7    128 x 2112 x 7168 (264 workgroups): 13.8, 14.8   65 x 7168 x 18432: 49, 33
 //   64 x 7168 x 18432   split 4 x 2: 28,  64 tiles: 32      65: 50, 33

@@ -80,8 +80,8 @@ struct Matrix {
 // Rows of x are 16-bit numbers, or with F32 fp32 ones, R / 2 of them: each is the sum of three bf16, the nearest, the nearest to what that leaves, and the rest, which
 // has six bits at most (parts below 2^-126 may count as 0).  Every part has a product of its own.  A lane makes the parts of eight numbers, those of one step in R / 2 rows of
 // the MFMA and of the next in the R / 2 behind them, so that none makes what another has; a product of one step then fills those rows, and what it leaves in the others is
-// of no use.  (Instructions bound this: with lanes that exchange their parts, first and second in the rows of one product, as long, and with every lane making the parts of both
-// 8 % longer.)  Sums of the first parts stay apart: what an infinity leaves is no number.
+// of no use.  Instructions bound this (16 tokens x 8 of 32 experts, 7168 x 2048 e2m1, eight tokens a pass: 102 us, with lanes that exchange their parts, first and second in the
+// rows of one product, 103; rows of 16 bits 73).  Sums of the first parts stay apart: what an infinity leaves is no number.
 //
 // A 16-byte piece of a row lies at another place of it, by the row, so that a read of 16 rows meets every bank once: of x piece ^ row, of weights
 // piece ^ (row / 2).  Steps of an MFMA are 32 columns: of e4m3 eight from each quarter's 16-byte piece, of e2m1 a group, a word of its 16 bytes a
